@@ -9,5 +9,6 @@ from .codec import (AstcEncoder, EncodedTensor, align, attention, attention_metr
 from .ops import (Attention, DevicePlane, contiguous_astc_plane, contiguous_fp16_plane, decode_attention,
                   decode_blocks, decode_image, host_encode, init, paged_astc_plane, paged_fp16_plane,
                   random_blocks, restore_plane)
+from .q8 import (Q8Attention, Q8Cache, Q8Evict, Q8Restore, Q8Store, q8_attention, q8_evict, q8_restore, q8_store)
 
 __version__ = "0.1.0"

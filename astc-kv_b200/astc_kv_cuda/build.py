@@ -19,10 +19,11 @@ CSRC = ROOT / "csrc"
 INCLUDE = ROOT.parent / "include"
 LIB = PKG / "libakv_cuda.so"
 
-SOURCES = ["akv_cuda.cu", "akv_tables.cpp", "akv_encode.cpp"]
+SOURCES = ["akv_cuda.cu", "akv_q8.cu", "akv_tables.cpp", "akv_encode.cpp"]
 HEADERS = ["akv_astc_device.cuh", "akv_common.cuh", "akv_decode_kernels.cuh", "akv_attention_kernels.cuh", "akv_tables.h",
            "akv_attn_fp16.cuh",
-           "akv_attn_fast.cuh", "akv_decode_fast.cuh"]
+           "akv_attn_fast.cuh", "akv_decode_fast.cuh",
+           "akv_q8_common.cuh", "akv_q8_store.cuh", "akv_q8_attend.cuh", "akv_q8_evict.cuh"]
 
 
 def nvcc() -> str:
@@ -36,7 +37,7 @@ def _stale() -> bool:
     if not LIB.exists():
         return True
     mtime = LIB.stat().st_mtime
-    deps = [CSRC / s for s in SOURCES + HEADERS] + [INCLUDE / "akv_cuda.h", INCLUDE / "akv_host.h", Path(__file__)]
+    deps = [CSRC / s for s in SOURCES + HEADERS] + [INCLUDE / "akv_cuda.h", INCLUDE / "akv_host.h", INCLUDE / "akv_q8.h", Path(__file__)]
     return any(d.stat().st_mtime > mtime for d in deps if d.exists())
 
 
@@ -44,7 +45,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not _stale():
         return LIB
     cmd = [nvcc(), "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-           "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-shared", "-I", str(INCLUDE),
+           "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-shared", "-t", "0", "-I", str(INCLUDE),
            "-o", str(LIB)] + [str(CSRC / s) for s in SOURCES]
     if verbose:
         cmd.insert(1, "-Xptxas=-v")

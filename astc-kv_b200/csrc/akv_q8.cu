@@ -1,0 +1,194 @@
+// C-ABI entry points of the 8-bit KV cache (declared in include/akv_q8.h):
+// argument validation, launch shapes, template dispatch.
+#include <cuda_runtime.h>
+
+#include <cmath>
+
+#include "../../include/akv_q8.h"
+#include "akv_q8_attend.cuh"
+#include "akv_q8_evict.cuh"
+#include "akv_q8_store.cuh"
+
+namespace akv {
+namespace q8 {
+namespace {
+
+constexpr int kMaxGridYZ = 65535;
+
+inline int launched() { return cudaPeekAtLastError() == cudaSuccess ? AKV_OK : (cudaGetLastError(), AKV_ERR_CUDA); }
+
+bool valid_dtype(int t) { return t >= AKV_Q_F32 && t <= AKV_Q_F16; }
+
+bool valid_side(const AkvQ8Side& s) {
+    return s.codes && s.scales && reinterpret_cast<uintptr_t>(s.codes) % 16 == 0 && reinterpret_cast<uintptr_t>(s.scales) % 4 == 0 &&
+           s.stride_batch % 16 == 0 && s.stride_head % 16 == 0 && s.stride_page % 16 == 0 && s.stride_token % 16 == 0;
+}
+
+int check_cache(const AkvQ8Cache& c) {
+    if (c.format != AKV_Q8_INT8 && c.format != AKV_Q8_E4M3) return AKV_ERR_INVALID_ARGUMENT;
+    if (c.batch < 0 || c.kv_heads <= 0 || c.head_dim <= 0 || c.max_tokens <= 0 || c.page_tokens <= 0) return AKV_ERR_INVALID_ARGUMENT;
+    if (!valid_side(c.k) || !valid_side(c.v)) return AKV_ERR_INVALID_ARGUMENT;
+    if (c.block_tokens <= 0 || c.page_tokens % c.block_tokens) return AKV_ERR_INVALID_ARGUMENT;
+    if (c.block_table_dev &&
+        (c.pages_per_seq <= 0 || c.num_pages <= 0 || static_cast<int64_t>(c.pages_per_seq) * c.page_tokens < c.max_tokens))
+        return AKV_ERR_INVALID_ARGUMENT;
+    if (c.block_tokens != 16 && c.block_tokens != 32 && c.block_tokens != 64 && c.block_tokens != 128) return AKV_ERR_UNSUPPORTED;
+    if (c.head_dim % 16 || c.head_dim > 256 || c.kv_heads > kMaxGridYZ || c.batch > kMaxGridYZ / 2) return AKV_ERR_UNSUPPORTED;
+    return AKV_OK;
+}
+
+// Calls fn with a value of the element type of an AKV_Q_* code.
+template <typename F>
+void with_type(int dtype, F fn) {
+    if (dtype == AKV_Q_F32) fn(float{});
+    else if (dtype == AKV_Q_BF16) fn(__nv_bfloat16{});
+    else fn(__half{});
+}
+
+int check_attention(const AkvQ8AttnDesc* d) {
+    if (!d) return AKV_ERR_INVALID_ARGUMENT;
+    if (int st = check_cache(d->cache)) return st;
+    if (d->q_heads <= 0 || d->q_heads % d->cache.kv_heads || d->q_tokens < 0 || !valid_dtype(d->q_dtype) || !valid_dtype(d->out_dtype))
+        return AKV_ERR_INVALID_ARGUMENT;
+    if (d->split_tokens < 0 || d->split_tokens % 16 || !(d->scale >= 0.f) || std::isinf(d->scale)) return AKV_ERR_INVALID_ARGUMENT;
+    if (d->weights_dev && d->weights_stride < d->cache.max_tokens) return AKV_ERR_INVALID_ARGUMENT;
+    if (d->q_heads > kMaxGridYZ || d->q_tokens > kMaxGridYZ) return AKV_ERR_UNSUPPORTED;
+    return AKV_OK;
+}
+
+size_t attention_workspace(const AkvQ8AttnDesc* d) {
+    return (static_cast<size_t>(d->cache.batch) * d->q_tokens * d->q_heads * sizeof(float) + 16 + 15) / 16 * 16;
+}
+
+}  // namespace
+}  // namespace q8
+}  // namespace akv
+
+using namespace akv;
+using namespace akv::q8;
+
+extern "C" {
+
+size_t akv_q8_struct_size(int which) {
+    switch (which) {
+        case 0: return sizeof(AkvQ8Cache);
+        case 1: return sizeof(AkvQ8StoreDesc);
+        case 2: return sizeof(AkvQ8RestoreDesc);
+        case 3: return sizeof(AkvQ8AttnDesc);
+        case 4: return sizeof(AkvQ8EvictDesc);
+        default: return 0;
+    }
+}
+
+int akv_q8_store(const AkvQ8StoreDesc* d, void* stream) {
+    if (!d) return AKV_ERR_INVALID_ARGUMENT;
+    if (int st = check_cache(d->cache)) return st;
+    if (d->tokens < 0 || !valid_dtype(d->dtype)) return AKV_ERR_INVALID_ARGUMENT;
+    if (d->cache.batch == 0 || d->tokens == 0) return AKV_OK;
+    const uintptr_t elem = d->dtype == AKV_Q_F32 ? 4 : 2;
+    if (!d->k_dev || !d->v_dev || !d->start_dev || reinterpret_cast<uintptr_t>(d->k_dev) % elem ||
+        reinterpret_cast<uintptr_t>(d->v_dev) % elem)
+        return AKV_ERR_INVALID_ARGUMENT;
+    StoreParams p;
+    p.c = to_dev(d->cache);
+    p.x[0] = d->k_dev; p.x[1] = d->v_dev;
+    p.xB[0] = d->k_stride[0]; p.xT[0] = d->k_stride[1]; p.xH[0] = d->k_stride[2];
+    p.xB[1] = d->v_stride[0]; p.xT[1] = d->v_stride[1]; p.xH[1] = d->v_stride[2];
+    p.start = d->start_dev; p.counts = d->counts_dev; p.n = d->tokens;
+    const int blocks = static_cast<int>((static_cast<int64_t>(d->tokens) + 2 * p.c.blk - 2) / p.c.blk);
+    const dim3 grid(blocks, p.c.H, 2 * p.c.B);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    with_type(d->dtype, [&](auto t) {
+        using T = decltype(t);
+        if (p.c.fmt == AKV_Q8_INT8) store_kernel<AKV_Q8_INT8, T><<<grid, kStoreThreads, 0, s>>>(p);
+        else store_kernel<AKV_Q8_E4M3, T><<<grid, kStoreThreads, 0, s>>>(p);
+    });
+    return launched();
+}
+
+int akv_q8_restore(const AkvQ8RestoreDesc* d, void* stream) {
+    if (!d) return AKV_ERR_INVALID_ARGUMENT;
+    if (int st = check_cache(d->cache)) return st;
+    if (d->tokens < 0 || !valid_dtype(d->dtype)) return AKV_ERR_INVALID_ARGUMENT;
+    if (d->cache.batch == 0 || d->tokens == 0) return AKV_OK;
+    if (!d->k_dev || !d->v_dev || reinterpret_cast<uintptr_t>(d->k_dev) % 16 || reinterpret_cast<uintptr_t>(d->v_dev) % 16)
+        return AKV_ERR_INVALID_ARGUMENT;
+    RestoreParams p;
+    p.c = to_dev(d->cache);
+    p.out[0] = d->k_dev; p.out[1] = d->v_dev;
+    p.start = d->start_dev; p.n = d->tokens;
+    const int64_t pieces = static_cast<int64_t>(p.c.B) * p.n * p.c.H * (p.c.D / 16);
+    const int64_t ctas = (pieces + 255) / 256;
+    if (ctas > 0x7FFFFFFF) return AKV_ERR_UNSUPPORTED;
+    const dim3 grid(static_cast<unsigned>(ctas), 2);
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    with_type(d->dtype, [&](auto t) {
+        using T = decltype(t);
+        if (p.c.fmt == AKV_Q8_INT8) restore_kernel<AKV_Q8_INT8, T><<<grid, 256, 0, s>>>(p);
+        else restore_kernel<AKV_Q8_E4M3, T><<<grid, 256, 0, s>>>(p);
+    });
+    return launched();
+}
+
+size_t akv_q8_attention_workspace(const AkvQ8AttnDesc* d) { return check_attention(d) == AKV_OK ? attention_workspace(d) : 0; }
+
+int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
+    if (int st = check_attention(d)) return st;
+    if (d->cache.batch == 0 || d->q_tokens == 0) return AKV_OK;
+    const uintptr_t elem = d->q_dtype == AKV_Q_F32 ? 4 : 2;
+    if (!d->q_dev || !d->out_dev || reinterpret_cast<uintptr_t>(d->q_dev) % elem || reinterpret_cast<uintptr_t>(d->out_dev) % 16)
+        return AKV_ERR_INVALID_ARGUMENT;
+    if (!d->workspace_dev || d->workspace_bytes < attention_workspace(d)) return AKV_ERR_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(d->workspace_dev) % 16) return AKV_ERR_INVALID_ARGUMENT;
+    AttnParams p;
+    p.c = to_dev(d->cache);
+    p.Hq = d->q_heads; p.G = d->q_heads / d->cache.kv_heads; p.n = d->q_tokens;
+    p.q_dtype = d->q_dtype; p.out_dtype = d->out_dtype; p.causal = d->causal; p.accumulate = d->accumulate;
+    p.c2 = (d->scale > 0.f ? d->scale : 1.0f / std::sqrt(static_cast<float>(p.c.D))) * 1.4426950408889634f;
+    p.q = d->q_dev; p.qB = d->q_stride[0]; p.qT = d->q_stride[1]; p.qH = d->q_stride[2];
+    p.lens = d->seq_lens_dev; p.q_lens = d->q_lens_dev;
+    p.out = d->out_dev; p.lse = static_cast<float*>(d->workspace_dev); p.lse_out = d->lse_dev;
+    p.weights = d->weights_dev; p.wstride = d->weights_stride;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const dim3 grid(p.Hq, p.n, p.c.B), wgrid((p.c.T + kRowThreads - 1) / kRowThreads, p.c.H, p.c.B);
+    const bool int8 = p.c.fmt == AKV_Q8_INT8;
+    if (int8) attend_kernel<AKV_Q8_INT8><<<grid, kRowThreads, 0, s>>>(p);
+    else attend_kernel<AKV_Q8_E4M3><<<grid, kRowThreads, 0, s>>>(p);
+    if (int st = launched()) return st;
+    if (p.weights) {
+        if (int8) weights_kernel<AKV_Q8_INT8><<<wgrid, kRowThreads, 0, s>>>(p);
+        else weights_kernel<AKV_Q8_E4M3><<<wgrid, kRowThreads, 0, s>>>(p);
+    }
+    return launched();
+}
+
+int akv_q8_evict(const AkvQ8EvictDesc* d, void* stream) {
+    if (!d) return AKV_ERR_INVALID_ARGUMENT;
+    if (int st = check_cache(d->src)) return st;
+    if (int st = check_cache(d->dst)) return st;
+    const AkvQ8Cache &a = d->src, &c = d->dst;
+    if (a.format != c.format || a.batch != c.batch || a.kv_heads != c.kv_heads || a.head_dim != c.head_dim) return AKV_ERR_INVALID_ARGUMENT;
+    if (d->keep <= 0 || d->keep > c.max_tokens || d->sinks < 0 || d->recent < 0 ||
+        static_cast<int64_t>(d->sinks) + d->recent > d->keep)
+        return AKV_ERR_INVALID_ARGUMENT;
+    if (a.k.codes == c.k.codes || a.v.codes == c.v.codes || a.k.scales == c.k.scales || a.v.scales == c.v.scales)
+        return AKV_ERR_INVALID_ARGUMENT;
+    if (!d->weights_dev || !d->kept_dev || !d->out_lens_dev || !d->out_weights_dev || d->weights_stride < a.max_tokens ||
+        d->out_weights_stride < d->keep)
+        return AKV_ERR_INVALID_ARGUMENT;
+    if (a.batch == 0) return AKV_OK;
+    EvictParams p;
+    p.src = to_dev(a); p.dst = to_dev(c);
+    p.weights = d->weights_dev; p.wstride = d->weights_stride; p.lens = d->seq_lens_dev;
+    p.keep = d->keep; p.sinks = d->sinks; p.recent = d->recent;
+    p.kept = d->kept_dev; p.out_lens = d->out_lens_dev; p.out_weights = d->out_weights_dev; p.ostride = d->out_weights_stride;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    select_kernel<<<dim3(a.kv_heads, a.batch), kSelectThreads, 0, s>>>(p);
+    if (int st = launched()) return st;
+    const dim3 grid((p.keep + p.dst.blk - 1) / p.dst.blk, a.kv_heads, 2 * a.batch);
+    if (a.format == AKV_Q8_INT8) pack_kernel<AKV_Q8_INT8><<<grid, 256, 0, s>>>(p);
+    else pack_kernel<AKV_Q8_E4M3><<<grid, 256, 0, s>>>(p);
+    return launched();
+}
+
+}  // extern "C"

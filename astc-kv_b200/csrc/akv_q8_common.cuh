@@ -1,0 +1,114 @@
+// 8-bit KV cache: kernel-side view of an AkvQ8Cache, code conversions.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cstdint>
+
+#include "../../include/akv_q8.h"
+
+namespace akv {
+namespace q8 {
+
+struct SideDev {
+    uint8_t* codes;
+    float* scales;
+    int64_t sB, sH, sP, sT;  // bytes
+    int64_t cB, cH, cP;      // scales, elements
+};
+
+struct CacheDev {
+    SideDev k, v;
+    const int32_t* table;
+    int B, H, D, T, P, pps, num_pages, blk, fmt;
+    int32_t* status;
+};
+
+inline SideDev to_dev(const AkvQ8Side& s) {
+    return {static_cast<uint8_t*>(s.codes), s.scales, s.stride_batch, s.stride_head, s.stride_page, s.stride_token,
+            s.scale_stride_batch, s.scale_stride_head, s.scale_stride_page};
+}
+
+inline CacheDev to_dev(const AkvQ8Cache& c) {
+    CacheDev d;
+    d.k = to_dev(c.k);
+    d.v = to_dev(c.v);
+    d.table = c.block_table_dev;
+    d.B = c.batch; d.H = c.kv_heads; d.D = c.head_dim; d.T = c.max_tokens; d.P = c.page_tokens;
+    d.pps = c.pages_per_seq; d.num_pages = c.num_pages; d.blk = c.block_tokens; d.fmt = c.format;
+    d.status = c.status_dev;
+    return d;
+}
+
+__device__ __forceinline__ void report(int32_t* status, int code) {
+    if (status) atomicExch(status, code);
+}
+
+// Physical page of token t (0 <= t < T) of sequence b, -1 for a table entry
+// outside the pool.
+__device__ __forceinline__ int page_of(const CacheDev& c, int b, int t) {
+    const int p = t / c.P;
+    if (!c.table) return p;
+    const int v = __ldg(c.table + static_cast<int64_t>(b) * c.pps + p);
+    if (static_cast<unsigned>(v) >= static_cast<unsigned>(c.num_pages)) {
+        report(c.status, AKV_ERR_BAD_BLOCK_TABLE);
+        return -1;
+    }
+    return v;
+}
+
+__device__ __forceinline__ int64_t code_offset(const SideDev& s, int b, int h, int phys, int row) {
+    return b * s.sB + h * s.sH + phys * s.sP + row * s.sT;
+}
+
+__device__ __forceinline__ int64_t scale_offset(const SideDev& s, int b, int h, int phys, int block) {
+    return b * s.cB + h * s.cH + phys * s.cP + block;
+}
+
+// The code of y = x / scale: nearest, ties to even, saturating.
+template <int FMT>
+__device__ __forceinline__ uint8_t to_code(float y) {
+    if (FMT == AKV_Q8_INT8) return static_cast<uint8_t>(static_cast<int8_t>(__float2int_rn(fminf(fmaxf(y, -127.f), 127.f))));
+    return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+}
+
+template <int FMT>
+__device__ __forceinline__ float from_code(uint8_t c) {
+    if (FMT == AKV_Q8_INT8) return static_cast<float>(static_cast<int8_t>(c));
+    return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+}
+
+// Scale of a block from the largest |x| of its rows, given as the bits of
+// |x| (so that an infinity or a NaN, whose bits exceed every number's, is
+// seen): amax / M as a product with 1/M; NaN for what is not finite, 0 where
+// the scale would be subnormal (its reciprocal could overflow).
+template <int FMT>
+__device__ __forceinline__ float block_scale(uint32_t amax_bits) {
+    if (amax_bits >= 0x7F800000u) return __uint_as_float(0x7FC00000u);
+    constexpr float inv_most = FMT == AKV_Q8_INT8 ? 1.0f / 127.0f : 1.0f / 448.0f;
+    const float s = __fmul_rn(__uint_as_float(amax_bits), inv_most);
+    return s < 1.17549435e-38f ? 0.f : s;
+}
+
+// 1 / scale; 0 for a block of zeros or one that holds no numbers.
+__device__ __forceinline__ float block_inverse(float scale) { return scale > 0.f ? __frcp_rn(scale) : 0.f; }
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
+
+// Element loads and stores of the three 16/32-bit types.
+template <typename T>
+__device__ __forceinline__ float to_f32(T x) { return static_cast<float>(x); }
+template <>
+__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
+template <>
+__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float x) { return static_cast<T>(x); }
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+}  // namespace q8
+}  // namespace akv
