@@ -7,7 +7,9 @@
 #include "../../include/akv_q8.h"
 #include "akv_q8_attend.cuh"
 #include "akv_q8_evict.cuh"
+#include "akv_q8_step.cuh"
 #include "akv_q8_store.cuh"
+#include "akv_q8_weights.cuh"
 
 namespace akv {
 namespace q8 {
@@ -33,7 +35,9 @@ int check_cache(const AkvQ8Cache& c) {
         (c.pages_per_seq <= 0 || c.num_pages <= 0 || static_cast<int64_t>(c.pages_per_seq) * c.page_tokens < c.max_tokens))
         return AKV_ERR_INVALID_ARGUMENT;
     if (c.block_tokens != 16 && c.block_tokens != 32 && c.block_tokens != 64 && c.block_tokens != 128) return AKV_ERR_UNSUPPORTED;
-    if (c.head_dim % 16 || c.head_dim > 256 || c.kv_heads > kMaxGridYZ || c.batch > kMaxGridYZ / 2) return AKV_ERR_UNSUPPORTED;
+    if (c.head_dim % 16 || c.head_dim > 256 || c.kv_heads > kMaxGridYZ || c.batch > kMaxGridYZ / 2 ||
+        c.max_tokens > 1 << 30)
+        return AKV_ERR_UNSUPPORTED;
     return AKV_OK;
 }
 
@@ -52,12 +56,92 @@ int check_attention(const AkvQ8AttnDesc* d) {
         return AKV_ERR_INVALID_ARGUMENT;
     if (d->split_tokens < 0 || d->split_tokens % 16 || !(d->scale >= 0.f) || std::isinf(d->scale)) return AKV_ERR_INVALID_ARGUMENT;
     if (d->weights_dev && d->weights_stride < d->cache.max_tokens) return AKV_ERR_INVALID_ARGUMENT;
-    if (d->q_heads > kMaxGridYZ || d->q_tokens > kMaxGridYZ) return AKV_ERR_UNSUPPORTED;
+    if (static_cast<int64_t>(d->q_heads) * d->q_tokens > 1 << 24) return AKV_ERR_UNSUPPORTED;
     return AKV_OK;
 }
 
-size_t attention_workspace(const AkvQ8AttnDesc* d) {
-    return (static_cast<size_t>(d->cache.batch) * d->q_tokens * d->q_heads * sizeof(float) + 16 + 15) / 16 * 16;
+int sm_count() {
+    int dev = 0, n = 0;
+    cudaGetDevice(&dev);
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) cudaGetLastError();
+    return n > 0 ? n : 148;
+}
+
+struct AttnPlan {
+    int rows;         // per kv head
+    int nt;           // groups of eight rows per CTA
+    int split, nsplits;
+    bool keep_scores; // the step kernel stores its scores for the token weights
+    size_t part_ml, part_o, scores, lse, bytes;  // offsets into the workspace, and its size
+};
+
+constexpr int kSplitAlign = 16 * kStepWarps;
+
+// Rows whose scores are stored for the token weights rather than computed
+// again: storing costs 8 bytes per row and token, a second pass over K
+// head_dim bytes per token.
+constexpr int kScoreRows = 16;
+
+AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
+    AttnPlan a;
+    const AkvQ8Cache& c = d->cache;
+    const int64_t bh = static_cast<int64_t>(c.batch) * c.kv_heads;
+    a.rows = d->q_tokens * (d->q_heads / c.kv_heads);
+    a.nt = c.head_dim <= 128 && a.rows > 8 ? 2 : 1;
+    a.keep_scores = d->weights_dev && a.rows <= 8 * a.nt && a.rows <= kScoreRows;
+    a.split = d->split_tokens;
+    if (a.split == 0) {
+        const int64_t units = bh * ((a.rows + 8 * a.nt - 1) / (8 * a.nt));
+        const int64_t want = (static_cast<int64_t>(sm_count()) * 16 + units - 1) / (units ? units : 1);
+        const int64_t per = (c.max_tokens + want - 1) / (want ? want : 1);
+        a.split = static_cast<int>((per + kSplitAlign - 1) / kSplitAlign * kSplitAlign);
+        if (a.split < 4 * kSplitAlign) a.split = 4 * kSplitAlign;
+    }
+    a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);
+    const int64_t most = 0x7FFFFFFF / ((a.rows + 8 * a.nt - 1) / (8 * a.nt) + 1);
+    while (a.nsplits > most) {  // the grid holds splits x row groups
+        a.split *= 2;
+        a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);
+    }
+    const auto up = [](size_t x) { return (x + 15) / 16 * 16; };
+    const size_t parts = static_cast<size_t>(bh) * a.nsplits * a.rows;
+    a.part_ml = 0;
+    a.part_o = up(parts * sizeof(float2));
+    a.scores = a.part_o + (a.nsplits > 1 ? up(parts * c.head_dim * sizeof(float)) : 0);
+    a.lse = a.scores + (a.keep_scores ? up(static_cast<size_t>(bh) * c.max_tokens * a.rows * sizeof(float)) : 0);
+    a.bytes = a.lse + (d->weights_dev && !a.keep_scores ? up(static_cast<size_t>(c.batch) * d->q_tokens * d->q_heads * sizeof(float)) : 0) + 16;
+    return a;
+}
+
+template <int FMT, int DP, int NT>
+void launch_step(const AttnParams& p, cudaStream_t s) {
+    const dim3 grid(p.nsplits * ((p.R + 8 * NT - 1) / (8 * NT)), p.c.H, p.c.B);
+    const bool plo = p.out_dtype == AKV_Q_F32, qlo = p.q_dtype == AKV_Q_F32;
+    if (plo && qlo) step_kernel<FMT, DP, NT, true, true><<<grid, kStepThreads, 0, s>>>(p);
+    else if (plo) step_kernel<FMT, DP, NT, true, false><<<grid, kStepThreads, 0, s>>>(p);
+    else if (qlo) step_kernel<FMT, DP, NT, false, true><<<grid, kStepThreads, 0, s>>>(p);
+    else step_kernel<FMT, DP, NT, false, false><<<grid, kStepThreads, 0, s>>>(p);
+}
+
+template <int FMT>
+void launch_step(const AttnParams& p, int nt, cudaStream_t s) {
+    if (p.c.D > 128) launch_step<FMT, 256, 1>(p, s);
+    else if (p.c.D > 64) nt == 2 ? launch_step<FMT, 128, 2>(p, s) : launch_step<FMT, 128, 1>(p, s);
+    else nt == 2 ? launch_step<FMT, 64, 2>(p, s) : launch_step<FMT, 64, 1>(p, s);
+}
+
+template <int FMT, int DP>
+void launch_weights(const AttnParams& p, cudaStream_t s) {
+    const dim3 grid((p.c.T + kWeightTile - 1) / kWeightTile, p.c.H, p.c.B);
+    if (p.q_dtype == AKV_Q_F32) weights_kernel<FMT, DP, true><<<grid, kWeightThreads, 0, s>>>(p);
+    else weights_kernel<FMT, DP, false><<<grid, kWeightThreads, 0, s>>>(p);
+}
+
+template <int FMT>
+void launch_weights(const AttnParams& p, cudaStream_t s) {
+    if (p.c.D > 128) launch_weights<FMT, 256>(p, s);
+    else if (p.c.D > 64) launch_weights<FMT, 128>(p, s);
+    else launch_weights<FMT, 64>(p, s);
 }
 
 }  // namespace
@@ -130,7 +214,7 @@ int akv_q8_restore(const AkvQ8RestoreDesc* d, void* stream) {
     return launched();
 }
 
-size_t akv_q8_attention_workspace(const AkvQ8AttnDesc* d) { return check_attention(d) == AKV_OK ? attention_workspace(d) : 0; }
+size_t akv_q8_attention_workspace(const AkvQ8AttnDesc* d) { return check_attention(d) == AKV_OK ? plan_attention(d).bytes : 0; }
 
 int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     if (int st = check_attention(d)) return st;
@@ -138,27 +222,37 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     const uintptr_t elem = d->q_dtype == AKV_Q_F32 ? 4 : 2;
     if (!d->q_dev || !d->out_dev || reinterpret_cast<uintptr_t>(d->q_dev) % elem || reinterpret_cast<uintptr_t>(d->out_dev) % 16)
         return AKV_ERR_INVALID_ARGUMENT;
-    if (!d->workspace_dev || d->workspace_bytes < attention_workspace(d)) return AKV_ERR_WORKSPACE;
+    const AttnPlan plan = plan_attention(d);
+    if (!d->workspace_dev || d->workspace_bytes < plan.bytes) return AKV_ERR_WORKSPACE;
     if (reinterpret_cast<uintptr_t>(d->workspace_dev) % 16) return AKV_ERR_INVALID_ARGUMENT;
+    char* ws = static_cast<char*>(d->workspace_dev);
     AttnParams p;
     p.c = to_dev(d->cache);
-    p.Hq = d->q_heads; p.G = d->q_heads / d->cache.kv_heads; p.n = d->q_tokens;
+    p.Hq = d->q_heads; p.G = d->q_heads / d->cache.kv_heads; p.n = d->q_tokens; p.R = plan.rows;
     p.q_dtype = d->q_dtype; p.out_dtype = d->out_dtype; p.causal = d->causal; p.accumulate = d->accumulate;
+    p.q_vec = reinterpret_cast<uintptr_t>(d->q_dev) % 16 == 0;
+    for (int i = 0; i < 3; ++i) p.q_vec &= d->q_stride[i] * static_cast<int64_t>(elem) % 16 == 0;
     p.c2 = (d->scale > 0.f ? d->scale : 1.0f / std::sqrt(static_cast<float>(p.c.D))) * 1.4426950408889634f;
     p.q = d->q_dev; p.qB = d->q_stride[0]; p.qT = d->q_stride[1]; p.qH = d->q_stride[2];
     p.lens = d->seq_lens_dev; p.q_lens = d->q_lens_dev;
-    p.out = d->out_dev; p.lse = static_cast<float*>(d->workspace_dev); p.lse_out = d->lse_dev;
+    p.split = plan.split; p.nsplits = plan.nsplits;
+    p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
+    p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
+    p.scores = plan.keep_scores ? reinterpret_cast<float*>(ws + plan.scores) : nullptr;
+    p.lse = d->weights_dev && !plan.keep_scores ? reinterpret_cast<float*>(ws + plan.lse) : nullptr;
+    p.out = d->out_dev; p.lse_out = d->lse_dev;
     p.weights = d->weights_dev; p.wstride = d->weights_stride;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const dim3 grid(p.Hq, p.n, p.c.B), wgrid((p.c.T + kRowThreads - 1) / kRowThreads, p.c.H, p.c.B);
     const bool int8 = p.c.fmt == AKV_Q8_INT8;
-    if (int8) attend_kernel<AKV_Q8_INT8><<<grid, kRowThreads, 0, s>>>(p);
-    else attend_kernel<AKV_Q8_E4M3><<<grid, kRowThreads, 0, s>>>(p);
+    int8 ? launch_step<AKV_Q8_INT8>(p, plan.nt, s) : launch_step<AKV_Q8_E4M3>(p, plan.nt, s);
     if (int st = launched()) return st;
-    if (p.weights) {
-        if (int8) weights_kernel<AKV_Q8_INT8><<<wgrid, kRowThreads, 0, s>>>(p);
-        else weights_kernel<AKV_Q8_E4M3><<<wgrid, kRowThreads, 0, s>>>(p);
-    }
+    const int64_t rows = plan.nsplits > 1 ? static_cast<int64_t>(p.c.B) * p.c.H * p.R : 0;
+    const int wblocks = plan.keep_scores ? (p.c.T + kWeightTokens - 1) / kWeightTokens : 0;
+    const int64_t blocks = rows + static_cast<int64_t>(p.c.B) * p.c.H * wblocks;
+    if (blocks > 0x7FFFFFFF) return AKV_ERR_UNSUPPORTED;
+    if (blocks) combine_kernel<<<static_cast<unsigned>(blocks), kCombineThreads, 0, s>>>(p, static_cast<int>(rows), wblocks);
+    if (int st = launched()) return st;
+    if (p.weights && !plan.keep_scores) int8 ? launch_weights<AKV_Q8_INT8>(p, s) : launch_weights<AKV_Q8_E4M3>(p, s);
     return launched();
 }
 

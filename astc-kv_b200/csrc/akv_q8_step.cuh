@@ -1,0 +1,363 @@
+// Attention of few rows (query tokens x heads of a kv head) over the 8-bit
+// cache: decode steps, and any other shape sixteen rows at a time.
+//
+// Every K and V byte of the cache is read once per group of 8 or 16 rows, so
+// a decode step is bound by HBM. One warp takes 16 tokens at a time; the
+// codes go from global memory straight into the registers that the tensor
+// cores read, no shared memory between. That works because the contracted
+// index of a matrix product may be permuted freely if both operands agree:
+//
+//   S^T = K Q^T (m = token, n = row, k = d): lane (g, c) of m16n8k16 (g =
+//   lane / 4, c = lane % 4) holds d-groups c of tokens g and g + 8. It loads
+//   16 consecutive bytes of each of these rows, and the query fragments
+//   take their d in the same order.
+//   O^T += V^T P^T (m = d, n = row, k = token): the lane holds tokens 2c,
+//   2c + 1, 2c + 8, 2c + 9 for its own d. It loads 16 consecutive bytes of
+//   these four rows (eight lanes cover a row), pairs tokens by byte permutes,
+//   and the output's d follow: fragment row g of tile i is byte 2i of lane
+//   group g's bytes, row g + 8 is byte 2i + 1.
+//
+// Codes are exact in fp16; a query row is exact in fp16 after a power of two
+// (fp32 queries in two parts); the block scale of K and the power go to the
+// fp32 score. V's block scale v is folded into the exponent: P' = 2^(s +
+// log2 v - m) and the row sum adds P' / v, so V needs no product. P' is
+// scaled to at most 2^14 to use fp16's range; fp32 outputs carry it in two
+// fp16 parts (the rest is then below 2^-24 of the largest).
+// The running maximum m is raised only when some score exceeds it, which a
+// vote finds; after the first tiles that is rare.
+#pragma once
+#include "akv_q8_attend.cuh"
+
+namespace akv {
+namespace q8 {
+
+constexpr int kStepWarps = 4;
+constexpr int kStepThreads = 32 * kStepWarps;
+
+// DP: head_dim rounded up to 64, 128 or 256; NT: groups of 8 rows; PLO: P in
+// two parts; QLO: queries in two parts.
+template <int FMT, int DP, int NT, bool PLO, bool QLO>
+__global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) step_kernel(AttnParams p) {
+    constexpr int KS = DP / 16;       // k-steps of S, d-tiles of O
+    constexpr int VW = DP / 32;       // words of a V row per lane
+    constexpr int ROWS = 8 * NT;
+    constexpr bool QREG = NT == 1 && !QLO && DP <= 128;
+    __shared__ float red[kStepWarps][ROWS][DP];
+    __shared__ float2 ml[kStepWarps][ROWS];
+    __shared__ uint2 qs[QREG ? 1 : KS][NT][QLO ? 2 : 1][32];
+
+    const CacheDev& c = p.c;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
+    const int h = blockIdx.y, b = blockIdx.z, split = blockIdx.x % p.nsplits, r0 = blockIdx.x / p.nsplits * ROWS;
+    const int len = len_of(p, b), qlen = q_len_of(p, b);
+    const int rows = min(ROWS, p.R - r0);
+    const int bh = b * c.H + h;
+    const int64_t unit = (static_cast<int64_t>(bh) * p.nsplits + split) * p.R + r0;
+    // The last query of the group sees the most.
+    int end = 0;
+    if (p.causal) end = seen_by(p, min((r0 + rows - 1) / p.G, qlen - 1), len, qlen);
+    else end = r0 / p.G < qlen ? len : 0;
+    if (qlen == 0 || r0 / p.G >= qlen) end = 0;
+    const int t_begin = split * p.split, t_end = min(t_begin + p.split, end);
+    if (t_begin >= t_end) {
+        if (p.nsplits > 1) {
+            if (threadIdx.x < rows) p.part_ml[unit + threadIdx.x] = make_float2(-CUDART_INF_F, 0.f);
+            return;
+        }
+        // The only split: rows that see nothing.
+        for (int i = threadIdx.x; i < rows * c.D; i += kStepThreads)
+            store_elem(p.out, p.out_dtype, out_row(p, b, h, r0 + i / c.D) * c.D + i % c.D, 0.f);
+        if (threadIdx.x < rows) {
+            const int64_t row = out_row(p, b, h, r0 + threadIdx.x);
+            if (p.lse) p.lse[row] = -CUDART_INF_F;
+            if (p.lse_out) p.lse_out[row] = -CUDART_INF_F;
+            p.part_ml[unit + threadIdx.x] = make_float2(-CUDART_INF_F, 0.f);
+        }
+        return;
+    }
+
+    const int64_t k_head = b * c.k.sB + h * c.k.sH, v_head = b * c.v.sB + h * c.v.sH;
+    const int64_t ks_head = b * c.k.cB + h * c.k.cH, vs_head = b * c.v.cB + h * c.v.cH;
+    uint32_t kr[2][KS], vr[4][VW];
+    float kscale = 0.f, vscale = 0.f;
+    // Physical page and first row of the tile at t0.
+    auto locate = [&](int t0, int& phys, int& row) {
+        phys = t0 < t_end ? page_of(c, b, t0) : -1;
+        row = t0 % c.P;
+    };
+    auto load_k = [&](int t0, int phys, int row) {
+        const uint8_t* base = c.k.codes + k_head + phys * c.k.sP + row * c.k.sT;
+        kscale = phys >= 0 ? __ldg(c.k.scales + ks_head + phys * c.k.cP + row / c.blk) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < DP / 64; ++j) {
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (phys >= 0 && t0 + g + 8 * i < t_end && 16 * cc + 64 * j < c.D)
+                    w = load_stream(base + (g + 8 * i) * c.k.sT + 16 * cc + 64 * j);
+                kr[i][4 * j] = w.x; kr[i][4 * j + 1] = w.y; kr[i][4 * j + 2] = w.z; kr[i][4 * j + 3] = w.w;
+            }
+    };
+    auto load_v = [&](int t0, int phys, int row) {
+        const uint8_t* base = c.v.codes + v_head + phys * c.v.sP + row * c.v.sT;
+        vscale = phys >= 0 ? __ldg(c.v.scales + vs_head + phys * c.v.cP + row / c.blk) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = 2 * cc + (i & 1) + 8 * (i >> 1);
+            const bool in = phys >= 0 && t0 + r < t_end;
+            if (DP == 64) {
+                uint2 w = make_uint2(0, 0);
+                if (in && 8 * g < c.D) w = load_stream8(base + r * c.v.sT + 8 * g);
+                vr[i][0] = w.x; vr[i][1] = w.y;
+            } else {
+#pragma unroll
+                for (int j = 0; j < DP / 128; ++j) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (in && 16 * g + 128 * j < c.D) w = load_stream(base + r * c.v.sT + 16 * g + 128 * j);
+                    vr[i][4 * j] = w.x; vr[i][4 * j + 1] = w.y; vr[i][4 * j + 2] = w.z; vr[i][4 * j + 3] = w.w;
+                }
+            }
+        }
+    };
+
+    int t0 = t_begin + 16 * warp, phys, row;
+    locate(t0, phys, row);
+    load_k(t0, phys, row);
+    load_v(t0, phys, row);
+
+    // Query fragments: n = g, d as in load_k.
+    uint32_t qf[QREG ? KS : 1][2];
+    float factor[NT][2];   // of the lane's score columns, rows 2c and 2c + 1
+    int bound[NT][2];      // tokens that those rows see
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = 8 * nt + g;
+        const bool in = r < rows;
+        float x[DP / 64][16];
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < DP / 64; ++j) {
+            if (in && 16 * cc + 64 * j < c.D) {
+                load_q16(p, q_row(p, b, h, r0 + r) + 16 * cc + 64 * j, x[j]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) x[j][k] = 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 16; ++k) top = __uint_as_float(max(__float_as_uint(top), abs_bits(x[j][k])));
+        }
+        uint32_t tb = __float_as_uint(top);
+        tb = max(tb, __shfl_xor_sync(0xFFFFFFFFu, tb, 1));
+        tb = max(tb, __shfl_xor_sync(0xFFFFFFFFu, tb, 2));
+        const int e = row_exponent(__uint_as_float(tb));
+        const float up = power_of_two(e);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            float y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = x[s / 4][4 * (s % 4) + k] * up;
+            const uint32_t h0 = pack_half2(y[0], y[1]), h1 = pack_half2(y[2], y[3]);
+            if (QREG) {
+                qf[s][0] = h0;
+                qf[s][1] = h1;
+            } else if (warp == 0) {
+                qs[s][nt][0][lane] = make_uint2(h0, h1);
+                if (QLO) qs[s][nt][1][lane] = make_uint2(pack_rest(y[0], y[1], h0), pack_rest(y[2], y[3], h1));
+            }
+        }
+        const float f = p.c2 * power_of_two(-e);
+        const int bnd = in ? seen_by(p, (r0 + r) / p.G, len, qlen) : 0;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            factor[nt][k] = __shfl_sync(0xFFFFFFFFu, f, 8 * cc + 4 * k);
+            bound[nt][k] = __shfl_sync(0xFFFFFFFFu, bnd, 8 * cc + 4 * k);
+        }
+    }
+    if (!QREG) __syncthreads();
+
+    float o[KS][NT][4];
+    float m[NT][2], base[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) { m[nt][k] = -CUDART_INF_F; base[nt][k] = 0.f; l[nt][k] = 0.f; }
+    }
+
+    for (; t0 < t_end; t0 += 16 * kStepWarps) {
+        int phys_next, row_next;
+        locate(t0 + 16 * kStepWarps, phys_next, row_next);
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+            uint32_t a0, a1, a2, a3;
+            codes_to_half<FMT>(kr[0][k], a0, a2);
+            codes_to_half<FMT>(kr[1][k], a1, a3);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                if (QREG) {
+                    mma16816(s[nt], a0, a1, a2, a3, qf[k][0], qf[k][1]);
+                } else {
+                    const uint2 q = qs[k][nt][0][lane];
+                    mma16816(s[nt], a0, a1, a2, a3, q.x, q.y);
+                    if (QLO) {
+                        const uint2 ql = qs[k][nt][QLO ? 1 : 0][lane];
+                        mma16816(s[nt], a0, a1, a2, a3, ql.x, ql.y);
+                    }
+                }
+            }
+        }
+        const float ks = kscale;
+        load_k(t0 + 16 * kStepWarps, phys_next, row_next);
+
+        // A NaN scale has to stay one.
+        const float vs = vscale < 8.0779357e-28f ? 8.0779357e-28f : vscale;
+        const float lv = __log2f(vs), iv = __frcp_rn(vs);
+        bool above = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[nt][k] *= ks * factor[nt][k & 1];
+            if (p.scores) {
+                float* at = p.scores + (static_cast<int64_t>(bh) * c.T + t0 + g) * p.R + r0 + 8 * nt + 2 * cc;
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (t0 + g + 8 * (k >> 1) < t_end && 8 * nt + 2 * cc + (k & 1) < rows) at[(k >> 1) * 8 * p.R + (k & 1)] = s[nt][k];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                s[nt][k] = t0 + g + 8 * (k >> 1) < bound[nt][k & 1] ? s[nt][k] + lv : -CUDART_INF_F;
+                above |= s[nt][k] > m[nt][k & 1];
+            }
+        }
+        if (__any_sync(0xFFFFFFFFu, above)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float x = fmaxf(s[nt][k], s[nt][k + 2]);
+                    x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
+                    x = fmaxf(x, m[nt][k]);
+                    const float alpha = m[nt][k] == -CUDART_INF_F ? 0.f : exp2_fast(m[nt][k] - x);
+                    m[nt][k] = x;
+                    base[nt][k] = x == -CUDART_INF_F ? 0.f : x - 14.f;
+                    l[nt][k] *= alpha;
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) {
+                        o[i][nt][k] *= alpha;
+                        o[i][nt][k + 2] *= alpha;
+                    }
+                }
+        }
+        uint32_t ph[NT][2], pl[PLO ? NT : 1][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                s[nt][k] = exp2_fast(s[nt][k] - base[nt][k & 1]);
+                l[nt][k & 1] = fmaf(s[nt][k], iv, l[nt][k & 1]);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t hi = pack_half2(s[nt][2 * k], s[nt][2 * k + 1]);
+                ph[nt][k] = transpose8x8(hi);
+                if (PLO) pl[nt][k] = transpose8x8(pack_rest(s[nt][2 * k], s[nt][2 * k + 1], hi));
+            }
+        }
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+            // Bytes of tokens (0, 1) and (2, 3) of the lane side by side: four d, two d-tiles.
+            const uint32_t e0 = __byte_perm(vr[0][w], vr[1][w], 0x5140), e1 = __byte_perm(vr[0][w], vr[1][w], 0x7362);
+            const uint32_t f0 = __byte_perm(vr[2][w], vr[3][w], 0x5140), f1 = __byte_perm(vr[2][w], vr[3][w], 0x7362);
+            uint32_t a[2][4];
+            codes_to_half<FMT>(e0, a[0][0], a[0][1]);
+            codes_to_half<FMT>(f0, a[0][2], a[0][3]);
+            codes_to_half<FMT>(e1, a[1][0], a[1][1]);
+            codes_to_half<FMT>(f1, a[1][2], a[1][3]);
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma16816(o[2 * w + j][nt], a[j][0], a[j][1], a[j][2], a[j][3], ph[nt][0], ph[nt][1]);
+                    if (PLO) mma16816(o[2 * w + j][nt], a[j][0], a[j][1], a[j][2], a[j][3], pl[PLO ? nt : 0][0], pl[PLO ? nt : 0][1]);
+                }
+        }
+        load_v(t0 + 16 * kStepWarps, phys_next, row_next);
+    }
+
+    // Join the warps in their order: (m, l) first, then O under the common maximum.
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            float x = l[nt][k];
+            x += __shfl_xor_sync(0xFFFFFFFFu, x, 4);
+            x += __shfl_xor_sync(0xFFFFFFFFu, x, 8);
+            x += __shfl_xor_sync(0xFFFFFFFFu, x, 16);
+            if (isnan(x)) m[nt][k] = x;  // NaN scores never raise the maximum
+            if (g == 0) ml[warp][8 * nt + 2 * cc + k] = make_float2(m[nt][k], x);
+        }
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int r = 8 * nt + 2 * cc + k;
+            float top = ml[0][r].x;
+#pragma unroll
+            for (int w = 1; w < kStepWarps; ++w) top = fmaxf(top, ml[w][r].x);
+            const float a = m[nt][k] == -CUDART_INF_F ? 0.f : exp2f(m[nt][k] - top);
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                // Byte x of the lane group's bytes.
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int x = 2 * i + j;
+                    const int d = DP == 64 ? 8 * g + x : 128 * (x / 16) + 16 * g + x % 16;
+                    red[warp][r][d] = o[i][nt][k + 2 * j] * a;
+                }
+            }
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * c.D; i += kStepThreads) {
+        const int r = i / c.D, d = i % c.D;
+        float top = ml[0][r].x, sum = 0.f, acc = red[0][r][d];
+#pragma unroll
+        for (int w = 1; w < kStepWarps; ++w) {
+            top = fmaxf(top, ml[w][r].x);
+            acc += red[w][r][d];
+        }
+        if (p.nsplits > 1 && d > 0) {
+            p.part_o[(unit + r) * c.D + d] = acc;
+            continue;
+        }
+#pragma unroll
+        for (int w = 0; w < kStepWarps; ++w)
+            if (ml[w][r].x != -CUDART_INF_F) sum += ml[w][r].y * exp2f(ml[w][r].x - top);
+        const bool none = top == -CUDART_INF_F && !isnan(sum);
+        if (isnan(sum)) top = sum;
+        if (p.nsplits > 1) {
+            p.part_o[(unit + r) * c.D] = acc;
+        } else {
+            store_elem(p.out, p.out_dtype, out_row(p, b, h, r0 + r) * c.D + d, none ? 0.f : acc / sum);
+        }
+        if (d == 0) {
+            // The exponent's shift by 14 is taken off here.
+            p.part_ml[unit + r] = make_float2(none ? top : top - 14.f, sum);
+            if (p.nsplits == 1) {
+                const float lse = none ? top : top - 14.f + log2f(sum);
+                const int64_t orow = out_row(p, b, h, r0 + r);
+                if (p.lse) p.lse[orow] = lse;
+                if (p.lse_out) p.lse_out[orow] = lse * 0.69314718055994531f;
+            }
+        }
+    }
+}
+
+}  // namespace q8
+}  // namespace akv
