@@ -67,6 +67,22 @@ int sm_count() {
     return n > 0 ? n : 148;
 }
 
+// Launches a kernel that calls wait_for_previous_kernel() so that it may be
+// brought onto the SMs while the kernel before it ends.
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t s, A... args) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...) == cudaSuccess ? AKV_OK : (cudaGetLastError(), AKV_ERR_CUDA);
+}
+
 struct AttnPlan {
     int rows;         // per kv head
     int nt;           // groups of eight rows per CTA
@@ -76,6 +92,7 @@ struct AttnPlan {
 };
 
 constexpr int kSplitAlign = 16 * kStepWarps;
+constexpr int kMinSplit = 64, kMaxSplit = 4096;
 
 // Rows whose scores are stored for the token weights rather than computed
 // again: storing costs 8 bytes per row and token, a second pass over K
@@ -91,11 +108,14 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
     a.keep_scores = d->weights_dev && a.rows <= 8 * a.nt && a.rows <= kScoreRows;
     a.split = d->split_tokens;
     if (a.split == 0) {
+        // One wave of CTAs where that makes splits of at most kMaxSplit
+        // tokens, else splits of that length, several waves of them (lengths
+        // may be ragged, and are not known here).
         const int64_t units = bh * ((a.rows + 8 * a.nt - 1) / (8 * a.nt));
-        const int64_t want = (static_cast<int64_t>(sm_count()) * 16 + units - 1) / (units ? units : 1);
-        const int64_t per = (c.max_tokens + want - 1) / (want ? want : 1);
-        a.split = static_cast<int>((per + kSplitAlign - 1) / kSplitAlign * kSplitAlign);
-        if (a.split < 4 * kSplitAlign) a.split = 4 * kSplitAlign;
+        const int64_t slots = static_cast<int64_t>(sm_count()) * (c.head_dim > 128 || a.nt == 2 ? 2 : 4);
+        const int64_t want = units > 0 && slots > units ? slots / units : 1;
+        const int64_t per = ((c.max_tokens + want - 1) / want + kSplitAlign - 1) / kSplitAlign * kSplitAlign;
+        a.split = static_cast<int>(per < kMinSplit ? kMinSplit : per > kMaxSplit ? kMaxSplit : per);
     }
     a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);
     const int64_t most = 0x7FFFFFFF / ((a.rows + 8 * a.nt - 1) / (8 * a.nt) + 1);
@@ -250,8 +270,10 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     const int wblocks = plan.keep_scores ? (p.c.T + kWeightTokens - 1) / kWeightTokens : 0;
     const int64_t blocks = rows + static_cast<int64_t>(p.c.B) * p.c.H * wblocks;
     if (blocks > 0x7FFFFFFF) return AKV_ERR_UNSUPPORTED;
-    if (blocks) combine_kernel<<<static_cast<unsigned>(blocks), kCombineThreads, 0, s>>>(p, static_cast<int>(rows), wblocks);
-    if (int st = launched()) return st;
+    if (blocks) {
+        if (int st = launch_after(combine_kernel, dim3(static_cast<unsigned>(blocks)), kCombineThreads, s, p, static_cast<int>(rows), wblocks))
+            return st;
+    }
     if (p.weights && !plan.keep_scores) int8 ? launch_weights<AKV_Q8_INT8>(p, s) : launch_weights<AKV_Q8_E4M3>(p, s);
     return launched();
 }

@@ -1,6 +1,8 @@
 // Attention over the 8-bit KV cache: parameters and helpers shared by the
 // kernels, the split combine, and the accumulated token weights.
 #pragma once
+#include <climits>
+
 #include <math_constants.h>
 
 #include "akv_q8_common.cuh"
@@ -102,6 +104,12 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
+__device__ __forceinline__ float log2_fast(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -157,62 +165,101 @@ __device__ __forceinline__ uint2 load_stream8(const void* p) {
 
 // ------------------------------------------------------------------ combine
 
-constexpr int kCombineThreads = 128;
+// Ordering with the kernel before or after on the stream when both are
+// launched as programmatic dependents (no effect otherwise): the next one may
+// be brought onto the SMs, and wait until everything before has finished.
+__device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+constexpr int kCombineThreads = 256;
 constexpr int kWeightTokens = 512;   // per CTA of the weights part
 
 // Base-2 log-sum-exp of row r over the splits, by one warp; all lanes get it.
 __device__ __forceinline__ float combined_lse(const float2* ml, int nsplits, int R) {
     const int lane = threadIdx.x & 31;
-    float m = -CUDART_INF_F;
-    for (int s = lane; s < nsplits; s += 32) m = fmaxf(m, ml[static_cast<int64_t>(s) * R].x);
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    float l = 0.f;
+    float m = -CUDART_INF_F, l = 0.f;
     for (int s = lane; s < nsplits; s += 32) {
         const float2 v = ml[static_cast<int64_t>(s) * R];
-        if (v.x != -CUDART_INF_F) l += v.y * exp2f(v.x - m);
+        if (v.x == -CUDART_INF_F) continue;
+        const float top = fmaxf(m, v.x);
+        l = (m == -CUDART_INF_F ? 0.f : l * exp2f(m - top)) + v.y * exp2f(v.x - top);
+        m = top;
     }
+    float all = m;
+    for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
+    l = m == -CUDART_INF_F && !isnan(l) ? 0.f : l * exp2f(m - all);
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
-    return isnan(l) ? l : m == -CUDART_INF_F ? m : m + log2f(l);
+    return isnan(l) ? l : all == -CUDART_INF_F ? all : all + log2f(l);
 }
 
 // Blocks [0, rows): one row of the output each: the splits' partials weighted
-// by 2^(m - lse), added in the order of the splits. Blocks from `rows` on:
-// 512 tokens of one kv head each: the stored scores of its rows become
-// softmax weights, which are added up.
+// by 2^(m - lse). Groups of D / 4 threads take every so many-th split, four
+// loads in flight each (the kernel is bound by load latency: 37 partials of
+// 64 rows 4 us, against 24 us with one thread per dimension); their sums are
+// added in a fixed order. Blocks from `rows` on: 512 tokens of one kv head
+// each: the stored scores of its rows become softmax weights, added up.
 __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, int rows, int wblocks) {
     __shared__ float lse[16];
     __shared__ int ends[16];
+    __shared__ float w[kCombineThreads];
+    __shared__ float4 part[kCombineThreads];
     const int tid = threadIdx.x;
+    wait_for_previous_kernel();
     if (static_cast<int>(blockIdx.x) < rows) {
-        const int r = blockIdx.x % p.R, bh = blockIdx.x / p.R, h = bh % p.c.H, b = bh / p.c.H;
+        const int r = blockIdx.x % p.R, bh = blockIdx.x / p.R, h = bh % p.c.H, b = bh / p.c.H, D = p.c.D;
         const float2* ml = p.part_ml + static_cast<int64_t>(bh) * p.nsplits * p.R + r;
-        const float all = combined_lse(ml, p.nsplits, p.R);
+        const float all = combined_lse(ml, p.nsplits, p.R);  // every warp for itself
         const int64_t row = out_row(p, b, h, r);
         if (tid == 0) {
             if (p.lse) p.lse[row] = all;
             if (p.lse_out) p.lse_out[row] = all * 0.69314718055994531f;
         }
-        const float* o = p.part_o + (static_cast<int64_t>(bh) * p.nsplits * p.R + r) * p.c.D;
-        const int64_t step = static_cast<int64_t>(p.R) * p.c.D;
-        for (int d = tid; d < p.c.D; d += kCombineThreads) {
-            float a = 0.f;
-            for (int s0 = 0; s0 < p.nsplits; s0 += 8) {
-                float x[8], w[8];
+        const int lanes = D / 4, groups = kCombineThreads / lanes, x = tid % lanes, grp = tid / lanes;
+        const float4* o = reinterpret_cast<const float4*>(p.part_o) + (static_cast<int64_t>(bh) * p.nsplits * p.R + r) * lanes + x;
+        const int64_t step = static_cast<int64_t>(p.R) * lanes;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s0 = 0; s0 < p.nsplits; s0 += kCombineThreads) {
+            __syncthreads();
+            if (s0 + tid < p.nsplits) {
+                const float m = ml[static_cast<int64_t>(s0 + tid) * p.R].x;
+                w[tid] = m == -CUDART_INF_F ? 0.f : exp2f(m - all);
+            }
+            __syncthreads();
+            const int n = min(kCombineThreads, p.nsplits - s0);
+            for (int s = grp; s < n && grp < groups; s += 4 * groups) {
+                float4 v[4];
+                float f[4];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const int s = s0 + k;
-                    w[k] = s < p.nsplits ? ml[static_cast<int64_t>(s) * p.R].x : -CUDART_INF_F;
-                    x[k] = w[k] != -CUDART_INF_F ? o[s * step + d] : 0.f;
+                for (int k = 0; k < 4; ++k) {
+                    const int sk = s + k * groups;
+                    f[k] = sk < n ? w[sk] : 0.f;
+                    // A split that has nothing has no partial either.
+                    v[k] = f[k] != 0.f ? o[static_cast<int64_t>(s0 + sk) * step] : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (w[k] != -CUDART_INF_F) a = fmaf(x[k], exp2f(w[k] - all), a);
+                for (int k = 0; k < 4; ++k) {
+                    a.x = fmaf(v[k].x, f[k], a.x);
+                    a.y = fmaf(v[k].y, f[k], a.y);
+                    a.z = fmaf(v[k].z, f[k], a.z);
+                    a.w = fmaf(v[k].w, f[k], a.w);
+                }
             }
-            store_elem(p.out, p.out_dtype, row * p.c.D + d, a);
         }
+        part[tid] = a;
+        __syncthreads();
+        if (grp != 0) return;
+        for (int k = 1; k < groups; ++k) {
+            const float4 v = part[k * lanes + x];
+            a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
+        }
+        const int64_t at = row * D + 4 * x;
+        store_elem(p.out, p.out_dtype, at, a.x);
+        store_elem(p.out, p.out_dtype, at + 1, a.y);
+        store_elem(p.out, p.out_dtype, at + 2, a.z);
+        store_elem(p.out, p.out_dtype, at + 3, a.w);
         return;
     }
-    const int wb = blockIdx.x - rows, bh = wb / wblocks, h = bh % p.c.H, b = bh / p.c.H, t0 = wb % wblocks * kWeightTokens;
+    const int wb = blockIdx.x - rows, bh = wb / wblocks, b = bh / p.c.H, t0 = wb % wblocks * kWeightTokens;
     const int len = len_of(p, b), qlen = q_len_of(p, b);
     if (p.accumulate && t0 >= len) return;
     for (int r = tid >> 5; r < p.R; r += kCombineThreads / 32) {
@@ -226,11 +273,22 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, 
     const float* sc = p.scores + static_cast<int64_t>(bh) * p.c.T * p.R;
     float* at = p.weights + static_cast<int64_t>(bh) * p.wstride;
     for (int t = t0 + tid; t < min(t0 + kWeightTokens, p.c.T); t += kCombineThreads) {
-        float w = 0.f;
-        for (int r = 0; r < p.R; ++r)
-            if (t < ends[r]) w += exp2f(sc[static_cast<int64_t>(t) * p.R + r] - lse[r]);
-        if (!p.accumulate) at[t] = w;
-        else if (t < len) at[t] += w;
+        float sum = 0.f;
+        if (p.R % 4 == 0) {
+            for (int r = 0; r < p.R; r += 4) {
+                if (t >= len) break;
+                const float4 v = *reinterpret_cast<const float4*>(sc + static_cast<int64_t>(t) * p.R + r);
+                if (t < ends[r]) sum += exp2_fast(v.x - lse[r]);
+                if (t < ends[r + 1]) sum += exp2_fast(v.y - lse[r + 1]);
+                if (t < ends[r + 2]) sum += exp2_fast(v.z - lse[r + 2]);
+                if (t < ends[r + 3]) sum += exp2_fast(v.w - lse[r + 3]);
+            }
+        } else {
+            for (int r = 0; r < p.R; ++r)
+                if (t < ends[r]) sum += exp2_fast(sc[static_cast<int64_t>(t) * p.R + r] - lse[r]);
+        }
+        if (!p.accumulate) at[t] = sum;
+        else if (t < len) at[t] += sum;
     }
 }
 

@@ -41,10 +41,9 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     constexpr int KS = DP / 16;       // k-steps of S, d-tiles of O
     constexpr int VW = DP / 32;       // words of a V row per lane
     constexpr int ROWS = 8 * NT;
-    constexpr bool QREG = NT == 1 && !QLO && DP <= 128;
     __shared__ float red[kStepWarps][ROWS][DP];
     __shared__ float2 ml[kStepWarps][ROWS];
-    __shared__ uint2 qs[QREG ? 1 : KS][NT][QLO ? 2 : 1][32];
+    __shared__ uint2 qs[KS][NT][QLO ? 2 : 1][32];
 
     const CacheDev& c = p.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
@@ -76,59 +75,113 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
         return;
     }
 
-    const int64_t k_head = b * c.k.sB + h * c.k.sH, v_head = b * c.v.sB + h * c.v.sH;
-    const int64_t ks_head = b * c.k.cB + h * c.k.cH, vs_head = b * c.v.cB + h * c.v.cH;
-    uint32_t kr[2][KS], vr[4][VW];
-    float kscale = 0.f, vscale = 0.f;
-    // Physical page and first row of the tile at t0.
-    auto locate = [&](int t0, int& phys, int& row) {
-        phys = t0 < t_end ? page_of(c, b, t0) : -1;
-        row = t0 % c.P;
-    };
-    auto load_k = [&](int t0, int phys, int row) {
-        const uint8_t* base = c.k.codes + k_head + phys * c.k.sP + row * c.k.sT;
-        kscale = phys >= 0 ? __ldg(c.k.scales + ks_head + phys * c.k.cP + row / c.blk) : 0.f;
+    // The lane's own places in a tile. Columns past head_dim read column 0
+    // instead: the query is 0 there, and such output columns are not stored.
+    int k_col[DP / 64], v_col[DP > 128 ? 2 : 1];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < DP / 64; ++j) k_col[j] = 16 * cc + 64 * j < c.D ? 16 * cc + 64 * j : 0;
+    if (DP == 64) {
+        v_col[0] = 8 * g < c.D ? 8 * g : 0;
+    } else {
 #pragma unroll
-            for (int j = 0; j < DP / 64; ++j) {
-                uint4 w = make_uint4(0, 0, 0, 0);
-                if (phys >= 0 && t0 + g + 8 * i < t_end && 16 * cc + 64 * j < c.D)
-                    w = load_stream(base + (g + 8 * i) * c.k.sT + 16 * cc + 64 * j);
-                kr[i][4 * j] = w.x; kr[i][4 * j + 1] = w.y; kr[i][4 * j + 2] = w.z; kr[i][4 * j + 3] = w.w;
+        for (int j = 0; j < DP / 128; ++j) v_col[j] = 16 * g + 128 * j < c.D ? 16 * g + 128 * j : 0;
+    }
+    const int blk_shift = 31 - __clz(c.blk);
+    uint32_t kr[2][KS], va[4][VW], vb[4][VW];
+    float kscale = 0.f, vscale_a = 0.f, vscale_b = 0.f;
+    // The tile to be loaded next: its first token, its place in its page, and
+    // pointers that move along with it and start anew in every page.
+    int t_load = t_begin + 16 * warp, page = t_load / c.P, row = t_load - page * c.P;
+    bool mapped = false;
+    const uint8_t *k_at = nullptr, *v_at = nullptr;
+    const float *ks_at = nullptr, *vs_at = nullptr;
+    auto enter_page = [&]() {
+        mapped = false;
+        if (t_load >= t_end) return;
+        int phys = page;
+        if (c.table) {
+            phys = __ldg(c.table + static_cast<int64_t>(b) * c.pps + page);
+            if (static_cast<unsigned>(phys) >= static_cast<unsigned>(c.num_pages)) {
+                report(c.status, AKV_ERR_BAD_BLOCK_TABLE);
+                return;
             }
+        }
+        mapped = true;
+        k_at = c.k.codes + code_offset(c.k, b, h, phys, row) + g * c.k.sT;
+        v_at = c.v.codes + code_offset(c.v, b, h, phys, row) + 2 * cc * c.v.sT;
+        ks_at = c.k.scales + scale_offset(c.k, b, h, phys, 0);
+        vs_at = c.v.scales + scale_offset(c.v, b, h, phys, 0);
     };
-    auto load_v = [&](int t0, int phys, int row) {
-        const uint8_t* base = c.v.codes + v_head + phys * c.v.sP + row * c.v.sT;
-        vscale = phys >= 0 ? __ldg(c.v.scales + vs_head + phys * c.v.cP + row / c.blk) : 0.f;
+    const int64_t k_step = 16 * kStepWarps * c.k.sT, v_step = 16 * kStepWarps * c.v.sT;
+    auto next_tile = [&]() {
+        t_load += 16 * kStepWarps;
+        row += 16 * kStepWarps;
+        k_at += k_step;
+        v_at += v_step;
+        if (row >= c.P) {
+            do {
+                row -= c.P;
+                ++page;
+            } while (row >= c.P);
+            enter_page();
+        }
+    };
+    auto load_k = [&]() {
+        const uint8_t* at8 = k_at + 8 * c.k.sT;
+        auto load_rows = [&](auto in) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = 2 * cc + (i & 1) + 8 * (i >> 1);
-            const bool in = phys >= 0 && t0 + r < t_end;
-            if (DP == 64) {
-                uint2 w = make_uint2(0, 0);
-                if (in && 8 * g < c.D) w = load_stream8(base + r * c.v.sT + 8 * g);
-                vr[i][0] = w.x; vr[i][1] = w.y;
-            } else {
+            for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int j = 0; j < DP / 128; ++j) {
+                for (int j = 0; j < DP / 64; ++j) {
                     uint4 w = make_uint4(0, 0, 0, 0);
-                    if (in && 16 * g + 128 * j < c.D) w = load_stream(base + r * c.v.sT + 16 * g + 128 * j);
-                    vr[i][4 * j] = w.x; vr[i][4 * j + 1] = w.y; vr[i][4 * j + 2] = w.z; vr[i][4 * j + 3] = w.w;
+                    if (in(i)) w = load_stream((i ? at8 : k_at) + k_col[j]);
+                    kr[i][4 * j] = w.x; kr[i][4 * j + 1] = w.y; kr[i][4 * j + 2] = w.z; kr[i][4 * j + 3] = w.w;
+                }
+        };
+        if (mapped && t_load + 16 <= t_end) {
+            kscale = __ldg(ks_at + (row >> blk_shift));
+            load_rows([](int) { return true; });
+        } else {
+            kscale = mapped && t_load < t_end ? __ldg(ks_at + (row >> blk_shift)) : 0.f;
+            load_rows([&](int i) { return mapped && t_load + g + 8 * i < t_end; });
+        }
+    };
+    auto load_v = [&](uint32_t (&vr)[4][VW], float& vscale) {
+        auto load_rows = [&](auto in) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint8_t* at = v_at + (i & 1 ? c.v.sT : 0) + (i & 2 ? 8 * c.v.sT : 0);
+                if (DP == 64) {
+                    uint2 w = make_uint2(0, 0);
+                    if (in(i)) w = load_stream8(at + v_col[0]);
+                    vr[i][0] = w.x; vr[i][1] = w.y;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < DP / 128; ++j) {
+                        uint4 w = make_uint4(0, 0, 0, 0);
+                        if (in(i)) w = load_stream(at + v_col[j]);
+                        vr[i][4 * j] = w.x; vr[i][4 * j + 1] = w.y; vr[i][4 * j + 2] = w.z; vr[i][4 * j + 3] = w.w;
+                    }
                 }
             }
+        };
+        if (mapped && t_load + 16 <= t_end) {
+            vscale = __ldg(vs_at + (row >> blk_shift));
+            load_rows([](int) { return true; });
+        } else {
+            vscale = mapped && t_load < t_end ? __ldg(vs_at + (row >> blk_shift)) : 0.f;
+            load_rows([&](int i) { return mapped && t_load + 2 * cc + (i & 1) + 8 * (i >> 1) < t_end; });
         }
     };
 
-    int t0 = t_begin + 16 * warp, phys, row;
-    locate(t0, phys, row);
-    load_k(t0, phys, row);
-    load_v(t0, phys, row);
+    enter_page();
+    load_k();
+    load_v(va, vscale_a);
 
     // Query fragments: n = g, d as in load_k.
-    uint32_t qf[QREG ? KS : 1][2];
     float factor[NT][2];   // of the lane's score columns, rows 2c and 2c + 1
-    int bound[NT][2];      // tokens that those rows see
+    int bound[NT][2];      // tokens that those rows see (rows past the last: all)
+    int bound_min = INT_MAX;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int r = 8 * nt + g;
@@ -157,23 +210,21 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
 #pragma unroll
             for (int k = 0; k < 4; ++k) y[k] = x[s / 4][4 * (s % 4) + k] * up;
             const uint32_t h0 = pack_half2(y[0], y[1]), h1 = pack_half2(y[2], y[3]);
-            if (QREG) {
-                qf[s][0] = h0;
-                qf[s][1] = h1;
-            } else if (warp == 0) {
+            if (warp == 0) {
                 qs[s][nt][0][lane] = make_uint2(h0, h1);
                 if (QLO) qs[s][nt][1][lane] = make_uint2(pack_rest(y[0], y[1], h0), pack_rest(y[2], y[3], h1));
             }
         }
         const float f = p.c2 * power_of_two(-e);
-        const int bnd = in ? seen_by(p, (r0 + r) / p.G, len, qlen) : 0;
+        const int bnd = in ? seen_by(p, (r0 + r) / p.G, len, qlen) : INT_MAX;
+        bound_min = min(bound_min, __reduce_min_sync(0xFFFFFFFFu, bnd));
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             factor[nt][k] = __shfl_sync(0xFFFFFFFFu, f, 8 * cc + 4 * k);
             bound[nt][k] = __shfl_sync(0xFFFFFFFFu, bnd, 8 * cc + 4 * k);
         }
     }
-    if (!QREG) __syncthreads();
+    __syncthreads();
 
     float o[KS][NT][4];
     float m[NT][2], base[NT][2], l[NT][2];
@@ -185,12 +236,13 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
         for (int k = 0; k < 2; ++k) { m[nt][k] = -CUDART_INF_F; base[nt][k] = 0.f; l[nt][k] = 0.f; }
     }
 
-    for (; t0 < t_end; t0 += 16 * kStepWarps) {
-        int phys_next, row_next;
-        locate(t0 + 16 * kStepWarps, phys_next, row_next);
-        float s[NT][4];
+    auto tile = [&](int t0, const uint32_t (&vr)[4][VW], float vscale, uint32_t (&v_next)[4][VW], float& vscale_next) {
+        // Two sums per score: the tensor cores truncate as they add.
+        float s[NT][4], s1[NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[nt][k] = s1[nt][k] = 0.f;
 #pragma unroll
         for (int k = 0; k < KS; ++k) {
             uint32_t a0, a1, a2, a3;
@@ -198,38 +250,41 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
             codes_to_half<FMT>(kr[1][k], a1, a3);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                if (QREG) {
-                    mma16816(s[nt], a0, a1, a2, a3, qf[k][0], qf[k][1]);
-                } else {
-                    const uint2 q = qs[k][nt][0][lane];
-                    mma16816(s[nt], a0, a1, a2, a3, q.x, q.y);
-                    if (QLO) {
-                        const uint2 ql = qs[k][nt][QLO ? 1 : 0][lane];
-                        mma16816(s[nt], a0, a1, a2, a3, ql.x, ql.y);
-                    }
+                float(&d)[4] = k & 1 ? s1[nt] : s[nt];
+                const uint2 q = qs[k][nt][0][lane];
+                mma16816(d, a0, a1, a2, a3, q.x, q.y);
+                if (QLO) {
+                    const uint2 ql = qs[k][nt][QLO ? 1 : 0][lane];
+                    mma16816(d, a0, a1, a2, a3, ql.x, ql.y);
                 }
             }
         }
         const float ks = kscale;
-        load_k(t0 + 16 * kStepWarps, phys_next, row_next);
-
         // A NaN scale has to stay one.
         const float vs = vscale < 8.0779357e-28f ? 8.0779357e-28f : vscale;
-        const float lv = __log2f(vs), iv = __frcp_rn(vs);
+        const float lv = log2_fast(vs), iv = exp2_fast(-lv);
+        next_tile();
+        load_k();
+        load_v(v_next, vscale_next);
+
+        const bool all_seen = t0 + 16 <= bound_min;
         bool above = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            const float f[2] = {ks * factor[nt][0], ks * factor[nt][1]};
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s[nt][k] *= ks * factor[nt][k & 1];
+            for (int k = 0; k < 4; ++k) s[nt][k] += s1[nt][k];
             if (p.scores) {
                 float* at = p.scores + (static_cast<int64_t>(bh) * c.T + t0 + g) * p.R + r0 + 8 * nt + 2 * cc;
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (t0 + g + 8 * (k >> 1) < t_end && 8 * nt + 2 * cc + (k & 1) < rows) at[(k >> 1) * 8 * p.R + (k & 1)] = s[nt][k];
+                    if (t0 + g + 8 * (k >> 1) < t_end && 8 * nt + 2 * cc + (k & 1) < rows)
+                        at[(k >> 1) * 8 * p.R + (k & 1)] = s[nt][k] * f[k & 1];
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                s[nt][k] = t0 + g + 8 * (k >> 1) < bound[nt][k & 1] ? s[nt][k] + lv : -CUDART_INF_F;
+                s[nt][k] = fmaf(s[nt][k], f[k & 1], lv);
+                if (!all_seen && t0 + g + 8 * (k >> 1) >= bound[nt][k & 1]) s[nt][k] = -CUDART_INF_F;
                 above |= s[nt][k] > m[nt][k & 1];
             }
         }
@@ -287,9 +342,13 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
                     if (PLO) mma16816(o[2 * w + j][nt], a[j][0], a[j][1], a[j][2], a[j][3], pl[PLO ? nt : 0][0], pl[PLO ? nt : 0][1]);
                 }
         }
-        load_v(t0 + 16 * kStepWarps, phys_next, row_next);
+    };
+    for (int t0 = t_begin + 16 * warp; t0 < t_end; t0 += 32 * kStepWarps) {
+        tile(t0, va, vscale_a, vb, vscale_b);
+        if (t0 + 16 * kStepWarps < t_end) tile(t0 + 16 * kStepWarps, vb, vscale_b, va, vscale_a);
     }
 
+    allow_next_kernel();
     // Join the warps in their order: (m, l) first, then O under the common maximum.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
