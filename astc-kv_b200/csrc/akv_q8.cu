@@ -2,6 +2,7 @@
 // argument validation, launch shapes, template dispatch.
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 
 #include "../../include/akv_q8.h"
@@ -41,6 +42,22 @@ int check_cache(const AkvQ8Cache& c) {
     return AKV_OK;
 }
 
+// Launches a kernel that calls wait_for_previous_kernel() so that it may be
+// brought onto the SMs while the kernel before it ends.
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t s, A... args) {
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, P(args)...) == cudaSuccess ? AKV_OK : (cudaGetLastError(), AKV_ERR_CUDA);
+}
+
 // Calls fn with a value of the element type of an AKV_Q_* code.
 template <typename F>
 void with_type(int dtype, F fn) {
@@ -60,27 +77,16 @@ int check_attention(const AkvQ8AttnDesc* d) {
     return AKV_OK;
 }
 
+// SMs of the current device, asked once per device.
 int sm_count() {
+    static std::atomic<int> known[64];
     int dev = 0, n = 0;
-    cudaGetDevice(&dev);
+    if (cudaGetDevice(&dev) != cudaSuccess) cudaGetLastError();
+    if (dev >= 0 && dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) cudaGetLastError();
-    return n > 0 ? n : 148;
-}
-
-// Launches a kernel that calls wait_for_previous_kernel() so that it may be
-// brought onto the SMs while the kernel before it ends.
-template <typename... P, typename... A>
-int launch_after(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t s, A... args) {
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, P(args)...) == cudaSuccess ? AKV_OK : (cudaGetLastError(), AKV_ERR_CUDA);
+    if (n <= 0) return 148;
+    if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
+    return n;
 }
 
 struct AttnPlan {
@@ -199,13 +205,27 @@ int akv_q8_store(const AkvQ8StoreDesc* d, void* stream) {
     p.xB[0] = d->k_stride[0]; p.xT[0] = d->k_stride[1]; p.xH[0] = d->k_stride[2];
     p.xB[1] = d->v_stride[0]; p.xT[1] = d->v_stride[1]; p.xH[1] = d->v_stride[2];
     p.start = d->start_dev; p.counts = d->counts_dev; p.n = d->tokens;
+    for (int i = 0; i < 2; ++i) {
+        p.vec[i] = reinterpret_cast<uintptr_t>(p.x[i]) % 16 == 0;
+        for (const int64_t st : {p.xB[i], p.xT[i], p.xH[i]}) p.vec[i] = p.vec[i] && st * static_cast<int64_t>(elem) % 16 == 0;
+    }
     const int blocks = static_cast<int>((static_cast<int64_t>(d->tokens) + 2 * p.c.blk - 2) / p.c.blk);
     const dim3 grid(blocks, p.c.H, 2 * p.c.B);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    // A block's new rows in pieces: a few threads for a few rows, else 256
+    // with two or eight pieces each.
+    const int pieces = (d->tokens < p.c.blk ? d->tokens : p.c.blk) * (p.c.D / 16);
+    const int threads = pieces <= 128 ? 64 : 256;
     with_type(d->dtype, [&](auto t) {
         using T = decltype(t);
-        if (p.c.fmt == AKV_Q8_INT8) store_kernel<AKV_Q8_INT8, T><<<grid, kStoreThreads, 0, s>>>(p);
-        else store_kernel<AKV_Q8_E4M3, T><<<grid, kStoreThreads, 0, s>>>(p);
+        const bool few = pieces <= 2 * threads;
+        if (p.c.fmt == AKV_Q8_INT8) {
+            if (few) store_kernel<AKV_Q8_INT8, T, 2><<<grid, threads, 0, s>>>(p);
+            else store_kernel<AKV_Q8_INT8, T, 8><<<grid, threads, 0, s>>>(p);
+        } else {
+            if (few) store_kernel<AKV_Q8_E4M3, T, 2><<<grid, threads, 0, s>>>(p);
+            else store_kernel<AKV_Q8_E4M3, T, 8><<<grid, threads, 0, s>>>(p);
+        }
     });
     return launched();
 }
@@ -221,17 +241,17 @@ int akv_q8_restore(const AkvQ8RestoreDesc* d, void* stream) {
     p.c = to_dev(d->cache);
     p.out[0] = d->k_dev; p.out[1] = d->v_dev;
     p.start = d->start_dev; p.n = d->tokens;
-    const int64_t pieces = static_cast<int64_t>(p.c.B) * p.n * p.c.H * (p.c.D / 16);
-    const int64_t ctas = (pieces + 255) / 256;
-    if (ctas > 0x7FFFFFFF) return AKV_ERR_UNSUPPORTED;
-    const dim3 grid(static_cast<unsigned>(ctas), 2);
+    const int64_t pieces = static_cast<int64_t>(p.n) * p.c.H * (p.c.D / 16);  // of a sequence's side
+    if (pieces > 0x7FFFFFFF) return AKV_ERR_UNSUPPORTED;
+    const dim3 grid(static_cast<unsigned>((pieces + 255) / 256), 2 * p.c.B);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    int st = AKV_OK;
     with_type(d->dtype, [&](auto t) {
         using T = decltype(t);
-        if (p.c.fmt == AKV_Q8_INT8) restore_kernel<AKV_Q8_INT8, T><<<grid, 256, 0, s>>>(p);
-        else restore_kernel<AKV_Q8_E4M3, T><<<grid, 256, 0, s>>>(p);
+        if (p.c.fmt == AKV_Q8_INT8) st = launch_after(restore_kernel<AKV_Q8_INT8, T>, grid, 256, s, p);
+        else st = launch_after(restore_kernel<AKV_Q8_E4M3, T>, grid, 256, s, p);
     });
-    return launched();
+    return st;
 }
 
 size_t akv_q8_attention_workspace(const AkvQ8AttnDesc* d) { return check_attention(d) == AKV_OK ? plan_attention(d).bytes : 0; }
@@ -302,9 +322,10 @@ int akv_q8_evict(const AkvQ8EvictDesc* d, void* stream) {
     select_kernel<<<dim3(a.kv_heads, a.batch), kSelectThreads, 0, s>>>(p);
     if (int st = launched()) return st;
     const dim3 grid((p.keep + p.dst.blk - 1) / p.dst.blk, a.kv_heads, 2 * a.batch);
-    if (a.format == AKV_Q8_INT8) pack_kernel<AKV_Q8_INT8><<<grid, 256, 0, s>>>(p);
-    else pack_kernel<AKV_Q8_E4M3><<<grid, 256, 0, s>>>(p);
-    return launched();
+    const bool few = c.block_tokens * (c.head_dim / 16) <= 512;  // pieces of a block
+    if (a.format == AKV_Q8_INT8)
+        return few ? launch_after(pack_kernel<AKV_Q8_INT8, 2>, grid, 256, s, p) : launch_after(pack_kernel<AKV_Q8_INT8, 8>, grid, 256, s, p);
+    return few ? launch_after(pack_kernel<AKV_Q8_E4M3, 2>, grid, 256, s, p) : launch_after(pack_kernel<AKV_Q8_E4M3, 8>, grid, 256, s, p);
 }
 
 }  // extern "C"

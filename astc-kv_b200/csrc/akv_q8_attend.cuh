@@ -165,12 +165,6 @@ __device__ __forceinline__ uint2 load_stream8(const void* p) {
 
 // ------------------------------------------------------------------ combine
 
-// Ordering with the kernel before or after on the stream when both are
-// launched as programmatic dependents (no effect otherwise): the next one may
-// be brought onto the SMs, and wait until everything before has finished.
-__device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 constexpr int kCombineThreads = 256;
 constexpr int kWeightTokens = 512;   // per CTA of the weights part
 

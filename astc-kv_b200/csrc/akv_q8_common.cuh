@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cstdint>
+#include <type_traits>
 
 #include "../../include/akv_q8.h"
 
@@ -40,6 +41,12 @@ inline CacheDev to_dev(const AkvQ8Cache& c) {
     return d;
 }
 
+// Ordering with the kernel before or after on the stream when both are
+// launched as programmatic dependents (no effect otherwise): the next one may
+// be brought onto the SMs, and wait until everything before has finished.
+__device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ void report(int32_t* status, int code) {
     if (status) atomicExch(status, code);
 }
@@ -65,17 +72,35 @@ __device__ __forceinline__ int64_t scale_offset(const SideDev& s, int b, int h, 
     return b * s.cB + h * s.cH + phys * s.cP + block;
 }
 
-// The code of y = x / scale: nearest, ties to even, saturating.
+// Four codes as floats, exactly.
 template <int FMT>
-__device__ __forceinline__ uint8_t to_code(float y) {
-    if (FMT == AKV_Q8_INT8) return static_cast<uint8_t>(static_cast<int8_t>(__float2int_rn(fminf(fmaxf(y, -127.f), 127.f))));
-    return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ void from_codes4(uint32_t w, float (&x)[4]) {
+    if (FMT == AKV_Q8_INT8) {
+        // code + 128 in the low byte of 2^23, less 2^23 + 128.
+        const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7440 | k)) - 8388736.f;
+    } else {
+        const __half2 a = __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w & 0xFFFF), __NV_E4M3));
+        const __half2 b = __half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> 16), __NV_E4M3));
+        const float2 f = __half22float2(a), g = __half22float2(b);
+        x[0] = f.x; x[1] = f.y; x[2] = g.x; x[3] = g.y;
+    }
 }
 
+// Codes of four y = x / scale with |y| <= M up to rounding (M = 127 or 448).
 template <int FMT>
-__device__ __forceinline__ float from_code(uint8_t c) {
-    if (FMT == AKV_Q8_INT8) return static_cast<float>(static_cast<int8_t>(c));
-    return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
+__device__ __forceinline__ uint32_t to_codes4(const float (&y)[4]) {
+    if (FMT == AKV_Q8_INT8) {
+        // The sum with 1.5 * 2^23 rounds to the nearest whole number, ties to
+        // even; its low byte is that number's.
+        uint32_t u[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = __float_as_uint(__fadd_rn(y[k], 12582912.f));
+        return __byte_perm(__byte_perm(u[0], u[1], 0x0040), __byte_perm(u[2], u[3], 0x0040), 0x5410);
+    }
+    return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3)) |
+           static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3)) << 16;
 }
 
 // Scale of a block from the largest |x| of its rows, given as the bits of

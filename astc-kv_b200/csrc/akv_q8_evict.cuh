@@ -52,12 +52,18 @@ __device__ __forceinline__ int cta_scan(int v, int* warp_sums, int* total) {
     return x - v + (warp ? warp_sums[warp - 1] : 0);
 }
 
-// One CTA per (kv head, sequence). The middle tokens' cut-off is found one
-// byte of the key at a time, by a histogram of the keys that still agree with
-// the bytes found; then one pass in order writes what lies above it, and of
-// what equals it the first few.
+// Runs of the row that a thread looks at, so that its kept tokens are in
+// order: whole groups of four where the row allows vector loads.
+__device__ __forceinline__ int run_length(int n) { return ((n + kSelectThreads - 1) / kSelectThreads + 3) / 4 * 4; }
+
+// One CTA per (kv head, sequence). The middle tokens' cut-off is the key of
+// the last one that stays; it is found 11, 11 and 10 bits at a time, by a
+// histogram of the keys that agree with the bits found. Then every thread
+// counts what its own run of tokens keeps (keys above the cut-off, and of the
+// equal ones the first few), a scan over the threads gives the places, and a
+// second look writes. The row is read five times, from L2 after the first.
 __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictParams p) {
-    __shared__ int hist[256];
+    __shared__ int hist[2048];
     __shared__ int sums[32];
     __shared__ uint32_t s_prefix;
     __shared__ int s_want;
@@ -68,6 +74,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictParams p) {
     float* ow = p.out_weights + unit * p.ostride;
     const int len = p.lens ? min(max(p.lens[b], 0), p.src.T) : p.src.T;
     const int n = min(len, p.keep);
+    allow_next_kernel();
     if (h == 0 && tid == 0) p.out_lens[b] = n;
     for (int i = n + tid; i < p.keep; i += kSelectThreads) {
         kept[i] = -1;
@@ -83,73 +90,127 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictParams p) {
     const int lo = p.sinks, hi = len - p.recent;
     uint32_t prefix = 0;
     int want = p.keep - p.sinks - p.recent;  // of the tokens whose key agrees with `prefix` so far
-    for (int shift = 24; want > 0 && shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
+    const bool none = want == 0;
+    for (int pass = 0; pass < 3 && !none; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+        const uint32_t mask = pass == 2 ? 1023u : 2047u;
+        hist[tid] = hist[tid + kSelectThreads] = 0;
         __syncthreads();
-        for (int t = lo + tid; t < hi; t += kSelectThreads) {
-            const uint32_t k = order_key(w[t]);
-            if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255], 1);
+        for (int t = lo + tid; t < hi; t += 8 * kSelectThreads) {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = t + k * kSelectThreads < hi ? w[t + k * kSelectThreads] : 0.f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t key = order_key(x[k]);
+                if (t + k * kSelectThreads < hi && (pass == 0 || ((key ^ prefix) >> (shift + (pass == 1 ? 11 : 10))) == 0))
+                    atomicAdd(&hist[(key >> shift) & mask], 1);
+            }
         }
         __syncthreads();
-        if (tid == 0) {
-            int d = 255, left = want;
-            while (left > hist[d]) left -= hist[d--];
-            s_prefix = prefix | static_cast<uint32_t>(d) << shift;
-            s_want = left;
+        // Bins from the highest down, two a thread.
+        const int d = 2047 - 2 * tid, upper = hist[d], lower = hist[d - 1];
+        int total;
+        const int before = cta_scan(upper + lower, sums, &total);
+        if (before < want && want <= before + upper + lower) {
+            const bool first = want <= before + upper;
+            s_prefix = prefix | static_cast<uint32_t>(first ? d : d - 1) << shift;
+            s_want = want - before - (first ? 0 : upper);
         }
         __syncthreads();
         prefix = s_prefix;
         want = s_want;
     }
-    const bool none = p.keep == p.sinks + p.recent;
-    int out = 0, equal = 0;
-    for (int t0 = 0; t0 < len; t0 += kSelectThreads) {
-        const int t = t0 + tid;
-        const bool in = t < len, fixed = in && (t < lo || t >= hi);
-        const float x = in ? w[t] : 0.f;
-        const uint32_t k = order_key(x);
-        const bool same = in && !fixed && !none && k == prefix;
-        int total, all;
-        const int before = equal + cta_scan(same, sums, &all);
-        const bool take = fixed || (in && !none && (k > prefix || (same && before < want)));
-        const int at = out + cta_scan(take, sums, &total);
-        if (take) {
+    const int run = run_length(len), t0 = min(tid * run, len), t1 = min(t0 + run, len);
+    int above = 0, equal = 0;
+    for (int t = t0; t < t1; ++t) {
+        const uint32_t key = order_key(w[t]);
+        const bool fixed = t < lo || t >= hi;
+        above += fixed || (!none && key > prefix);
+        equal += !fixed && !none && key == prefix;
+    }
+    int total;
+    const int equal_before = cta_scan(equal, sums, &total);
+    const int take = max(0, min(equal, want - equal_before));
+    int at = cta_scan(above + take, sums, &total), left = take;
+    for (int t = t0; t < t1; ++t) {
+        const float x = w[t];
+        const uint32_t key = order_key(x);
+        const bool fixed = t < lo || t >= hi;
+        bool in = fixed || (!none && key > prefix);
+        if (!in && !none && key == prefix && left > 0) {
+            in = true;
+            --left;
+        }
+        if (in) {
             kept[at] = t;
             ow[at] = x;
+            ++at;
         }
-        equal += all;
-        out += total;
     }
 }
 
-// One CTA per (block of the new cache, kv head, sequence x side).
-template <int FMT>
+// One CTA per (block of the new cache, kv head, sequence x side). The rows'
+// codes stay in registers (PP pieces of 16 a thread) between finding the
+// largest value and coding them under the new scale.
+template <int FMT, int PP>
 __global__ void __launch_bounds__(256) pack_kernel(EvictParams p) {
     __shared__ uint32_t red[8];
     const CacheDev &a = p.src, &c = p.dst;
     const int h = blockIdx.y, b = blockIdx.z >> 1, side = blockIdx.z & 1;
     const SideDev &from = side ? a.v : a.k, &to = side ? c.v : c.k;
-    const int64_t unit = static_cast<int64_t>(b) * a.H + h;
-    const int32_t* kept = p.kept + unit * p.keep;
-    const int row0 = blockIdx.x * c.blk;
+    const int32_t* kept = p.kept + (static_cast<int64_t>(b) * a.H + h) * p.keep;
+    const int row0 = blockIdx.x * c.blk, per_row = c.D / 16;
+    wait_for_previous_kernel();
     const int n = min(p.out_lens[b] - row0, c.blk);
     if (n <= 0) return;
     const int phys = page_of(c, b, row0);
     if (phys < 0) return;
-    auto value = [&](int r, int d) {
-        const int t = kept[row0 + r], pg = page_of(a, b, t), row = t % a.P;
-        if (pg < 0) return 0.f;
-        return __fmul_rn(from_code<FMT>(from.codes[code_offset(from, b, h, pg, row) + d]),
-                         from.scales[scale_offset(from, b, h, pg, row / a.blk)]);
-    };
+    uint4 w[PP];
+    float sc[PP];
     uint32_t top = 0;
-    for (int i = threadIdx.x; i < n * c.D; i += 256) top = max(top, abs_bits(value(i / c.D, i % c.D)));
+#pragma unroll
+    for (int k = 0; k < PP; ++k) {
+        const int i = threadIdx.x + k * 256, r = i / per_row;
+        w[k] = make_uint4(0, 0, 0, 0);
+        sc[k] = 0.f;
+        if (r >= n) continue;
+        const int t = kept[row0 + r], pg = page_of(a, b, t), row = t % a.P;
+        if (pg < 0) continue;
+        w[k] = __ldg(reinterpret_cast<const uint4*>(from.codes + code_offset(from, b, h, pg, row)) + (i - r * per_row));
+        sc[k] = from.scales[scale_offset(from, b, h, pg, row / a.blk)];
+    }
+#pragma unroll
+    for (int k = 0; k < PP; ++k) {
+        const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+        uint32_t m = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float f[4];
+            from_codes4<FMT>(u[j], f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = max(m, abs_bits(f[e]));
+        }
+        // Rounding keeps the order: the largest code gives the largest value.
+        top = max(top, abs_bits(__fmul_rn(__uint_as_float(m), sc[k])));
+    }
     const float scale = block_scale<FMT>(cta_max(top, red)), inv = block_inverse(scale);
     const int in_page = row0 % c.P;
     uint8_t* codes = to.codes + code_offset(to, b, h, phys, in_page);
-    for (int i = threadIdx.x; i < c.blk * c.D; i += 256) {
-        const int r = i / c.D, d = i % c.D;
-        codes[r * to.sT + d] = r < n ? to_code<FMT>(__fmul_rn(value(r, d), inv)) : 0;
+#pragma unroll
+    for (int k = 0; k < PP; ++k) {
+        const int i = threadIdx.x + k * 256, r = i / per_row;
+        if (r >= c.blk) break;
+        uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float f[4];
+            from_codes4<FMT>(u[j], f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(__fmul_rn(f[e], sc[k]), inv);
+            u[j] = to_codes4<FMT>(f);
+        }
+        reinterpret_cast<uint4*>(codes + r * to.sT)[i - r * per_row] = make_uint4(u[0], u[1], u[2], u[3]);
     }
     if (threadIdx.x == 0) to.scales[scale_offset(to, b, h, phys, in_page / c.blk)] = scale;
 }

@@ -1,16 +1,18 @@
 // Store and restore of the 8-bit KV cache.
+//
+// Both move every element once and are bound by HBM. A thread holds pieces of
+// 16 consecutive elements of a row: 16 bytes of codes, the widest access.
 #pragma once
 #include "akv_q8_common.cuh"
 
 namespace akv {
 namespace q8 {
 
-constexpr int kStoreThreads = 256;
-
 struct StoreParams {
     CacheDev c;
-    const void* x[2];       // K, V rows
+    const void* x[2];             // K, V rows
     int64_t xB[2], xT[2], xH[2];  // elements
+    bool vec[2];                  // rows start on 16-byte boundaries
     const int32_t* start;
     const int32_t* counts;
     int n;
@@ -26,11 +28,40 @@ __device__ __forceinline__ uint32_t cta_max(uint32_t v, uint32_t* red) {
     return v;
 }
 
-// One CTA per (touched block, kv head, sequence x side). Reads its rows twice
-// (the second time from L1/L2): once for the largest value, once to code.
-template <int FMT, typename T>
-__global__ void __launch_bounds__(kStoreThreads) store_kernel(StoreParams p) {
-    __shared__ uint32_t red[kStoreThreads / 32];
+// 16 elements as they are in memory, and element i of them as a float.
+template <typename T>
+struct Piece {
+    uint4 w[sizeof(T)];
+
+    __device__ __forceinline__ void load(const T* at, bool vec) {
+        if (vec) {
+#pragma unroll
+            for (int k = 0; k < static_cast<int>(sizeof(T)); ++k) w[k] = __ldg(reinterpret_cast<const uint4*>(at) + k);
+        } else {
+            T* e = reinterpret_cast<T*>(w);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) e[k] = at[k];
+        }
+    }
+    __device__ __forceinline__ uint32_t word(int i) const {
+        const uint4& v = w[i >> 2];
+        return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if (sizeof(T) == 4) return __uint_as_float(word(i));
+        const uint32_t v = word(i >> 1);
+        if (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i & 1 ? v & 0xFFFF0000u : v << 16);
+        return __half2float(__ushort_as_half(static_cast<uint16_t>(i & 1 ? v >> 16 : v)));
+    }
+};
+
+// One CTA per (touched block, kv head, sequence x side). The new rows stay in
+// registers (PP pieces a thread) between finding their largest value and
+// coding them. Rows that a growing block holds already are read, coded again
+// and written in place.
+template <int FMT, typename T, int PP>
+__global__ void __launch_bounds__(256) store_kernel(StoreParams p) {
+    __shared__ uint32_t red[8];
     const CacheDev& c = p.c;
     const int h = blockIdx.y, b = blockIdx.z >> 1, side = blockIdx.z & 1;
     const int64_t start = p.start[b];
@@ -52,33 +83,58 @@ __global__ void __launch_bounds__(kStoreThreads) store_kernel(StoreParams p) {
     float* scale_at = s.scales + scale_offset(s, b, h, phys, row0 / c.blk);
     const T* x = static_cast<const T*>(p.x[side]) + b * p.xB[side] + h * p.xH[side] + (block0 - start) * p.xT[side];
     const int64_t xT = p.xT[side];
-    const int n = (last - first) * c.D;
+    const int per_row = c.D / 16, pieces = (last - first) * per_row;
+    Piece<T> v[PP];
     uint32_t top = 0;
-    for (int i = threadIdx.x; i < n; i += kStoreThreads) top = max(top, abs_bits(to_f32(x[(first + i / c.D) * xT + i % c.D])));
-    top = cta_max(top, red);
+#pragma unroll
+    for (int k = 0; k < PP; ++k) {
+        const int i = threadIdx.x + k * blockDim.x;
+        if (i >= pieces) break;
+        const int r = first + i / per_row, d = i % per_row * 16;
+        v[k].load(x + r * xT + d, p.vec[side]);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top = max(top, abs_bits(v[k].get(j)));
+    }
+    float had = first > 0 ? *scale_at : 0.f;
+    top = cta_max(top, red);  // its barrier: everyone has read the scale
     float scale = block_scale<FMT>(top);
     if (first > 0) {
-        const float had = *scale_at;
-        __syncthreads();  // everyone has read it
-        if (!(scale <= had)) {
-            if (!isnan(had)) {
-                // The rows that are there already, under the larger scale.
-                const float inv = block_inverse(scale);
-                for (int i = threadIdx.x; i < first * c.D; i += kStoreThreads) {
-                    uint8_t* at = codes + (i / c.D) * s.sT + i % c.D;
-                    *at = to_code<FMT>(__fmul_rn(__fmul_rn(from_code<FMT>(*at), had), inv));
-                }
-            } else {
-                scale = had;
-            }
-        } else {
+        if (scale <= had || isnan(had)) {
             scale = had;
+        } else {
+            // The rows that are there already, under the larger scale.
+            const float inv = block_inverse(scale);
+            for (int i = threadIdx.x; i < first * per_row; i += blockDim.x) {
+                uint4* at = reinterpret_cast<uint4*>(codes + (i / per_row) * s.sT + i % per_row * 16);
+                uint4 w = *at;
+                uint32_t* u = reinterpret_cast<uint32_t*>(&w);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    float f[4];
+                    from_codes4<FMT>(u[k], f);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) f[j] = __fmul_rn(__fmul_rn(f[j], had), inv);
+                    u[k] = to_codes4<FMT>(f);
+                }
+                *at = w;
+            }
         }
     }
     const float inv = block_inverse(scale);
-    for (int i = threadIdx.x; i < n; i += kStoreThreads) {
-        const int r = first + i / c.D, d = i % c.D;
-        codes[r * s.sT + d] = to_code<FMT>(__fmul_rn(to_f32(x[r * xT + d]), inv));
+#pragma unroll
+    for (int k = 0; k < PP; ++k) {
+        const int i = threadIdx.x + k * blockDim.x;
+        if (i >= pieces) break;
+        const int r = first + i / per_row, d = i % per_row * 16;
+        uint32_t u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float f[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(v[k].get(4 * j + e), inv);
+            u[j] = to_codes4<FMT>(f);
+        }
+        *reinterpret_cast<uint4*>(codes + r * s.sT + d) = make_uint4(u[0], u[1], u[2], u[3]);
     }
     if (threadIdx.x == 0) *scale_at = scale;
 }
@@ -90,34 +146,38 @@ struct RestoreParams {
     int n;
 };
 
-// One thread per 16 codes, in the order of the output.
+// One thread per piece, in the order of the output; grid.y: sequence x side.
 template <int FMT, typename T>
 __global__ void __launch_bounds__(256) restore_kernel(RestoreParams p) {
     const CacheDev& c = p.c;
-    const int side = blockIdx.y;
+    const int b = blockIdx.y >> 1, side = blockIdx.y & 1;
     const SideDev& s = side ? c.v : c.k;
-    const int per_row = c.D / 16;
-    const int64_t total = static_cast<int64_t>(c.B) * p.n * c.H * per_row;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
-    if (i >= total) return;
-    const int d16 = static_cast<int>(i % per_row);
-    const int64_t rowi = i / per_row;
-    const int h = static_cast<int>(rowi % c.H);
-    const int64_t bt = rowi / c.H;
-    const int b = static_cast<int>(bt / p.n);
-    const int64_t t = bt % p.n + (p.start ? p.start[b] : 0);
-    __align__(16) T o[16];
+    const unsigned per_row = c.D / 16, per_token = per_row * c.H;
+    const unsigned i = blockIdx.x * 256u + threadIdx.x;
+    if (i >= per_token * p.n) return;
+    const unsigned ti = i / per_token, rest = i - ti * per_token;
+    const int h = rest / per_row, d = (rest - h * per_row) * 16;
+    wait_for_previous_kernel();
+    const int64_t t = static_cast<int64_t>(ti) + (p.start ? p.start[b] : 0);
     const int phys = t >= 0 && t < c.T ? page_of(c, b, static_cast<int>(t)) : -1;
-    if (phys < 0) {
-        for (int k = 0; k < 16; ++k) o[k] = from_f32<T>(0.f);
-    } else {
+    uint4 w = make_uint4(0, 0, 0, 0);
+    float scale = 0.f;
+    if (phys >= 0) {
         const int row = static_cast<int>(t % c.P);
-        const uint4 w = *reinterpret_cast<const uint4*>(s.codes + code_offset(s, b, h, phys, row) + d16 * 16);
-        const float scale = s.scales[scale_offset(s, b, h, phys, row / c.blk)];
-        const uint8_t* q = reinterpret_cast<const uint8_t*>(&w);
-        for (int k = 0; k < 16; ++k) o[k] = from_f32<T>(__fmul_rn(from_code<FMT>(q[k]), scale));
+        w = *reinterpret_cast<const uint4*>(s.codes + code_offset(s, b, h, phys, row) + d);
+        scale = s.scales[scale_offset(s, b, h, phys, row / c.blk)];
     }
-    uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.out[side]) + i * 16);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    __align__(16) T o[16];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        float f[4];
+        from_codes4<FMT>(u[k], f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[4 * k + j] = from_f32<T>(__fmul_rn(f[j], scale));
+    }
+    uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.out[side]) + (static_cast<int64_t>(b) * p.n * per_token + i) * 16);
+#pragma unroll
     for (int k = 0; k < static_cast<int>(sizeof(T)); ++k) out[k] = reinterpret_cast<const uint4*>(o)[k];
 }
 
