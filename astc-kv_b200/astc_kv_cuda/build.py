@@ -23,7 +23,7 @@ SOURCES = ["akv_cuda.cu", "akv_q8.cu", "akv_tables.cpp", "akv_encode.cpp"]
 HEADERS = ["akv_astc_device.cuh", "akv_common.cuh", "akv_decode_kernels.cuh", "akv_attention_kernels.cuh", "akv_tables.h",
            "akv_attn_fp16.cuh",
            "akv_attn_fast.cuh", "akv_decode_fast.cuh",
-           "akv_q8_common.cuh", "akv_q8_store.cuh", "akv_q8_attend.cuh", "akv_q8_step.cuh", "akv_q8_weights.cuh", "akv_q8_evict.cuh"]
+           "akv_q8_common.cuh", "akv_q8_store.cuh", "akv_q8_attend.cuh", "akv_q8_chunk.cuh", "akv_q8_step.cuh", "akv_q8_weights.cuh", "akv_q8_evict.cuh"]
 
 
 def nvcc() -> str:

@@ -7,6 +7,7 @@
 
 #include "../../include/akv_q8.h"
 #include "akv_q8_attend.cuh"
+#include "akv_q8_chunk.cuh"
 #include "akv_q8_evict.cuh"
 #include "akv_q8_step.cuh"
 #include "akv_q8_store.cuh"
@@ -91,6 +92,7 @@ int sm_count() {
 
 struct AttnPlan {
     int rows;         // per kv head
+    bool chunk;       // the tcgen05 kernel, else the step kernel
     int nt;           // groups of eight rows per CTA
     int split, nsplits;
     bool keep_scores; // the step kernel stores its scores for the token weights
@@ -98,6 +100,9 @@ struct AttnPlan {
 };
 
 constexpr int kSplitAlign = 16 * kStepWarps;
+// Rows from which the tcgen05 kernel, whose CTA does 128 or 256 rows for the
+// price of one, is ahead of the step kernel, which does 16.
+constexpr int kChunkMinRows = 33;
 constexpr int kMinSplit = 64, kMaxSplit = 4096;
 
 // Rows whose scores are stored for the token weights rather than computed
@@ -111,20 +116,37 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
     const int64_t bh = static_cast<int64_t>(c.batch) * c.kv_heads;
     a.rows = d->q_tokens * (d->q_heads / c.kv_heads);
     a.nt = c.head_dim <= 128 && a.rows > 8 ? 2 : 1;
-    a.keep_scores = d->weights_dev && a.rows <= 8 * a.nt && a.rows <= kScoreRows;
+    a.chunk = a.rows >= kChunkMinRows && c.head_dim <= 128 && d->q_dtype != AKV_Q_F32 && d->out_dtype != AKV_Q_F32;
+    a.keep_scores = !a.chunk && d->weights_dev && a.rows <= 8 * a.nt && a.rows <= kScoreRows;
     a.split = d->split_tokens;
-    if (a.split == 0) {
+    const int group = a.chunk ? kChunkRows : 8 * a.nt;  // rows of a CTA
+    if (a.split == 0 && a.chunk) {
+        // One CTA per SM: the number of splits (up to eight) whose last wave
+        // is fullest; each costs a partial to write and read again.
+        const int64_t units = bh * ((a.rows + group - 1) / group), sms = sm_count();
+        const int64_t steps = (static_cast<int64_t>(c.max_tokens) + kChunkTokens - 1) / kChunkTokens;
+        int64_t best = 1;
+        double least = 0;
+        for (int64_t n = 1; n <= 8 && n * 4 <= steps + 3; ++n) {
+            const double waves = static_cast<double>((units * n + sms - 1) / sms) * ((steps + n - 1) / n) * (n > 1 ? 1.02 + 0.01 * n : 1.0);
+            if (n == 1 || waves < least) {
+                best = n;
+                least = waves;
+            }
+        }
+        a.split = static_cast<int>((steps + best - 1) / best * kChunkTokens);
+    } else if (a.split == 0) {
         // One wave of CTAs where that makes splits of at most kMaxSplit
         // tokens, else splits of that length, several waves of them (lengths
         // may be ragged, and are not known here).
-        const int64_t units = bh * ((a.rows + 8 * a.nt - 1) / (8 * a.nt));
+        const int64_t units = bh * ((a.rows + group - 1) / group);
         const int64_t slots = static_cast<int64_t>(sm_count()) * (c.head_dim > 128 || a.nt == 2 ? 2 : 4);
         const int64_t want = units > 0 && slots > units ? slots / units : 1;
         const int64_t per = ((c.max_tokens + want - 1) / want + kSplitAlign - 1) / kSplitAlign * kSplitAlign;
         a.split = static_cast<int>(per < kMinSplit ? kMinSplit : per > kMaxSplit ? kMaxSplit : per);
     }
     a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);
-    const int64_t most = 0x7FFFFFFF / ((a.rows + 8 * a.nt - 1) / (8 * a.nt) + 1);
+    const int64_t most = 0x7FFFFFFF / ((a.rows + group - 1) / group + 1);
     while (a.nsplits > most) {  // the grid holds splits x row groups
         a.split *= 2;
         a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);
@@ -154,6 +176,24 @@ void launch_step(const AttnParams& p, int nt, cudaStream_t s) {
     if (p.c.D > 128) launch_step<FMT, 256, 1>(p, s);
     else if (p.c.D > 64) nt == 2 ? launch_step<FMT, 128, 2>(p, s) : launch_step<FMT, 128, 1>(p, s);
     else nt == 2 ? launch_step<FMT, 64, 2>(p, s) : launch_step<FMT, 64, 1>(p, s);
+}
+
+template <int FMT, int DP>
+int launch_chunk(const AttnParams& p, cudaStream_t s) {
+    const auto kern = chunk_kernel<FMT, DP>;
+    constexpr int bytes = sizeof(ChunkSmem<DP>) + 1024;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return AKV_ERR_CUDA;
+    }
+    const dim3 grid(p.nsplits * ((p.R + kChunkRows - 1) / kChunkRows), p.c.H, p.c.B);
+    kern<<<grid, kChunkThreads, bytes, s>>>(p);
+    return launched();
+}
+
+template <int FMT>
+int launch_chunk(const AttnParams& p, cudaStream_t s) {
+    return p.c.D > 64 ? launch_chunk<FMT, 128>(p, s) : launch_chunk<FMT, 64>(p, s);
 }
 
 template <int FMT, int DP>
@@ -284,13 +324,22 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     p.weights = d->weights_dev; p.wstride = d->weights_stride;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool int8 = p.c.fmt == AKV_Q8_INT8;
-    int8 ? launch_step<AKV_Q8_INT8>(p, plan.nt, s) : launch_step<AKV_Q8_E4M3>(p, plan.nt, s);
-    if (int st = launched()) return st;
+    if (plan.chunk) {
+        if (int st = int8 ? launch_chunk<AKV_Q8_INT8>(p, s) : launch_chunk<AKV_Q8_E4M3>(p, s)) return st;
+    } else {
+        int8 ? launch_step<AKV_Q8_INT8>(p, plan.nt, s) : launch_step<AKV_Q8_E4M3>(p, plan.nt, s);
+        if (int st = launched()) return st;
+    }
     const int64_t rows = plan.nsplits > 1 ? static_cast<int64_t>(p.c.B) * p.c.H * p.R : 0;
     const int wblocks = plan.keep_scores ? (p.c.T + kWeightTokens - 1) / kWeightTokens : 0;
     const int64_t blocks = rows + static_cast<int64_t>(p.c.B) * p.c.H * wblocks;
     if (blocks > 0x7FFFFFFF) return AKV_ERR_UNSUPPORTED;
-    if (blocks) {
+    if (blocks && !wblocks && p.nsplits <= 16 && rows >= 4096) {
+        constexpr int per = kCombineThreads / 32;
+        if (int st = launch_after(combine_rows_kernel, dim3(static_cast<unsigned>((rows + per - 1) / per)), kCombineThreads, s, p,
+                                  static_cast<int>(rows)))
+            return st;
+    } else if (blocks) {
         if (int st = launch_after(combine_kernel, dim3(static_cast<unsigned>(blocks)), kCombineThreads, s, p, static_cast<int>(rows), wblocks))
             return st;
     }

@@ -286,5 +286,40 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, 
     }
 }
 
+// The combine where rows are many and splits few: a warp per row.
+__global__ void __launch_bounds__(kCombineThreads) combine_rows_kernel(AttnParams p, int rows) {
+    const int i = blockIdx.x * (kCombineThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    wait_for_previous_kernel();
+    if (i >= rows) return;
+    const int r = i % p.R, bh = i / p.R, h = bh % p.c.H, b = bh / p.c.H, lanes = p.c.D / 4;
+    const int64_t unit = static_cast<int64_t>(bh) * p.nsplits * p.R + r;
+    const float2* ml = p.part_ml + unit;
+    const float all = combined_lse(ml, p.nsplits, p.R);
+    const int64_t row = out_row(p, b, h, r);
+    if (lane == 0) {
+        if (p.lse) p.lse[row] = all;
+        if (p.lse_out) p.lse_out[row] = all * 0.69314718055994531f;
+    }
+    for (int x = lane; x < lanes; x += 32) {
+        const float4* o = reinterpret_cast<const float4*>(p.part_o) + unit * lanes + x;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < p.nsplits; ++s) {
+            const float m = ml[static_cast<int64_t>(s) * p.R].x;
+            if (m == -CUDART_INF_F) continue;
+            const float f = exp2f(m - all);
+            const float4 v = o[static_cast<int64_t>(s) * p.R * lanes];
+            a.x = fmaf(v.x, f, a.x);
+            a.y = fmaf(v.y, f, a.y);
+            a.z = fmaf(v.z, f, a.z);
+            a.w = fmaf(v.w, f, a.w);
+        }
+        const int64_t at = row * p.c.D + 4 * x;
+        store_elem(p.out, p.out_dtype, at, a.x);
+        store_elem(p.out, p.out_dtype, at + 1, a.y);
+        store_elem(p.out, p.out_dtype, at + 2, a.z);
+        store_elem(p.out, p.out_dtype, at + 3, a.w);
+    }
+}
+
 }  // namespace q8
 }  // namespace akv

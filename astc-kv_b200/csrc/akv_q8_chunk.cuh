@@ -1,0 +1,539 @@
+// Attention of many rows (query tokens x heads of a kv head) over the 8-bit
+// cache with 16-bit outputs: prompt chunks, on the fifth-generation tensor
+// cores.
+//
+// A CTA takes 256 rows of one kv head as two tiles of 128 and goes through a
+// split of the tokens 128 at a time. Its warps have roles:
+//
+//   warps 0-3, 4-7  softmax of tile 0 and 1, one thread per row
+//   warps 8-11      K and V: codes from global memory to fp16 in shared
+//                   memory (the conversion is shared by all 256 rows)
+//   warp 12         one thread issues tcgen05.mma
+//
+// S = Q K^T (M 128 rows, N 128 tokens) and O += P V (N head_dim) accumulate
+// in tensor memory: two S tiles and two O tiles fill its 512 columns. P is
+// written as fp16 over its own S and is the A operand of the second product.
+// While one tile's softmax runs, the other tile's products do; the order of
+// the issues (P0 V, Q0 K', P1 V, Q1 K') is the order of execution, so an S
+// that is there tells that the P V before it is done.
+//
+// Shared memory operands are K-major with the 128-byte swizzle: Q and K
+// [row][d], V transposed to [d][token] (eight tokens of a d are paired by byte
+// permutes in registers and stored as 16 bytes). Codes are exact in fp16, and
+// 16-bit query rows after a power of two.
+//
+// Softmax: t = s * factor + log2 v - base per token block, p = 2^t, and the
+// row sum adds p / v (see the step kernel for V's scale in the exponent).
+// `base` follows the row maximum loosely: the first tokens set it so that
+// their largest p is 2^6, and only a t above 15 (p would leave fp16) moves it
+// and scales O, which after the first tokens hardly ever happens.
+//
+// Per step and tile the tensor cores need 1024 cycles (D = 128) and the
+// special-function units as many for the 128 x 128 exp2: the two are the
+// bound, softmax's other instructions come close.
+#pragma once
+#include "akv_q8_attend.cuh"
+
+namespace akv {
+namespace q8 {
+
+constexpr int kChunkRows = 256;    // rows of a CTA
+constexpr int kChunkTokens = 128;  // per step
+constexpr int kChunkThreads = 32 * 13;
+constexpr int kMetaSlots = 4;      // K may be written three steps ahead of a softmax
+
+template <int DP>
+struct ChunkSmem {
+    // Operand tiles of 64 x 16-bit columns, 128 bytes a row, swizzled.
+    uint8_t q[2][DP / 64][128 * 128];
+    uint8_t k[2][DP / 64][128 * 128];
+    uint8_t v[2][2][DP * 128];
+    float4 meta[kMetaSlots][kChunkTokens / 16];  // K's scale, log2 and reciprocal of V's
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], done;
+    uint32_t tmem;
+    int abort;
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ void bar_init(uint64_t* bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_addr(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+// Waits for the phase of `parity` to end, a bounded number of times; false
+// (and the CTA's abort flag) when it does not, or when another warp gave up.
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, int parity, volatile int* abort) {
+    for (int i = 0; i < 1 << 22; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity) : "memory");
+        if (ok) return true;
+        if (*abort) return false;
+    }
+    *abort = 1;
+    return false;
+}
+
+// Descriptor of a K-major operand with the 128-byte swizzle: rows of 128
+// bytes, groups of eight rows 1024 bytes apart.
+__device__ __forceinline__ uint64_t operand_desc(const void* p) {
+    return static_cast<uint64_t>((smem_addr(p) & 0x3FFFF) >> 4) | 1ull << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61;
+}
+// kind::f16 with fp16 operands, fp32 accumulation, both K-major.
+__device__ __forceinline__ constexpr uint32_t mma_desc(int m, int n) {
+    return 1u << 4 | static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(m >> 4) << 24;
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b),
+        "r"(desc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b),
+        "r"(desc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+// The barrier's phase ends when every MMA issued so far has finished.
+__device__ __forceinline__ void mma_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t (&x)[16], uint32_t at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]), "=r"(x[4]), "=r"(x[5]), "=r"(x[6]), "=r"(x[7]), "=r"(x[8]), "=r"(x[9]),
+          "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
+        : "r"(at) : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* x) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(x[0]),
+        "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]), "r"(x[11]),
+        "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Byte offset of 16-byte chunk c of row r in a swizzled tile.
+__device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
+
+template <int FMT, int DP>
+__global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
+    using Smem = ChunkSmem<DP>;
+    extern __shared__ uint8_t smem_raw[];
+    // The swizzle counts from 1024-byte boundaries.
+    Smem& sm = *reinterpret_cast<Smem*>(smem_raw + (-smem_addr(smem_raw) & 1023));
+    const CacheDev& c = p.c;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int tiles = (p.R + kChunkRows - 1) / kChunkRows;
+    // Later rows see more tokens: they go first.
+    const int split = blockIdx.x % p.nsplits, r0 = (tiles - 1 - blockIdx.x / p.nsplits) * kChunkRows, h = blockIdx.y, b = blockIdx.z;
+    const int len = len_of(p, b), qlen = q_len_of(p, b), rows = min(kChunkRows, p.R - r0);
+    const int bh = b * c.H + h;
+    const int64_t unit = (static_cast<int64_t>(bh) * p.nsplits + split) * p.R + r0;
+    const int end = r0 / p.G < qlen ? seen_by(p, min((r0 + rows - 1) / p.G, qlen - 1), len, qlen) : 0;
+    const int t_begin = split * p.split, t_end = min(t_begin + p.split, end);
+    const int steps = t_end > t_begin ? (t_end - t_begin + kChunkTokens - 1) / kChunkTokens : 0;
+    if (steps == 0) {
+        // Nothing to see for any row.
+        for (int i = threadIdx.x; i < rows; i += kChunkThreads) {
+            p.part_ml[unit + i] = make_float2(-CUDART_INF_F, 0.f);
+            if (p.nsplits > 1) continue;
+            const int64_t row = out_row(p, b, h, r0 + i);
+            if (p.lse) p.lse[row] = -CUDART_INF_F;
+            if (p.lse_out) p.lse_out[row] = -CUDART_INF_F;
+        }
+        if (p.nsplits == 1)
+            for (int i = threadIdx.x; i < rows * c.D; i += kChunkThreads)
+                store_elem(p.out, p.out_dtype, out_row(p, b, h, r0 + i / c.D) * c.D + i % c.D, 0.f);
+        return;
+    }
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&sm.k_full[i], 128);
+            bar_init(&sm.v_full[i], 128);
+            bar_init(&sm.k_empty[i], 1);
+            bar_init(&sm.v_empty[i], 1);
+            bar_init(&sm.s_full[i], 2);
+            bar_init(&sm.p_full[i], 128);
+        }
+        bar_init(&sm.done, 1);
+        sm.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sm.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+
+    // Query rows: thread = row, to fp16 after a power of two.
+    float factor = 0.f;
+    int bound = 0;
+    if (warp < 8) {
+        const int tile = warp >> 2, r = threadIdx.x & 127, row = r0 + threadIdx.x;
+        const bool in = static_cast<int>(threadIdx.x) < rows;
+        const int64_t at = in ? q_row(p, b, h, row) : 0;
+        uint32_t top = 0;
+        for (int d = 0; in && d < c.D; d += 16) {
+            float x[16];
+            load_q16(p, at + d, x);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) top = max(top, abs_bits(x[k]));
+        }
+        const int e = row_exponent(__uint_as_float(top));
+        const float up = power_of_two(e);
+        for (int d = 0; d < DP; d += 16) {
+            float x[16];
+            if (in && d < c.D) {
+                load_q16(p, at + d, x);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) x[k] = 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                uint4 w;
+                w.x = pack_half2(x[8 * k] * up, x[8 * k + 1] * up);
+                w.y = pack_half2(x[8 * k + 2] * up, x[8 * k + 3] * up);
+                w.z = pack_half2(x[8 * k + 4] * up, x[8 * k + 5] * up);
+                w.w = pack_half2(x[8 * k + 6] * up, x[8 * k + 7] * up);
+                *reinterpret_cast<uint4*>(sm.q[tile][d / 64] + swizzled(r, d / 8 % 8 + k)) = w;
+            }
+        }
+        factor = p.c2 * power_of_two(-e);
+        bound = in ? seen_by(p, row / p.G, len, qlen) : 0;
+        fence_async();
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sm.tmem;
+
+    const bool two = rows > 128;  // with fewer rows the second tile rests
+    if (warp < 4 || (two && warp < 8)) {
+        // ------------------------------------------------------------ softmax
+        const int tile = warp >> 2;
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes
+        const uint32_t s_at = tmem + tile * 128 + lanes, o_at = tmem + 256 + tile * 128 + lanes;
+        float base = 0.f, l = 0.f;
+        bool started = false;
+        bool alive = true;
+        for (int j = 0; j < steps && alive; ++j) {
+            const int t0 = t_begin + j * kChunkTokens;
+            const float4* meta = sm.meta[j % kMetaSlots];
+            alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.s_full[tile], j & 1, &sm.abort));
+            if (!alive) break;
+            fence_after();
+            const bool masked = __any_sync(0xFFFFFFFFu, t0 + kChunkTokens > bound);
+            // The largest t of the row's tokens under base 0.
+            auto row_max = [&]() {
+                float m = -CUDART_INF_F;
+#pragma unroll 1
+                for (int g = 0; g < 8; ++g) {
+                    uint32_t s[16];
+                    tmem_ld16(s, s_at + 16 * g);
+                    tmem_wait_ld();
+                    const float4 mt = meta[g];
+                    const float f = factor * mt.x;
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        const float t = fmaf(__uint_as_float(s[k]), f, mt.y);
+                        if (t0 + 16 * g + k < bound) m = fmaxf(m, t);
+                    }
+                }
+                return m;
+            };
+            if (__any_sync(0xFFFFFFFFu, !started)) {
+                const float m = row_max();
+                if (!started && m != -CUDART_INF_F) {
+                    base = m - 6.f;
+                    started = true;
+                }
+                __syncwarp();
+            }
+            uint32_t pk[64];
+            float add, m;
+            auto weights = [&](auto check) {
+                add = 0.f;
+                m = -CUDART_INF_F;
+#pragma unroll
+                for (int g = 0; g < 8; ++g) {
+                    uint32_t s[16];
+                    tmem_ld16(s, s_at + 16 * g);
+                    const float4 mt = meta[g];
+                    const float f = factor * mt.x, off = mt.y - base;
+                    tmem_wait_ld();
+                    float sum = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2) {
+                        float a = fmaf(__uint_as_float(s[k]), f, off), d = fmaf(__uint_as_float(s[k + 1]), f, off);
+                        if (check(0)) {
+                            if (t0 + 16 * g + k >= bound) a = -CUDART_INF_F;
+                            if (t0 + 16 * g + k + 1 >= bound) d = -CUDART_INF_F;
+                        }
+                        m = fmaxf(m, fmaxf(a, d));
+                        a = exp2_fast(a);
+                        d = exp2_fast(d);
+                        sum += a + d;
+                        pk[8 * g + k / 2] = pack_half2(a, d);
+                    }
+                    add = fmaf(sum, mt.z, add);
+                }
+            };
+            if (masked) weights([](int) { return true; });
+            else weights([](int) { return false; });
+            if (__any_sync(0xFFFFFFFFu, m > 15.f)) {
+                // Some row's p leaves fp16: raise its base, scale its sums, again.
+                const float up = m > 15.f ? m - 6.f : 0.f;
+                const float alpha = exp2_fast(-up);
+                base += up;
+                l *= alpha;
+                if (j > 0) {
+#pragma unroll 1
+                    for (int g = 0; g < DP / 16; ++g) {
+                        uint32_t o[16];
+                        tmem_ld16(o, o_at + 16 * g);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                        tmem_st16(o_at + 16 * g, o);
+                    }
+                }
+                weights([](int) { return true; });
+            }
+            l += add;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) tmem_st16(s_at + 16 * g, pk + 16 * g);
+            tmem_wait_st();
+            fence_before();
+            bar_arrive(&sm.p_full[tile]);
+        }
+        // ---------------------------------------------------------- write rows
+        alive = __all_sync(0xFFFFFFFFu, alive && bar_wait(&sm.done, 0, &sm.abort));
+        fence_after();
+        const bool in = static_cast<int>(threadIdx.x) < rows;
+        const int r = r0 + threadIdx.x;
+        const bool none = !started && !isnan(l);
+        const float inv = none ? 0.f : 1.f / l;
+        const int64_t row = in ? out_row(p, b, h, r) : 0;
+#pragma unroll 1
+        for (int g = 0; g < DP / 16; ++g) {
+            uint32_t o[16];
+            tmem_ld16(o, o_at + 16 * g);
+            tmem_wait_ld();
+            if (!in || 16 * g >= c.D || !alive) {
+            } else if (p.nsplits > 1) {
+                uint4* to = reinterpret_cast<uint4*>(p.part_o + (unit + threadIdx.x) * c.D + 16 * g);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) to[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            } else {
+                uint32_t w[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float x = none ? 0.f : __uint_as_float(o[2 * k]) * inv, y = none ? 0.f : __uint_as_float(o[2 * k + 1]) * inv;
+                    if (p.out_dtype == AKV_Q_BF16) {
+                        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+                        w[k] = *reinterpret_cast<const uint32_t*>(&v);
+                    } else {
+                        w[k] = pack_half2(x, y);
+                    }
+                }
+                uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * c.D + 16 * g);
+                to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                to[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+            __syncwarp();
+        }
+        if (in) {
+            if (!alive) l = CUDART_NAN_F;
+            p.part_ml[unit + threadIdx.x] = make_float2(isnan(l) ? l : none ? -CUDART_INF_F : base, l);
+            if (p.nsplits == 1) {
+                const float lse = isnan(l) ? l : none ? -CUDART_INF_F : base + log2f(l);
+                if (p.lse) p.lse[row] = lse;
+                if (p.lse_out) p.lse_out[row] = lse * 0.69314718055994531f;
+            }
+        }
+    } else if (warp >= 8 && warp < 12) {
+        // ---------------------------------------------------- K and V to fp16
+        const int tid = threadIdx.x - 256, w = tid >> 5;
+        constexpr int KP = DP / 16;                  // 16-byte pieces per lane and step, = pieces of a row
+        constexpr int KROWS = 128 / KP;              // rows that the warps cover at a time
+        constexpr int VW = DP / 32;                  // words of a token per lane
+        const int k_row = tid / KP, k_piece = tid % KP;
+        const int k_col = 16 * k_piece < c.D ? 16 * k_piece : 0;
+        const int v_tok = 64 * (w & 1) + 8 * (lane & 7), v_d = (w >> 1) * (DP / 2) + (lane >> 3) * (DP / 8);
+        const int v_col = v_d < c.D ? v_d : 0;
+        const uint8_t* k_head = c.k.codes + b * c.k.sB + h * c.k.sH + k_col;
+        const uint8_t* v_head = c.v.codes + b * c.v.sB + h * c.v.sH + v_col;
+        uint4 kr[KP];
+        uint32_t vr[8][VW];
+        auto load_k = [&](int t0) {
+#pragma unroll
+            for (int i = 0; i < KP; ++i) {
+                const int t = t0 + i * KROWS + k_row;
+                kr[i] = make_uint4(0, 0, 0, 0);
+                if (t >= t_end) continue;
+                int row;
+                const int phys = page_of(c, b, t, row);
+                if (phys >= 0) kr[i] = load_stream(k_head + phys * c.k.sP + row * c.k.sT);
+            }
+        };
+        auto load_v = [&](int t0) {
+            const int t = t0 + v_tok;
+            int row = 0;
+            const int phys = t < t_end ? page_of(c, b, t, row) : -1;
+            const uint8_t* at = v_head + phys * c.v.sP + row * c.v.sT;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool in = phys >= 0 && t + i < t_end;
+                if (DP == 64) {
+                    const uint2 x = in ? load_stream8(at + i * c.v.sT) : make_uint2(0, 0);
+                    vr[i][0] = x.x; vr[i][1] = x.y;
+                } else {
+                    const uint4 x = in ? load_stream(at + i * c.v.sT) : make_uint4(0, 0, 0, 0);
+                    vr[i][0] = x.x; vr[i][1] = x.y; vr[i][VW - 2] = x.z; vr[i][VW - 1] = x.w;
+                }
+            }
+        };
+        float ks = 0.f, vs = 0.f;
+        auto load_meta = [&](int t0) {
+            ks = 0.f;
+            vs = 1.f;
+            const int t = t0 + 16 * tid;
+            if (tid >= 8 || t >= t_end) return;
+            int row;
+            const int phys = page_of(c, b, t, row);
+            if (phys < 0) return;
+            ks = __ldg(c.k.scales + scale_offset(c.k, b, h, phys, row / c.blk));
+            vs = __ldg(c.v.scales + scale_offset(c.v, b, h, phys, row / c.blk));
+            vs = vs < 8.0779357e-28f ? 8.0779357e-28f : vs;  // a NaN stays one
+        };
+        load_meta(t_begin);
+        load_k(t_begin);
+        load_v(t_begin);
+        bool alive = true;
+        for (int j = 0; j < steps && alive; ++j) {
+            const int st = j & 1, t_next = t_begin + (j + 1) * kChunkTokens;
+            // The phase before a stage's first use counts as over.
+            alive = bar_wait(&sm.k_empty[st], (j >> 1 & 1) ^ 1, &sm.abort);
+            if (!alive) break;
+            if (tid < 8) {
+                const float lv = log2_fast(vs);
+                sm.meta[j % kMetaSlots][tid] = make_float4(ks, lv, exp2_fast(-lv), 0.f);
+            }
+#pragma unroll
+            for (int i = 0; i < KP; ++i) {
+                const int r = i * KROWS + k_row, chunk = 2 * k_piece % 8;
+                uint8_t* tile = sm.k[st][k_piece / 4];
+                uint4 a, d;
+                codes_to_half<FMT>(kr[i].x, a.x, a.y);
+                codes_to_half<FMT>(kr[i].y, a.z, a.w);
+                codes_to_half<FMT>(kr[i].z, d.x, d.y);
+                codes_to_half<FMT>(kr[i].w, d.z, d.w);
+                // The second half of a row's lanes start with their second
+                // chunk, so that a row's stores fall into different banks.
+                const bool swap = k_piece >= 4;
+                *reinterpret_cast<uint4*>(tile + swizzled(r, chunk + swap)) = swap ? d : a;
+                *reinterpret_cast<uint4*>(tile + swizzled(r, chunk + !swap)) = swap ? a : d;
+            }
+            fence_async();
+            bar_arrive(&sm.k_full[st]);
+            load_meta(t_next);
+            load_k(t_next);
+            alive = bar_wait(&sm.v_empty[st], (j >> 1 & 1) ^ 1, &sm.abort);
+            if (!alive) break;
+            uint8_t* tile = sm.v[st][w & 1];
+#pragma unroll
+            for (int x = 0; x < VW; ++x) {
+                uint32_t y[4][4];  // [d of the word][pair of tokens]
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const uint32_t u = vr[2 * q][x], z = vr[2 * q + 1][x];
+                    codes_to_half<FMT>(__byte_perm(u, z, 0x5140), y[0][q], y[1][q]);
+                    codes_to_half<FMT>(__byte_perm(u, z, 0x7362), y[2][q], y[3][q]);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    *reinterpret_cast<uint4*>(tile + swizzled(v_d + 4 * x + k, lane & 7)) = make_uint4(y[k][0], y[k][1], y[k][2], y[k][3]);
+            }
+            fence_async();
+            bar_arrive(&sm.v_full[st]);
+            load_v(t_next);
+        }
+    } else if (warp == 12) {
+        // --------------------------------------------------------- the products
+        bool alive = true;
+        if (lane == 0) {
+            constexpr uint32_t qk = mma_desc(128, 128), pv = mma_desc(128, DP);
+            auto scores = [&](int tile, int st) {
+#pragma unroll
+                for (int k = 0; k < DP / 16; ++k)
+                    mma_ss(tmem + tile * 128, operand_desc(sm.q[tile][k / 4]) + k % 4 * 2, operand_desc(sm.k[st][k / 4]) + k % 4 * 2, qk, k > 0);
+                mma_commit(&sm.s_full[tile]);
+                bar_arrive(&sm.s_full[tile]);  // hands on what k_full has shown: the block scales
+            };
+            auto values = [&](int tile, int st, bool add) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                    mma_ts(tmem + 256 + tile * 128, tmem + tile * 128 + 8 * k, operand_desc(sm.v[st][k / 4]) + k % 4 * 2, pv, add || k > 0);
+            };
+            alive = bar_wait(&sm.k_full[0], 0, &sm.abort);
+            if (alive) {
+                fence_after();
+                scores(0, 0);
+                if (two) scores(1, 0);
+                mma_commit(&sm.k_empty[0]);
+            }
+            for (int j = 0; j < steps && alive; ++j) {
+                const int st = j & 1, nx = st ^ 1;
+                const bool more = j + 1 < steps;
+                alive = bar_wait(&sm.v_full[st], j >> 1 & 1, &sm.abort) && bar_wait(&sm.p_full[0], j & 1, &sm.abort);
+                if (!alive) break;
+                fence_after();
+                values(0, st, j > 0);
+                if (more) {
+                    alive = bar_wait(&sm.k_full[nx], (j + 1) >> 1 & 1, &sm.abort);
+                    if (!alive) break;
+                    fence_after();
+                    scores(0, nx);
+                }
+                if (two) {
+                    alive = bar_wait(&sm.p_full[1], j & 1, &sm.abort);
+                    if (!alive) break;
+                    fence_after();
+                    values(1, st, j > 0);
+                }
+                mma_commit(&sm.v_empty[st]);
+                if (more) {
+                    if (two) scores(1, nx);
+                    mma_commit(&sm.k_empty[nx]);
+                }
+            }
+            // Also after giving up: nothing may be in flight when the tensor
+            // memory is given back.
+            mma_commit(&sm.done);
+            int none = 0;
+            bar_wait(&sm.done, 0, &none);
+        }
+        __syncwarp();
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        if (lane == 0 && sm.abort) report(c.status, AKV_ERR_TIMEOUT);
+    }
+}
+
+}  // namespace q8
+}  // namespace akv

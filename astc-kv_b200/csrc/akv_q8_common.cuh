@@ -22,6 +22,7 @@ struct CacheDev {
     SideDev k, v;
     const int32_t* table;
     int B, H, D, T, P, pps, num_pages, blk, fmt;
+    int page_shift;          // log2 of P, 31 where one page holds every token, -1 otherwise
     int32_t* status;
 };
 
@@ -38,6 +39,9 @@ inline CacheDev to_dev(const AkvQ8Cache& c) {
     d.B = c.batch; d.H = c.kv_heads; d.D = c.head_dim; d.T = c.max_tokens; d.P = c.page_tokens;
     d.pps = c.pages_per_seq; d.num_pages = c.num_pages; d.blk = c.block_tokens; d.fmt = c.format;
     d.status = c.status_dev;
+    d.page_shift = c.page_tokens >= c.max_tokens ? 31 : -1;
+    for (int i = 4; i < 31 && d.page_shift < 0; ++i)
+        if (c.page_tokens == 1 << i) d.page_shift = i;
     return d;
 }
 
@@ -51,10 +55,11 @@ __device__ __forceinline__ void report(int32_t* status, int code) {
     if (status) atomicExch(status, code);
 }
 
-// Physical page of token t (0 <= t < T) of sequence b, -1 for a table entry
-// outside the pool.
-__device__ __forceinline__ int page_of(const CacheDev& c, int b, int t) {
-    const int p = t / c.P;
+// Physical page of token t (0 <= t < T) of sequence b and the token's row in
+// it; -1 for a table entry outside the pool.
+__device__ __forceinline__ int page_of(const CacheDev& c, int b, int t, int& row) {
+    const int p = c.page_shift >= 0 ? t >> c.page_shift : t / c.P;
+    row = t - p * c.P;
     if (!c.table) return p;
     const int v = __ldg(c.table + static_cast<int64_t>(b) * c.pps + p);
     if (static_cast<unsigned>(v) >= static_cast<unsigned>(c.num_pages)) {

@@ -164,7 +164,8 @@ __global__ void __launch_bounds__(256) pack_kernel(EvictParams p) {
     wait_for_previous_kernel();
     const int n = min(p.out_lens[b] - row0, c.blk);
     if (n <= 0) return;
-    const int phys = page_of(c, b, row0);
+    int in_page;
+    const int phys = page_of(c, b, row0, in_page);
     if (phys < 0) return;
     uint4 w[PP];
     float sc[PP];
@@ -175,7 +176,8 @@ __global__ void __launch_bounds__(256) pack_kernel(EvictParams p) {
         w[k] = make_uint4(0, 0, 0, 0);
         sc[k] = 0.f;
         if (r >= n) continue;
-        const int t = kept[row0 + r], pg = page_of(a, b, t), row = t % a.P;
+        int row;
+        const int pg = page_of(a, b, kept[row0 + r], row);
         if (pg < 0) continue;
         w[k] = __ldg(reinterpret_cast<const uint4*>(from.codes + code_offset(from, b, h, pg, row)) + (i - r * per_row));
         sc[k] = from.scales[scale_offset(from, b, h, pg, row / a.blk)];
@@ -195,7 +197,6 @@ __global__ void __launch_bounds__(256) pack_kernel(EvictParams p) {
         top = max(top, abs_bits(__fmul_rn(__uint_as_float(m), sc[k])));
     }
     const float scale = block_scale<FMT>(cta_max(top, red)), inv = block_inverse(scale);
-    const int in_page = row0 % c.P;
     uint8_t* codes = to.codes + code_offset(to, b, h, phys, in_page);
 #pragma unroll
     for (int k = 0; k < PP; ++k) {

@@ -75,10 +75,10 @@ __global__ void __launch_bounds__(256) store_kernel(StoreParams p) {
     const int first = static_cast<int>(max(start, block0) - block0);  // rows [first, last) are new
     const int last = static_cast<int>(min(end - block0, static_cast<int64_t>(c.blk)));
     if (last <= first) return;
-    const int phys = page_of(c, b, static_cast<int>(block0));
+    int row0;
+    const int phys = page_of(c, b, static_cast<int>(block0), row0);
     if (phys < 0) return;
     const SideDev& s = side ? c.v : c.k;
-    const int row0 = static_cast<int>(block0 % c.P);
     uint8_t* codes = s.codes + code_offset(s, b, h, phys, row0);
     float* scale_at = s.scales + scale_offset(s, b, h, phys, row0 / c.blk);
     const T* x = static_cast<const T*>(p.x[side]) + b * p.xB[side] + h * p.xH[side] + (block0 - start) * p.xT[side];
@@ -159,11 +159,11 @@ __global__ void __launch_bounds__(256) restore_kernel(RestoreParams p) {
     const int h = rest / per_row, d = (rest - h * per_row) * 16;
     wait_for_previous_kernel();
     const int64_t t = static_cast<int64_t>(ti) + (p.start ? p.start[b] : 0);
-    const int phys = t >= 0 && t < c.T ? page_of(c, b, static_cast<int>(t)) : -1;
+    int row = 0;
+    const int phys = t >= 0 && t < c.T ? page_of(c, b, static_cast<int>(t), row) : -1;
     uint4 w = make_uint4(0, 0, 0, 0);
     float scale = 0.f;
     if (phys >= 0) {
-        const int row = static_cast<int>(t % c.P);
         w = *reinterpret_cast<const uint4*>(s.codes + code_offset(s, b, h, phys, row) + d);
         scale = s.scales[scale_offset(s, b, h, phys, row / c.blk)];
     }

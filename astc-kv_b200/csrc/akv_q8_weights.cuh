@@ -41,7 +41,8 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(AttnParams p) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int tt = t0 + 16 * i;
-        const int phys = tt < len ? page_of(c, b, tt) : -1, row = tt % c.P;
+        int row = 0;
+        const int phys = tt < len ? page_of(c, b, tt, row) : -1;
         const uint8_t* base = c.k.codes + b * c.k.sB + h * c.k.sH + phys * c.k.sP + row * c.k.sT;
         ks[i] = phys >= 0 ? c.k.scales[b * c.k.cB + h * c.k.cH + phys * c.k.cP + row / c.blk] : 0.f;
 #pragma unroll
