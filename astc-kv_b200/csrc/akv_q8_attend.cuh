@@ -163,6 +163,24 @@ __device__ __forceinline__ uint2 load_stream8(const void* p) {
     return v;
 }
 
+// The same, or zeros without a load; nothing waits for what is loaded.
+__device__ __forceinline__ uint4 load_stream_if(const void* p, bool in) {
+    uint4 v;
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %5, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\nmov.b32 %2, 0;\nmov.b32 %3, 0;\n"
+        "@p ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];\n}\n"
+        : "=&r"(v.x), "=&r"(v.y), "=&r"(v.z), "=&r"(v.w) : "l"(p), "r"(static_cast<uint32_t>(in)));
+    return v;
+}
+__device__ __forceinline__ uint2 load_stream8_if(const void* p, bool in) {
+    uint2 v;
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.u32 p, %3, 0;\nmov.b32 %0, 0;\nmov.b32 %1, 0;\n"
+        "@p ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];\n}\n"
+        : "=&r"(v.x), "=&r"(v.y) : "l"(p), "r"(static_cast<uint32_t>(in)));
+    return v;
+}
+
 // ------------------------------------------------------------------ combine
 
 constexpr int kCombineThreads = 256;

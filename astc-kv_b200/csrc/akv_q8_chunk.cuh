@@ -39,7 +39,7 @@ namespace q8 {
 
 constexpr int kChunkRows = 256;    // rows of a CTA
 constexpr int kChunkTokens = 128;  // per step
-constexpr int kChunkThreads = 32 * 13;
+constexpr int kChunkThreads = 32 * 16;  // four warpgroups; warps 13-15 only give their registers away
 constexpr int kMetaSlots = 4;      // K may be written three steps ahead of a softmax
 
 template <int DP>
@@ -116,11 +116,41 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* x) {
         "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15])
         : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Ends the loads in flight; x is one of them and must not be used before.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&x)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(x[0]), "+r"(x[1]), "+r"(x[2]), "+r"(x[3]), "+r"(x[4]), "+r"(x[5]), "+r"(x[6]), "+r"(x[7]), "+r"(x[8]), "+r"(x[9]),
+                   "+r"(x[10]), "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]), "+r"(x[15])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(lo), "r"(hi));
+    return v;
+}
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) { return pair_of(__float_as_uint(lo), __float_as_uint(hi)); }
+__device__ __forceinline__ float2 halves(uint64_t v) {
+    uint32_t lo, hi;
+    asm("mov.b64 {%0, %1}, %2;" : "=r"(lo), "=r"(hi) : "l"(v));
+    return make_float2(__uint_as_float(lo), __uint_as_float(hi));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 
 // Byte offset of 16-byte chunk c of row r in a swizzled tile.
 __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
@@ -183,18 +213,22 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         const bool in = static_cast<int>(threadIdx.x) < rows;
         const int64_t at = in ? q_row(p, b, h, row) : 0;
         uint32_t top = 0;
-        for (int d = 0; in && d < c.D; d += 16) {
-            float x[16];
-            load_q16(p, at + d, x);
+        if (in) {
+#pragma unroll 4
+            for (int d = 0; d < c.D; d += 16) {
+                float x[16];
+                load_q16(p, at + d, x);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) top = max(top, abs_bits(x[k]));
+                for (int k = 0; k < 16; ++k) top = max(top, abs_bits(x[k]));
+            }
         }
         const int e = row_exponent(__uint_as_float(top));
         const float up = power_of_two(e);
+#pragma unroll 4
         for (int d = 0; d < DP; d += 16) {
             float x[16];
             if (in && d < c.D) {
-                load_q16(p, at + d, x);
+                load_q16(p, at + d, x);  // from L1
             } else {
 #pragma unroll
                 for (int k = 0; k < 16; ++k) x[k] = 0.f;
@@ -219,41 +253,51 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     const uint32_t tmem = sm.tmem;
 
     const bool two = rows > 128;  // with fewer rows the second tile rests
-    if (warp < 4 || (two && warp < 8)) {
+    // Registers go to where they are needed: 2 x 168 + 104 + 72 = 4 x 128.
+    if (warp < 8) {
         // ------------------------------------------------------------ softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
         const int tile = warp >> 2;
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes
         const uint32_t s_at = tmem + tile * 128 + lanes, o_at = tmem + 256 + tile * 128 + lanes;
         float base = 0.f, l = 0.f;
         bool started = false;
         bool alive = true;
-        for (int j = 0; j < steps && alive; ++j) {
+        const int my_steps = tile == 0 || two ? steps : 0;
+        for (int j = 0; j < my_steps && alive; ++j) {
             const int t0 = t_begin + j * kChunkTokens;
             const float4* meta = sm.meta[j % kMetaSlots];
             alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.s_full[tile], j & 1, &sm.abort));
             if (!alive) break;
             fence_after();
-            const bool masked = __any_sync(0xFFFFFFFFu, t0 + kChunkTokens > bound);
-            // The largest t of the row's tokens under base 0.
-            auto row_max = [&]() {
+            if (__any_sync(0xFFFFFFFFu, t0 + kChunkTokens > bound)) {
+                // What a row does not see becomes a score that no factor
+                // brings back.
+#pragma unroll 1
+                for (int g = 0; g < 8; ++g) {
+                    uint32_t s[16];
+                    tmem_ld16(s, s_at + 16 * g);
+                    tmem_wait_ld(s);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (t0 + 16 * g + k >= bound) s[k] = __float_as_uint(-3e38f);
+                    tmem_st16(s_at + 16 * g, s);
+                }
+                tmem_wait_st();
+            }
+            if (__any_sync(0xFFFFFFFFu, !started)) {
+                // The largest t of the row's tokens.
                 float m = -CUDART_INF_F;
 #pragma unroll 1
                 for (int g = 0; g < 8; ++g) {
                     uint32_t s[16];
                     tmem_ld16(s, s_at + 16 * g);
-                    tmem_wait_ld();
                     const float4 mt = meta[g];
-                    const float f = factor * mt.x;
+                    tmem_wait_ld(s);
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        const float t = fmaf(__uint_as_float(s[k]), f, mt.y);
-                        if (t0 + 16 * g + k < bound) m = fmaxf(m, t);
-                    }
+                    for (int k = 0; k < 16; ++k)
+                        if (t0 + 16 * g + k < bound) m = fmaxf(m, fmaf(__uint_as_float(s[k]), fmaxf(factor * mt.x, 1e-30f), mt.y));
                 }
-                return m;
-            };
-            if (__any_sync(0xFFFFFFFFu, !started)) {
-                const float m = row_max();
                 if (!started && m != -CUDART_INF_F) {
                     base = m - 6.f;
                     started = true;
@@ -261,37 +305,35 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                 __syncwarp();
             }
             uint32_t pk[64];
-            float add, m;
-            auto weights = [&](auto check) {
+            float add;
+            while (true) {
+                float m = -CUDART_INF_F;
                 add = 0.f;
-                m = -CUDART_INF_F;
+                uint32_t s[2][16];
+                tmem_ld16(s[0], s_at);
 #pragma unroll
                 for (int g = 0; g < 8; ++g) {
-                    uint32_t s[16];
-                    tmem_ld16(s, s_at + 16 * g);
+                    uint32_t(&x)[16] = s[g & 1];
+                    tmem_wait_ld(x);
+                    if (g < 7) tmem_ld16(s[(g + 1) & 1], s_at + 16 * (g + 1));
                     const float4 mt = meta[g];
-                    const float f = factor * mt.x, off = mt.y - base;
-                    tmem_wait_ld();
-                    float sum = 0.f;
+                    // A NaN scale has to stay one.
+                    const float f0 = factor * mt.x, f = f0 < 1e-30f ? 1e-30f : f0, off = mt.y - base;
+                    const uint64_t f2 = pair_of(f, f), off2 = pair_of(off, off);
+                    uint64_t sum = 0;
 #pragma unroll
                     for (int k = 0; k < 16; k += 2) {
-                        float a = fmaf(__uint_as_float(s[k]), f, off), d = fmaf(__uint_as_float(s[k + 1]), f, off);
-                        if (check(0)) {
-                            if (t0 + 16 * g + k >= bound) a = -CUDART_INF_F;
-                            if (t0 + 16 * g + k + 1 >= bound) d = -CUDART_INF_F;
-                        }
-                        m = fmaxf(m, fmaxf(a, d));
-                        a = exp2_fast(a);
-                        d = exp2_fast(d);
-                        sum += a + d;
-                        pk[8 * g + k / 2] = pack_half2(a, d);
+                        float2 t = halves(fma2(pair_of(x[k], x[k + 1]), f2, off2));
+                        m = fmaxf(m, fmaxf(t.x, t.y));
+                        t.x = exp2_fast(t.x);
+                        t.y = exp2_fast(t.y);
+                        sum = add2(sum, pair_of(t.x, t.y));
+                        pk[8 * g + k / 2] = pack_half2(t.x, t.y);
                     }
-                    add = fmaf(sum, mt.z, add);
+                    const float2 both = halves(sum);
+                    add = fmaf(both.x + both.y, mt.z, add);
                 }
-            };
-            if (masked) weights([](int) { return true; });
-            else weights([](int) { return false; });
-            if (__any_sync(0xFFFFFFFFu, m > 15.f)) {
+                if (!__any_sync(0xFFFFFFFFu, m > 15.f)) break;
                 // Some row's p leaves fp16: raise its base, scale its sums, again.
                 const float up = m > 15.f ? m - 6.f : 0.f;
                 const float alpha = exp2_fast(-up);
@@ -302,13 +344,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                     for (int g = 0; g < DP / 16; ++g) {
                         uint32_t o[16];
                         tmem_ld16(o, o_at + 16 * g);
-                        tmem_wait_ld();
+                        tmem_wait_ld(o);
 #pragma unroll
                         for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
                         tmem_st16(o_at + 16 * g, o);
                     }
                 }
-                weights([](int) { return true; });
             }
             l += add;
 #pragma unroll
@@ -329,7 +370,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         for (int g = 0; g < DP / 16; ++g) {
             uint32_t o[16];
             tmem_ld16(o, o_at + 16 * g);
-            tmem_wait_ld();
+            tmem_wait_ld(o);
             if (!in || 16 * g >= c.D || !alive) {
             } else if (p.nsplits > 1) {
                 uint4* to = reinterpret_cast<uint4*>(p.part_o + (unit + threadIdx.x) * c.D + 16 * g);
@@ -362,29 +403,51 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                 if (p.lse_out) p.lse_out[row] = lse * 0.69314718055994531f;
             }
         }
-    } else if (warp >= 8 && warp < 12) {
+    } else if (warp < 12) {
         // ---------------------------------------------------- K and V to fp16
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
         const int tid = threadIdx.x - 256, w = tid >> 5;
-        constexpr int KP = DP / 16;                  // 16-byte pieces per lane and step, = pieces of a row
-        constexpr int KROWS = 128 / KP;              // rows that the warps cover at a time
+        // K: four lanes a row of a 64-column tile, 32 rows at a time, so that
+        // the stores of eight lanes (two rows, every other chunk) fall into
+        // different banks. V: eight lanes a tile row of 64 tokens, likewise.
+        constexpr int KP = DP / 16;                  // 16-byte pieces per lane and step
         constexpr int VW = DP / 32;                  // words of a token per lane
-        const int k_row = tid / KP, k_piece = tid % KP;
-        const int k_col = 16 * k_piece < c.D ? 16 * k_piece : 0;
+        const int k_row = tid >> 2, k_piece = tid & 3;
         const int v_tok = 64 * (w & 1) + 8 * (lane & 7), v_d = (w >> 1) * (DP / 2) + (lane >> 3) * (DP / 8);
         const int v_col = v_d < c.D ? v_d : 0;
-        const uint8_t* k_head = c.k.codes + b * c.k.sB + h * c.k.sH + k_col;
+        int k_col[DP / 64];
+#pragma unroll
+        for (int i = 0; i < DP / 64; ++i) k_col[i] = 64 * i + 16 * k_piece < c.D ? 64 * i + 16 * k_piece : 0;
+        const uint8_t* k_head = c.k.codes + b * c.k.sB + h * c.k.sH;
         const uint8_t* v_head = c.v.codes + b * c.v.sB + h * c.v.sH + v_col;
+        const int blk_shift = 31 - __clz(c.blk);
+        // Every step within one page: one look at the table for all its rows.
+        const bool one_page = c.page_shift == 31 || (c.P % kChunkTokens == 0 && t_begin % kChunkTokens == 0);
+        const int64_t k_row32 = 32 * c.k.sT;
         uint4 kr[KP];
         uint32_t vr[8][VW];
         auto load_k = [&](int t0) {
-#pragma unroll
-            for (int i = 0; i < KP; ++i) {
-                const int t = t0 + i * KROWS + k_row;
-                kr[i] = make_uint4(0, 0, 0, 0);
-                if (t >= t_end) continue;
+            if (one_page) {
                 int row;
-                const int phys = page_of(c, b, t, row);
-                if (phys >= 0) kr[i] = load_stream(k_head + phys * c.k.sP + row * c.k.sT);
+                const int phys = t0 < t_end ? page_of(c, b, t0, row) : -1;
+                const uint8_t* at = k_head + phys * c.k.sP + (row + k_row) * c.k.sT;
+                const int left = phys >= 0 ? t_end - t0 - k_row : 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                    for (int k = 0; k < DP / 64; ++k) kr[4 * k + i] = load_stream_if(at + k_col[k], 32 * i < left);
+                    at += k_row32;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int t = t0 + 32 * i + k_row;
+                    int row = 0;
+                    const int phys = t < t_end ? page_of(c, b, t, row) : -1;
+#pragma unroll
+                    for (int k = 0; k < DP / 64; ++k)
+                        kr[4 * k + i] = load_stream_if(k_head + phys * c.k.sP + row * c.k.sT + k_col[k], phys >= 0);
+                }
             }
         };
         auto load_v = [&](int t0) {
@@ -392,30 +455,31 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             int row = 0;
             const int phys = t < t_end ? page_of(c, b, t, row) : -1;
             const uint8_t* at = v_head + phys * c.v.sP + row * c.v.sT;
+            const int left = phys >= 0 ? t_end - t : 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const bool in = phys >= 0 && t + i < t_end;
                 if (DP == 64) {
-                    const uint2 x = in ? load_stream8(at + i * c.v.sT) : make_uint2(0, 0);
+                    const uint2 x = load_stream8_if(at, i < left);
                     vr[i][0] = x.x; vr[i][1] = x.y;
                 } else {
-                    const uint4 x = in ? load_stream(at + i * c.v.sT) : make_uint4(0, 0, 0, 0);
+                    const uint4 x = load_stream_if(at, i < left);
                     vr[i][0] = x.x; vr[i][1] = x.y; vr[i][VW - 2] = x.z; vr[i][VW - 1] = x.w;
                 }
+                at += c.v.sT;
             }
         };
+        // Read now, looked at when the step comes.
         float ks = 0.f, vs = 0.f;
         auto load_meta = [&](int t0) {
+            const int t = t0 + 16 * tid;
             ks = 0.f;
             vs = 1.f;
-            const int t = t0 + 16 * tid;
             if (tid >= 8 || t >= t_end) return;
             int row;
             const int phys = page_of(c, b, t, row);
             if (phys < 0) return;
-            ks = __ldg(c.k.scales + scale_offset(c.k, b, h, phys, row / c.blk));
-            vs = __ldg(c.v.scales + scale_offset(c.v, b, h, phys, row / c.blk));
-            vs = vs < 8.0779357e-28f ? 8.0779357e-28f : vs;  // a NaN stays one
+            ks = __ldg(c.k.scales + scale_offset(c.k, b, h, phys, row >> blk_shift));
+            vs = __ldg(c.v.scales + scale_offset(c.v, b, h, phys, row >> blk_shift));
         };
         load_meta(t_begin);
         load_k(t_begin);
@@ -427,23 +491,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             alive = bar_wait(&sm.k_empty[st], (j >> 1 & 1) ^ 1, &sm.abort);
             if (!alive) break;
             if (tid < 8) {
-                const float lv = log2_fast(vs);
+                const float lv = log2_fast(vs < 8.0779357e-28f ? 8.0779357e-28f : vs);  // a NaN stays one
                 sm.meta[j % kMetaSlots][tid] = make_float4(ks, lv, exp2_fast(-lv), 0.f);
             }
 #pragma unroll
             for (int i = 0; i < KP; ++i) {
-                const int r = i * KROWS + k_row, chunk = 2 * k_piece % 8;
-                uint8_t* tile = sm.k[st][k_piece / 4];
-                uint4 a, d;
-                codes_to_half<FMT>(kr[i].x, a.x, a.y);
-                codes_to_half<FMT>(kr[i].y, a.z, a.w);
-                codes_to_half<FMT>(kr[i].z, d.x, d.y);
-                codes_to_half<FMT>(kr[i].w, d.z, d.w);
-                // The second half of a row's lanes start with their second
-                // chunk, so that a row's stores fall into different banks.
-                const bool swap = k_piece >= 4;
-                *reinterpret_cast<uint4*>(tile + swizzled(r, chunk + swap)) = swap ? d : a;
-                *reinterpret_cast<uint4*>(tile + swizzled(r, chunk + !swap)) = swap ? a : d;
+                uint8_t* tile = sm.k[st][i / 4];
+                const int r = 32 * (i & 3) + k_row;
+                uint4 x, y;
+                codes_to_half<FMT>(kr[i].x, x.x, x.y);
+                codes_to_half<FMT>(kr[i].y, x.z, x.w);
+                codes_to_half<FMT>(kr[i].z, y.x, y.y);
+                codes_to_half<FMT>(kr[i].w, y.z, y.w);
+                *reinterpret_cast<uint4*>(tile + swizzled(r, 2 * k_piece)) = x;
+                *reinterpret_cast<uint4*>(tile + swizzled(r, 2 * k_piece + 1)) = y;
             }
             fence_async();
             bar_arrive(&sm.k_full[st]);
@@ -469,10 +530,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             bar_arrive(&sm.v_full[st]);
             load_v(t_next);
         }
-    } else if (warp == 12) {
+    } else {
         // --------------------------------------------------------- the products
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         bool alive = true;
-        if (lane == 0) {
+        if (warp == 12 && lane == 0) {
             constexpr uint32_t qk = mma_desc(128, 128), pv = mma_desc(128, DP);
             auto scores = [&](int tile, int st) {
 #pragma unroll
