@@ -6,16 +6,18 @@
 // split of the tokens 128 at a time. Its warps have roles:
 //
 //   warps 0-3, 4-7  softmax of tile 0 and 1, one thread per row
-//   warps 8-11      K and V: codes from global memory to fp16 in shared
-//                   memory (the conversion is shared by all 256 rows)
-//   warp 12         one thread issues tcgen05.mma
+//   warps 8-11      K, warps 12-15 V: codes from global memory to fp16 in
+//                   shared memory (the conversion is shared by all 256 rows)
+//   warp 16         one thread issues tcgen05.mma
 //
-// S = Q K^T (M 128 rows, N 128 tokens) and O += P V (N head_dim) accumulate
-// in tensor memory: two S tiles and two O tiles fill its 512 columns. P is
-// written as fp16 over its own S and is the A operand of the second product.
-// While one tile's softmax runs, the other tile's products do; the order of
-// the issues (P0 V, Q0 K', P1 V, Q1 K') is the order of execution, so an S
-// that is there tells that the P V before it is done.
+// S = Q K^T (M 128 rows, N 64 tokens at a time) and O += P V (N head_dim)
+// accumulate in tensor memory: two S tiles of 2 x 64 columns and two O tiles
+// fill its 512 columns. P is written as fp16 over its own S and is the A
+// operand of the second product. A tile's softmax works on one half of S
+// while the products of the other half run (with S in one piece it waited
+// for them: 1.43 ms against XXXX for 2048 of 32768 tokens, 32/8 heads, D
+// 128). The order of the issues is the order of execution, so an S that is
+// there tells that the P V before it is done.
 //
 // Shared memory operands are K-major with the 128-byte swizzle: Q and K
 // [row][d], V transposed to [d][token] (eight tokens of a d are paired by byte
@@ -39,7 +41,8 @@ namespace q8 {
 
 constexpr int kChunkRows = 256;    // rows of a CTA
 constexpr int kChunkTokens = 128;  // per step
-constexpr int kChunkThreads = 32 * 16;  // four warpgroups; warps 13-15 only give their registers away
+constexpr int kChunkHalf = 64;     // tokens of one S
+constexpr int kChunkThreads = 32 * 20;  // five warpgroups; warps 17-19 only give their registers away
 constexpr int kMetaSlots = 4;      // K may be written three steps ahead of a softmax
 
 template <int DP>
@@ -48,8 +51,8 @@ struct ChunkSmem {
     uint8_t q[2][DP / 64][128 * 128];
     uint8_t k[2][DP / 64][128 * 128];
     uint8_t v[2][2][DP * 128];
-    float4 meta[kMetaSlots][kChunkTokens / 16];  // K's scale, log2 and reciprocal of V's
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], done;
+    float4 meta[kMetaSlots][kChunkTokens / 16];  // K's scale, log2 and reciprocal of V's, for 16 tokens
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2], done;
     uint32_t tmem;
     int abort;
 };
@@ -77,26 +80,30 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, int parity, volatile int
     return false;
 }
 
-// Descriptor of a K-major operand with the 128-byte swizzle: rows of 128
-// bytes, groups of eight rows 1024 bytes apart.
-__device__ __forceinline__ uint64_t operand_desc(const void* p) {
-    return static_cast<uint64_t>((smem_addr(p) & 0x3FFFF) >> 4) | 1ull << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61;
-}
+// Low word of the descriptor of a K-major operand with the 128-byte swizzle:
+// its address in units of 16 bytes. The high word is the same for all: rows of
+// 128 bytes, groups of eight rows 1024 bytes apart, descriptor version 1.
+__device__ __forceinline__ uint32_t operand_desc(const void* p) { return (smem_addr(p) & 0x3FFFF) >> 4 | 1u << 16; }
 // kind::f16 with fp16 operands, fp32 accumulation, both K-major.
 __device__ __forceinline__ constexpr uint32_t mma_desc(int m, int n) {
     return 1u << 4 | static_cast<uint32_t>(n >> 3) << 17 | static_cast<uint32_t>(m >> 4) << 24;
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, bool add) {
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b),
-        "r"(desc), "r"(static_cast<uint32_t>(add))
+        "{\n.reg .pred p;\n.reg .b64 x, y;\nsetp.ne.u32 p, %4, 0;\nmov.b64 x, {%1, 0x40004040};\nmov.b64 y, {%2, 0x40004040};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(desc), "r"(static_cast<uint32_t>(add))
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, bool add) {
     asm volatile(
-        "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b),
-        "r"(desc), "r"(static_cast<uint32_t>(add))
+        "{\n.reg .pred p;\n.reg .b64 y;\nsetp.ne.u32 p, %4, 0;\nmov.b64 y, {%2, 0x40004040};\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d), "r"(a), "r"(b), "r"(desc), "r"(static_cast<uint32_t>(add))
         : "memory");
+}
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t p;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xFFFFFFFF;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+    return p != 0;
 }
 // The barrier's phase ends when every MMA issued so far has finished.
 __device__ __forceinline__ void mma_commit(uint64_t* bar) {
@@ -193,14 +200,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             bar_init(&sm.v_full[i], 128);
             bar_init(&sm.k_empty[i], 1);
             bar_init(&sm.v_empty[i], 1);
-            bar_init(&sm.s_full[i], 2);
-            bar_init(&sm.p_full[i], 128);
+            bar_init(&sm.pv_done[i], 1);
+            for (int k = 0; k < 2; ++k) {
+                bar_init(&sm.s_full[i][k], 2);
+                bar_init(&sm.p_full[i][k], 128);
+            }
         }
         bar_init(&sm.done, 1);
         sm.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sm.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -253,28 +263,30 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     const uint32_t tmem = sm.tmem;
 
     const bool two = rows > 128;  // with fewer rows the second tile rests
-    // Registers go to where they are needed: 2 x 168 + 104 + 72 = 4 x 128.
+    // Registers go to where they are needed: 2 x 136 + 2 x 80 + 48 = 5 x 96.
     if (warp < 8) {
         // ------------------------------------------------------------ softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         const int tile = warp >> 2;
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes
-        const uint32_t s_at = tmem + tile * 128 + lanes, o_at = tmem + 256 + tile * 128 + lanes;
+        const uint32_t s_tile = tmem + tile * 128 + lanes, o_at = tmem + 256 + tile * 128 + lanes;
         float base = 0.f, l = 0.f;
         bool started = false;
         bool alive = true;
         const int my_steps = tile == 0 || two ? steps : 0;
-        for (int j = 0; j < my_steps && alive; ++j) {
-            const int t0 = t_begin + j * kChunkTokens;
-            const float4* meta = sm.meta[j % kMetaSlots];
-            alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.s_full[tile], j & 1, &sm.abort));
+        for (int i = 0; i < 2 * my_steps && alive; ++i) {
+            const int j = i >> 1, half = i & 1;
+            const int t0 = t_begin + i * kChunkHalf;
+            const float4* meta = sm.meta[j % kMetaSlots] + 4 * half;
+            const uint32_t s_at = s_tile + kChunkHalf * half;
+            alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.s_full[tile][half], j & 1, &sm.abort));
             if (!alive) break;
             fence_after();
-            if (__any_sync(0xFFFFFFFFu, t0 + kChunkTokens > bound)) {
+            if (__any_sync(0xFFFFFFFFu, t0 + kChunkHalf > bound)) {
                 // What a row does not see becomes a score that no factor
                 // brings back.
 #pragma unroll 1
-                for (int g = 0; g < 8; ++g) {
+                for (int g = 0; g < 4; ++g) {
                     uint32_t s[16];
                     tmem_ld16(s, s_at + 16 * g);
                     tmem_wait_ld(s);
@@ -289,7 +301,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                 // The largest t of the row's tokens.
                 float m = -CUDART_INF_F;
 #pragma unroll 1
-                for (int g = 0; g < 8; ++g) {
+                for (int g = 0; g < 4; ++g) {
                     uint32_t s[16];
                     tmem_ld16(s, s_at + 16 * g);
                     const float4 mt = meta[g];
@@ -304,7 +316,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                 }
                 __syncwarp();
             }
-            uint32_t pk[64];
+            uint32_t pk[32];
             float add;
             while (true) {
                 float m = -CUDART_INF_F;
@@ -312,10 +324,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                 uint32_t s[2][16];
                 tmem_ld16(s[0], s_at);
 #pragma unroll
-                for (int g = 0; g < 8; ++g) {
+                for (int g = 0; g < 4; ++g) {
                     uint32_t(&x)[16] = s[g & 1];
                     tmem_wait_ld(x);
-                    if (g < 7) tmem_ld16(s[(g + 1) & 1], s_at + 16 * (g + 1));
+                    if (g < 3) tmem_ld16(s[(g + 1) & 1], s_at + 16 * (g + 1));
                     const float4 mt = meta[g];
                     // A NaN scale has to stay one.
                     const float f0 = factor * mt.x, f = f0 < 1e-30f ? 1e-30f : f0, off = mt.y - base;
@@ -339,7 +351,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                 const float alpha = exp2_fast(-up);
                 base += up;
                 l *= alpha;
-                if (j > 0) {
+                if (i > 0) {
+                    // The last P V of the tile may still be running.
+                    alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.pv_done[tile], (i - 1) & 1, &sm.abort));
+                    if (!alive) break;
+                    fence_after();
 #pragma unroll 1
                     for (int g = 0; g < DP / 16; ++g) {
                         uint32_t o[16];
@@ -353,10 +369,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             }
             l += add;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) tmem_st16(s_at + 16 * g, pk + 16 * g);
+            for (int g = 0; g < 2; ++g) tmem_st16(s_at + 16 * g, pk + 16 * g);
             tmem_wait_st();
             fence_before();
-            bar_arrive(&sm.p_full[tile]);
+            bar_arrive(&sm.p_full[tile][half]);
         }
         // ---------------------------------------------------------- write rows
         alive = __all_sync(0xFFFFFFFFu, alive && bar_wait(&sm.done, 0, &sm.abort));
@@ -404,39 +420,34 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             }
         }
     } else if (warp < 12) {
-        // ---------------------------------------------------- K and V to fp16
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
-        const int tid = threadIdx.x - 256, w = tid >> 5;
-        // K: four lanes a row of a 64-column tile, 32 rows at a time, so that
-        // the stores of eight lanes (two rows, every other chunk) fall into
-        // different banks. V: eight lanes a tile row of 64 tokens, likewise.
-        constexpr int KP = DP / 16;                  // 16-byte pieces per lane and step
-        constexpr int VW = DP / 32;                  // words of a token per lane
+        // ---------------------------------------------------------- K to fp16
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        // Four lanes a row of a 64-column tile, 32 rows at a time: the stores
+        // of eight lanes (two rows, every other chunk) fall into different
+        // banks.
+        const int tid = threadIdx.x - 256;
+        constexpr int KP = DP / 16;  // 16-byte pieces per lane and step
         const int k_row = tid >> 2, k_piece = tid & 3;
-        const int v_tok = 64 * (w & 1) + 8 * (lane & 7), v_d = (w >> 1) * (DP / 2) + (lane >> 3) * (DP / 8);
-        const int v_col = v_d < c.D ? v_d : 0;
         int k_col[DP / 64];
 #pragma unroll
         for (int i = 0; i < DP / 64; ++i) k_col[i] = 64 * i + 16 * k_piece < c.D ? 64 * i + 16 * k_piece : 0;
-        const uint8_t* k_head = c.k.codes + b * c.k.sB + h * c.k.sH;
-        const uint8_t* v_head = c.v.codes + b * c.v.sB + h * c.v.sH + v_col;
+        const uint8_t* head = c.k.codes + b * c.k.sB + h * c.k.sH;
         const int blk_shift = 31 - __clz(c.blk);
         // Every step within one page: one look at the table for all its rows.
         const bool one_page = c.page_shift == 31 || (c.P % kChunkTokens == 0 && t_begin % kChunkTokens == 0);
-        const int64_t k_row32 = 32 * c.k.sT;
+        const int64_t row32 = 32 * c.k.sT;
         uint4 kr[KP];
-        uint32_t vr[8][VW];
         auto load_k = [&](int t0) {
             if (one_page) {
-                int row;
+                int row = 0;
                 const int phys = t0 < t_end ? page_of(c, b, t0, row) : -1;
-                const uint8_t* at = k_head + phys * c.k.sP + (row + k_row) * c.k.sT;
+                const uint8_t* at = head + phys * c.k.sP + (row + k_row) * c.k.sT;
                 const int left = phys >= 0 ? t_end - t0 - k_row : 0;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
 #pragma unroll
                     for (int k = 0; k < DP / 64; ++k) kr[4 * k + i] = load_stream_if(at + k_col[k], 32 * i < left);
-                    at += k_row32;
+                    at += row32;
                 }
             } else {
 #pragma unroll
@@ -446,26 +457,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                     const int phys = t < t_end ? page_of(c, b, t, row) : -1;
 #pragma unroll
                     for (int k = 0; k < DP / 64; ++k)
-                        kr[4 * k + i] = load_stream_if(k_head + phys * c.k.sP + row * c.k.sT + k_col[k], phys >= 0);
+                        kr[4 * k + i] = load_stream_if(head + phys * c.k.sP + row * c.k.sT + k_col[k], phys >= 0);
                 }
-            }
-        };
-        auto load_v = [&](int t0) {
-            const int t = t0 + v_tok;
-            int row = 0;
-            const int phys = t < t_end ? page_of(c, b, t, row) : -1;
-            const uint8_t* at = v_head + phys * c.v.sP + row * c.v.sT;
-            const int left = phys >= 0 ? t_end - t : 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                if (DP == 64) {
-                    const uint2 x = load_stream8_if(at, i < left);
-                    vr[i][0] = x.x; vr[i][1] = x.y;
-                } else {
-                    const uint4 x = load_stream_if(at, i < left);
-                    vr[i][0] = x.x; vr[i][1] = x.y; vr[i][VW - 2] = x.z; vr[i][VW - 1] = x.w;
-                }
-                at += c.v.sT;
             }
         };
         // Read now, looked at when the step comes.
@@ -483,13 +476,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         };
         load_meta(t_begin);
         load_k(t_begin);
-        load_v(t_begin);
-        bool alive = true;
-        for (int j = 0; j < steps && alive; ++j) {
-            const int st = j & 1, t_next = t_begin + (j + 1) * kChunkTokens;
+        for (int j = 0; j < steps; ++j) {
+            const int st = j & 1;
             // The phase before a stage's first use counts as over.
-            alive = bar_wait(&sm.k_empty[st], (j >> 1 & 1) ^ 1, &sm.abort);
-            if (!alive) break;
+            if (!bar_wait(&sm.k_empty[st], (j >> 1 & 1) ^ 1, &sm.abort)) break;
             if (tid < 8) {
                 const float lv = log2_fast(vs < 8.0779357e-28f ? 8.0779357e-28f : vs);  // a NaN stays one
                 sm.meta[j % kMetaSlots][tid] = make_float4(ks, lv, exp2_fast(-lv), 0.f);
@@ -508,10 +498,40 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             }
             fence_async();
             bar_arrive(&sm.k_full[st]);
-            load_meta(t_next);
-            load_k(t_next);
-            alive = bar_wait(&sm.v_empty[st], (j >> 1 & 1) ^ 1, &sm.abort);
-            if (!alive) break;
+            load_meta(t_begin + (j + 1) * kChunkTokens);
+            load_k(t_begin + (j + 1) * kChunkTokens);
+        }
+    } else if (warp < 16) {
+        // ---------------------------------------------------------- V to fp16
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        // Eight lanes take the 64 tokens of a tile row, eight tokens each.
+        const int w = warp & 3;
+        constexpr int VW = DP / 32;  // words of a token per lane
+        const int v_tok = 64 * (w & 1) + 8 * (lane & 7), v_d = (w >> 1) * (DP / 2) + (lane >> 3) * (DP / 8);
+        const uint8_t* head = c.v.codes + b * c.v.sB + h * c.v.sH + (v_d < c.D ? v_d : 0);
+        uint32_t vr[8][VW];
+        auto load_v = [&](int t0) {
+            const int t = t0 + v_tok;
+            int row = 0;
+            const int phys = t < t_end ? page_of(c, b, t, row) : -1;
+            const uint8_t* at = head + phys * c.v.sP + row * c.v.sT;
+            const int left = phys >= 0 ? t_end - t : 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (DP == 64) {
+                    const uint2 x = load_stream8_if(at, i < left);
+                    vr[i][0] = x.x; vr[i][1] = x.y;
+                } else {
+                    const uint4 x = load_stream_if(at, i < left);
+                    vr[i][0] = x.x; vr[i][1] = x.y; vr[i][VW - 2] = x.z; vr[i][VW - 1] = x.w;
+                }
+                at += c.v.sT;
+            }
+        };
+        load_v(t_begin);
+        for (int j = 0; j < steps; ++j) {
+            const int st = j & 1;
+            if (!bar_wait(&sm.v_empty[st], (j >> 1 & 1) ^ 1, &sm.abort)) break;
             uint8_t* tile = sm.v[st][w & 1];
 #pragma unroll
             for (int x = 0; x < VW; ++x) {
@@ -528,61 +548,71 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             }
             fence_async();
             bar_arrive(&sm.v_full[st]);
-            load_v(t_next);
+            load_v(t_begin + (j + 1) * kChunkTokens);
         }
     } else {
         // --------------------------------------------------------- the products
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        bool alive = true;
-        if (warp == 12 && lane == 0) {
-            constexpr uint32_t qk = mma_desc(128, 128), pv = mma_desc(128, DP);
-            auto scores = [&](int tile, int st) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == 16) {
+            // The whole warp goes through the loop, so that addresses stay in
+            // uniform registers; one lane issues.
+            constexpr uint32_t qk = mma_desc(128, kChunkHalf), pv = mma_desc(128, DP);
+            constexpr uint32_t kTile = 128 * 128 / 16, kStage = DP / 64 * kTile, kHalf = kChunkHalf * 128 / 16;
+            constexpr uint32_t vHalf = DP * 128 / 16, vStage = 2 * vHalf;
+            const uint32_t q0 = operand_desc(sm.q), k0 = operand_desc(sm.k), v0 = operand_desc(sm.v);
+            const bool lead = elect_lane();
+            auto scores = [&](int tile, int half, int st) {
+                const uint32_t d = tmem + tile * 128 + half * kChunkHalf, a = q0 + tile * kStage, x = k0 + st * kStage + half * kHalf;
+                if (lead) {
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k)
-                    mma_ss(tmem + tile * 128, operand_desc(sm.q[tile][k / 4]) + k % 4 * 2, operand_desc(sm.k[st][k / 4]) + k % 4 * 2, qk, k > 0);
-                mma_commit(&sm.s_full[tile]);
-                bar_arrive(&sm.s_full[tile]);  // hands on what k_full has shown: the block scales
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint32_t off = k / 4 * kTile + k % 4 * 2;
+                        mma_ss(d, a + off, x + off, qk, k > 0);
+                    }
+                    mma_commit(&sm.s_full[tile][half]);
+                    bar_arrive(&sm.s_full[tile][half]);  // hands on what k_full has shown: the block scales
+                }
             };
-            auto values = [&](int tile, int st, bool add) {
+            auto values = [&](int tile, int half, int st, bool add) {
+                const uint32_t d = tmem + 256 + tile * 128, a = tmem + tile * 128 + half * kChunkHalf, x = v0 + st * vStage + half * vHalf;
+                if (lead) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    mma_ts(tmem + 256 + tile * 128, tmem + tile * 128 + 8 * k, operand_desc(sm.v[st][k / 4]) + k % 4 * 2, pv, add || k > 0);
+                    for (int k = 0; k < kChunkHalf / 16; ++k) mma_ts(d, a + 8 * k, x + 2 * k, pv, add || k > 0);
+                    mma_commit(&sm.pv_done[tile]);
+                }
             };
-            alive = bar_wait(&sm.k_full[0], 0, &sm.abort);
+            const int tiles_here = two ? 2 : 1;
+            bool alive = bar_wait(&sm.k_full[0], 0, &sm.abort);
+            alive = __all_sync(0xFFFFFFFFu, alive);
             if (alive) {
                 fence_after();
-                scores(0, 0);
-                if (two) scores(1, 0);
-                mma_commit(&sm.k_empty[0]);
+                for (int half = 0; half < 2; ++half)
+                    for (int tile = 0; tile < tiles_here; ++tile) scores(tile, half, 0);
+                if (lead) mma_commit(&sm.k_empty[0]);
             }
             for (int j = 0; j < steps && alive; ++j) {
                 const int st = j & 1, nx = st ^ 1;
                 const bool more = j + 1 < steps;
-                alive = bar_wait(&sm.v_full[st], j >> 1 & 1, &sm.abort) && bar_wait(&sm.p_full[0], j & 1, &sm.abort);
+                alive = bar_wait(&sm.v_full[st], j >> 1 & 1, &sm.abort);
+                if (more) alive = bar_wait(&sm.k_full[nx], (j + 1) >> 1 & 1, &sm.abort) && alive;
+                for (int i = 0; i < 4; ++i) {
+                    const int half = i >> 1, tile = i & 1;
+                    if (tile >= tiles_here) continue;
+                    alive = __all_sync(0xFFFFFFFFu, alive && bar_wait(&sm.p_full[tile][half], j & 1, &sm.abort));
+                    if (!alive) break;
+                    fence_after();
+                    values(tile, half, st, j > 0 || half > 0);
+                    if (more) scores(tile, half, nx);
+                }
                 if (!alive) break;
-                fence_after();
-                values(0, st, j > 0);
-                if (more) {
-                    alive = bar_wait(&sm.k_full[nx], (j + 1) >> 1 & 1, &sm.abort);
-                    if (!alive) break;
-                    fence_after();
-                    scores(0, nx);
-                }
-                if (two) {
-                    alive = bar_wait(&sm.p_full[1], j & 1, &sm.abort);
-                    if (!alive) break;
-                    fence_after();
-                    values(1, st, j > 0);
-                }
-                mma_commit(&sm.v_empty[st]);
-                if (more) {
-                    if (two) scores(1, nx);
-                    mma_commit(&sm.k_empty[nx]);
+                if (lead) {
+                    mma_commit(&sm.v_empty[st]);
+                    if (more) mma_commit(&sm.k_empty[nx]);
                 }
             }
             // Also after giving up: nothing may be in flight when the tensor
             // memory is given back.
-            mma_commit(&sm.done);
+            if (lead) mma_commit(&sm.done);
             int none = 0;
             bar_wait(&sm.done, 0, &none);
         }
@@ -590,7 +620,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     }
     fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
         if (lane == 0 && sm.abort) report(c.status, AKV_ERR_TIMEOUT);
