@@ -10,14 +10,14 @@
 //                   shared memory (the conversion is shared by all 256 rows)
 //   warp 16         one thread issues tcgen05.mma
 //
-// S = Q K^T (M 128 rows, N 64 tokens at a time) and O += P V (N head_dim)
-// accumulate in tensor memory: two S tiles of 2 x 64 columns and two O tiles
-// fill its 512 columns. P is written as fp16 over its own S and is the A
-// operand of the second product. A tile's softmax works on one half of S
-// while the products of the other half run (with S in one piece it waited
-// for them: 1.43 ms against XXXX for 2048 of 32768 tokens, 32/8 heads, D
-// 128). The order of the issues is the order of execution, so an S that is
-// there tells that the P V before it is done.
+// S = Q K^T (M 128 rows, N 128 tokens) and O += P V (N head_dim) accumulate
+// in tensor memory: two S tiles and two O tiles fill its 512 columns. P is
+// written as fp16 over its own S, 64 tokens at a time, and is the A operand of
+// the second product. While one tile's softmax runs, the other tile's products
+// do. The order of the issues is the order of execution, so an S that is there
+// tells that the P V before it is done. (With S in two pieces of 64 tokens,
+// each computed while the softmax worked on the other, the products took
+// longer than that saved: from shared memory, N 64 costs what N 128 does.)
 //
 // Shared memory operands are K-major with the 128-byte swizzle: Q and K
 // [row][d], V transposed to [d][token] (eight tokens of a d are paired by byte
@@ -41,7 +41,7 @@ namespace q8 {
 
 constexpr int kChunkRows = 256;    // rows of a CTA
 constexpr int kChunkTokens = 128;  // per step
-constexpr int kChunkHalf = 64;     // tokens of one S
+constexpr int kChunkHalf = 64;     // P goes to the tensor cores in two parts
 constexpr int kChunkThreads = 32 * 20;  // five warpgroups; warps 17-19 only give their registers away
 constexpr int kMetaSlots = 4;      // K may be written three steps ahead of a softmax
 
@@ -52,7 +52,7 @@ struct ChunkSmem {
     uint8_t k[2][DP / 64][128 * 128];
     uint8_t v[2][2][DP * 128];
     float4 meta[kMetaSlots][kChunkTokens / 16];  // K's scale, log2 and reciprocal of V's, for 16 tokens
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2][2], p_full[2][2], pv_done[2], done;
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], pv_done[2], done;
     uint32_t tmem;
     int abort;
 };
@@ -201,10 +201,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             bar_init(&sm.k_empty[i], 1);
             bar_init(&sm.v_empty[i], 1);
             bar_init(&sm.pv_done[i], 1);
-            for (int k = 0; k < 2; ++k) {
-                bar_init(&sm.s_full[i][k], 2);
-                bar_init(&sm.p_full[i][k], 128);
-            }
+            bar_init(&sm.s_full[i], 2);
+            bar_init(&sm.p_full[i][0], 128);
+            bar_init(&sm.p_full[i][1], 128);
         }
         bar_init(&sm.done, 1);
         sm.abort = 0;
@@ -279,9 +278,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             const int t0 = t_begin + i * kChunkHalf;
             const float4* meta = sm.meta[j % kMetaSlots] + 4 * half;
             const uint32_t s_at = s_tile + kChunkHalf * half;
-            alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.s_full[tile][half], j & 1, &sm.abort));
-            if (!alive) break;
-            fence_after();
+            if (half == 0) {
+                alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.s_full[tile], j & 1, &sm.abort));
+                if (!alive) break;
+                fence_after();
+            }
             if (__any_sync(0xFFFFFFFFu, t0 + kChunkHalf > bound)) {
                 // What a row does not see becomes a score that no factor
                 // brings back.
@@ -556,21 +557,21 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         if (warp == 16) {
             // The whole warp goes through the loop, so that addresses stay in
             // uniform registers; one lane issues.
-            constexpr uint32_t qk = mma_desc(128, kChunkHalf), pv = mma_desc(128, DP);
-            constexpr uint32_t kTile = 128 * 128 / 16, kStage = DP / 64 * kTile, kHalf = kChunkHalf * 128 / 16;
+            constexpr uint32_t qk = mma_desc(128, kChunkTokens), pv = mma_desc(128, DP);
+            constexpr uint32_t kTile = 128 * 128 / 16, kStage = DP / 64 * kTile;
             constexpr uint32_t vHalf = DP * 128 / 16, vStage = 2 * vHalf;
             const uint32_t q0 = operand_desc(sm.q), k0 = operand_desc(sm.k), v0 = operand_desc(sm.v);
             const bool lead = elect_lane();
-            auto scores = [&](int tile, int half, int st) {
-                const uint32_t d = tmem + tile * 128 + half * kChunkHalf, a = q0 + tile * kStage, x = k0 + st * kStage + half * kHalf;
+            auto scores = [&](int tile, int st) {
+                const uint32_t d = tmem + tile * 128, a = q0 + tile * kStage, x = k0 + st * kStage;
                 if (lead) {
 #pragma unroll
                     for (int k = 0; k < DP / 16; ++k) {
                         const uint32_t off = k / 4 * kTile + k % 4 * 2;
                         mma_ss(d, a + off, x + off, qk, k > 0);
                     }
-                    mma_commit(&sm.s_full[tile][half]);
-                    bar_arrive(&sm.s_full[tile][half]);  // hands on what k_full has shown: the block scales
+                    mma_commit(&sm.s_full[tile]);
+                    bar_arrive(&sm.s_full[tile]);  // hands on what k_full has shown: the block scales
                 }
             };
             auto values = [&](int tile, int half, int st, bool add) {
@@ -586,8 +587,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             alive = __all_sync(0xFFFFFFFFu, alive);
             if (alive) {
                 fence_after();
-                for (int half = 0; half < 2; ++half)
-                    for (int tile = 0; tile < tiles_here; ++tile) scores(tile, half, 0);
+                for (int tile = 0; tile < tiles_here; ++tile) scores(tile, 0);
                 if (lead) mma_commit(&sm.k_empty[0]);
             }
             for (int j = 0; j < steps && alive; ++j) {
@@ -596,13 +596,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                 alive = bar_wait(&sm.v_full[st], j >> 1 & 1, &sm.abort);
                 if (more) alive = bar_wait(&sm.k_full[nx], (j + 1) >> 1 & 1, &sm.abort) && alive;
                 for (int i = 0; i < 4; ++i) {
-                    const int half = i >> 1, tile = i & 1;
+                    const int tile = i >> 1, half = i & 1;
                     if (tile >= tiles_here) continue;
                     alive = __all_sync(0xFFFFFFFFu, alive && bar_wait(&sm.p_full[tile][half], j & 1, &sm.abort));
                     if (!alive) break;
                     fence_after();
                     values(tile, half, st, j > 0 || half > 0);
-                    if (more) scores(tile, half, nx);
+                    if (more && half == 1) scores(tile, nx);
                 }
                 if (!alive) break;
                 if (lead) {
