@@ -121,13 +121,14 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
     a.split = d->split_tokens;
     const int group = a.chunk ? kChunkRows : 8 * a.nt;  // rows of a CTA
     if (a.split == 0 && a.chunk) {
-        // One CTA per SM: the number of splits (up to eight) whose last wave
-        // is fullest; each costs a partial to write and read again.
+        // One CTA per SM: the number of splits whose last wave is fullest, up
+        // to eight or one wave; each costs a partial to write and read again.
         const int64_t units = bh * ((a.rows + group - 1) / group), sms = sm_count();
         const int64_t steps = (static_cast<int64_t>(c.max_tokens) + kChunkTokens - 1) / kChunkTokens;
+        const int64_t most = units > 0 && sms / units > 8 ? sms / units : 8;
         int64_t best = 1;
         double least = 0;
-        for (int64_t n = 1; n <= 8 && n * 4 <= steps + 3; ++n) {
+        for (int64_t n = 1; n <= most && n * 4 <= steps + 3; ++n) {
             const double waves = static_cast<double>((units * n + sms - 1) / sms) * ((steps + n - 1) / n) * (n > 1 ? 1.02 + 0.01 * n : 1.0);
             if (n == 1 || waves < least) {
                 best = n;
@@ -151,6 +152,7 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
         a.split *= 2;
         a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);
     }
+    if (a.chunk && a.rows <= 128) a.nsplits *= 2;  // its two tiles share the rows and take every other step
     const auto up = [](size_t x) { return (x + 15) / 16 * 16; };
     const size_t parts = static_cast<size_t>(bh) * a.nsplits * a.rows;
     a.part_ml = 0;
@@ -178,22 +180,24 @@ void launch_step(const AttnParams& p, int nt, cudaStream_t s) {
     else nt == 2 ? launch_step<FMT, 64, 2>(p, s) : launch_step<FMT, 64, 1>(p, s);
 }
 
-template <int FMT, int DP>
+template <int FMT, int DP, bool SHARED>
 int launch_chunk(const AttnParams& p, cudaStream_t s) {
-    const auto kern = chunk_kernel<FMT, DP>;
+    const auto kern = chunk_kernel<FMT, DP, SHARED>;
     constexpr int bytes = sizeof(ChunkSmem<DP>) + 1024;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
         cudaGetLastError();
         return AKV_ERR_CUDA;
     }
-    const dim3 grid(p.nsplits * ((p.R + kChunkRows - 1) / kChunkRows), p.c.H, p.c.B);
+    const int parts = SHARED ? p.nsplits / 2 : p.nsplits;
+    const dim3 grid(parts * ((p.R + kChunkRows - 1) / kChunkRows), p.c.H, p.c.B);
     kern<<<grid, kChunkThreads, bytes, s>>>(p);
     return launched();
 }
 
 template <int FMT>
 int launch_chunk(const AttnParams& p, cudaStream_t s) {
-    return p.c.D > 64 ? launch_chunk<FMT, 128>(p, s) : launch_chunk<FMT, 64>(p, s);
+    if (p.R <= 128) return p.c.D > 64 ? launch_chunk<FMT, 128, true>(p, s) : launch_chunk<FMT, 64, true>(p, s);
+    return p.c.D > 64 ? launch_chunk<FMT, 128, false>(p, s) : launch_chunk<FMT, 64, false>(p, s);
 }
 
 template <int FMT, int DP>

@@ -116,13 +116,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t (&x)[16], uint32_t at) {
           "=r"(x[10]), "=r"(x[11]), "=r"(x[12]), "=r"(x[13]), "=r"(x[14]), "=r"(x[15])
         : "r"(at) : "memory");
 }
-__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* x) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(x[0]),
-        "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]), "r"(x[11]),
-        "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15])
-        : "memory");
-}
 // Ends the loads in flight; x is one of them and must not be used before.
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&x)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -130,6 +123,13 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&x)[16]) {
                    "+r"(x[10]), "+r"(x[11]), "+r"(x[12]), "+r"(x[13]), "+r"(x[14]), "+r"(x[15])
                  :
                  : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* x) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(at), "r"(x[0]),
+        "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]), "r"(x[11]),
+        "r"(x[12]), "r"(x[13]), "r"(x[14]), "r"(x[15])
+        : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -162,7 +162,9 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // Byte offset of 16-byte chunk c of row r in a swizzled tile.
 __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
 
-template <int FMT, int DP>
+// SHARED: 128 rows or fewer a kv head; both tiles take the same rows and every
+// other step, as two splits.
+template <int FMT, int DP, bool SHARED>
 __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     using Smem = ChunkSmem<DP>;
     extern __shared__ uint8_t smem_raw[];
@@ -172,10 +174,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int tiles = (p.R + kChunkRows - 1) / kChunkRows;
     // Later rows see more tokens: they go first.
-    const int split = blockIdx.x % p.nsplits, r0 = (tiles - 1 - blockIdx.x / p.nsplits) * kChunkRows, h = blockIdx.y, b = blockIdx.z;
+    const int parts = SHARED ? p.nsplits / 2 : p.nsplits;  // CTAs along the tokens
+    const int split = blockIdx.x % parts, r0 = (tiles - 1 - blockIdx.x / parts) * kChunkRows, h = blockIdx.y, b = blockIdx.z;
     const int len = len_of(p, b), qlen = q_len_of(p, b), rows = min(kChunkRows, p.R - r0);
     const int bh = b * c.H + h;
-    const int64_t unit = (static_cast<int64_t>(bh) * p.nsplits + split) * p.R + r0;
+    const int64_t unit = (static_cast<int64_t>(bh) * p.nsplits + (SHARED ? 2 * split : split)) * p.R + r0;
     const int end = r0 / p.G < qlen ? seen_by(p, min((r0 + rows - 1) / p.G, qlen - 1), len, qlen) : 0;
     const int t_begin = split * p.split, t_end = min(t_begin + p.split, end);
     const int steps = t_end > t_begin ? (t_end - t_begin + kChunkTokens - 1) / kChunkTokens : 0;
@@ -183,6 +186,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         // Nothing to see for any row.
         for (int i = threadIdx.x; i < rows; i += kChunkThreads) {
             p.part_ml[unit + i] = make_float2(-CUDART_INF_F, 0.f);
+            if (SHARED) p.part_ml[unit + p.R + i] = make_float2(-CUDART_INF_F, 0.f);
             if (p.nsplits > 1) continue;
             const int64_t row = out_row(p, b, h, r0 + i);
             if (p.lse) p.lse[row] = -CUDART_INF_F;
@@ -217,9 +221,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     // Query rows: thread = row, to fp16 after a power of two.
     float factor = 0.f;
     int bound = 0;
+    bool blind = true;
     if (warp < 8) {
-        const int tile = warp >> 2, r = threadIdx.x & 127, row = r0 + threadIdx.x;
-        const bool in = static_cast<int>(threadIdx.x) < rows;
+        const int tile = warp >> 2, r = threadIdx.x & 127, at_row = SHARED ? r : threadIdx.x, row = r0 + at_row;
+        const bool in = at_row < rows;
         const int64_t at = in ? q_row(p, b, h, row) : 0;
         uint32_t top = 0;
         if (in) {
@@ -253,7 +258,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             }
         }
         factor = p.c2 * power_of_two(-e);
-        bound = in ? seen_by(p, row / p.G, len, qlen) : 0;
+        // A row without tokens goes along unmasked and is dropped at the end.
+        const int seen = in ? seen_by(p, row / p.G, len, qlen) : 0;
+        blind = seen == 0;
+        bound = blind ? INT_MAX : seen;
         fence_async();
     }
     fence_before();
@@ -261,7 +269,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     fence_after();
     const uint32_t tmem = sm.tmem;
 
-    const bool two = rows > 128;  // with fewer rows the second tile rests
+    // Steps of a tile: all, or every other one.
+    const bool two = SHARED || rows > 128;  // else the second tile rests
     // Registers go to where they are needed: 2 x 136 + 2 x 80 + 48 = 5 x 96.
     if (warp < 8) {
         // ------------------------------------------------------------ softmax
@@ -272,14 +281,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         float base = 0.f, l = 0.f;
         bool started = false;
         bool alive = true;
-        const int my_steps = tile == 0 || two ? steps : 0;
+        const int my_steps = SHARED ? (steps + 1 - tile) / 2 : tile == 0 || two ? steps : 0;
         for (int i = 0; i < 2 * my_steps && alive; ++i) {
-            const int j = i >> 1, half = i & 1;
-            const int t0 = t_begin + i * kChunkHalf;
+            const int turn = i >> 1, half = i & 1, j = SHARED ? 2 * turn + tile : turn;
+            const int t0 = t_begin + j * kChunkTokens + half * kChunkHalf;
             const float4* meta = sm.meta[j % kMetaSlots] + 4 * half;
             const uint32_t s_at = s_tile + kChunkHalf * half;
             if (half == 0) {
-                alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.s_full[tile], j & 1, &sm.abort));
+                alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.s_full[tile], turn & 1, &sm.abort));
                 if (!alive) break;
                 fence_after();
             }
@@ -378,9 +387,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         // ---------------------------------------------------------- write rows
         alive = __all_sync(0xFFFFFFFFu, alive && bar_wait(&sm.done, 0, &sm.abort));
         fence_after();
-        const bool in = static_cast<int>(threadIdx.x) < rows;
-        const int r = r0 + threadIdx.x;
-        const bool none = !started && !isnan(l);
+        const int my_row = SHARED ? threadIdx.x & 127 : threadIdx.x;
+        const bool in = my_row < rows;
+        const int r = r0 + my_row;
+        const int64_t part = unit + my_row + (SHARED && tile ? p.R : 0);
+        const bool none = blind || (!started && !isnan(l));
         const float inv = none ? 0.f : 1.f / l;
         const int64_t row = in ? out_row(p, b, h, r) : 0;
 #pragma unroll 1
@@ -390,7 +401,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             tmem_wait_ld(o);
             if (!in || 16 * g >= c.D || !alive) {
             } else if (p.nsplits > 1) {
-                uint4* to = reinterpret_cast<uint4*>(p.part_o + (unit + threadIdx.x) * c.D + 16 * g);
+                uint4* to = reinterpret_cast<uint4*>(p.part_o + part * c.D + 16 * g);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) to[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
             } else {
@@ -413,9 +424,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         }
         if (in) {
             if (!alive) l = CUDART_NAN_F;
-            p.part_ml[unit + threadIdx.x] = make_float2(isnan(l) ? l : none ? -CUDART_INF_F : base, l);
+            p.part_ml[part] = make_float2(none ? -CUDART_INF_F : isnan(l) ? l : base, l);
             if (p.nsplits == 1) {
-                const float lse = isnan(l) ? l : none ? -CUDART_INF_F : base + log2f(l);
+                const float lse = none ? -CUDART_INF_F : isnan(l) ? l : base + log2f(l);
                 if (p.lse) p.lse[row] = lse;
                 if (p.lse_out) p.lse_out[row] = lse * 0.69314718055994531f;
             }
@@ -583,26 +594,37 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                 }
             };
             const int tiles_here = two ? 2 : 1;
-            bool alive = bar_wait(&sm.k_full[0], 0, &sm.abort);
-            alive = __all_sync(0xFFFFFFFFu, alive);
-            if (alive) {
+            bool alive = true;
+            // A tile's first scores; with both tiles on the same rows, the
+            // second tile's are those of step 1.
+            for (int tile = 0; tile < tiles_here && alive; ++tile) {
+                const int st = SHARED ? tile : 0;
+                if (SHARED && tile >= steps) break;
+                alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.k_full[st], 0, &sm.abort));
+                if (!alive) break;
                 fence_after();
-                for (int tile = 0; tile < tiles_here; ++tile) scores(tile, 0);
-                if (lead) mma_commit(&sm.k_empty[0]);
+                scores(tile, st);
+                if (lead && (SHARED || tile == tiles_here - 1)) mma_commit(&sm.k_empty[st]);
             }
             for (int j = 0; j < steps && alive; ++j) {
-                const int st = j & 1, nx = st ^ 1;
-                const bool more = j + 1 < steps;
+                // The step after this one of the same tiles.
+                const int st = j & 1, next = SHARED ? j + 2 : j + 1, nx = next & 1, turn = SHARED ? j >> 1 : j;
+                const bool more = next < steps;
                 alive = bar_wait(&sm.v_full[st], j >> 1 & 1, &sm.abort);
-                if (more) alive = bar_wait(&sm.k_full[nx], (j + 1) >> 1 & 1, &sm.abort) && alive;
-                for (int i = 0; i < 4; ++i) {
+                if (more && !SHARED) alive = bar_wait(&sm.k_full[nx], next >> 1 & 1, &sm.abort) && alive;
+                for (int i = SHARED ? 2 * st : 0; i < (SHARED ? 2 * st + 2 : 2 * tiles_here); ++i) {
                     const int tile = i >> 1, half = i & 1;
-                    if (tile >= tiles_here) continue;
-                    alive = __all_sync(0xFFFFFFFFu, alive && bar_wait(&sm.p_full[tile][half], j & 1, &sm.abort));
+                    alive = __all_sync(0xFFFFFFFFu, alive && bar_wait(&sm.p_full[tile][half], turn & 1, &sm.abort));
                     if (!alive) break;
                     fence_after();
-                    values(tile, half, st, j > 0 || half > 0);
-                    if (more && half == 1) scores(tile, nx);
+                    values(tile, half, st, turn > 0 || half > 0);
+                    if (!more || half == 0) continue;
+                    if (SHARED) {
+                        alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.k_full[nx], next >> 1 & 1, &sm.abort));
+                        if (!alive) break;
+                        fence_after();
+                    }
+                    scores(tile, nx);
                 }
                 if (!alive) break;
                 if (lead) {
