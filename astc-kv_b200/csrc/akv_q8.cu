@@ -94,16 +94,16 @@ struct AttnPlan {
     int rows;         // per kv head
     bool chunk;       // the tcgen05 kernel, else the step kernel
     int nt;           // groups of eight rows per CTA
-    int split, nsplits;
+    int split, nsplits;          // chunk kernel
+    int share_ctas, share_min;   // step kernel
     bool keep_scores; // the step kernel stores its scores for the token weights
     size_t part_ml, part_o, scores, lse, bytes;  // offsets into the workspace, and its size
 };
 
-constexpr int kSplitAlign = 16 * kStepWarps;
+static_assert(kShareTokens == 16 * kStepWarps, "a tile of 16 tokens for each warp");
 // Rows from which the tcgen05 kernel, whose CTA does 128 or 256 rows for the
 // price of one, is ahead of the step kernel, which does 16.
 constexpr int kChunkMinRows = 33;
-constexpr int kMinSplit = 64, kMaxSplit = 4096;
 
 // Rows whose scores are stored for the token weights rather than computed
 // again: storing costs 8 bytes per row and token, a second pass over K
@@ -111,7 +111,7 @@ constexpr int kMinSplit = 64, kMaxSplit = 4096;
 constexpr int kScoreRows = 16;
 
 AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
-    AttnPlan a;
+    AttnPlan a = {};
     const AkvQ8Cache& c = d->cache;
     const int64_t bh = static_cast<int64_t>(c.batch) * c.kv_heads;
     a.rows = d->q_tokens * (d->q_heads / c.kv_heads);
@@ -136,36 +136,40 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
             }
         }
         a.split = static_cast<int>((steps + best - 1) / best * kChunkTokens);
-    } else if (a.split == 0) {
-        // One wave of CTAs where that makes splits of at most kMaxSplit
-        // tokens, else splits of that length, several waves of them (lengths
-        // may be ragged, and are not known here).
-        const int64_t units = bh * ((a.rows + group - 1) / group);
-        const int64_t slots = static_cast<int64_t>(sm_count()) * (c.head_dim > 128 || a.nt == 2 ? 2 : 4);
-        const int64_t want = units > 0 && slots > units ? slots / units : 1;
-        const int64_t per = ((c.max_tokens + want - 1) / want + kSplitAlign - 1) / kSplitAlign * kSplitAlign;
-        a.split = static_cast<int>(per < kMinSplit ? kMinSplit : per > kMaxSplit ? kMaxSplit : per);
     }
-    a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);
-    const int64_t most = 0x7FFFFFFF / ((a.rows + group - 1) / group + 1);
-    while (a.nsplits > most) {  // the grid holds splits x row groups
-        a.split *= 2;
+    size_t parts;  // rows of partials
+    if (a.chunk) {
         a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);
+        const int64_t limit = 0x7FFFFFFF / ((a.rows + group - 1) / group + 1);
+        while (a.nsplits > limit) {  // the grid holds splits x row groups
+            a.split *= 2;
+            a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);
+        }
+        if (a.rows <= 128) a.nsplits *= 2;  // its two tiles share the rows and take every other step
+        parts = a.nsplits > 1 ? static_cast<size_t>(bh) * a.nsplits * a.rows : 0;
+    } else {
+        // One wave of CTAs (see the step kernel), two pieces each; no more
+        // CTAs than there can be chunks.
+        const int64_t chunks = bh * ((a.rows + group - 1) / group) * ((c.max_tokens + kShareTokens - 1) / kShareTokens);
+        const int64_t slots = static_cast<int64_t>(sm_count()) * (c.head_dim > 128 || a.nt == 2 ? 2 : 4);
+        a.share_min = a.split > kShareTokens ? a.split / kShareTokens : 1;
+        const int64_t ctas = chunks / a.share_min < slots ? chunks / a.share_min : slots;
+        a.share_ctas = static_cast<int>(ctas > 0 ? ctas : 1);
+        a.nsplits = 0;
+        parts = 2 * static_cast<size_t>(a.share_ctas) * group;
     }
-    if (a.chunk && a.rows <= 128) a.nsplits *= 2;  // its two tiles share the rows and take every other step
     const auto up = [](size_t x) { return (x + 15) / 16 * 16; };
-    const size_t parts = static_cast<size_t>(bh) * a.nsplits * a.rows;
     a.part_ml = 0;
     a.part_o = up(parts * sizeof(float2));
-    a.scores = a.part_o + (a.nsplits > 1 ? up(parts * c.head_dim * sizeof(float)) : 0);
+    a.scores = a.part_o + up(parts * c.head_dim * sizeof(float));
     a.lse = a.scores + (a.keep_scores ? up(static_cast<size_t>(bh) * c.max_tokens * a.rows * sizeof(float)) : 0);
-    a.bytes = a.lse + (d->weights_dev && !a.keep_scores ? up(static_cast<size_t>(c.batch) * d->q_tokens * d->q_heads * sizeof(float)) : 0) + 16;
+    a.bytes = a.lse + (d->weights_dev ? up(static_cast<size_t>(c.batch) * d->q_tokens * d->q_heads * sizeof(float)) : 0) + 16;
     return a;
 }
 
 template <int FMT, int DP, int NT>
 void launch_step(const AttnParams& p, cudaStream_t s) {
-    const dim3 grid(p.nsplits * ((p.R + 8 * NT - 1) / (8 * NT)), p.c.H, p.c.B);
+    const int grid = p.share_ctas;
     const bool plo = p.out_dtype == AKV_Q_F32, qlo = p.q_dtype == AKV_Q_F32;
     if (plo && qlo) step_kernel<FMT, DP, NT, true, true><<<grid, kStepThreads, 0, s>>>(p);
     else if (plo) step_kernel<FMT, DP, NT, true, false><<<grid, kStepThreads, 0, s>>>(p);
@@ -320,10 +324,11 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     p.q = d->q_dev; p.qB = d->q_stride[0]; p.qT = d->q_stride[1]; p.qH = d->q_stride[2];
     p.lens = d->seq_lens_dev; p.q_lens = d->q_lens_dev;
     p.split = plan.split; p.nsplits = plan.nsplits;
+    p.share_ctas = plan.chunk ? 0 : plan.share_ctas; p.share_min = plan.share_min; p.row_group = 8 * plan.nt;
     p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
     p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     p.scores = plan.keep_scores ? reinterpret_cast<float*>(ws + plan.scores) : nullptr;
-    p.lse = d->weights_dev && !plan.keep_scores ? reinterpret_cast<float*>(ws + plan.lse) : nullptr;
+    p.lse = d->weights_dev ? reinterpret_cast<float*>(ws + plan.lse) : nullptr;
     p.out = d->out_dev; p.lse_out = d->lse_dev;
     p.weights = d->weights_dev; p.wstride = d->weights_stride;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -334,7 +339,9 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
         int8 ? launch_step<AKV_Q8_INT8>(p, plan.nt, s) : launch_step<AKV_Q8_E4M3>(p, plan.nt, s);
         if (int st = launched()) return st;
     }
-    const int64_t rows = plan.nsplits > 1 ? static_cast<int64_t>(p.c.B) * p.c.H * p.R : 0;
+    // A step kernel of one CTA leaves nothing to combine.
+    const bool combine = plan.chunk ? plan.nsplits > 1 : plan.share_ctas > 1;
+    const int64_t rows = combine ? static_cast<int64_t>(p.c.B) * p.c.H * p.R : 0;
     const int wblocks = plan.keep_scores ? (p.c.T + kWeightTokens - 1) / kWeightTokens : 0;
     const int64_t blocks = rows + static_cast<int64_t>(p.c.B) * p.c.H * wblocks;
     if (blocks > 0x7FFFFFFF) return AKV_ERR_UNSUPPORTED;

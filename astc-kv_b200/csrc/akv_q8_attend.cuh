@@ -21,9 +21,14 @@ struct AttnParams {
     int64_t qB, qT, qH;         // elements
     const int32_t* lens;
     const int32_t* q_lens;
+    // Partials: of the chunk kernel [B][H][nsplits][R] rows, of the step
+    // kernel two pieces for each CTA, row_group rows each (see Parts).
     int split, nsplits;         // tokens per split
-    float* part_o;              // [B][H][nsplits][R][D]
-    float2* part_ml;            // [B][H][nsplits][R]
+    int share_ctas;             // CTAs of the step kernel, 0 for the chunk kernel
+    int share_min;              // chunks that a share has at least
+    int row_group;
+    float* part_o;              // ... [D], weighted by 2^-base
+    float2* part_ml;            // base (-inf: nothing seen), sum
     float* scores;              // [B][H][T][R], base 2, or NULL
     void* out;
     float* lse;                 // [B][n][Hq], base 2, or NULL
@@ -186,12 +191,126 @@ __device__ __forceinline__ uint2 load_stream8_if(const void* p, bool in) {
 constexpr int kCombineThreads = 256;
 constexpr int kWeightTokens = 512;   // per CTA of the weights part
 
-// Base-2 log-sum-exp of row r over the splits, by one warp; all lanes get it.
-__device__ __forceinline__ float combined_lse(const float2* ml, int nsplits, int R) {
+// ------------------------------------------------- the step kernel's shares
+
+constexpr int kShareTokens = 64;
+
+// 64-token chunks of each (kv head, row group) of sequence b.
+__device__ __forceinline__ int share_chunks(const AttnParams& p, int b) {
+    return q_len_of(p, b) > 0 ? (len_of(p, b) + kShareTokens - 1) / kShareTokens : 0;
+}
+
+// CTA i does chunks [start(i), start(i + 1)) of all, counted by sequence, kv
+// head and row group, and along the tokens.
+struct Shares {
+    int64_t chunks;
+    int ctas;
+    __device__ __forceinline__ int64_t start(int i) const { return i * chunks / ctas; }
+    __device__ __forceinline__ int owner(int64_t chunk) const { return static_cast<int>(((chunk + 1) * ctas + chunks - 1) / chunks) - 1; }
+};
+__device__ __forceinline__ Shares make_shares(const AttnParams& p, int64_t chunks) {
+    const int64_t most = chunks / p.share_min;
+    return {chunks, static_cast<int>(max(static_cast<int64_t>(1), min(most, static_cast<int64_t>(p.share_ctas))))};
+}
+
+struct ShareScratch {
+    int64_t sums[32];
+    int64_t before;
+    int b;
+};
+
+// Counts all chunks with the whole CTA (ctas 0 when there are none).
+__device__ __forceinline__ Shares count_shares(const AttnParams& p, int units, ShareScratch& sh) {
+    int64_t n = 0;
+    for (int b = threadIdx.x; b < p.c.B; b += blockDim.x) n += share_chunks(p, b);
+    for (int o = 16; o; o >>= 1) n += __shfl_xor_sync(0xFFFFFFFFu, n, o);
+    if ((threadIdx.x & 31) == 0) sh.sums[threadIdx.x >> 5] = n;
+    __syncthreads();
+    n = 0;
+    for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) n += sh.sums[w];
+    Shares s = make_shares(p, n * units);
+    if (n == 0) s.ctas = 0;
+    return s;
+}
+
+// The sequence that chunk `at` belongs to, and the chunks before it.
+__device__ __forceinline__ int find_sequence(const AttnParams& p, int64_t at, int units, ShareScratch& sh, int64_t& before) {
+    const int lane = threadIdx.x & 31;
+    if (threadIdx.x < 32) {
+        int64_t done = 0;
+        bool found = false;
+        for (int b0 = 0; b0 < p.c.B && !found; b0 += 32) {
+            const int64_t n = b0 + lane < p.c.B ? static_cast<int64_t>(share_chunks(p, b0 + lane)) * units : 0;
+            int64_t x = n;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int64_t y = __shfl_up_sync(0xFFFFFFFFu, x, o);
+                if (lane >= o) x += y;
+            }
+            const uint32_t hit = __ballot_sync(0xFFFFFFFFu, at < done + x);
+            if (hit) {
+                found = true;
+                if (lane == __ffs(hit) - 1) {
+                    sh.b = b0 + lane;
+                    sh.before = done + x - n;
+                }
+            }
+            done += __shfl_sync(0xFFFFFFFFu, x, 31);
+        }
+    }
+    __syncthreads();
+    before = sh.before;
+    return sh.b;
+}
+
+// The partials of a row: part_ml[row(k)], k < n; `done` when its one piece
+// wrote the row itself.
+struct Parts {
+    int n;
+    bool done;
+    int64_t first, rest, step;
+    __device__ __forceinline__ int64_t row(int k) const { return k == 0 ? first : rest + k * step; }
+};
+
+// Chunks before sequence b and all chunks, by one warp (shares only).
+__device__ __forceinline__ void warp_chunks(const AttnParams& p, int b, int64_t& before, int64_t& all) {
+    const int lane = threadIdx.x & 31;
+    before = all = 0;
+    for (int i = lane; i < p.c.B; i += 32) {
+        const int n = share_chunks(p, i);
+        all += n;
+        before += i < b ? n : 0;
+    }
+    for (int o = 16; o; o >>= 1) {
+        all += __shfl_xor_sync(0xFFFFFFFFu, all, o);
+        before += __shfl_xor_sync(0xFFFFFFFFu, before, o);
+    }
+}
+
+// Of row r of kv head h; by a whole warp.
+__device__ __forceinline__ Parts find_parts(const AttnParams& p, int b, int h, int r) {
+    const int bh = b * p.c.H + h;
+    if (p.share_ctas == 0) {
+        const int64_t first = static_cast<int64_t>(bh) * p.nsplits * p.R + r;
+        return {p.nsplits, false, first, first, p.R};
+    }
+    int64_t before, chunks;
+    warp_chunks(p, b, before, chunks);
+    const int n = share_chunks(p, b);
+    if (n == 0) return {0, true, 0, 0, 0};
+    const int groups = (p.R + p.row_group - 1) / p.row_group, units = p.c.H * groups;
+    const Shares s = make_shares(p, chunks * units);
+    const int64_t at = before * units + static_cast<int64_t>(h * groups + r / p.row_group) * n;
+    const int i0 = s.owner(at), i1 = s.owner(at + n - 1), rr = r % p.row_group;
+    const int64_t step = 2 * static_cast<int64_t>(p.row_group), rest = i0 * step + rr;
+    return {i1 - i0 + 1, i0 == i1, rest + (s.start(i0) == at ? 0 : p.row_group), rest, step};
+}
+
+// Base-2 log-sum-exp of a row over its partials, by one warp; all lanes get it.
+__device__ __forceinline__ float combined_lse(const AttnParams& p, const Parts& parts) {
     const int lane = threadIdx.x & 31;
     float m = -CUDART_INF_F, l = 0.f;
-    for (int s = lane; s < nsplits; s += 32) {
-        const float2 v = ml[static_cast<int64_t>(s) * R];
+    for (int s = lane; s < parts.n; s += 32) {
+        const float2 v = p.part_ml[parts.row(s)];
         if (v.x == -CUDART_INF_F) continue;
         const float top = fmaxf(m, v.x);
         l = (m == -CUDART_INF_F ? 0.f : l * exp2f(m - top)) + v.y * exp2f(v.x - top);
@@ -204,8 +323,8 @@ __device__ __forceinline__ float combined_lse(const float2* ml, int nsplits, int
     return isnan(l) ? l : all == -CUDART_INF_F ? all : all + log2f(l);
 }
 
-// Blocks [0, rows): one row of the output each: the splits' partials weighted
-// by 2^(m - lse). Groups of D / 4 threads take every so many-th split, four
+// Blocks [0, rows): one row of the output each: its partials weighted
+// by 2^(m - lse). Groups of D / 4 threads take every so many-th partial, four
 // loads in flight each (the kernel is bound by load latency: 37 partials of
 // 64 rows 4 us, against 24 us with one thread per dimension); their sums are
 // added in a fixed order. Blocks from `rows` on: 512 tokens of one kv head
@@ -219,25 +338,25 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, 
     wait_for_previous_kernel();
     if (static_cast<int>(blockIdx.x) < rows) {
         const int r = blockIdx.x % p.R, bh = blockIdx.x / p.R, h = bh % p.c.H, b = bh / p.c.H, D = p.c.D;
-        const float2* ml = p.part_ml + static_cast<int64_t>(bh) * p.nsplits * p.R + r;
-        const float all = combined_lse(ml, p.nsplits, p.R);  // every warp for itself
+        const Parts parts = find_parts(p, b, h, r);  // every warp for itself
+        if (parts.done) return;
+        const float all = combined_lse(p, parts);
         const int64_t row = out_row(p, b, h, r);
         if (tid == 0) {
             if (p.lse) p.lse[row] = all;
             if (p.lse_out) p.lse_out[row] = all * 0.69314718055994531f;
         }
         const int lanes = D / 4, groups = kCombineThreads / lanes, x = tid % lanes, grp = tid / lanes;
-        const float4* o = reinterpret_cast<const float4*>(p.part_o) + (static_cast<int64_t>(bh) * p.nsplits * p.R + r) * lanes + x;
-        const int64_t step = static_cast<int64_t>(p.R) * lanes;
+        const float4* o = reinterpret_cast<const float4*>(p.part_o) + x;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s0 = 0; s0 < p.nsplits; s0 += kCombineThreads) {
+        for (int s0 = 0; s0 < parts.n; s0 += kCombineThreads) {
             __syncthreads();
-            if (s0 + tid < p.nsplits) {
-                const float m = ml[static_cast<int64_t>(s0 + tid) * p.R].x;
+            if (s0 + tid < parts.n) {
+                const float m = p.part_ml[parts.row(s0 + tid)].x;
                 w[tid] = m == -CUDART_INF_F ? 0.f : exp2f(m - all);
             }
             __syncthreads();
-            const int n = min(kCombineThreads, p.nsplits - s0);
+            const int n = min(kCombineThreads, parts.n - s0);
             for (int s = grp; s < n && grp < groups; s += 4 * groups) {
                 float4 v[4];
                 float f[4];
@@ -246,7 +365,7 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, 
                     const int sk = s + k * groups;
                     f[k] = sk < n ? w[sk] : 0.f;
                     // A split that has nothing has no partial either.
-                    v[k] = f[k] != 0.f ? o[static_cast<int64_t>(s0 + sk) * step] : make_float4(0.f, 0.f, 0.f, 0.f);
+                    v[k] = f[k] != 0.f ? o[parts.row(s0 + sk) * lanes] : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -274,8 +393,10 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, 
     const int wb = blockIdx.x - rows, bh = wb / wblocks, b = bh / p.c.H, t0 = wb % wblocks * kWeightTokens;
     const int len = len_of(p, b), qlen = q_len_of(p, b);
     if (p.accumulate && t0 >= len) return;
+    const int h = bh % p.c.H;
     for (int r = tid >> 5; r < p.R; r += kCombineThreads / 32) {
-        const float v = combined_lse(p.part_ml + static_cast<int64_t>(bh) * p.nsplits * p.R + r, p.nsplits, p.R);
+        const Parts parts = find_parts(p, b, h, r);
+        const float v = parts.done ? p.lse[out_row(p, b, h, r)] : combined_lse(p, parts);
         if ((tid & 31) == 0) {
             lse[r] = v;
             ends[r] = seen_by(p, r / p.G, len, qlen);
@@ -304,28 +425,28 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, 
     }
 }
 
-// The combine where rows are many and splits few: a warp per row.
+// The combine where rows are many and partials few: a warp per row.
 __global__ void __launch_bounds__(kCombineThreads) combine_rows_kernel(AttnParams p, int rows) {
     const int i = blockIdx.x * (kCombineThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     wait_for_previous_kernel();
     if (i >= rows) return;
     const int r = i % p.R, bh = i / p.R, h = bh % p.c.H, b = bh / p.c.H, lanes = p.c.D / 4;
-    const int64_t unit = static_cast<int64_t>(bh) * p.nsplits * p.R + r;
-    const float2* ml = p.part_ml + unit;
-    const float all = combined_lse(ml, p.nsplits, p.R);
+    const Parts parts = find_parts(p, b, h, r);
+    if (parts.done) return;
+    const float all = combined_lse(p, parts);
     const int64_t row = out_row(p, b, h, r);
     if (lane == 0) {
         if (p.lse) p.lse[row] = all;
         if (p.lse_out) p.lse_out[row] = all * 0.69314718055994531f;
     }
     for (int x = lane; x < lanes; x += 32) {
-        const float4* o = reinterpret_cast<const float4*>(p.part_o) + unit * lanes + x;
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < p.nsplits; ++s) {
-            const float m = ml[static_cast<int64_t>(s) * p.R].x;
+        for (int s = 0; s < parts.n; ++s) {
+            const int64_t at = parts.row(s);
+            const float m = p.part_ml[at].x;
             if (m == -CUDART_INF_F) continue;
             const float f = exp2f(m - all);
-            const float4 v = o[static_cast<int64_t>(s) * p.R * lanes];
+            const float4 v = reinterpret_cast<const float4*>(p.part_o)[at * lanes + x];
             a.x = fmaf(v.x, f, a.x);
             a.y = fmaf(v.y, f, a.y);
             a.z = fmaf(v.z, f, a.z);

@@ -185,9 +185,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     if (steps == 0) {
         // Nothing to see for any row.
         for (int i = threadIdx.x; i < rows; i += kChunkThreads) {
-            p.part_ml[unit + i] = make_float2(-CUDART_INF_F, 0.f);
-            if (SHARED) p.part_ml[unit + p.R + i] = make_float2(-CUDART_INF_F, 0.f);
-            if (p.nsplits > 1) continue;
+            if (p.nsplits > 1) {
+                p.part_ml[unit + i] = make_float2(-CUDART_INF_F, 0.f);
+                if (SHARED) p.part_ml[unit + p.R + i] = make_float2(-CUDART_INF_F, 0.f);
+                continue;
+            }
             const int64_t row = out_row(p, b, h, r0 + i);
             if (p.lse) p.lse[row] = -CUDART_INF_F;
             if (p.lse_out) p.lse_out[row] = -CUDART_INF_F;
@@ -424,8 +426,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         }
         if (in) {
             if (!alive) l = CUDART_NAN_F;
-            p.part_ml[part] = make_float2(none ? -CUDART_INF_F : isnan(l) ? l : base, l);
-            if (p.nsplits == 1) {
+            if (p.nsplits > 1) {
+                p.part_ml[part] = make_float2(none ? -CUDART_INF_F : isnan(l) ? l : base, l);
+            } else {
                 const float lse = none ? -CUDART_INF_F : isnan(l) ? l : base + log2f(l);
                 if (p.lse) p.lse[row] = lse;
                 if (p.lse_out) p.lse_out[row] = lse * 0.69314718055994531f;

@@ -21,10 +21,16 @@
 // (fp32 queries in two parts); the block scale of K and the power go to the
 // fp32 score. V's block scale v is folded into the exponent: P' = 2^(s +
 // log2 v - m) and the row sum adds P' / v, so V needs no product. P' is
-// scaled to at most 2^14 to use fp16's range; fp32 outputs carry it in two
-// fp16 parts (the rest is then below 2^-24 of the largest).
-// The running maximum m is raised only when some score exceeds it, which a
-// vote finds; after the first tiles that is rare.
+// scaled to between 2^8 and 2^15.5 to use fp16's range; fp32 outputs carry it
+// in two fp16 parts.
+// `m` follows the row maximum loosely: a score that would take P' past fp16
+// raises it so that the largest P' is 2^8 again. A vote finds such scores;
+// after the first tiles they are rare.
+//
+// The work, 64-token chunks of every (sequence, kv head, group of rows), is
+// divided evenly over the CTAs of one wave, whatever the lengths: a CTA's
+// share may start and end inside a unit, whose pieces the combine kernel adds
+// up.
 #pragma once
 #include "akv_q8_attend.cuh"
 
@@ -45,35 +51,43 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     __shared__ float2 ml[kStepWarps][ROWS];
     __shared__ uint2 qs[KS][NT][QLO ? 2 : 1][32];
 
+    __shared__ ShareScratch scratch;
+
     const CacheDev& c = p.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
-    const int h = blockIdx.y, b = blockIdx.z, split = blockIdx.x % p.nsplits, r0 = blockIdx.x / p.nsplits * ROWS;
+    const int groups = (p.R + ROWS - 1) / ROWS, units = c.H * groups;  // of a sequence
+    // Sequences without tokens or queries are nobody's share.
+    for (int b = blockIdx.x; b < c.B; b += gridDim.x) {
+        if (share_chunks(p, b) > 0) continue;
+        for (int i = threadIdx.x; i < p.n * p.Hq * c.D; i += kStepThreads)
+            store_elem(p.out, p.out_dtype, static_cast<int64_t>(b) * p.n * p.Hq * c.D + i, 0.f);
+        for (int i = threadIdx.x; i < p.n * p.Hq; i += kStepThreads) {
+            const int64_t row = static_cast<int64_t>(b) * p.n * p.Hq + i;
+            if (p.lse) p.lse[row] = -CUDART_INF_F;
+            if (p.lse_out) p.lse_out[row] = -CUDART_INF_F;
+        }
+    }
+    const Shares all = count_shares(p, units, scratch);
+    if (static_cast<int>(blockIdx.x) >= all.ctas) return;
+    int64_t at = all.start(blockIdx.x);                 // the next chunk of this CTA's share
+    const int64_t stop = all.start(blockIdx.x + 1);
+    int b, unit_of_b, chunk;
+    {
+        int64_t before;
+        b = find_sequence(p, at, units, scratch, before);
+        const int n = share_chunks(p, b);
+        unit_of_b = static_cast<int>((at - before) / n);
+        chunk = static_cast<int>((at - before) % n);
+    }
+    for (bool first = true; at < stop; first = false) {
+    const int n_chunks = share_chunks(p, b), n_mine = static_cast<int>(min(static_cast<int64_t>(n_chunks - chunk), stop - at));
+    const bool whole = n_mine == n_chunks;
+    const int h = unit_of_b / groups, r0 = unit_of_b % groups * ROWS;
     const int len = len_of(p, b), qlen = q_len_of(p, b);
     const int rows = min(ROWS, p.R - r0);
     const int bh = b * c.H + h;
-    const int64_t unit = (static_cast<int64_t>(bh) * p.nsplits + split) * p.R + r0;
-    // The last query of the group sees the most.
-    int end = 0;
-    if (p.causal) end = seen_by(p, min((r0 + rows - 1) / p.G, qlen - 1), len, qlen);
-    else end = r0 / p.G < qlen ? len : 0;
-    if (qlen == 0 || r0 / p.G >= qlen) end = 0;
-    const int t_begin = split * p.split, t_end = min(t_begin + p.split, end);
-    if (t_begin >= t_end) {
-        if (p.nsplits > 1) {
-            if (threadIdx.x < rows) p.part_ml[unit + threadIdx.x] = make_float2(-CUDART_INF_F, 0.f);
-            return;
-        }
-        // The only split: rows that see nothing.
-        for (int i = threadIdx.x; i < rows * c.D; i += kStepThreads)
-            store_elem(p.out, p.out_dtype, out_row(p, b, h, r0 + i / c.D) * c.D + i % c.D, 0.f);
-        if (threadIdx.x < rows) {
-            const int64_t row = out_row(p, b, h, r0 + threadIdx.x);
-            if (p.lse) p.lse[row] = -CUDART_INF_F;
-            if (p.lse_out) p.lse_out[row] = -CUDART_INF_F;
-            p.part_ml[unit + threadIdx.x] = make_float2(-CUDART_INF_F, 0.f);
-        }
-        return;
-    }
+    const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (first ? 0 : 1)) * ROWS;  // where a piece of a unit goes
+    const int t_begin = chunk * kShareTokens, t_end = min(t_begin + n_mine * kShareTokens, len);
 
     // The lane's own places in a tile. Columns past head_dim read column 0
     // instead: the query is 0 there, and such output columns are not stored.
@@ -227,13 +241,13 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     __syncthreads();
 
     float o[KS][NT][4];
-    float m[NT][2], base[NT][2], l[NT][2];
+    float base[NT][2], limit[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int i = 0; i < KS; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) { m[nt][k] = -CUDART_INF_F; base[nt][k] = 0.f; l[nt][k] = 0.f; }
+        for (int k = 0; k < 2; ++k) { base[nt][k] = 0.f; limit[nt][k] = -CUDART_INF_F; l[nt][k] = 0.f; }
     }
 
     auto tile = [&](int t0, const uint32_t (&vr)[4][VW], float vscale, uint32_t (&v_next)[4][VW], float& vscale_next) {
@@ -285,7 +299,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
             for (int k = 0; k < 4; ++k) {
                 s[nt][k] = fmaf(s[nt][k], f[k & 1], lv);
                 if (!all_seen && t0 + g + 8 * (k >> 1) >= bound[nt][k & 1]) s[nt][k] = -CUDART_INF_F;
-                above |= s[nt][k] > m[nt][k & 1];
+                above |= s[nt][k] > limit[nt][k & 1];
             }
         }
         if (__any_sync(0xFFFFFFFFu, above)) {
@@ -297,10 +311,13 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
                     x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
-                    x = fmaxf(x, m[nt][k]);
-                    const float alpha = m[nt][k] == -CUDART_INF_F ? 0.f : exp2_fast(m[nt][k] - x);
-                    m[nt][k] = x;
-                    base[nt][k] = x == -CUDART_INF_F ? 0.f : x - 14.f;
+                    // The row's largest p is to be 2^8 again; rows below
+                    // their limit stay as they are.
+                    const bool up = x > limit[nt][k];
+                    const float to = up ? x - 8.f : base[nt][k];
+                    const float alpha = limit[nt][k] == -CUDART_INF_F ? 0.f : exp2_fast(base[nt][k] - to);
+                    base[nt][k] = to;
+                    limit[nt][k] = up ? to + 15.5f : limit[nt][k];
                     l[nt][k] *= alpha;
 #pragma unroll
                     for (int i = 0; i < KS; ++i) {
@@ -358,8 +375,10 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
             x += __shfl_xor_sync(0xFFFFFFFFu, x, 4);
             x += __shfl_xor_sync(0xFFFFFFFFu, x, 8);
             x += __shfl_xor_sync(0xFFFFFFFFu, x, 16);
-            if (isnan(x)) m[nt][k] = x;  // NaN scores never raise the maximum
-            if (g == 0) ml[warp][8 * nt + 2 * cc + k] = make_float2(m[nt][k], x);
+            // A row that saw nothing has no base; NaN scores never set one.
+            if (limit[nt][k] == -CUDART_INF_F) base[nt][k] = -CUDART_INF_F;
+            if (isnan(x)) base[nt][k] = x;
+            if (g == 0) ml[warp][8 * nt + 2 * cc + k] = make_float2(base[nt][k], x);
         }
     __syncthreads();
 #pragma unroll
@@ -370,7 +389,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
             float top = ml[0][r].x;
 #pragma unroll
             for (int w = 1; w < kStepWarps; ++w) top = fmaxf(top, ml[w][r].x);
-            const float a = m[nt][k] == -CUDART_INF_F ? 0.f : exp2f(m[nt][k] - top);
+            const float a = base[nt][k] == -CUDART_INF_F ? 0.f : exp2f(base[nt][k] - top);
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
                 // Byte x of the lane group's bytes.
@@ -391,30 +410,33 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
             top = fmaxf(top, ml[w][r].x);
             acc += red[w][r][d];
         }
-        if (p.nsplits > 1 && d > 0) {
-            p.part_o[(unit + r) * c.D + d] = acc;
-            continue;
-        }
+        if (!whole) p.part_o[(part + r) * c.D + d] = acc;
+        if (!whole && d > 0) continue;
 #pragma unroll
         for (int w = 0; w < kStepWarps; ++w)
             if (ml[w][r].x != -CUDART_INF_F) sum += ml[w][r].y * exp2f(ml[w][r].x - top);
         const bool none = top == -CUDART_INF_F && !isnan(sum);
         if (isnan(sum)) top = sum;
-        if (p.nsplits > 1) {
-            p.part_o[(unit + r) * c.D] = acc;
+        const int64_t row = out_row(p, b, h, r0 + r);
+        if (whole) store_elem(p.out, p.out_dtype, row * c.D + d, none ? 0.f : acc / sum);
+        if (d > 0) continue;
+        if (!whole) {
+            p.part_ml[part + r] = make_float2(none ? -CUDART_INF_F : top, sum);
         } else {
-            store_elem(p.out, p.out_dtype, out_row(p, b, h, r0 + r) * c.D + d, none ? 0.f : acc / sum);
+            const float lse = none ? -CUDART_INF_F : top + log2f(sum);
+            if (p.lse) p.lse[row] = lse;
+            if (p.lse_out) p.lse_out[row] = lse * 0.69314718055994531f;
         }
-        if (d == 0) {
-            // The exponent's shift by 14 is taken off here.
-            p.part_ml[unit + r] = make_float2(none ? top : top - 14.f, sum);
-            if (p.nsplits == 1) {
-                const float lse = none ? top : top - 14.f + log2f(sum);
-                const int64_t orow = out_row(p, b, h, r0 + r);
-                if (p.lse) p.lse[orow] = lse;
-                if (p.lse_out) p.lse_out[orow] = lse * 0.69314718055994531f;
-            }
-        }
+    }
+    // On to the next unit.
+    at += n_mine;
+    chunk = 0;
+    if (++unit_of_b == units) {
+        unit_of_b = 0;
+        do ++b;
+        while (b < c.B && share_chunks(p, b) == 0);
+    }
+    __syncthreads();
     }
 }
 

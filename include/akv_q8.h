@@ -116,7 +116,7 @@ typedef struct AkvQ8AttnDesc {
     int32_t q_heads, q_tokens;
     int32_t q_dtype, out_dtype;     /* AKV_Q_* */
     int32_t causal, accumulate;
-    int32_t split_tokens;           /* tokens per split, a multiple of 16; 0 = library choice */
+    int32_t split_tokens;           /* tokens per split at least, a multiple of 16; 0 = library choice */
     float scale;                    /* 0 = head_dim^-0.5 */
     const void* q_dev;              /* element strides batch / token / head */
     int64_t q_stride[3];
