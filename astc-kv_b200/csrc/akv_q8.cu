@@ -171,10 +171,17 @@ template <int FMT, int DP, int NT>
 void launch_step(const AttnParams& p, cudaStream_t s) {
     const int grid = p.share_ctas;
     const bool plo = p.out_dtype == AKV_Q_F32, qlo = p.q_dtype == AKV_Q_F32;
-    if (plo && qlo) step_kernel<FMT, DP, NT, true, true><<<grid, kStepThreads, 0, s>>>(p);
-    else if (plo) step_kernel<FMT, DP, NT, true, false><<<grid, kStepThreads, 0, s>>>(p);
-    else if (qlo) step_kernel<FMT, DP, NT, false, true><<<grid, kStepThreads, 0, s>>>(p);
-    else step_kernel<FMT, DP, NT, false, false><<<grid, kStepThreads, 0, s>>>(p);
+    if constexpr (NT == 1) {
+        if (plo && p.R <= 4) {
+            if (qlo) step_kernel<FMT, DP, 1, true, true, true><<<grid, kStepThreads, 0, s>>>(p);
+            else step_kernel<FMT, DP, 1, true, false, true><<<grid, kStepThreads, 0, s>>>(p);
+            return;
+        }
+    }
+    if (plo && qlo) step_kernel<FMT, DP, NT, true, true, false><<<grid, kStepThreads, 0, s>>>(p);
+    else if (plo) step_kernel<FMT, DP, NT, true, false, false><<<grid, kStepThreads, 0, s>>>(p);
+    else if (qlo) step_kernel<FMT, DP, NT, false, true, false><<<grid, kStepThreads, 0, s>>>(p);
+    else step_kernel<FMT, DP, NT, false, false, false><<<grid, kStepThreads, 0, s>>>(p);
 }
 
 template <int FMT>
@@ -342,7 +349,11 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     // A step kernel of one CTA leaves nothing to combine.
     const bool combine = plan.chunk ? plan.nsplits > 1 : plan.share_ctas > 1;
     const int64_t rows = combine ? static_cast<int64_t>(p.c.B) * p.c.H * p.R : 0;
-    const int wblocks = plan.keep_scores ? (p.c.T + kWeightTokens - 1) / kWeightTokens : 0;
+    // Tokens per CTA of the weights part: some 1000 CTAs where there are tokens
+    // enough, since each first works out the rows' log-sum-exps.
+    int wtokens = kCombineThreads;
+    while (wtokens < 2048 && static_cast<int64_t>(p.c.B) * p.c.H * p.c.T / wtokens > 8 * sm_count()) wtokens *= 2;
+    const int wblocks = plan.keep_scores ? (p.c.T + wtokens - 1) / wtokens : 0;
     const int64_t blocks = rows + static_cast<int64_t>(p.c.B) * p.c.H * wblocks;
     if (blocks > 0x7FFFFFFF) return AKV_ERR_UNSUPPORTED;
     if (blocks && !wblocks && p.nsplits <= 16 && rows >= 4096) {
@@ -351,7 +362,7 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
                                   static_cast<int>(rows)))
             return st;
     } else if (blocks) {
-        if (int st = launch_after(combine_kernel, dim3(static_cast<unsigned>(blocks)), kCombineThreads, s, p, static_cast<int>(rows), wblocks))
+        if (int st = launch_after(combine_kernel, dim3(static_cast<unsigned>(blocks)), kCombineThreads, s, p, static_cast<int>(rows), wblocks, wtokens))
             return st;
     }
     if (p.weights && !plan.keep_scores) int8 ? launch_weights<AKV_Q8_INT8>(p, s) : launch_weights<AKV_Q8_E4M3>(p, s);

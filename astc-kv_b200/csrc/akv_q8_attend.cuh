@@ -189,7 +189,6 @@ __device__ __forceinline__ uint2 load_stream8_if(const void* p, bool in) {
 // ------------------------------------------------------------------ combine
 
 constexpr int kCombineThreads = 256;
-constexpr int kWeightTokens = 512;   // per CTA of the weights part
 
 // ------------------------------------------------- the step kernel's shares
 
@@ -327,9 +326,9 @@ __device__ __forceinline__ float combined_lse(const AttnParams& p, const Parts& 
 // by 2^(m - lse). Groups of D / 4 threads take every so many-th partial, four
 // loads in flight each (the kernel is bound by load latency: 37 partials of
 // 64 rows 4 us, against 24 us with one thread per dimension); their sums are
-// added in a fixed order. Blocks from `rows` on: 512 tokens of one kv head
+// added in a fixed order. Blocks from `rows` on: wtokens tokens of one kv head
 // each: the stored scores of its rows become softmax weights, added up.
-__global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, int rows, int wblocks) {
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, int rows, int wblocks, int wtokens) {
     __shared__ float lse[16];
     __shared__ int ends[16];
     __shared__ float w[kCombineThreads];
@@ -390,7 +389,7 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, 
         store_elem(p.out, p.out_dtype, at + 3, a.w);
         return;
     }
-    const int wb = blockIdx.x - rows, bh = wb / wblocks, b = bh / p.c.H, t0 = wb % wblocks * kWeightTokens;
+    const int wb = blockIdx.x - rows, bh = wb / wblocks, b = bh / p.c.H, t0 = wb % wblocks * wtokens;
     const int len = len_of(p, b), qlen = q_len_of(p, b);
     if (p.accumulate && t0 >= len) return;
     const int h = bh % p.c.H;
@@ -405,7 +404,7 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, 
     __syncthreads();
     const float* sc = p.scores + static_cast<int64_t>(bh) * p.c.T * p.R;
     float* at = p.weights + static_cast<int64_t>(bh) * p.wstride;
-    for (int t = t0 + tid; t < min(t0 + kWeightTokens, p.c.T); t += kCombineThreads) {
+    for (int t = t0 + tid; t < min(t0 + wtokens, p.c.T); t += kCombineThreads) {
         float sum = 0.f;
         if (p.R % 4 == 0) {
             for (int r = 0; r < p.R; r += 4) {

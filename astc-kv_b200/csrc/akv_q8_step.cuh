@@ -40,9 +40,12 @@ namespace q8 {
 constexpr int kStepWarps = 4;
 constexpr int kStepThreads = 32 * kStepWarps;
 
+// TWIN (with PLO, four rows or fewer): rows 4 to 7 are rows 0 to 3 again; their
+// P is the second part, so that one product does both. The power that the
+// products draw slows the clock: B32, 32768 tokens int8 XXX us against XXX.
 // DP: head_dim rounded up to 64, 128 or 256; NT: groups of 8 rows; PLO: P in
 // two parts; QLO: queries in two parts.
-template <int FMT, int DP, int NT, bool PLO, bool QLO>
+template <int FMT, int DP, int NT, bool PLO, bool QLO, bool TWIN>
 __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) step_kernel(AttnParams p) {
     constexpr int KS = DP / 16;       // k-steps of S, d-tiles of O
     constexpr int VW = DP / 32;       // words of a V row per lane
@@ -55,6 +58,8 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
 
     const CacheDev& c = p.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
+    static_assert(!TWIN || (PLO && NT == 1), "twin rows carry P's second part");
+    constexpr bool SECOND = PLO && !TWIN;  // P's second part in products of its own
     const int groups = (p.R + ROWS - 1) / ROWS, units = c.H * groups;  // of a sequence
     // Sequences without tokens or queries are nobody's share.
     for (int b = blockIdx.x; b < c.B; b += gridDim.x) {
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     int bound_min = INT_MAX;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int r = 8 * nt + g;
+        const int r = TWIN ? g & 3 : 8 * nt + g;
         const bool in = r < rows;
         float x[DP / 64][16];
         float top = 0.f;
@@ -289,11 +294,17 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
 #pragma unroll
             for (int k = 0; k < 4; ++k) s[nt][k] += s1[nt][k];
             if (p.scores) {
-                float* at = p.scores + (static_cast<int64_t>(bh) * c.T + t0 + g) * p.R + r0 + 8 * nt + 2 * cc;
+                float* to = p.scores + (static_cast<int64_t>(bh) * c.T + t0 + g) * p.R + r0 + 8 * nt + 2 * cc;
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (t0 + g + 8 * (k >> 1) < t_end && 8 * nt + 2 * cc + (k & 1) < rows)
-                        at[(k >> 1) * 8 * p.R + (k & 1)] = s[nt][k] * f[k & 1];
+                for (int k = 0; k < 4; k += 2) {
+                    if (t0 + g + 4 * k >= t_end || 8 * nt + 2 * cc >= rows) continue;
+                    if (p.R % 2 == 0) {
+                        *reinterpret_cast<float2*>(to + k * 4 * p.R) = make_float2(s[nt][k] * f[0], s[nt][k + 1] * f[1]);
+                    } else {
+                        to[k * 4 * p.R] = s[nt][k] * f[0];
+                        if (8 * nt + 2 * cc + 1 < rows) to[k * 4 * p.R + 1] = s[nt][k + 1] * f[1];
+                    }
+                }
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -326,7 +337,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
                     }
                 }
         }
-        uint32_t ph[NT][2], pl[PLO ? NT : 1][2];
+        uint32_t ph[NT][2], pl[SECOND ? NT : 1][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -336,9 +347,10 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const uint32_t hi = pack_half2(s[nt][2 * k], s[nt][2 * k + 1]);
+                uint32_t hi = pack_half2(s[nt][2 * k], s[nt][2 * k + 1]);
+                if (SECOND) pl[nt][k] = transpose8x8(pack_rest(s[nt][2 * k], s[nt][2 * k + 1], hi));
+                if (TWIN && cc >= 2) hi = pack_rest(s[nt][2 * k], s[nt][2 * k + 1], hi);
                 ph[nt][k] = transpose8x8(hi);
-                if (PLO) pl[nt][k] = transpose8x8(pack_rest(s[nt][2 * k], s[nt][2 * k + 1], hi));
             }
         }
 #pragma unroll
@@ -356,7 +368,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     mma16816(o[2 * w + j][nt], a[j][0], a[j][1], a[j][2], a[j][3], ph[nt][0], ph[nt][1]);
-                    if (PLO) mma16816(o[2 * w + j][nt], a[j][0], a[j][1], a[j][2], a[j][3], pl[PLO ? nt : 0][0], pl[PLO ? nt : 0][1]);
+                    if (SECOND) mma16816(o[2 * w + j][nt], a[j][0], a[j][1], a[j][2], a[j][3], pl[SECOND ? nt : 0][0], pl[SECOND ? nt : 0][1]);
                 }
         }
     };
@@ -405,10 +417,12 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     for (int i = threadIdx.x; i < rows * c.D; i += kStepThreads) {
         const int r = i / c.D, d = i % c.D;
         float top = ml[0][r].x, sum = 0.f, acc = red[0][r][d];
+        if (TWIN) acc += red[0][r + 4][d];
 #pragma unroll
         for (int w = 1; w < kStepWarps; ++w) {
             top = fmaxf(top, ml[w][r].x);
             acc += red[w][r][d];
+            if (TWIN) acc += red[w][r + 4][d];
         }
         if (!whole) p.part_o[(part + r) * c.D + d] = acc;
         if (!whole && d > 0) continue;
