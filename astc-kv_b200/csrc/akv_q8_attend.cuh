@@ -63,6 +63,20 @@ __device__ __forceinline__ void store_elem(void* o, int dtype, int64_t i, float 
     else static_cast<__half*>(o)[i] = __float2half_rn(v);
 }
 
+__device__ __forceinline__ void store4(void* o, int dtype, int64_t i, float4 v) {
+    if (dtype == AKV_Q_F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(o) + i) = v;
+    } else if (dtype == AKV_Q_BF16) {
+        const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+        *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(o) + i) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    } else {
+        const __half2 a = __floats2half2_rn(v.x, v.y), b = __floats2half2_rn(v.z, v.w);
+        *reinterpret_cast<uint2*>(static_cast<__half*>(o) + i) =
+            make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
+}
+
 // 16 consecutive query elements as floats.
 __device__ __forceinline__ void load_q16(const AttnParams& p, int64_t at, float (&x)[16]) {
     if (!p.q_vec) {
@@ -199,16 +213,23 @@ __device__ __forceinline__ int share_chunks(const AttnParams& p, int b) {
     return q_len_of(p, b) > 0 ? (len_of(p, b) + kShareTokens - 1) / kShareTokens : 0;
 }
 
+// a / b of numbers that are not negative; most fit 32 bits, whose division is
+// several times shorter.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
+}
+
 // CTA i does chunks [start(i), start(i + 1)) of all, counted by sequence, kv
 // head and row group, and along the tokens.
 struct Shares {
     int64_t chunks;
     int ctas;
-    __device__ __forceinline__ int64_t start(int i) const { return i * chunks / ctas; }
-    __device__ __forceinline__ int owner(int64_t chunk) const { return static_cast<int>(((chunk + 1) * ctas + chunks - 1) / chunks) - 1; }
+    __device__ __forceinline__ int64_t start(int i) const { return quotient(i * chunks, ctas); }
+    __device__ __forceinline__ int owner(int64_t chunk) const { return static_cast<int>(quotient((chunk + 1) * ctas + chunks - 1, chunks)) - 1; }
 };
 __device__ __forceinline__ Shares make_shares(const AttnParams& p, int64_t chunks) {
-    const int64_t most = chunks / p.share_min;
+    const int64_t most = p.share_min == 1 ? chunks : chunks / p.share_min;
     return {chunks, static_cast<int>(max(static_cast<int64_t>(1), min(most, static_cast<int64_t>(p.share_ctas))))};
 }
 
@@ -382,11 +403,7 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, 
             const float4 v = part[k * lanes + x];
             a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
         }
-        const int64_t at = row * D + 4 * x;
-        store_elem(p.out, p.out_dtype, at, a.x);
-        store_elem(p.out, p.out_dtype, at + 1, a.y);
-        store_elem(p.out, p.out_dtype, at + 2, a.z);
-        store_elem(p.out, p.out_dtype, at + 3, a.w);
+        store4(p.out, p.out_dtype, row * D + 4 * x, a);
         return;
     }
     const int wb = blockIdx.x - rows, bh = wb / wblocks, b = bh / p.c.H, t0 = wb % wblocks * wtokens;
@@ -404,23 +421,45 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, 
     __syncthreads();
     const float* sc = p.scores + static_cast<int64_t>(bh) * p.c.T * p.R;
     float* at = p.weights + static_cast<int64_t>(bh) * p.wstride;
-    for (int t = t0 + tid; t < min(t0 + wtokens, p.c.T); t += kCombineThreads) {
-        float sum = 0.f;
+    const int t_end = min(t0 + wtokens, p.c.T);
+    for (int t = t0 + tid; t < t_end; t += 4 * kCombineThreads) {
+        float sum[4] = {0.f, 0.f, 0.f, 0.f}, old[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int tk = t + k * kCombineThreads;
+            old[k] = p.accumulate && tk < min(t_end, len) ? at[tk] : 0.f;
+        }
         if (p.R % 4 == 0) {
             for (int r = 0; r < p.R; r += 4) {
-                if (t >= len) break;
-                const float4 v = *reinterpret_cast<const float4*>(sc + static_cast<int64_t>(t) * p.R + r);
-                if (t < ends[r]) sum += exp2_fast(v.x - lse[r]);
-                if (t < ends[r + 1]) sum += exp2_fast(v.y - lse[r + 1]);
-                if (t < ends[r + 2]) sum += exp2_fast(v.z - lse[r + 2]);
-                if (t < ends[r + 3]) sum += exp2_fast(v.w - lse[r + 3]);
+                float4 v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int tk = t + k * kCombineThreads;
+                    v[k] = tk < min(t_end, len) ? *reinterpret_cast<const float4*>(sc + static_cast<int64_t>(tk) * p.R + r)
+                                                : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int tk = t + k * kCombineThreads;
+                    if (tk < ends[r]) sum[k] += exp2_fast(v[k].x - lse[r]);
+                    if (tk < ends[r + 1]) sum[k] += exp2_fast(v[k].y - lse[r + 1]);
+                    if (tk < ends[r + 2]) sum[k] += exp2_fast(v[k].z - lse[r + 2]);
+                    if (tk < ends[r + 3]) sum[k] += exp2_fast(v[k].w - lse[r + 3]);
+                }
             }
         } else {
             for (int r = 0; r < p.R; ++r)
-                if (t < ends[r]) sum += exp2_fast(sc[static_cast<int64_t>(t) * p.R + r] - lse[r]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int tk = t + k * kCombineThreads;
+                    if (tk < min(ends[r], t_end)) sum[k] += exp2_fast(sc[static_cast<int64_t>(tk) * p.R + r] - lse[r]);
+                }
         }
-        if (!p.accumulate) at[t] = sum;
-        else if (t < len) at[t] += sum;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int tk = t + k * kCombineThreads;
+            if (tk < t_end && (!p.accumulate || tk < len)) at[tk] = old[k] + sum[k];
+        }
     }
 }
 
@@ -451,11 +490,7 @@ __global__ void __launch_bounds__(kCombineThreads) combine_rows_kernel(AttnParam
             a.z = fmaf(v.z, f, a.z);
             a.w = fmaf(v.w, f, a.w);
         }
-        const int64_t at = row * p.c.D + 4 * x;
-        store_elem(p.out, p.out_dtype, at, a.x);
-        store_elem(p.out, p.out_dtype, at + 1, a.y);
-        store_elem(p.out, p.out_dtype, at + 2, a.z);
-        store_elem(p.out, p.out_dtype, at + 3, a.w);
+        store4(p.out, p.out_dtype, row * p.c.D + 4 * x, a);
     }
 }
 

@@ -50,8 +50,9 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     constexpr int KS = DP / 16;       // k-steps of S, d-tiles of O
     constexpr int VW = DP / 32;       // words of a V row per lane
     constexpr int ROWS = 8 * NT;
-    __shared__ float red[kStepWarps][ROWS][DP];
+    __shared__ __align__(16) float red[kStepWarps][ROWS][DP];
     __shared__ float2 ml[kStepWarps][ROWS];
+    __shared__ float row_scale[ROWS];
     __shared__ uint2 qs[KS][NT][QLO ? 2 : 1][32];
 
     __shared__ ShareScratch scratch;
@@ -81,8 +82,8 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
         int64_t before;
         b = find_sequence(p, at, units, scratch, before);
         const int n = share_chunks(p, b);
-        unit_of_b = static_cast<int>((at - before) / n);
-        chunk = static_cast<int>((at - before) % n);
+        unit_of_b = static_cast<int>(quotient(at - before, n));
+        chunk = static_cast<int>(at - before - static_cast<int64_t>(unit_of_b) * n);
     }
     for (bool first = true; at < stop; first = false) {
     const int n_chunks = share_chunks(p, b), n_mine = static_cast<int>(min(static_cast<int64_t>(n_chunks - chunk), stop - at));
@@ -413,33 +414,43 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
                 }
             }
         }
-    __syncthreads();
-    for (int i = threadIdx.x; i < rows * c.D; i += kStepThreads) {
-        const int r = i / c.D, d = i % c.D;
-        float top = ml[0][r].x, sum = 0.f, acc = red[0][r][d];
-        if (TWIN) acc += red[0][r + 4][d];
+    if (static_cast<int>(threadIdx.x) < rows) {
+        const int r = threadIdx.x;
+        float top = ml[0][r].x, sum = 0.f;
 #pragma unroll
-        for (int w = 1; w < kStepWarps; ++w) {
-            top = fmaxf(top, ml[w][r].x);
-            acc += red[w][r][d];
-            if (TWIN) acc += red[w][r + 4][d];
-        }
-        if (!whole) p.part_o[(part + r) * c.D + d] = acc;
-        if (!whole && d > 0) continue;
+        for (int w = 1; w < kStepWarps; ++w) top = fmaxf(top, ml[w][r].x);
 #pragma unroll
         for (int w = 0; w < kStepWarps; ++w)
             if (ml[w][r].x != -CUDART_INF_F) sum += ml[w][r].y * exp2f(ml[w][r].x - top);
         const bool none = top == -CUDART_INF_F && !isnan(sum);
         if (isnan(sum)) top = sum;
-        const int64_t row = out_row(p, b, h, r0 + r);
-        if (whole) store_elem(p.out, p.out_dtype, row * c.D + d, none ? 0.f : acc / sum);
-        if (d > 0) continue;
+        row_scale[r] = none ? 0.f : 1.f / sum;
         if (!whole) {
             p.part_ml[part + r] = make_float2(none ? -CUDART_INF_F : top, sum);
         } else {
+            const int64_t row = out_row(p, b, h, r0 + r);
             const float lse = none ? -CUDART_INF_F : top + log2f(sum);
             if (p.lse) p.lse[row] = lse;
             if (p.lse_out) p.lse_out[row] = lse * 0.69314718055994531f;
+        }
+    }
+    __syncthreads();
+    // Four dimensions a thread, so many rows at a time.
+    const int lanes = c.D / 4, row_step = kStepThreads / lanes, d = threadIdx.x % lanes * 4;
+    for (int r = threadIdx.x / lanes; r < rows && threadIdx.x < lanes * row_step; r += row_step) {
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kStepWarps; ++w)
+#pragma unroll
+            for (int k = 0; k < (TWIN ? 2 : 1); ++k) {
+                const float4 v = *reinterpret_cast<const float4*>(&red[w][r + 4 * k][d]);
+                acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+            }
+        if (!whole) {
+            *reinterpret_cast<float4*>(p.part_o + (part + r) * c.D + d) = acc;
+        } else {
+            const float f = row_scale[r];  // 0 for a row that saw nothing
+            store4(p.out, p.out_dtype, out_row(p, b, h, r0 + r) * c.D + d, f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
         }
     }
     // On to the next unit.
