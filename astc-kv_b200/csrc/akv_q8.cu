@@ -93,6 +93,7 @@ int sm_count() {
 struct AttnPlan {
     int rows;         // per kv head
     bool chunk;       // the tcgen05 kernel, else the step kernel
+    bool cluster;     // the step kernel's clusters
     int nt;           // groups of eight rows per CTA
     int split, nsplits;          // chunk kernel
     int share_ctas, share_min;   // step kernel
@@ -104,6 +105,10 @@ static_assert(kShareTokens == 16 * kStepWarps, "a tile of 16 tokens for each war
 // Rows from which the tcgen05 kernel, whose CTA does 128 or 256 rows for the
 // price of one, is ahead of the step kernel, which does 16.
 constexpr int kChunkMinRows = 33;
+
+// Tokens up to which a cluster of eight CTAs for each kv head (which all have
+// to fit the GPU at once) beats even shares of all CTAs and a second launch.
+constexpr int kClusterTokens = 4096;
 
 // Rows whose scores are stored for the token weights rather than computed
 // again: storing costs 8 bytes per row and token, a second pass over K
@@ -157,6 +162,7 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
         a.share_ctas = static_cast<int>(ctas > 0 ? ctas : 1);
         a.nsplits = 0;
         parts = 2 * static_cast<size_t>(a.share_ctas) * group;
+        a.cluster = a.split == 0 && a.rows <= 8 && bh * kStepCluster <= slots && c.max_tokens <= kClusterTokens;
     }
     const auto up = [](size_t x) { return (x + 15) / 16 * 16; };
     a.part_ml = 0;
@@ -167,28 +173,43 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
     return a;
 }
 
-template <int FMT, int DP, int NT>
-void launch_step(const AttnParams& p, cudaStream_t s) {
-    const int grid = p.share_ctas;
-    const bool plo = p.out_dtype == AKV_Q_F32, qlo = p.q_dtype == AKV_Q_F32;
+template <int FMT, int DP, int NT, bool PLO, bool QLO, bool TWIN>
+int launch_step(const AttnParams& p, cudaStream_t s) {
     if constexpr (NT == 1) {
-        if (plo && p.R <= 4) {
-            if (qlo) step_kernel<FMT, DP, 1, true, true, true><<<grid, kStepThreads, 0, s>>>(p);
-            else step_kernel<FMT, DP, 1, true, false, true><<<grid, kStepThreads, 0, s>>>(p);
-            return;
+        if (p.share_ctas < 0) {
+            cudaLaunchAttribute attr;
+            attr.id = cudaLaunchAttributeClusterDimension;
+            attr.val.clusterDim.x = kStepCluster;
+            attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3(static_cast<unsigned>(p.c.B * p.c.H * kStepCluster));
+            cfg.blockDim = dim3(kStepThreads);
+            cfg.stream = s;
+            cfg.attrs = &attr;
+            cfg.numAttrs = 1;
+            return cudaLaunchKernelEx(&cfg, step_kernel<FMT, DP, 1, PLO, QLO, TWIN, true>, p) == cudaSuccess
+                       ? AKV_OK : (cudaGetLastError(), AKV_ERR_CUDA);
         }
     }
-    if (plo && qlo) step_kernel<FMT, DP, NT, true, true, false><<<grid, kStepThreads, 0, s>>>(p);
-    else if (plo) step_kernel<FMT, DP, NT, true, false, false><<<grid, kStepThreads, 0, s>>>(p);
-    else if (qlo) step_kernel<FMT, DP, NT, false, true, false><<<grid, kStepThreads, 0, s>>>(p);
-    else step_kernel<FMT, DP, NT, false, false, false><<<grid, kStepThreads, 0, s>>>(p);
+    step_kernel<FMT, DP, NT, PLO, QLO, TWIN, false><<<p.share_ctas, kStepThreads, 0, s>>>(p);
+    return launched();
+}
+
+template <int FMT, int DP, int NT>
+int launch_step(const AttnParams& p, cudaStream_t s) {
+    const bool plo = p.out_dtype == AKV_Q_F32, qlo = p.q_dtype == AKV_Q_F32;
+    if constexpr (NT == 1) {
+        if (plo && p.R <= 4) return qlo ? launch_step<FMT, DP, 1, true, true, true>(p, s) : launch_step<FMT, DP, 1, true, false, true>(p, s);
+    }
+    if (plo) return qlo ? launch_step<FMT, DP, NT, true, true, false>(p, s) : launch_step<FMT, DP, NT, true, false, false>(p, s);
+    return qlo ? launch_step<FMT, DP, NT, false, true, false>(p, s) : launch_step<FMT, DP, NT, false, false, false>(p, s);
 }
 
 template <int FMT>
-void launch_step(const AttnParams& p, int nt, cudaStream_t s) {
-    if (p.c.D > 128) launch_step<FMT, 256, 1>(p, s);
-    else if (p.c.D > 64) nt == 2 ? launch_step<FMT, 128, 2>(p, s) : launch_step<FMT, 128, 1>(p, s);
-    else nt == 2 ? launch_step<FMT, 64, 2>(p, s) : launch_step<FMT, 64, 1>(p, s);
+int launch_step(const AttnParams& p, int nt, cudaStream_t s) {
+    if (p.c.D > 128) return launch_step<FMT, 256, 1>(p, s);
+    if (p.c.D > 64) return nt == 2 ? launch_step<FMT, 128, 2>(p, s) : launch_step<FMT, 128, 1>(p, s);
+    return nt == 2 ? launch_step<FMT, 64, 2>(p, s) : launch_step<FMT, 64, 1>(p, s);
 }
 
 template <int FMT, int DP, bool SHARED>
@@ -331,7 +352,7 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     p.q = d->q_dev; p.qB = d->q_stride[0]; p.qT = d->q_stride[1]; p.qH = d->q_stride[2];
     p.lens = d->seq_lens_dev; p.q_lens = d->q_lens_dev;
     p.split = plan.split; p.nsplits = plan.nsplits;
-    p.share_ctas = plan.chunk ? 0 : plan.share_ctas; p.share_min = plan.share_min; p.row_group = 8 * plan.nt;
+    p.share_ctas = plan.chunk ? 0 : plan.cluster ? -1 : plan.share_ctas; p.share_min = plan.share_min; p.row_group = 8 * plan.nt;
     p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
     p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     p.scores = plan.keep_scores ? reinterpret_cast<float*>(ws + plan.scores) : nullptr;
@@ -340,29 +361,26 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     p.weights = d->weights_dev; p.wstride = d->weights_stride;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool int8 = p.c.fmt == AKV_Q8_INT8;
-    if (plan.chunk) {
-        if (int st = int8 ? launch_chunk<AKV_Q8_INT8>(p, s) : launch_chunk<AKV_Q8_E4M3>(p, s)) return st;
-    } else {
-        int8 ? launch_step<AKV_Q8_INT8>(p, plan.nt, s) : launch_step<AKV_Q8_E4M3>(p, plan.nt, s);
-        if (int st = launched()) return st;
-    }
+    if (int st = plan.chunk ? (int8 ? launch_chunk<AKV_Q8_INT8>(p, s) : launch_chunk<AKV_Q8_E4M3>(p, s))
+                            : (int8 ? launch_step<AKV_Q8_INT8>(p, plan.nt, s) : launch_step<AKV_Q8_E4M3>(p, plan.nt, s)))
+        return st;
     // A step kernel of one CTA leaves nothing to combine.
-    const bool combine = plan.chunk ? plan.nsplits > 1 : plan.share_ctas > 1;
+    const bool combine = plan.chunk ? plan.nsplits > 1 : !plan.cluster && plan.share_ctas > 1;
     const int64_t rows = combine ? static_cast<int64_t>(p.c.B) * p.c.H * p.R : 0;
     // Tokens per CTA of the weights part: some 1000 CTAs where there are tokens
     // enough, since each first works out the rows' log-sum-exps.
     int wtokens = kCombineThreads;
     while (wtokens < 2048 && static_cast<int64_t>(p.c.B) * p.c.H * p.c.T / wtokens > 8 * sm_count()) wtokens *= 2;
     const int wblocks = plan.keep_scores ? (p.c.T + wtokens - 1) / wtokens : 0;
-    const int64_t blocks = rows + static_cast<int64_t>(p.c.B) * p.c.H * wblocks;
+    // Partials of a row: of all rows alike, or as the shares fall.
+    const int64_t pieces = plan.chunk ? plan.nsplits : plan.share_ctas / (static_cast<int64_t>(p.c.B) * p.c.H) + 1;
+    const bool by_warp = pieces <= 16 && rows >= 1024;
+    constexpr int per = kCombineThreads / 32;
+    const int64_t blocks = (by_warp ? (rows + per - 1) / per : rows) + static_cast<int64_t>(p.c.B) * p.c.H * wblocks;
     if (blocks > 0x7FFFFFFF) return AKV_ERR_UNSUPPORTED;
-    if (blocks && !wblocks && p.nsplits <= 16 && rows >= 4096) {
-        constexpr int per = kCombineThreads / 32;
-        if (int st = launch_after(combine_rows_kernel, dim3(static_cast<unsigned>((rows + per - 1) / per)), kCombineThreads, s, p,
-                                  static_cast<int>(rows)))
-            return st;
-    } else if (blocks) {
-        if (int st = launch_after(combine_kernel, dim3(static_cast<unsigned>(blocks)), kCombineThreads, s, p, static_cast<int>(rows), wblocks, wtokens))
+    if (blocks) {
+        if (int st = launch_after(combine_kernel, dim3(static_cast<unsigned>(blocks)), kCombineThreads, s, p, static_cast<int>(rows), by_warp,
+                                  wblocks, wtokens))
             return st;
     }
     if (p.weights && !plan.keep_scores) int8 ? launch_weights<AKV_Q8_INT8>(p, s) : launch_weights<AKV_Q8_E4M3>(p, s);

@@ -24,7 +24,7 @@ struct AttnParams {
     // Partials: of the chunk kernel [B][H][nsplits][R] rows, of the step
     // kernel two pieces for each CTA, row_group rows each (see Parts).
     int split, nsplits;         // tokens per split
-    int share_ctas;             // CTAs of the step kernel, 0 for the chunk kernel
+    int share_ctas;             // CTAs of the step kernel, 0 for the chunk kernel, -1 for the step kernel's clusters
     int share_min;              // chunks that a share has at least
     int row_group;
     float* part_o;              // ... [D], weighted by 2^-base
@@ -313,6 +313,7 @@ __device__ __forceinline__ Parts find_parts(const AttnParams& p, int b, int h, i
         const int64_t first = static_cast<int64_t>(bh) * p.nsplits * p.R + r;
         return {p.nsplits, false, first, first, p.R};
     }
+    if (p.share_ctas < 0) return {0, true, 0, 0, 0};
     int64_t before, chunks;
     warp_chunks(p, b, before, chunks);
     const int n = share_chunks(p, b);
@@ -343,28 +344,65 @@ __device__ __forceinline__ float combined_lse(const AttnParams& p, const Parts& 
     return isnan(l) ? l : all == -CUDART_INF_F ? all : all + log2f(l);
 }
 
-// Blocks [0, rows): one row of the output each: its partials weighted
+// A row by one warp.
+__device__ __forceinline__ void combine_row(const AttnParams& p, const Parts& parts, float all, int64_t row) {
+    const int lanes = p.c.D / 4;
+    for (int x = threadIdx.x & 31; x < lanes; x += 32) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s0 = 0; s0 < parts.n; s0 += 4) {
+            float4 v[4];
+            float f[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) f[k] = s0 + k < parts.n ? p.part_ml[parts.row(s0 + k)].x : -CUDART_INF_F;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                // What has seen nothing has no partial either.
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (f[k] != -CUDART_INF_F) v[k] = reinterpret_cast<const float4*>(p.part_o)[parts.row(s0 + k) * lanes + x];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float w = f[k] == -CUDART_INF_F ? 0.f : exp2f(f[k] - all);
+                a.x = fmaf(v[k].x, w, a.x);
+                a.y = fmaf(v[k].y, w, a.y);
+                a.z = fmaf(v[k].z, w, a.z);
+                a.w = fmaf(v[k].w, w, a.w);
+            }
+        }
+        store4(p.out, p.out_dtype, row * p.c.D + 4 * x, a);
+    }
+}
+
+// The first blocks: `rows` rows of the output, each its partials weighted
 // by 2^(m - lse). Groups of D / 4 threads take every so many-th partial, four
 // loads in flight each (the kernel is bound by load latency: 37 partials of
 // 64 rows 4 us, against 24 us with one thread per dimension); their sums are
-// added in a fixed order. Blocks from `rows` on: wtokens tokens of one kv head
+// added in a fixed order. Where partials are few a warp does a row (by_warp).
+// The other blocks: wtokens tokens of one kv head
 // each: the stored scores of its rows become softmax weights, added up.
-__global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, int rows, int wblocks, int wtokens) {
+__global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, int rows, bool by_warp, int wblocks, int wtokens) {
     __shared__ float lse[16];
     __shared__ int ends[16];
     __shared__ float w[kCombineThreads];
     __shared__ float4 part[kCombineThreads];
     const int tid = threadIdx.x;
     wait_for_previous_kernel();
-    if (static_cast<int>(blockIdx.x) < rows) {
-        const int r = blockIdx.x % p.R, bh = blockIdx.x / p.R, h = bh % p.c.H, b = bh / p.c.H, D = p.c.D;
+    const int row_blocks = by_warp ? (rows + kCombineThreads / 32 - 1) / (kCombineThreads / 32) : rows;
+    if (static_cast<int>(blockIdx.x) < row_blocks) {
+        const int i = by_warp ? blockIdx.x * (kCombineThreads / 32) + (tid >> 5) : blockIdx.x;
+        if (i >= rows) return;
+        const int r = i % p.R, bh = i / p.R, h = bh % p.c.H, b = bh / p.c.H, D = p.c.D;
         const Parts parts = find_parts(p, b, h, r);  // every warp for itself
         if (parts.done) return;
         const float all = combined_lse(p, parts);
         const int64_t row = out_row(p, b, h, r);
-        if (tid == 0) {
+        if (by_warp ? (tid & 31) == 0 : tid == 0) {
             if (p.lse) p.lse[row] = all;
             if (p.lse_out) p.lse_out[row] = all * 0.69314718055994531f;
+        }
+        if (by_warp) {
+            combine_row(p, parts, all, row);
+            return;
         }
         const int lanes = D / 4, groups = kCombineThreads / lanes, x = tid % lanes, grp = tid / lanes;
         const float4* o = reinterpret_cast<const float4*>(p.part_o) + x;
@@ -406,7 +444,7 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, 
         store4(p.out, p.out_dtype, row * D + 4 * x, a);
         return;
     }
-    const int wb = blockIdx.x - rows, bh = wb / wblocks, b = bh / p.c.H, t0 = wb % wblocks * wtokens;
+    const int wb = blockIdx.x - row_blocks, bh = wb / wblocks, b = bh / p.c.H, t0 = wb % wblocks * wtokens;
     const int len = len_of(p, b), qlen = q_len_of(p, b);
     if (p.accumulate && t0 >= len) return;
     const int h = bh % p.c.H;
@@ -460,37 +498,6 @@ __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, 
             const int tk = t + k * kCombineThreads;
             if (tk < t_end && (!p.accumulate || tk < len)) at[tk] = old[k] + sum[k];
         }
-    }
-}
-
-// The combine where rows are many and partials few: a warp per row.
-__global__ void __launch_bounds__(kCombineThreads) combine_rows_kernel(AttnParams p, int rows) {
-    const int i = blockIdx.x * (kCombineThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-    wait_for_previous_kernel();
-    if (i >= rows) return;
-    const int r = i % p.R, bh = i / p.R, h = bh % p.c.H, b = bh / p.c.H, lanes = p.c.D / 4;
-    const Parts parts = find_parts(p, b, h, r);
-    if (parts.done) return;
-    const float all = combined_lse(p, parts);
-    const int64_t row = out_row(p, b, h, r);
-    if (lane == 0) {
-        if (p.lse) p.lse[row] = all;
-        if (p.lse_out) p.lse_out[row] = all * 0.69314718055994531f;
-    }
-    for (int x = lane; x < lanes; x += 32) {
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < parts.n; ++s) {
-            const int64_t at = parts.row(s);
-            const float m = p.part_ml[at].x;
-            if (m == -CUDART_INF_F) continue;
-            const float f = exp2f(m - all);
-            const float4 v = reinterpret_cast<const float4*>(p.part_o)[at * lanes + x];
-            a.x = fmaf(v.x, f, a.x);
-            a.y = fmaf(v.y, f, a.y);
-            a.z = fmaf(v.z, f, a.z);
-            a.w = fmaf(v.w, f, a.w);
-        }
-        store4(p.out, p.out_dtype, row * p.c.D + 4 * x, a);
     }
 }
 

@@ -39,13 +39,38 @@ namespace q8 {
 
 constexpr int kStepWarps = 4;
 constexpr int kStepThreads = 32 * kStepWarps;
+constexpr int kStepCluster = 8;
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// `p`, a place in this CTA's shared memory, in that of CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t remote_addr(const void* p, int rank) {
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ float2 load_remote2(const void* p, int rank) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(remote_addr(p, rank)) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 load_remote4(const void* p, int rank) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote_addr(p, rank)) : "memory");
+    return v;
+}
 
 // TWIN (with PLO, four rows or fewer): rows 4 to 7 are rows 0 to 3 again; their
 // P is the second part, so that one product does both. The power that the
 // products draw slows the clock: B32, 32768 tokens int8 XXX us against XXX.
+// CLUSTER: eight CTAs divide one unit and add up its pieces through distributed
+// shared memory; for little work, where the scan of the lengths and a second
+// launch would cost more than an even division saves (B1, 384 tokens, 9/3
+// heads: XXXX us against XXXX).
 // DP: head_dim rounded up to 64, 128 or 256; NT: groups of 8 rows; PLO: P in
 // two parts; QLO: queries in two parts.
-template <int FMT, int DP, int NT, bool PLO, bool QLO, bool TWIN>
+template <int FMT, int DP, int NT, bool PLO, bool QLO, bool TWIN, bool CLUSTER>
 __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) step_kernel(AttnParams p) {
     constexpr int KS = DP / 16;       // k-steps of S, d-tiles of O
     constexpr int VW = DP / 32;       // words of a V row per lane
@@ -53,6 +78,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     __shared__ __align__(16) float red[kStepWarps][ROWS][DP];
     __shared__ float2 ml[kStepWarps][ROWS];
     __shared__ float row_scale[ROWS];
+    __shared__ float2 piece[CLUSTER ? ROWS : 1];
     __shared__ uint2 qs[KS][NT][QLO ? 2 : 1][32];
 
     __shared__ ShareScratch scratch;
@@ -62,23 +88,29 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     static_assert(!TWIN || (PLO && NT == 1), "twin rows carry P's second part");
     constexpr bool SECOND = PLO && !TWIN;  // P's second part in products of its own
     const int groups = (p.R + ROWS - 1) / ROWS, units = c.H * groups;  // of a sequence
-    // Sequences without tokens or queries are nobody's share.
-    for (int b = blockIdx.x; b < c.B; b += gridDim.x) {
-        if (share_chunks(p, b) > 0) continue;
-        for (int i = threadIdx.x; i < p.n * p.Hq * c.D; i += kStepThreads)
-            store_elem(p.out, p.out_dtype, static_cast<int64_t>(b) * p.n * p.Hq * c.D + i, 0.f);
-        for (int i = threadIdx.x; i < p.n * p.Hq; i += kStepThreads) {
-            const int64_t row = static_cast<int64_t>(b) * p.n * p.Hq + i;
-            if (p.lse) p.lse[row] = -CUDART_INF_F;
-            if (p.lse_out) p.lse_out[row] = -CUDART_INF_F;
-        }
-    }
-    const Shares all = count_shares(p, units, scratch);
-    if (static_cast<int>(blockIdx.x) >= all.ctas) return;
-    int64_t at = all.start(blockIdx.x);                 // the next chunk of this CTA's share
-    const int64_t stop = all.start(blockIdx.x + 1);
+    int64_t at = 0, stop = 1;  // the next chunk of this CTA's share, its end
     int b, unit_of_b, chunk;
-    {
+    const int rank = CLUSTER ? blockIdx.x % kStepCluster : 0;
+    if constexpr (CLUSTER) {
+        b = blockIdx.x / kStepCluster / units;
+        unit_of_b = blockIdx.x / kStepCluster % units;
+        chunk = 0;
+    } else {
+        // Sequences without tokens or queries are nobody's share.
+        for (int e = blockIdx.x; e < c.B; e += gridDim.x) {
+            if (share_chunks(p, e) > 0) continue;
+            for (int i = threadIdx.x; i < p.n * p.Hq * c.D; i += kStepThreads)
+                store_elem(p.out, p.out_dtype, static_cast<int64_t>(e) * p.n * p.Hq * c.D + i, 0.f);
+            for (int i = threadIdx.x; i < p.n * p.Hq; i += kStepThreads) {
+                const int64_t row = static_cast<int64_t>(e) * p.n * p.Hq + i;
+                if (p.lse) p.lse[row] = -CUDART_INF_F;
+                if (p.lse_out) p.lse_out[row] = -CUDART_INF_F;
+            }
+        }
+        const Shares all = count_shares(p, units, scratch);
+        if (static_cast<int>(blockIdx.x) >= all.ctas) return;
+        at = all.start(blockIdx.x);
+        stop = all.start(blockIdx.x + 1);
         int64_t before;
         b = find_sequence(p, at, units, scratch, before);
         const int n = share_chunks(p, b);
@@ -86,8 +118,16 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
         chunk = static_cast<int>(at - before - static_cast<int64_t>(unit_of_b) * n);
     }
     for (bool first = true; at < stop; first = false) {
-    const int n_chunks = share_chunks(p, b), n_mine = static_cast<int>(min(static_cast<int64_t>(n_chunks - chunk), stop - at));
-    const bool whole = n_mine == n_chunks;
+    const int n_chunks = share_chunks(p, b);
+    int n_mine;
+    if constexpr (CLUSTER) {
+        chunk = rank * n_chunks / kStepCluster;
+        n_mine = (rank + 1) * n_chunks / kStepCluster - chunk;
+        at = stop;
+    } else {
+        n_mine = static_cast<int>(min(static_cast<int64_t>(n_chunks - chunk), stop - at));
+    }
+    const bool whole = !CLUSTER && n_mine == n_chunks;
     const int h = unit_of_b / groups, r0 = unit_of_b % groups * ROWS;
     const int len = len_of(p, b), qlen = q_len_of(p, b);
     const int rows = min(ROWS, p.R - r0);
@@ -425,7 +465,9 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
         const bool none = top == -CUDART_INF_F && !isnan(sum);
         if (isnan(sum)) top = sum;
         row_scale[r] = none ? 0.f : 1.f / sum;
-        if (!whole) {
+        if (CLUSTER) {
+            piece[r] = make_float2(none ? -CUDART_INF_F : top, sum);
+        } else if (!whole) {
             p.part_ml[part + r] = make_float2(none ? -CUDART_INF_F : top, sum);
         } else {
             const int64_t row = out_row(p, b, h, r0 + r);
@@ -446,12 +488,54 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
                 const float4 v = *reinterpret_cast<const float4*>(&red[w][r + 4 * k][d]);
                 acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
             }
-        if (!whole) {
+        if (CLUSTER) {
+            *reinterpret_cast<float4*>(&red[0][r][d]) = acc;  // what this thread alone has read
+        } else if (!whole) {
             *reinterpret_cast<float4*>(p.part_o + (part + r) * c.D + d) = acc;
         } else {
             const float f = row_scale[r];  // 0 for a row that saw nothing
             store4(p.out, p.out_dtype, out_row(p, b, h, r0 + r) * c.D + d, f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
         }
+    }
+    if constexpr (CLUSTER) {
+        __syncthreads();
+        cluster_sync();
+        // Row r is finished by CTA r % 8, its pieces in the order of the CTAs.
+        for (int r = rank; r < rows; r += kStepCluster) {
+            float top = -CUDART_INF_F, sum = 0.f;
+            float2 v[kStepCluster];
+#pragma unroll
+            for (int k = 0; k < kStepCluster; ++k) {
+                v[k] = load_remote2(&piece[r], k);
+                top = fmaxf(top, v[k].x);
+            }
+#pragma unroll
+            for (int k = 0; k < kStepCluster; ++k)
+                if (v[k].x != -CUDART_INF_F) sum += v[k].y * exp2f(v[k].x - top);
+            const bool none = top == -CUDART_INF_F && !isnan(sum);
+            const int64_t row = out_row(p, b, h, r0 + r);
+            if (static_cast<int>(threadIdx.x) < lanes) {
+                float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int k = 0; k < kStepCluster; ++k) {
+                    if (v[k].x == -CUDART_INF_F) continue;
+                    const float f = exp2f(v[k].x - top);
+                    const float4 o = load_remote4(&red[0][r][d], k);
+                    acc.x = fmaf(o.x, f, acc.x); acc.y = fmaf(o.y, f, acc.y);
+                    acc.z = fmaf(o.z, f, acc.z); acc.w = fmaf(o.w, f, acc.w);
+                }
+                const float f = none ? 0.f : 1.f / sum;
+                store4(p.out, p.out_dtype, row * c.D + d, none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
+            }
+            if (threadIdx.x == 0) {
+                const float lse = none ? -CUDART_INF_F : isnan(sum) ? sum : top + log2f(sum);
+                if (p.lse) p.lse[row] = lse;
+                if (p.lse_out) p.lse_out[row] = lse * 0.69314718055994531f;
+            }
+        }
+        __syncthreads();
+        cluster_sync();  // nobody reads this CTA's memory any more
+        return;
     }
     // On to the next unit.
     at += n_mine;
