@@ -19,11 +19,12 @@ CSRC = ROOT / "csrc"
 INCLUDE = ROOT.parent / "include"
 LIB = PKG / "libakv_cuda.so"
 
-SOURCES = ["akv_cuda.cu", "akv_q8.cu", "akv_tables.cpp", "akv_encode.cpp"]
+SOURCES = ["akv_cuda.cu", "akv_q8.cu", "akv_q8_step_int8.cu", "akv_q8_step_e4m3.cu", "akv_tables.cpp", "akv_encode.cpp"]
 HEADERS = ["akv_astc_device.cuh", "akv_common.cuh", "akv_decode_kernels.cuh", "akv_attention_kernels.cuh", "akv_tables.h",
            "akv_attn_fp16.cuh",
            "akv_attn_fast.cuh", "akv_decode_fast.cuh",
-           "akv_q8_common.cuh", "akv_q8_store.cuh", "akv_q8_attend.cuh", "akv_q8_chunk.cuh", "akv_q8_step.cuh", "akv_q8_weights.cuh", "akv_q8_evict.cuh"]
+           "akv_q8_common.cuh", "akv_q8_store.cuh", "akv_q8_attend.cuh", "akv_q8_chunk.cuh", "akv_q8_step.cuh", "akv_q8_step_launch.cuh", "akv_q8_step_launch.h",
+           "akv_q8_weights.cuh", "akv_q8_evict.cuh"]
 
 
 def nvcc() -> str:

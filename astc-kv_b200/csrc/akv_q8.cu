@@ -9,7 +9,7 @@
 #include "akv_q8_attend.cuh"
 #include "akv_q8_chunk.cuh"
 #include "akv_q8_evict.cuh"
-#include "akv_q8_step.cuh"
+#include "akv_q8_step_launch.h"
 #include "akv_q8_store.cuh"
 #include "akv_q8_weights.cuh"
 
@@ -19,7 +19,6 @@ namespace {
 
 constexpr int kMaxGridYZ = 65535;
 
-inline int launched() { return cudaPeekAtLastError() == cudaSuccess ? AKV_OK : (cudaGetLastError(), AKV_ERR_CUDA); }
 
 bool valid_dtype(int t) { return t >= AKV_Q_F32 && t <= AKV_Q_F16; }
 
@@ -101,7 +100,6 @@ struct AttnPlan {
     size_t part_ml, part_o, scores, lse, bytes;  // offsets into the workspace, and its size
 };
 
-static_assert(kShareTokens == 16 * kStepWarps, "a tile of 16 tokens for each warp");
 // Rows from which the tcgen05 kernel, whose CTA does 128 or 256 rows for the
 // price of one, is ahead of the step kernel, which does 16.
 constexpr int kChunkMinRows = 33;
@@ -171,45 +169,6 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
     a.lse = a.scores + (a.keep_scores ? up(static_cast<size_t>(bh) * c.max_tokens * a.rows * sizeof(float)) : 0);
     a.bytes = a.lse + (d->weights_dev ? up(static_cast<size_t>(c.batch) * d->q_tokens * d->q_heads * sizeof(float)) : 0) + 16;
     return a;
-}
-
-template <int FMT, int DP, int NT, bool PLO, bool QLO, bool TWIN>
-int launch_step(const AttnParams& p, cudaStream_t s) {
-    if constexpr (NT == 1) {
-        if (p.share_ctas < 0) {
-            cudaLaunchAttribute attr;
-            attr.id = cudaLaunchAttributeClusterDimension;
-            attr.val.clusterDim.x = kStepCluster;
-            attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-            cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(static_cast<unsigned>(p.c.B * p.c.H * kStepCluster));
-            cfg.blockDim = dim3(kStepThreads);
-            cfg.stream = s;
-            cfg.attrs = &attr;
-            cfg.numAttrs = 1;
-            return cudaLaunchKernelEx(&cfg, step_kernel<FMT, DP, 1, PLO, QLO, TWIN, true>, p) == cudaSuccess
-                       ? AKV_OK : (cudaGetLastError(), AKV_ERR_CUDA);
-        }
-    }
-    step_kernel<FMT, DP, NT, PLO, QLO, TWIN, false><<<p.share_ctas, kStepThreads, 0, s>>>(p);
-    return launched();
-}
-
-template <int FMT, int DP, int NT>
-int launch_step(const AttnParams& p, cudaStream_t s) {
-    const bool plo = p.out_dtype == AKV_Q_F32, qlo = p.q_dtype == AKV_Q_F32;
-    if constexpr (NT == 1) {
-        if (plo && p.R <= 4) return qlo ? launch_step<FMT, DP, 1, true, true, true>(p, s) : launch_step<FMT, DP, 1, true, false, true>(p, s);
-    }
-    if (plo) return qlo ? launch_step<FMT, DP, NT, true, true, false>(p, s) : launch_step<FMT, DP, NT, true, false, false>(p, s);
-    return qlo ? launch_step<FMT, DP, NT, false, true, false>(p, s) : launch_step<FMT, DP, NT, false, false, false>(p, s);
-}
-
-template <int FMT>
-int launch_step(const AttnParams& p, int nt, cudaStream_t s) {
-    if (p.c.D > 128) return launch_step<FMT, 256, 1>(p, s);
-    if (p.c.D > 64) return nt == 2 ? launch_step<FMT, 128, 2>(p, s) : launch_step<FMT, 128, 1>(p, s);
-    return nt == 2 ? launch_step<FMT, 64, 2>(p, s) : launch_step<FMT, 64, 1>(p, s);
 }
 
 template <int FMT, int DP, bool SHARED>
@@ -362,7 +321,7 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool int8 = p.c.fmt == AKV_Q8_INT8;
     if (int st = plan.chunk ? (int8 ? launch_chunk<AKV_Q8_INT8>(p, s) : launch_chunk<AKV_Q8_E4M3>(p, s))
-                            : (int8 ? launch_step<AKV_Q8_INT8>(p, plan.nt, s) : launch_step<AKV_Q8_E4M3>(p, plan.nt, s)))
+                            : (int8 ? launch_step_int8(p, plan.nt, s) : launch_step_e4m3(p, plan.nt, s)))
         return st;
     // A step kernel of one CTA leaves nothing to combine.
     const bool combine = plan.chunk ? plan.nsplits > 1 : !plan.cluster && plan.share_ctas > 1;
@@ -410,7 +369,7 @@ int akv_q8_evict(const AkvQ8EvictDesc* d, void* stream) {
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     select_kernel<<<dim3(a.kv_heads, a.batch), kSelectThreads, 0, s>>>(p);
     if (int st = launched()) return st;
-    const dim3 grid((p.keep + p.dst.blk - 1) / p.dst.blk, a.kv_heads, 2 * a.batch);
+    const dim3 grid((p.keep + p.dst.blk - 1) / p.dst.blk, a.kv_heads, a.batch);
     const bool few = c.block_tokens * (c.head_dim / 16) <= 512;  // pieces of a block
     if (a.format == AKV_Q8_INT8)
         return few ? launch_after(pack_kernel<AKV_Q8_INT8, 2>, grid, 256, s, p) : launch_after(pack_kernel<AKV_Q8_INT8, 8>, grid, 256, s, p);

@@ -139,24 +139,6 @@ __device__ __forceinline__ uint32_t pack_rest(float a, float b, uint32_t hi) {
     return pack_half2(a - f.x, b - f.y);
 }
 
-// Four codes as two fp16 pairs, exactly. int8: code + 128 becomes the low
-// byte of 1024 + (code + 128), and 1152 is taken off. e4m3: the conversion
-// instruction.
-template <int FMT>
-__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
-    if (FMT == AKV_Q8_INT8) {
-        const uint32_t u = w ^ 0x80808080u;
-        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        const uint32_t c = 0x64806480u;
-        const __half2 base = *reinterpret_cast<const __half2*>(&c);
-        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), base), y = __hsub2(*reinterpret_cast<const __half2*>(&b), base);
-        lo = *reinterpret_cast<const uint32_t*>(&x);
-        hi = *reinterpret_cast<const uint32_t*>(&y);
-    } else {
-        asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}\n" : "=r"(lo), "=r"(hi) : "r"(w));
-    }
-}
-
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -380,7 +362,7 @@ __device__ __forceinline__ void combine_row(const AttnParams& p, const Parts& pa
 // added in a fixed order. Where partials are few a warp does a row (by_warp).
 // The other blocks: wtokens tokens of one kv head
 // each: the stored scores of its rows become softmax weights, added up.
-__global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, int rows, bool by_warp, int wblocks, int wtokens) {
+static __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, int rows, bool by_warp, int wblocks, int wtokens) {
     __shared__ float lse[16];
     __shared__ int ends[16];
     __shared__ float w[kCombineThreads];

@@ -93,6 +93,24 @@ __device__ __forceinline__ void from_codes4(uint32_t w, float (&x)[4]) {
     }
 }
 
+// Four codes as two fp16 pairs, exactly. int8: code + 128 becomes the low
+// byte of 1024 + (code + 128), and 1152 is taken off. e4m3: the conversion
+// instruction.
+template <int FMT>
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if (FMT == AKV_Q8_INT8) {
+        const uint32_t u = w ^ 0x80808080u;
+        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
+        const uint32_t c = 0x64806480u;
+        const __half2 base = *reinterpret_cast<const __half2*>(&c);
+        const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), base), y = __hsub2(*reinterpret_cast<const __half2*>(&b), base);
+        lo = *reinterpret_cast<const uint32_t*>(&x);
+        hi = *reinterpret_cast<const uint32_t*>(&y);
+    } else {
+        asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}\n" : "=r"(lo), "=r"(hi) : "r"(w));
+    }
+}
+
 // Codes of four y = x / scale with |y| <= M up to rounding (M = 127 or 448).
 template <int FMT>
 __device__ __forceinline__ uint32_t to_codes4(const float (&y)[4]) {

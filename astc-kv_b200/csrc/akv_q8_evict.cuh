@@ -62,7 +62,7 @@ __device__ __forceinline__ int run_length(int n) { return ((n + kSelectThreads -
 // counts what its own run of tokens keeps (keys above the cut-off, and of the
 // equal ones the first few), a scan over the threads gives the places, and a
 // second look writes. The row is read five times, from L2 after the first.
-__global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictParams p) {
+static __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictParams p) {
     __shared__ int hist[2048];
     __shared__ int sums[32];
     __shared__ uint32_t s_prefix;
@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictParams p) {
         const uint32_t mask = pass == 2 ? 1023u : 2047u;
         hist[tid] = hist[tid + kSelectThreads] = 0;
         __syncthreads();
+        int zeros = 0;  // tokens that never received weight are many: one bin
         for (int t = lo + tid; t < hi; t += 8 * kSelectThreads) {
             float x[8];
 #pragma unroll
@@ -103,10 +104,13 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictParams p) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const uint32_t key = order_key(x[k]);
-                if (t + k * kSelectThreads < hi && (pass == 0 || ((key ^ prefix) >> (shift + (pass == 1 ? 11 : 10))) == 0))
+                if (pass == 0 && key == 0x80000000u) zeros += t + k * kSelectThreads < hi;
+                else if (t + k * kSelectThreads < hi && (pass == 0 || ((key ^ prefix) >> (shift + (pass == 1 ? 11 : 10))) == 0))
                     atomicAdd(&hist[(key >> shift) & mask], 1);
             }
         }
+        zeros = __reduce_add_sync(0xFFFFFFFFu, zeros);
+        if (zeros && (tid & 31) == 0) atomicAdd(&hist[0x80000000u >> 21], zeros);
         __syncthreads();
         // Bins from the highest down, two a thread.
         const int d = 2047 - 2 * tid, upper = hist[d], lower = hist[d - 1];
@@ -150,15 +154,25 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictParams p) {
     }
 }
 
-// One CTA per (block of the new cache, kv head, sequence x side). The rows'
-// codes stay in registers (PP pieces of 16 a thread) between finding the
-// largest value and coding them under the new scale.
+// Largest |code| of four, as fp16 (exact; a NaN code stays one).
+template <int FMT>
+__device__ __forceinline__ __half2 max_of_codes(uint32_t w, __half2 m) {
+    uint32_t lo, hi;
+    codes_to_half<FMT>(w, lo, hi);
+    m = __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&lo)));
+    return __hmax2_nan(m, __habs2(*reinterpret_cast<const __half2*>(&hi)));
+}
+
+// One CTA per (block of the new cache, kv head, sequence), K and V together:
+// the kept tokens and their pages are looked up once, and both sides' rows are
+// in flight at a time. The rows' codes stay in registers (PP pieces of 16 a
+// thread and side) between finding the largest value and coding them under
+// the new scale.
 template <int FMT, int PP>
 __global__ void __launch_bounds__(256) pack_kernel(EvictParams p) {
-    __shared__ uint32_t red[8];
+    __shared__ uint32_t red[2][8];
     const CacheDev &a = p.src, &c = p.dst;
-    const int h = blockIdx.y, b = blockIdx.z >> 1, side = blockIdx.z & 1;
-    const SideDev &from = side ? a.v : a.k, &to = side ? c.v : c.k;
+    const int h = blockIdx.y, b = blockIdx.z;
     const int32_t* kept = p.kept + (static_cast<int64_t>(b) * a.H + h) * p.keep;
     const int row0 = blockIdx.x * c.blk, per_row = c.D / 16;
     wait_for_previous_kernel();
@@ -167,53 +181,66 @@ __global__ void __launch_bounds__(256) pack_kernel(EvictParams p) {
     int in_page;
     const int phys = page_of(c, b, row0, in_page);
     if (phys < 0) return;
-    uint4 w[PP];
-    float sc[PP];
-    uint32_t top = 0;
+    uint4 w[2][PP];
+    float sc[2][PP];
 #pragma unroll
     for (int k = 0; k < PP; ++k) {
         const int i = threadIdx.x + k * 256, r = i / per_row;
-        w[k] = make_uint4(0, 0, 0, 0);
-        sc[k] = 0.f;
+        w[0][k] = w[1][k] = make_uint4(0, 0, 0, 0);
+        sc[0][k] = sc[1][k] = 0.f;
         if (r >= n) continue;
         int row;
         const int pg = page_of(a, b, kept[row0 + r], row);
         if (pg < 0) continue;
-        w[k] = __ldg(reinterpret_cast<const uint4*>(from.codes + code_offset(from, b, h, pg, row)) + (i - r * per_row));
-        sc[k] = from.scales[scale_offset(from, b, h, pg, row / a.blk)];
+        const int piece = i - r * per_row;
+        w[0][k] = __ldg(reinterpret_cast<const uint4*>(a.k.codes + code_offset(a.k, b, h, pg, row)) + piece);
+        w[1][k] = __ldg(reinterpret_cast<const uint4*>(a.v.codes + code_offset(a.v, b, h, pg, row)) + piece);
+        sc[0][k] = a.k.scales[scale_offset(a.k, b, h, pg, row / a.blk)];
+        sc[1][k] = a.v.scales[scale_offset(a.v, b, h, pg, row / a.blk)];
     }
 #pragma unroll
-    for (int k = 0; k < PP; ++k) {
-        const uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
-        uint32_t m = 0;
+    for (int side = 0; side < 2; ++side) {
+        uint32_t top = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float f[4];
-            from_codes4<FMT>(u[j], f);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) m = max(m, abs_bits(f[e]));
+        for (int k = 0; k < PP; ++k) {
+            __half2 m = __float2half2_rn(0.f);
+            m = max_of_codes<FMT>(w[side][k].x, m);
+            m = max_of_codes<FMT>(w[side][k].y, m);
+            m = max_of_codes<FMT>(w[side][k].z, m);
+            m = max_of_codes<FMT>(w[side][k].w, m);
+            const float2 f = __half22float2(m);
+            // Rounding keeps the order: the largest code gives the largest value.
+            top = max(top, max(abs_bits(__fmul_rn(f.x, sc[side][k])), abs_bits(__fmul_rn(f.y, sc[side][k]))));
         }
-        // Rounding keeps the order: the largest code gives the largest value.
-        top = max(top, abs_bits(__fmul_rn(__uint_as_float(m), sc[k])));
+        top = __reduce_max_sync(0xFFFFFFFFu, top);
+        if ((threadIdx.x & 31) == 0) red[side][threadIdx.x >> 5] = top;
     }
-    const float scale = block_scale<FMT>(cta_max(top, red)), inv = block_inverse(scale);
-    uint8_t* codes = to.codes + code_offset(to, b, h, phys, in_page);
+    __syncthreads();
 #pragma unroll
-    for (int k = 0; k < PP; ++k) {
-        const int i = threadIdx.x + k * 256, r = i / per_row;
-        if (r >= c.blk) break;
-        uint32_t u[4] = {w[k].x, w[k].y, w[k].z, w[k].w};
+    for (int side = 0; side < 2; ++side) {
+        const SideDev& to = side ? c.v : c.k;
+        uint32_t top = red[side][0];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float f[4];
-            from_codes4<FMT>(u[j], f);
+        for (int k = 1; k < 8; ++k) top = max(top, red[side][k]);
+        const float scale = block_scale<FMT>(top), inv = block_inverse(scale);
+        uint8_t* codes = to.codes + code_offset(to, b, h, phys, in_page);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(__fmul_rn(f[e], sc[k]), inv);
-            u[j] = to_codes4<FMT>(f);
+        for (int k = 0; k < PP; ++k) {
+            const int i = threadIdx.x + k * 256, r = i / per_row;
+            if (r >= c.blk) break;
+            uint32_t u[4] = {w[side][k].x, w[side][k].y, w[side][k].z, w[side][k].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float f[4];
+                from_codes4<FMT>(u[j], f);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(__fmul_rn(f[e], sc[side][k]), inv);
+                u[j] = to_codes4<FMT>(f);
+            }
+            reinterpret_cast<uint4*>(codes + r * to.sT)[i - r * per_row] = make_uint4(u[0], u[1], u[2], u[3]);
         }
-        reinterpret_cast<uint4*>(codes + r * to.sT)[i - r * per_row] = make_uint4(u[0], u[1], u[2], u[3]);
+        if (threadIdx.x == 0) to.scales[scale_offset(to, b, h, phys, in_page / c.blk)] = scale;
     }
-    if (threadIdx.x == 0) to.scales[scale_offset(to, b, h, phys, in_page / c.blk)] = scale;
 }
 
 }  // namespace q8

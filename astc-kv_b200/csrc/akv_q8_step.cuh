@@ -33,13 +33,13 @@
 // up.
 #pragma once
 #include "akv_q8_attend.cuh"
+#include "akv_q8_step_launch.h"
 
 namespace akv {
 namespace q8 {
 
-constexpr int kStepWarps = 4;
 constexpr int kStepThreads = 32 * kStepWarps;
-constexpr int kStepCluster = 8;
+static_assert(kShareTokens == 16 * kStepWarps, "a tile of 16 tokens for each warp");
 
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");

@@ -47,6 +47,33 @@ struct Piece {
         const uint4& v = w[i >> 2];
         return (i & 3) == 0 ? v.x : (i & 3) == 1 ? v.y : (i & 3) == 2 ? v.z : v.w;
     }
+    // Bits of the largest |element|, as a float; an infinity or a NaN shows.
+    __device__ __forceinline__ uint32_t largest() const {
+        uint32_t top = 0;
+        if (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = max(top, word(i) & 0x7FFFFFFFu);
+        } else if (std::is_same<T, __nv_bfloat16>::value) {
+            // The order of the magnitudes is that of their bits.
+            uint32_t even = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                top = max(top, word(i) & 0x7FFF0000u);
+                even = max(even, word(i) & 0x7FFFu);
+            }
+            top = max(top, even << 16);
+        } else {
+            __half2 m = __float2half2_rn(0.f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t v = word(i) & 0x7FFF7FFFu;
+                m = __hmax2_nan(m, *reinterpret_cast<const __half2*>(&v));
+            }
+            const float2 f = __half22float2(m);
+            top = max(abs_bits(f.x), abs_bits(f.y));
+        }
+        return top;
+    }
     __device__ __forceinline__ float get(int i) const {
         if (sizeof(T) == 4) return __uint_as_float(word(i));
         const uint32_t v = word(i >> 1);
@@ -92,8 +119,7 @@ __global__ void __launch_bounds__(256) store_kernel(StoreParams p) {
         if (i >= pieces) break;
         const int r = first + i / per_row, d = i % per_row * 16;
         v[k].load(x + r * xT + d, p.vec[side]);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) top = max(top, abs_bits(v[k].get(j)));
+        top = max(top, v[k].largest());
     }
     float had = first > 0 ? *scale_at : 0.f;
     top = cta_max(top, red);  // its barrier: everyone has read the scale
