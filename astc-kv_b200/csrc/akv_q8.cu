@@ -97,7 +97,7 @@ struct AttnPlan {
     int split, nsplits;          // chunk kernel
     int share_ctas, share_min;   // step kernel
     bool keep_scores; // the step kernel stores its scores for the token weights
-    size_t part_ml, part_o, scores, lse, bytes;  // offsets into the workspace, and its size
+    size_t part_ml, part_o, scores, lse, q_rows, q_factors, bytes;  // offsets into the workspace, and its size
 };
 
 // Rows from which the tcgen05 kernel, whose CTA does 128 or 256 rows for the
@@ -167,7 +167,14 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
     a.part_o = up(parts * sizeof(float2));
     a.scores = a.part_o + up(parts * c.head_dim * sizeof(float));
     a.lse = a.scores + (a.keep_scores ? up(static_cast<size_t>(bh) * c.max_tokens * a.rows * sizeof(float)) : 0);
-    a.bytes = a.lse + (d->weights_dev ? up(static_cast<size_t>(c.batch) * d->q_tokens * d->q_heads * sizeof(float)) : 0) + 16;
+    a.q_rows = a.lse + (d->weights_dev ? up(static_cast<size_t>(c.batch) * d->q_tokens * d->q_heads * sizeof(float)) : 0);
+    a.q_factors = a.q_rows;
+    a.bytes = a.q_rows + 16;
+    if (d->weights_dev && !a.keep_scores) {
+        const size_t groups = static_cast<size_t>(bh) * ((a.rows + 7) / 8), dim = c.head_dim <= 64 ? 64 : c.head_dim <= 128 ? 128 : 256;
+        a.q_factors = a.q_rows + groups * 8 * dim * 2 * (d->q_dtype == AKV_Q_F32 ? 2 : 1);
+        a.bytes = a.q_factors + groups * 8 * sizeof(float) + 16;
+    }
     return a;
 }
 
@@ -192,17 +199,17 @@ int launch_chunk(const AttnParams& p, cudaStream_t s) {
 }
 
 template <int FMT, int DP>
-void launch_weights(const AttnParams& p, cudaStream_t s) {
+int launch_weights(const AttnParams& p, cudaStream_t s) {
     const dim3 grid((p.c.T + kWeightTile - 1) / kWeightTile, p.c.H, p.c.B);
-    if (p.q_dtype == AKV_Q_F32) weights_kernel<FMT, DP, true><<<grid, kWeightThreads, 0, s>>>(p);
-    else weights_kernel<FMT, DP, false><<<grid, kWeightThreads, 0, s>>>(p);
+    if (p.q_dtype == AKV_Q_F32) return launch_after(weights_kernel<FMT, DP, true>, grid, kWeightThreads, s, p);
+    return launch_after(weights_kernel<FMT, DP, false>, grid, kWeightThreads, s, p);
 }
 
 template <int FMT>
-void launch_weights(const AttnParams& p, cudaStream_t s) {
-    if (p.c.D > 128) launch_weights<FMT, 256>(p, s);
-    else if (p.c.D > 64) launch_weights<FMT, 128>(p, s);
-    else launch_weights<FMT, 64>(p, s);
+int launch_weights(const AttnParams& p, cudaStream_t s) {
+    if (p.c.D > 128) return launch_weights<FMT, 256>(p, s);
+    if (p.c.D > 64) return launch_weights<FMT, 128>(p, s);
+    return launch_weights<FMT, 64>(p, s);
 }
 
 }  // namespace
@@ -316,6 +323,8 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     p.scores = plan.keep_scores ? reinterpret_cast<float*>(ws + plan.scores) : nullptr;
     p.lse = d->weights_dev ? reinterpret_cast<float*>(ws + plan.lse) : nullptr;
+    p.q_rows = reinterpret_cast<uint2*>(ws + plan.q_rows);
+    p.q_factors = reinterpret_cast<float*>(ws + plan.q_factors);
     p.out = d->out_dev; p.lse_out = d->lse_dev;
     p.weights = d->weights_dev; p.wstride = d->weights_stride;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -335,15 +344,17 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     const int64_t pieces = plan.chunk ? plan.nsplits : plan.share_ctas / (static_cast<int64_t>(p.c.B) * p.c.H) + 1;
     const bool by_warp = pieces <= 16 && rows >= 1024;
     constexpr int per = kCombineThreads / 32;
-    const int64_t blocks = (by_warp ? (rows + per - 1) / per : rows) + static_cast<int64_t>(p.c.B) * p.c.H * wblocks;
+    const bool recompute = p.weights && !plan.keep_scores;
+    const int64_t packs = recompute ? static_cast<int64_t>(p.c.B) * p.c.H * ((p.R + 7) / 8) : 0;
+    const int64_t blocks = (by_warp ? (rows + per - 1) / per : rows) + (packs + per - 1) / per + static_cast<int64_t>(p.c.B) * p.c.H * wblocks;
     if (blocks > 0x7FFFFFFF) return AKV_ERR_UNSUPPORTED;
     if (blocks) {
         if (int st = launch_after(combine_kernel, dim3(static_cast<unsigned>(blocks)), kCombineThreads, s, p, static_cast<int>(rows), by_warp,
-                                  wblocks, wtokens))
+                                  wblocks, wtokens, static_cast<int>(packs)))
             return st;
     }
-    if (p.weights && !plan.keep_scores) int8 ? launch_weights<AKV_Q8_INT8>(p, s) : launch_weights<AKV_Q8_E4M3>(p, s);
-    return launched();
+    if (recompute) return int8 ? launch_weights<AKV_Q8_INT8>(p, s) : launch_weights<AKV_Q8_E4M3>(p, s);
+    return AKV_OK;
 }
 
 int akv_q8_evict(const AkvQ8EvictDesc* d, void* stream) {

@@ -29,6 +29,8 @@ struct AttnParams {
     int row_group;
     float* part_o;              // ... [D], weighted by 2^-base
     float2* part_ml;            // base (-inf: nothing seen), sum
+    uint2* q_rows;              // query rows as fragments for the weights kernel, see pack_rows
+    float* q_factors;
     float* scores;              // [B][H][T][R], base 2, or NULL
     void* out;
     float* lse;                 // [B][n][Hq], base 2, or NULL
@@ -326,6 +328,48 @@ __device__ __forceinline__ float combined_lse(const AttnParams& p, const Parts& 
     return isnan(l) ? l : all == -CUDART_INF_F ? all : all + log2f(l);
 }
 
+// Eight query rows as fragments of the second operand of S^T = K Q^T, in fp16
+// after a power of two (fp32 rows in two parts), and the factor that turns
+// their products with codes of scale 1 into base-2 scores; by one warp.
+__device__ __forceinline__ void pack_rows(const AttnParams& p, int b, int h, int group) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3, r = 8 * group + g;
+    const int steps = p.c.D <= 64 ? 4 : p.c.D <= 128 ? 8 : 16, parts = p.q_dtype == AKV_Q_F32 ? 2 : 1;
+    const int64_t at = r < p.R ? q_row(p, b, h, r) : 0;
+    uint32_t top = 0;
+    for (int d = 16 * cc; d < p.c.D && r < p.R; d += 64) {
+        float x[16];
+        load_q16(p, at + d, x);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) top = max(top, abs_bits(x[k]));
+    }
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+    top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+    const int e = row_exponent(__uint_as_float(top));
+    const float up = power_of_two(e);
+    const int64_t unit = static_cast<int64_t>(b * p.c.H + h) * ((p.R + 7) / 8) + group;
+    uint2* to = p.q_rows + unit * steps * parts * 32 + lane;
+    for (int j = 0; j < steps / 4; ++j) {
+        const int d = 16 * cc + 64 * j;
+        float x[16];
+        if (d < p.c.D && r < p.R) {
+            load_q16(p, at + d, x);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) x[k] = 0.f;
+        }
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            float y[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[k] = x[4 * s + k] * up;
+            const uint32_t h0 = pack_half2(y[0], y[1]), h1 = pack_half2(y[2], y[3]);
+            to[(4 * j + s) * parts * 32] = make_uint2(h0, h1);
+            if (parts == 2) to[((4 * j + s) * 2 + 1) * 32] = make_uint2(pack_rest(y[0], y[1], h0), pack_rest(y[2], y[3], h1));
+        }
+    }
+    if (cc == 0) p.q_factors[unit * 8 + g] = p.c2 * power_of_two(-e);
+}
+
 // A row by one warp.
 __device__ __forceinline__ void combine_row(const AttnParams& p, const Parts& parts, float all, int64_t row) {
     const int lanes = p.c.D / 4;
@@ -360,9 +404,9 @@ __device__ __forceinline__ void combine_row(const AttnParams& p, const Parts& pa
 // loads in flight each (the kernel is bound by load latency: 37 partials of
 // 64 rows 4 us, against 24 us with one thread per dimension); their sums are
 // added in a fixed order. Where partials are few a warp does a row (by_warp).
-// The other blocks: wtokens tokens of one kv head
-// each: the stored scores of its rows become softmax weights, added up.
-static __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, int rows, bool by_warp, int wblocks, int wtokens) {
+// The other blocks: `packs` groups of eight query rows for the weights kernel,
+// a warp each; or wtokens tokens of one kv head each: the stored scores of its rows become softmax weights, added up.
+static __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnParams p, int rows, bool by_warp, int wblocks, int wtokens, int packs) {
     __shared__ float lse[16];
     __shared__ int ends[16];
     __shared__ float w[kCombineThreads];
@@ -424,6 +468,11 @@ static __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnPar
             a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
         }
         store4(p.out, p.out_dtype, row * D + 4 * x, a);
+        return;
+    }
+    if (packs > 0) {
+        const int i = (blockIdx.x - row_blocks) * (kCombineThreads / 32) + (tid >> 5), groups = (p.R + 7) / 8;
+        if (i < packs) pack_rows(p, i / groups / p.c.H, i / groups % p.c.H, i % groups);
         return;
     }
     const int wb = blockIdx.x - row_blocks, bh = wb / wblocks, b = bh / p.c.H, t0 = wb % wblocks * wtokens;

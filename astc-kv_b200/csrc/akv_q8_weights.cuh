@@ -2,27 +2,42 @@
 // head) are too many to keep their scores: the scores are computed again
 // from K and the finished log-sum-exp, sum over rows of 2^(s - lse).
 //
-// A warp keeps 32 tokens' K as tensor-core fragments in registers and goes
-// through the rows, eight at a time, which the CTA brings to shared memory
-// as fragments (S^T = K Q^T as in the step kernel). A token's weight is
-// summed by one warp in the order of the rows, so it does not depend on
-// timing. Half the products of the attention itself, and one exp2 a score.
+// The query rows are laid out once as tensor-core fragments (by blocks of the
+// combine launch, pack_rows). A warp keeps 32 tokens' K as fragments in
+// registers and goes through the rows, eight at a time (S^T = K Q^T as in the
+// step kernel); the CTA's eight warps are four groups of 32 tokens times two
+// halves of the rows, and the rows' fragments come to shared memory by
+// asynchronous copies one stage ahead. A token's two sums are added in a fixed
+// order, so the result does not depend on timing.
+//
+// Half the products of the attention itself and one exp2 a score: bound by the
+// special-function units (16 exp2 per SM and cycle).
 #pragma once
 #include "akv_q8_attend.cuh"
 
 namespace akv {
 namespace q8 {
 
-constexpr int kWeightWarps = 4;
-constexpr int kWeightThreads = 32 * kWeightWarps;
-constexpr int kWeightTile = 32 * kWeightWarps;  // tokens per CTA
-constexpr int kWeightRows = 32;                 // rows in shared memory at a time
+constexpr int kWeightThreads = 256;
+constexpr int kWeightTile = 128;  // tokens per CTA
+
+// Row groups of a stage: 16 KB of fragments.
+template <int DP, bool QLO>
+constexpr int kWeightGroups = 64 / (DP / 16 * (QLO ? 2 : 1));
+
+__device__ __forceinline__ void copy_async16(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(to))), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <int FMT, int DP, bool QLO>
 __global__ void __launch_bounds__(kWeightThreads) weights_kernel(AttnParams p) {
-    constexpr int KS = DP / 16;
-    __shared__ uint2 qs[kWeightRows / 8][KS][QLO ? 2 : 1][32];
-    __shared__ float3 info[kWeightRows];  // factor, lse, tokens seen
+    constexpr int KS = DP / 16, GROUPS = kWeightGroups<DP, QLO>, PARTS = QLO ? 2 : 1;
+    __shared__ __align__(16) uint2 qs[2][GROUPS][KS][PARTS][32];
+    __shared__ float2 info[2][GROUPS * 8];  // factor, lse
+    __shared__ float half_sum[kWeightTile];
 
     const CacheDev& c = p.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
@@ -31,10 +46,10 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(AttnParams p) {
     const int first = blockIdx.x * kWeightTile;
     float* at = p.weights + static_cast<int64_t>(bh) * p.wstride;
     if (first >= len) {
-        if (!p.accumulate && first + threadIdx.x < c.T) at[first + threadIdx.x] = 0.f;
+        if (!p.accumulate && threadIdx.x < kWeightTile && first + threadIdx.x < c.T) at[first + threadIdx.x] = 0.f;
         return;
     }
-    const int t0 = first + 32 * warp;
+    const int t0 = first + 32 * (warp & 3);
 
     uint32_t a[2][KS][4];
     float ks[2];
@@ -44,16 +59,14 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(AttnParams p) {
         int row = 0;
         const int phys = tt < len ? page_of(c, b, tt, row) : -1;
         const uint8_t* base = c.k.codes + b * c.k.sB + h * c.k.sH + phys * c.k.sP + row * c.k.sT;
-        ks[i] = phys >= 0 ? c.k.scales[b * c.k.cB + h * c.k.cH + phys * c.k.cP + row / c.blk] : 0.f;
+        ks[i] = phys >= 0 ? c.k.scales[scale_offset(c.k, b, h, phys, row / c.blk)] : 0.f;
 #pragma unroll
         for (int j = 0; j < DP / 64; ++j) {
             uint4 w[2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                w[k] = make_uint4(0, 0, 0, 0);
-                if (phys >= 0 && tt + g + 8 * k < len && 16 * cc + 64 * j < c.D)
-                    w[k] = load_stream(base + (g + 8 * k) * c.k.sT + 16 * cc + 64 * j);
-            }
+            for (int k = 0; k < 2; ++k)
+                w[k] = load_stream_if(base + (g + 8 * k) * c.k.sT + 16 * cc + 64 * j,
+                                      phys >= 0 && tt + g + 8 * k < len && 16 * cc + 64 * j < c.D);
             codes_to_half<FMT>(w[0].x, a[i][4 * j][0], a[i][4 * j][2]);
             codes_to_half<FMT>(w[1].x, a[i][4 * j][1], a[i][4 * j][3]);
             codes_to_half<FMT>(w[0].y, a[i][4 * j + 1][0], a[i][4 * j + 1][2]);
@@ -65,85 +78,95 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(AttnParams p) {
         }
     }
 
-    // The first query that sees the CTA's first token; rows end with the queries.
-    const int i0 = p.causal ? max(first - (len - qlen), 0) : 0;
-    const int r_end = qlen * p.G;
+    // Rows from the group of the first query that sees the CTA's first token
+    // to the last query's.
+    const int groups = (p.R + 7) / 8, r_end = qlen * p.G;
+    const int g_first = p.causal ? max(first - (len - qlen), 0) * p.G / 8 : 0, g_end = (r_end + 7) / 8;
+    // Rows from here on see the whole tile. (A row that sees nothing has lse
+    // -inf, which the mask keeps out.)
+    const int r_full = max(p.causal ? first + kWeightTile - 1 - (len - qlen) : (len >= first + kWeightTile ? 0 : qlen), 0) * p.G;
+    const uint2* q = p.q_rows + static_cast<int64_t>(bh) * groups * KS * PARTS * 32;
+    const float* factors = p.q_factors + static_cast<int64_t>(bh) * groups * 8;
+    wait_for_previous_kernel();
+    auto fetch = [&](int g0, int stage) {
+        const int n = min(GROUPS, g_end - g0) * KS * PARTS * 16;  // 16-byte pieces
+        const uint4* from = reinterpret_cast<const uint4*>(q + static_cast<int64_t>(g0) * KS * PARTS * 32);
+        uint4* to = reinterpret_cast<uint4*>(qs[stage]);
+        for (int i = threadIdx.x; i < n; i += kWeightThreads) copy_async16(to + i, from + i);
+        copy_commit();
+        for (int i = threadIdx.x; i < GROUPS * 8; i += kWeightThreads) {
+            const int r = 8 * g0 + i;
+            info[stage][i] = r < r_end ? make_float2(factors[r], p.lse[out_row(p, b, h, r)]) : make_float2(0.f, CUDART_INF_F);
+        }
+    };
     float sum[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-    for (int r0 = i0 * p.G; r0 < r_end; r0 += kWeightRows) {
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < kWeightRows / 8 / kWeightWarps; ++q) {
-            const int grp = warp + q * kWeightWarps, r = r0 + 8 * grp + g;
-            float x[DP / 64][16];
-            float top = 0.f;
-#pragma unroll
-            for (int j = 0; j < DP / 64; ++j) {
-                if (r < r_end && 16 * cc + 64 * j < c.D) {
-                    load_q16(p, q_row(p, b, h, r) + 16 * cc + 64 * j, x[j]);
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) x[j][k] = 0.f;
-                }
-#pragma unroll
-                for (int k = 0; k < 16; ++k) top = __uint_as_float(max(__float_as_uint(top), abs_bits(x[j][k])));
-            }
-            uint32_t tb = __float_as_uint(top);
-            tb = max(tb, __shfl_xor_sync(0xFFFFFFFFu, tb, 1));
-            tb = max(tb, __shfl_xor_sync(0xFFFFFFFFu, tb, 2));
-            const int e = row_exponent(__uint_as_float(tb));
-            const float up = power_of_two(e);
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                float y[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) y[k] = x[s / 4][4 * (s % 4) + k] * up;
-                const uint32_t h0 = pack_half2(y[0], y[1]), h1 = pack_half2(y[2], y[3]);
-                qs[grp][s][0][lane] = make_uint2(h0, h1);
-                if (QLO) qs[grp][s][QLO ? 1 : 0][lane] = make_uint2(pack_rest(y[0], y[1], h0), pack_rest(y[2], y[3], h1));
-            }
-            if (cc == 0) {
-                const int seen = r < r_end ? seen_by(p, r / p.G, len, qlen) : 0;
-                info[8 * grp + g] = make_float3(p.c2 * power_of_two(-e), seen ? p.lse[out_row(p, b, h, r)] : 0.f, __int_as_float(seen));
-            }
+    if (g_first < g_end) fetch(g_first, 0);
+    for (int g0 = g_first, stage = 0; g0 < g_end; g0 += GROUPS, stage ^= 1) {
+        if (g0 + GROUPS < g_end) {
+            fetch(g0 + GROUPS, stage ^ 1);
+            copy_wait<1>();
+        } else {
+            copy_wait<0>();
         }
         __syncthreads();
-#pragma unroll
-        for (int grp = 0; grp < kWeightRows / 8; ++grp) {
-            if (r0 + 8 * grp >= r_end) break;
+        for (int grp = warp >> 2; grp < GROUPS && g0 + grp < g_end; grp += 2) {
             float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
 #pragma unroll
-                for (int q = 0; q < (QLO ? 2 : 1); ++q) {
-                    const uint2 f = qs[grp][k][q][lane];
+                for (int part = 0; part < PARTS; ++part) {
+                    const uint2 f = qs[stage][grp][k][part][lane];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) mma16816(s[i], a[i][k][0], a[i][k][1], a[i][k][2], a[i][k][3], f.x, f.y);
                 }
             }
+            const int r0 = 8 * (g0 + grp);
+            const bool all_seen = r0 >= r_full && r0 + 8 <= r_end;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float3 f = info[8 * grp + 2 * cc + k];
-                const int seen = __float_as_int(f.z);
+                const float2 f = info[stage][8 * grp + 2 * cc + k];
+                const float f0 = ks[0] * f.x, f1 = ks[1] * f.x;
+                float e[2][2];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    e[0][j] = exp2_fast(fmaf(s[0][2 * j + k], f0, -f.y));
+                    e[1][j] = exp2_fast(fmaf(s[1][2 * j + k], f1, -f.y));
+                }
+                if (!all_seen) {
+                    const int r = r0 + 2 * cc + k, seen = r < r_end ? seen_by(p, r / p.G, len, qlen) : 0;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+                            if (t0 + 16 * i + g + 8 * j >= seen) e[i][j] = 0.f;
+                }
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
-                        if (t0 + 16 * i + g + 8 * j < seen) sum[i][j] += exp2_fast(s[i][2 * j + k] * (ks[i] * f.x) - f.y);
+                    for (int j = 0; j < 2; ++j) sum[i][j] += e[i][j];
             }
         }
+        __syncthreads();  // the stage may be filled again
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            float w = sum[i][j];
-            w += __shfl_xor_sync(0xFFFFFFFFu, w, 1);
-            w += __shfl_xor_sync(0xFFFFFFFFu, w, 2);
+            sum[i][j] += __shfl_xor_sync(0xFFFFFFFFu, sum[i][j], 1);
+            sum[i][j] += __shfl_xor_sync(0xFFFFFFFFu, sum[i][j], 2);
+            if (warp >= 4 && cc == 0) half_sum[32 * (warp & 3) + 16 * i + g + 8 * j] = sum[i][j];
+        }
+    __syncthreads();
+    if (warp >= 4 || cc != 0) return;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
             const int t = t0 + 16 * i + g + 8 * j;
-            if (cc == 0 && t < c.T) {
-                if (!p.accumulate) at[t] = t < len ? w : 0.f;
-                else if (t < len) at[t] += w;
-            }
+            if (t >= c.T) continue;
+            const float w = sum[i][j] + half_sum[t - first];
+            if (!p.accumulate) at[t] = t < len ? w : 0.f;
+            else if (t < len) at[t] += w;
         }
 }
 
