@@ -59,7 +59,7 @@ def _rows(name: str, t: torch.Tensor, shape: tuple) -> tuple:
     return t.data_ptr(), t.stride()[:3]
 
 
-@dataclass
+@dataclass(eq=False)
 class Q8Cache:
     """K and V codes with their scales.
 
@@ -327,7 +327,7 @@ class Q8Attention(_Call):
 class Q8Evict(_Call):
     """Keep min(len, keep) tokens per sequence and kv head: the first `sinks`,
     the last `recent`, and those with the largest `weights` [B, H, T], packed
-    in their order into `dst`, a cache in other memory. run() returns (kept
+    in their order into `dst`, a cache in other memory that holds whole blocks. run() returns (kept
     token indices [B, H, keep] with -1 after the last, lengths [B], the kept
     tokens' weights [B, H, dst.max_tokens], 0 after the last): what the next
     steps go on with."""
@@ -341,6 +341,8 @@ class Q8Evict(_Call):
             raise ValueError("src and dst must agree in format, batch, kv_heads and head_dim")
         if not 0 < keep <= dst.max_tokens or sinks < 0 or recent < 0 or sinks + recent > keep:
             raise ValueError("keep must fit dst, and sinks + recent must fit keep")
+        if dst.k.shape[2] % dst.block_tokens:
+            raise ValueError("dst must hold whole blocks")
         B, H = src.batch, src.kv_heads
         if weights.dtype != torch.float32 or weights.dim() != 3 or tuple(weights.shape[:2]) != (B, H) or \
                 weights.shape[2] < src.max_tokens or not weights.is_contiguous():

@@ -73,7 +73,8 @@ int check_attention(const AkvQ8AttnDesc* d) {
         return AKV_ERR_INVALID_ARGUMENT;
     if (d->split_tokens < 0 || d->split_tokens % 16 || !(d->scale >= 0.f) || std::isinf(d->scale)) return AKV_ERR_INVALID_ARGUMENT;
     if (d->weights_dev && d->weights_stride < d->cache.max_tokens) return AKV_ERR_INVALID_ARGUMENT;
-    if (static_cast<int64_t>(d->q_heads) * d->q_tokens > 1 << 24) return AKV_ERR_UNSUPPORTED;
+    const int64_t rows = static_cast<int64_t>(d->q_heads) * d->q_tokens;
+    if (rows > 1 << 24 || rows * d->cache.batch > 1 << 30) return AKV_ERR_UNSUPPORTED;
     return AKV_OK;
 }
 
@@ -347,7 +348,6 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     const bool recompute = p.weights && !plan.keep_scores;
     const int64_t packs = recompute ? static_cast<int64_t>(p.c.B) * p.c.H * ((p.R + 7) / 8) : 0;
     const int64_t blocks = (by_warp ? (rows + per - 1) / per : rows) + (packs + per - 1) / per + static_cast<int64_t>(p.c.B) * p.c.H * wblocks;
-    if (blocks > 0x7FFFFFFF) return AKV_ERR_UNSUPPORTED;
     if (blocks) {
         if (int st = launch_after(combine_kernel, dim3(static_cast<unsigned>(blocks)), kCombineThreads, s, p, static_cast<int>(rows), by_warp,
                                   wblocks, wtokens, static_cast<int>(packs)))

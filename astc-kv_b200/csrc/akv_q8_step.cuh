@@ -99,8 +99,9 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
         // Sequences without tokens or queries are nobody's share.
         for (int e = blockIdx.x; e < c.B; e += gridDim.x) {
             if (share_chunks(p, e) > 0) continue;
-            for (int i = threadIdx.x; i < p.n * p.Hq * c.D; i += kStepThreads)
-                store_elem(p.out, p.out_dtype, static_cast<int64_t>(e) * p.n * p.Hq * c.D + i, 0.f);
+            const int64_t values = static_cast<int64_t>(p.n) * p.Hq * c.D;
+            for (int64_t i = 4 * threadIdx.x; i < values; i += 4 * kStepThreads)
+                store4(p.out, p.out_dtype, e * values + i, make_float4(0.f, 0.f, 0.f, 0.f));
             for (int i = threadIdx.x; i < p.n * p.Hq; i += kStepThreads) {
                 const int64_t row = static_cast<int64_t>(e) * p.n * p.Hq + i;
                 if (p.lse) p.lse[row] = -CUDART_INF_F;

@@ -30,7 +30,8 @@ extern "C" {
  *     scales[b*scale_stride_batch + h*scale_stride_head + phys*scale_stride_page
  *            + row / block_tokens].
  * Code strides are bytes and multiples of 16, codes 16-byte aligned; scale
- * strides are elements. Scales are >= 0; a scale below 2^-90 counts as 2^-90
+ * strides are elements. All page_tokens rows of a page are the cache's own
+ * memory (an eviction writes whole blocks). Scales are >= 0; a scale below 2^-90 counts as 2^-90
  * where V's softmax weights are formed. A NaN scale makes what reads it NaN.
  */
 typedef struct AkvQ8Side {
@@ -52,7 +53,8 @@ typedef struct AkvQ8Cache {
     AkvQ8Side k, v;
     int32_t* status_dev;            /* optional: kernels write AKV_ERR_BAD_BLOCK_TABLE (an entry outside
                                        [0, num_pages): reads as zeros, writes are dropped) or
-                                       AKV_ERR_INVALID_ARGUMENT (a store outside [0, max_tokens)) here */
+                                       AKV_ERR_INVALID_ARGUMENT (a store outside [0, max_tokens)) here, or
+                                       AKV_ERR_TIMEOUT (a bounded wait inside a kernel ran out: its rows are NaN) */
 } AkvQ8Cache;
 
 /*

@@ -622,6 +622,7 @@ def test_python_refusals(cuda):
         lambda: Q8Evict(cache, to, w, i, keep=8, sinks=4, recent=5),
         lambda: Q8Evict(cache, cache, w, i, keep=8),
         lambda: Q8Evict(cache, to, w[:1], i, keep=8),
+        lambda: Q8Evict(cache, Q8Cache(z[:, :, :40].clone(), z[:, :, :40].clone(), s.clone(), s.clone(), block_tokens=32), w, i, keep=8),
     ]
     for n, f in enumerate(refused):
         with pytest.raises(ValueError):
