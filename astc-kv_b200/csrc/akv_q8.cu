@@ -120,10 +120,11 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
     const int64_t bh = static_cast<int64_t>(c.batch) * c.kv_heads;
     a.rows = d->q_tokens * (d->q_heads / c.kv_heads);
     a.nt = c.head_dim <= 128 && a.rows > 8 ? 2 : 1;
-    a.chunk = a.rows >= kChunkMinRows && c.head_dim <= 128 && d->q_dtype != AKV_Q_F32 && d->out_dtype != AKV_Q_F32;
+    a.chunk = a.rows >= kChunkMinRows && d->q_dtype != AKV_Q_F32 && d->out_dtype != AKV_Q_F32;
     a.keep_scores = !a.chunk && d->weights_dev && a.rows <= 8 * a.nt && a.rows <= kScoreRows;
     a.split = d->split_tokens;
-    const int group = a.chunk ? kChunkRows : 8 * a.nt;  // rows of a CTA
+    const bool shared = a.chunk && a.rows <= 128 && c.head_dim <= 128;  // its two tiles share the rows and take every other step
+    const int group = a.chunk ? (c.head_dim <= 128 ? 256 : 128) : 8 * a.nt;  // rows of a CTA
     if (a.split == 0 && a.chunk) {
         // One CTA per SM: the number of splits whose last wave is fullest, up
         // to eight or one wave; each costs a partial to write and read again.
@@ -149,7 +150,7 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
             a.split *= 2;
             a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);
         }
-        if (a.rows <= 128) a.nsplits *= 2;  // its two tiles share the rows and take every other step
+        if (shared) a.nsplits *= 2;
         parts = a.nsplits > 1 ? static_cast<size_t>(bh) * a.nsplits * a.rows : 0;
     } else {
         // One wave of CTAs (see the step kernel), two pieces each; no more
@@ -188,13 +189,15 @@ int launch_chunk(const AttnParams& p, cudaStream_t s) {
         return AKV_ERR_CUDA;
     }
     const int parts = SHARED ? p.nsplits / 2 : p.nsplits;
-    const dim3 grid(parts * ((p.R + kChunkRows - 1) / kChunkRows), p.c.H, p.c.B);
+    constexpr int rows = 128 * kChunkTiles<DP>;
+    const dim3 grid(parts * ((p.R + rows - 1) / rows), p.c.H, p.c.B);
     kern<<<grid, kChunkThreads, bytes, s>>>(p);
     return launched();
 }
 
 template <int FMT>
 int launch_chunk(const AttnParams& p, cudaStream_t s) {
+    if (p.c.D > 128) return launch_chunk<FMT, 256, false>(p, s);
     if (p.R <= 128) return p.c.D > 64 ? launch_chunk<FMT, 128, true>(p, s) : launch_chunk<FMT, 64, true>(p, s);
     return p.c.D > 64 ? launch_chunk<FMT, 128, false>(p, s) : launch_chunk<FMT, 64, false>(p, s);
 }

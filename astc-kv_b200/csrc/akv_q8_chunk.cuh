@@ -39,7 +39,10 @@
 namespace akv {
 namespace q8 {
 
-constexpr int kChunkRows = 256;    // rows of a CTA
+// A CTA's tiles of 128 rows and its stages of K and V: with head_dim above 128
+// one O tile fills half of the tensor memory, and one stage the shared memory.
+template <int DP>
+constexpr int kChunkTiles = DP <= 128 ? 2 : 1;
 constexpr int kChunkTokens = 128;  // per step
 constexpr int kChunkHalf = 64;     // P goes to the tensor cores in two parts
 constexpr int kChunkThreads = 32 * 20;  // five warpgroups; warps 17-19 only give their registers away
@@ -48,9 +51,9 @@ constexpr int kMetaSlots = 4;      // K may be written three steps ahead of a so
 template <int DP>
 struct ChunkSmem {
     // Operand tiles of 64 x 16-bit columns, 128 bytes a row, swizzled.
-    uint8_t q[2][DP / 64][128 * 128];
-    uint8_t k[2][DP / 64][128 * 128];
-    uint8_t v[2][2][DP * 128];
+    uint8_t q[kChunkTiles<DP>][DP / 64][128 * 128];
+    uint8_t k[kChunkTiles<DP>][DP / 64][128 * 128];
+    uint8_t v[kChunkTiles<DP>][2][DP * 128];
     float4 meta[kMetaSlots][kChunkTokens / 16];  // K's scale, log2 and reciprocal of V's, for 16 tokens
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], pv_done[2], done;
     uint32_t tmem;
@@ -167,16 +170,18 @@ __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (
 template <int FMT, int DP, bool SHARED>
 __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     using Smem = ChunkSmem<DP>;
+    constexpr int TILES = kChunkTiles<DP>, STAGES = TILES, ROWS = 128 * TILES;
+    static_assert(!SHARED || TILES == 2, "two tiles to share rows");
     extern __shared__ uint8_t smem_raw[];
     // The swizzle counts from 1024-byte boundaries.
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw + (-smem_addr(smem_raw) & 1023));
     const CacheDev& c = p.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int tiles = (p.R + kChunkRows - 1) / kChunkRows;
+    const int tiles = (p.R + ROWS - 1) / ROWS;
     // Later rows see more tokens: they go first.
     const int parts = SHARED ? p.nsplits / 2 : p.nsplits;  // CTAs along the tokens
-    const int split = blockIdx.x % parts, r0 = (tiles - 1 - blockIdx.x / parts) * kChunkRows, h = blockIdx.y, b = blockIdx.z;
-    const int len = len_of(p, b), qlen = q_len_of(p, b), rows = min(kChunkRows, p.R - r0);
+    const int split = blockIdx.x % parts, r0 = (tiles - 1 - blockIdx.x / parts) * ROWS, h = blockIdx.y, b = blockIdx.z;
+    const int len = len_of(p, b), qlen = q_len_of(p, b), rows = min(ROWS, p.R - r0);
     const int bh = b * c.H + h;
     const int64_t unit = (static_cast<int64_t>(bh) * p.nsplits + (SHARED ? 2 * split : split)) * p.R + r0;
     const int end = r0 / p.G < qlen ? seen_by(p, min((r0 + rows - 1) / p.G, qlen - 1), len, qlen) : 0;
@@ -224,7 +229,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     float factor = 0.f;
     int bound = 0;
     bool blind = true;
-    if (warp < 8) {
+    if (warp < 4 * TILES) {
         const int tile = warp >> 2, r = threadIdx.x & 127, at_row = SHARED ? r : threadIdx.x, row = r0 + at_row;
         const bool in = at_row < rows;
         const int64_t at = in ? q_row(p, b, h, row) : 0;
@@ -272,9 +277,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     const uint32_t tmem = sm.tmem;
 
     // Steps of a tile: all, or every other one.
-    const bool two = SHARED || rows > 128;  // else the second tile rests
-    // Registers go to where they are needed: 2 x 136 + 2 x 80 + 48 = 5 x 96.
-    if (warp < 8) {
+    const bool two = TILES == 2 && (SHARED || rows > 128);  // else the second tile rests
+    // Registers go to where they are needed: 2 x 136 + 2 x 80 + 48 = 5 x 96,
+    // with one tile 136 + 24 + 2 x 136 + 48.
+    if (TILES == 1 && warp >= 4 && warp < 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
+    } else if (warp < 8) {
         // ------------------------------------------------------------ softmax
         asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         const int tile = warp >> 2;
@@ -436,7 +444,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         }
     } else if (warp < 12) {
         // ---------------------------------------------------------- K to fp16
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         // Four lanes a row of a 64-column tile, 32 rows at a time: the stores
         // of eight lanes (two rows, every other chunk) fall into different
         // banks.
@@ -492,9 +501,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         load_meta(t_begin);
         load_k(t_begin);
         for (int j = 0; j < steps; ++j) {
-            const int st = j & 1;
+            const int st = j % STAGES;
             // The phase before a stage's first use counts as over.
-            if (!bar_wait(&sm.k_empty[st], (j >> 1 & 1) ^ 1, &sm.abort)) break;
+            if (!bar_wait(&sm.k_empty[st], (j / STAGES & 1) ^ 1, &sm.abort)) break;
             if (tid < 8) {
                 const float lv = log2_fast(vs < 8.0779357e-28f ? 8.0779357e-28f : vs);  // a NaN stays one
                 sm.meta[j % kMetaSlots][tid] = make_float4(ks, lv, exp2_fast(-lv), 0.f);
@@ -518,12 +527,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         }
     } else if (warp < 16) {
         // ---------------------------------------------------------- V to fp16
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        if (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         // Eight lanes take the 64 tokens of a tile row, eight tokens each.
         const int w = warp & 3;
         constexpr int VW = DP / 32;  // words of a token per lane
         const int v_tok = 64 * (w & 1) + 8 * (lane & 7), v_d = (w >> 1) * (DP / 2) + (lane >> 3) * (DP / 8);
         const uint8_t* head = c.v.codes + b * c.v.sB + h * c.v.sH + (v_d < c.D ? v_d : 0);
+        const int next16 = v_d + 16 < c.D ? 16 : 0;  // of 32 bytes a lane the second half
         uint32_t vr[8][VW];
         auto load_v = [&](int t0) {
             const int t = t0 + v_tok;
@@ -538,15 +549,19 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                     vr[i][0] = x.x; vr[i][1] = x.y;
                 } else {
                     const uint4 x = load_stream_if(at, i < left);
-                    vr[i][0] = x.x; vr[i][1] = x.y; vr[i][VW - 2] = x.z; vr[i][VW - 1] = x.w;
+                    vr[i][0] = x.x; vr[i][1] = x.y; vr[i][VW > 2 ? 2 : 0] = x.z; vr[i][VW > 2 ? 3 : 1] = x.w;
+                }
+                if (DP == 256) {
+                    const uint4 x = load_stream_if(at + next16, i < left);
+                    vr[i][VW - 4 > 0 ? VW - 4 : 0] = x.x; vr[i][VW - 3 > 0 ? VW - 3 : 0] = x.y; vr[i][VW - 2] = x.z; vr[i][VW - 1] = x.w;
                 }
                 at += c.v.sT;
             }
         };
         load_v(t_begin);
         for (int j = 0; j < steps; ++j) {
-            const int st = j & 1;
-            if (!bar_wait(&sm.v_empty[st], (j >> 1 & 1) ^ 1, &sm.abort)) break;
+            const int st = j % STAGES;
+            if (!bar_wait(&sm.v_empty[st], (j / STAGES & 1) ^ 1, &sm.abort)) break;
             uint8_t* tile = sm.v[st][w & 1];
 #pragma unroll
             for (int x = 0; x < VW; ++x) {
@@ -611,28 +626,26 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             }
             for (int j = 0; j < steps && alive; ++j) {
                 // The step after this one of the same tiles.
-                const int st = j & 1, next = SHARED ? j + 2 : j + 1, nx = next & 1, turn = SHARED ? j >> 1 : j;
+                const int st = j % STAGES, next = SHARED ? j + 2 : j + 1, nx = next % STAGES, turn = SHARED ? j >> 1 : j;
                 const bool more = next < steps;
-                alive = bar_wait(&sm.v_full[st], j >> 1 & 1, &sm.abort);
-                if (more && !SHARED) alive = bar_wait(&sm.k_full[nx], next >> 1 & 1, &sm.abort) && alive;
-                for (int i = SHARED ? 2 * st : 0; i < (SHARED ? 2 * st + 2 : 2 * tiles_here); ++i) {
+                alive = bar_wait(&sm.v_full[st], j / STAGES & 1, &sm.abort);
+                if (more && !SHARED) alive = bar_wait(&sm.k_full[nx], next / STAGES & 1, &sm.abort) && alive;
+                const int i_end = SHARED ? 2 * st + 2 : 2 * tiles_here;
+                for (int i = SHARED ? 2 * st : 0; i < i_end; ++i) {
                     const int tile = i >> 1, half = i & 1;
                     alive = __all_sync(0xFFFFFFFFu, alive && bar_wait(&sm.p_full[tile][half], turn & 1, &sm.abort));
                     if (!alive) break;
                     fence_after();
                     values(tile, half, st, turn > 0 || half > 0);
+                    if (lead && i == i_end - 1) mma_commit(&sm.v_empty[st]);
                     if (!more || half == 0) continue;
                     if (SHARED) {
-                        alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.k_full[nx], next >> 1 & 1, &sm.abort));
+                        alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.k_full[nx], next / STAGES & 1, &sm.abort));
                         if (!alive) break;
                         fence_after();
                     }
                     scores(tile, nx);
-                }
-                if (!alive) break;
-                if (lead) {
-                    mma_commit(&sm.v_empty[st]);
-                    if (more) mma_commit(&sm.k_empty[nx]);
+                    if (lead && i == i_end - 1) mma_commit(&sm.k_empty[nx]);
                 }
             }
             // Also after giving up: nothing may be in flight when the tensor

@@ -166,6 +166,46 @@ def test_many_tokens(cuda, n, T, q_lens, lens, D, G, od):
     check_attention(cache, k, v, q, lens, q_lens, out_dtype=od)
 
 
+@pytest.mark.parametrize("D,G,n,T", [(256, 4, 9, 40), (256, 8, 33, 300), (240, 2, 64, 129), (144, 1, 200, 517), (256, 1, 33, 33)])
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_many_tokens_of_wide_heads(cuda, D, G, n, T, fmt):
+    cache, k, v = make(2, 1, T, D, fmt=fmt, block=16, seed=D + n)
+    q = torch.randn(2, n, G, D, device="cuda").half()
+    check_attention(cache, k, v, q, [T, max(T // 2, n)], [n, n // 2 + 1], out_dtype=torch.float16)
+
+
+@pytest.mark.parametrize("page,block", [(48, 16), (96, 32), (16, 16), (640, 128)])
+@pytest.mark.parametrize("n", [1, 9, 70])
+@pytest.mark.parametrize("D", [128, 256])
+def test_page_sizes_that_are_no_powers_of_two(cuda, page, block, n, D):
+    cache, k, v = make(2, 2, 1000, D, block=block, page=page, spare=3, seed=page + n)
+    q = torch.randn(2, n, 8, D, device="cuda").bfloat16()
+    check_attention(cache, k, v, q, [1000, 333], out_dtype=torch.bfloat16)
+    check_attention(cache, k, v, q, [997, 150])
+
+
+@pytest.mark.parametrize("n,od", [(1, torch.float32), (3, torch.float32), (20, torch.bfloat16)])
+def test_many_sequences(cuda, n, od):
+    """More sequences than a CTA has threads, many of them empty."""
+    B = 300
+    cache, k, v = make(B, 1, 200, 64, block=16, seed=n)
+    q = torch.randn(B, n, 2, 64, device="cuda").bfloat16()
+    r = np.random.default_rng(n)
+    lens = [int(x) if x % 3 else 0 for x in r.integers(0, 201, B)]
+    q_lens = [int(x) for x in r.integers(0, n + 1, B)]
+    check_attention(cache, k, v, q, lens, q_lens, out_dtype=od)
+    check_attention(cache, k, v, q, [0] * B, q_lens, out_dtype=od, accumulate=False)
+
+
+@pytest.mark.parametrize("T,lens", [(4096, [4096, 1]), (4000, [63, 0]), (700, [700, 449])])
+@pytest.mark.parametrize("G", [1, 4, 8])
+def test_one_token_of_few_heads(cuda, T, lens, G):
+    cache, k, v = make(2, 2, T, 128, fmt="fp8", block=64, seed=T + G)
+    q = torch.randn(2, 2 * G, 128, device="cuda")
+    check_attention(cache, k, v, q, lens)
+    check_attention(cache, k, v, q.half(), lens, out_dtype=torch.float16, accumulate=False)
+
+
 @pytest.mark.parametrize("n", [1, 4, 50])
 def test_not_causal_and_scale(cuda, n):
     cache, k, v = make(2, 1, 333, 64, seed=3)
