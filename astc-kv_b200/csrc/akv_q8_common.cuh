@@ -143,20 +143,16 @@ __device__ __forceinline__ float block_inverse(float scale) { return scale > 0.f
 
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 
-// Element loads and stores of the three 16/32-bit types.
+// Two floats as a pair of a 16-bit type.
 template <typename T>
-__device__ __forceinline__ float to_f32(T x) { return static_cast<float>(x); }
-template <>
-__device__ __forceinline__ float to_f32<__half>(__half x) { return __half2float(x); }
-template <>
-__device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-
-template <typename T>
-__device__ __forceinline__ T from_f32(float x) { return static_cast<T>(x); }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
 
 }  // namespace q8
 }  // namespace akv

@@ -91,23 +91,23 @@ __global__ void __launch_bounds__(256) store_kernel(StoreParams p) {
     __shared__ uint32_t red[8];
     const CacheDev& c = p.c;
     const int h = blockIdx.y, b = blockIdx.z >> 1, side = blockIdx.z & 1;
-    const int64_t start = p.start[b];
-    const int64_t count = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
-    if (start < 0 || start + count > c.T) {
+    const int start = p.start[b], count = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
+    if (start < 0 || static_cast<int64_t>(start) + count > c.T) {
         if (threadIdx.x == 0 && blockIdx.x == 0) report(c.status, AKV_ERR_INVALID_ARGUMENT);
-        if (start < 0) return;
+        if (start < 0 || start >= c.T) return;
     }
-    const int64_t end = min(start + count, static_cast<int64_t>(c.T));
-    const int64_t block0 = (start / c.blk + blockIdx.x) * c.blk;  // first token of this block
-    const int first = static_cast<int>(max(start, block0) - block0);  // rows [first, last) are new
-    const int last = static_cast<int>(min(end - block0, static_cast<int64_t>(c.blk)));
+    const int end = start + min(count, c.T - start), shift = 31 - __clz(c.blk);
+    const int64_t first_token = (static_cast<int64_t>(start >> shift) + blockIdx.x) << shift;  // of this block
+    if (first_token >= end) return;
+    const int block0 = static_cast<int>(first_token);
+    const int first = max(start - block0, 0), last = min(end - block0, c.blk);  // rows [first, last) are new
     if (last <= first) return;
     int row0;
-    const int phys = page_of(c, b, static_cast<int>(block0), row0);
+    const int phys = page_of(c, b, block0, row0);
     if (phys < 0) return;
     const SideDev& s = side ? c.v : c.k;
     uint8_t* codes = s.codes + code_offset(s, b, h, phys, row0);
-    float* scale_at = s.scales + scale_offset(s, b, h, phys, row0 / c.blk);
+    float* scale_at = s.scales + scale_offset(s, b, h, phys, row0 >> shift);
     const T* x = static_cast<const T*>(p.x[side]) + b * p.xB[side] + h * p.xH[side] + (block0 - start) * p.xT[side];
     const int64_t xT = p.xT[side];
     const int per_row = c.D / 16, pieces = (last - first) * per_row;
@@ -191,20 +191,27 @@ __global__ void __launch_bounds__(256) restore_kernel(RestoreParams p) {
     float scale = 0.f;
     if (phys >= 0) {
         w = *reinterpret_cast<const uint4*>(s.codes + code_offset(s, b, h, phys, row) + d);
-        scale = s.scales[scale_offset(s, b, h, phys, row / c.blk)];
+        scale = s.scales[scale_offset(s, b, h, phys, row >> (31 - __clz(c.blk)))];
     }
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-    __align__(16) T o[16];
+    uint32_t o[4 * sizeof(T)];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         float f[4];
         from_codes4<FMT>(u[k], f);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[4 * k + j] = from_f32<T>(__fmul_rn(f[j], scale));
+        for (int j = 0; j < 4; ++j) f[j] = __fmul_rn(f[j], scale);
+        if (sizeof(T) == 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[sizeof(T) == 4 ? 4 * k + j : 0] = __float_as_uint(f[j]);
+        } else {
+            o[2 * k] = pack2<T>(f[0], f[1]);
+            o[2 * k + 1] = pack2<T>(f[2], f[3]);
+        }
     }
     uint4* out = reinterpret_cast<uint4*>(static_cast<T*>(p.out[side]) + (static_cast<int64_t>(b) * p.n * per_token + i) * 16);
 #pragma unroll
-    for (int k = 0; k < static_cast<int>(sizeof(T)); ++k) out[k] = reinterpret_cast<const uint4*>(o)[k];
+    for (int k = 0; k < static_cast<int>(sizeof(T)); ++k) out[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
 }
 
 }  // namespace q8
