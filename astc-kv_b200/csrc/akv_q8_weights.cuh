@@ -10,8 +10,9 @@
 // asynchronous copies one stage ahead. A token's two sums are added in a fixed
 // order, so the result does not depend on timing.
 //
-// Half the products of the attention itself and one exp2 a score: bound by the
-// special-function units (16 exp2 per SM and cycle).
+// Half the products of the attention itself and one exp2 a score, of which an
+// SM does 16 a cycle: 90 us for 3 x 452 query tokens against 18578, 16/16
+// heads, D 64, where it takes 274 us.
 #pragma once
 #include "akv_q8_attend.cuh"
 
