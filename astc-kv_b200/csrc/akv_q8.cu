@@ -126,20 +126,27 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
     const bool shared = a.chunk && a.rows <= 128 && c.head_dim <= 128;  // its two tiles share the rows and take every other step
     const int group = a.chunk ? (c.head_dim <= 128 ? 256 : 128) : 8 * a.nt;  // rows of a CTA
     if (a.split == 0 && a.chunk) {
-        // One CTA per SM: the number of splits whose last wave is fullest, up
-        // to eight or one wave; each costs a partial to write and read again.
+        // One CTA per SM. In steps of 128 tokens a CTA costs its share of the
+        // tokens, about three to start and, when split, 2.5 (D 128) for a
+        // partial written and read; the number of splits, up to eight or one
+        // wave, is that of the least cost over the waves. Where lengths may be
+        // ragged more splits are taken for up to 15 %: short sequences then
+        // leave SMs to long ones (4 sequences of 559 to 8190 tokens, 9/3
+        // heads, 509 query tokens and their weights: 118 against 148 us).
         const int64_t units = bh * ((a.rows + group - 1) / group), sms = sm_count();
         const int64_t steps = (static_cast<int64_t>(c.max_tokens) + kChunkTokens - 1) / kChunkTokens;
         const int64_t most = units > 0 && sms / units > 8 ? sms / units : 8;
+        const auto cost = [&](int64_t n) {
+            const double each = static_cast<double>((steps + n - 1) / n) + 3.0 + (n > 1 ? 2.5 * c.head_dim / 128 : 0.0);
+            return static_cast<double>((units * n + sms - 1) / sms) * each;
+        };
+        double least = cost(1);
+        for (int64_t n = 2; n <= most && n <= steps; ++n) least = cost(n) < least ? cost(n) : least;
         int64_t best = 1;
-        double least = 0;
-        for (int64_t n = 1; n <= most && n * 4 <= steps + 3; ++n) {
-            const double waves = static_cast<double>((units * n + sms - 1) / sms) * ((steps + n - 1) / n) * (n > 1 ? 1.02 + 0.01 * n : 1.0);
-            if (n == 1 || waves < least) {
-                best = n;
-                least = waves;
-            }
-        }
+        const double limit = d->seq_lens_dev && c.batch > 1 ? 1.15 * least : least;
+        for (int64_t n = 2; n <= most && n <= steps; ++n)
+            if (cost(n) <= limit) best = n;
+        if (cost(1) <= least) best = best > 1 && limit > least ? best : 1;
         a.split = static_cast<int>((steps + best - 1) / best * kChunkTokens);
     }
     size_t parts;  // rows of partials
@@ -381,7 +388,8 @@ int akv_q8_evict(const AkvQ8EvictDesc* d, void* stream) {
     p.keep = d->keep; p.sinks = d->sinks; p.recent = d->recent;
     p.kept = d->kept_dev; p.out_lens = d->out_lens_dev; p.out_weights = d->out_weights_dev; p.ostride = d->out_weights_stride;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    select_kernel<<<dim3(a.kv_heads, a.batch), kSelectThreads, 0, s>>>(p);
+    if (a.max_tokens <= 8 * kSelectThreads) select_kernel<8><<<dim3(a.kv_heads, a.batch), kSelectThreads, 0, s>>>(p);
+    else select_kernel<32><<<dim3(a.kv_heads, a.batch), kSelectThreads, 0, s>>>(p);
     if (int st = launched()) return st;
     const dim3 grid((p.keep + p.dst.blk - 1) / p.dst.blk, a.kv_heads, a.batch);
     const bool few = c.block_tokens * (c.head_dim / 16) <= 512;  // pieces of a block

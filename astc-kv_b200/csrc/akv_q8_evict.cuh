@@ -52,24 +52,25 @@ __device__ __forceinline__ int cta_scan(int v, int* warp_sums, int* total) {
     return x - v + (warp ? warp_sums[warp - 1] : 0);
 }
 
-// Runs of the row that a thread looks at, so that its kept tokens are in
-// order: whole groups of four where the row allows vector loads.
-__device__ __forceinline__ int run_length(int n) { return ((n + kSelectThreads - 1) / kSelectThreads + 3) / 4 * 4; }
-
 // One CTA per (kv head, sequence). The middle tokens' cut-off is the key of
 // the last one that stays; it is found 11, 11 and 10 bits at a time, by a
-// histogram of the keys that agree with the bits found. Then every thread
-// counts what its own run of tokens keeps (keys above the cut-off, and of the
-// equal ones the first few), a scan over the threads gives the places, and a
-// second look writes. The row is read five times, from L2 after the first.
-// Measured, 256 rows of 841 to 32768 weights: 70 us, as long as the longest
-// row takes one CTA.
-static __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictParams p) {
+// histogram of the keys that agree with the bits found. Then votes give every
+// kept token its place among its warp's (keys above the cut-off, and of the
+// equal ones the first few of the row), and a scan over the warps the rest.
+//
+// A warp has a run of the row of its own and a lane every 32nd token of it, of
+// which it keeps HELD weights in registers; of rows of more than 1024 x HELD
+// the rest is read again in every pass, from L2. (HELD 8 for caches of up to
+// 8192 tokens: an eviction of 8192 to 1001 tokens takes 17 us with its restore, 25 us with
+// the code unrolled for 32.) Measured, 256 rows of 841
+// to 32768 weights: 40 us; reading the row in each of five passes 70 us.
+template <int HELD>
+__global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictParams p) {
     __shared__ int hist[2048];
     __shared__ int sums[32];
     __shared__ uint32_t s_prefix;
     __shared__ int s_want;
-    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+    const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int64_t unit = static_cast<int64_t>(b) * p.src.H + h;
     const float* w = p.weights + unit * p.wstride;
     int32_t* kept = p.kept + unit * p.keep;
@@ -90,6 +91,19 @@ static __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictPara
         return;
     }
     const int lo = p.sinks, hi = len - p.recent;
+    const int rounds = (len + kSelectThreads - 1) / kSelectThreads;  // of a warp's run, 32 tokens each
+    const int t0 = warp * rounds * 32 + lane;
+    float held[HELD];
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) held[k] = k < rounds && t0 + 32 * k < len ? w[t0 + 32 * k] : 0.f;
+    // Calls f with the token and its weight, in order, every lane of the warp
+    // alike; tokens from len on are not there.
+    auto for_tokens = [&](auto f) {
+#pragma unroll
+        for (int k = 0; k < HELD; ++k)
+            if (k < rounds) f(t0 + 32 * k, held[k]);
+        for (int k = HELD; k < rounds; ++k) f(t0 + 32 * k, t0 + 32 * k < len ? w[t0 + 32 * k] : 0.f);
+    };
     uint32_t prefix = 0;
     int want = p.keep - p.sinks - p.recent;  // of the tokens whose key agrees with `prefix` so far
     const bool none = want == 0;
@@ -99,20 +113,14 @@ static __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictPara
         hist[tid] = hist[tid + kSelectThreads] = 0;
         __syncthreads();
         int zeros = 0;  // tokens that never received weight are many: one bin
-        for (int t = lo + tid; t < hi; t += 8 * kSelectThreads) {
-            float x[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = t + k * kSelectThreads < hi ? w[t + k * kSelectThreads] : 0.f;
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const uint32_t key = order_key(x[k]);
-                if (pass == 0 && key == 0x80000000u) zeros += t + k * kSelectThreads < hi;
-                else if (t + k * kSelectThreads < hi && (pass == 0 || ((key ^ prefix) >> (shift + (pass == 1 ? 11 : 10))) == 0))
-                    atomicAdd(&hist[(key >> shift) & mask], 1);
-            }
-        }
+        for_tokens([&](int t, float x) {
+            const uint32_t key = order_key(x);
+            if (t < lo || t >= hi) return;
+            if (pass == 0 && key == 0x80000000u) ++zeros;
+            else if (pass == 0 || ((key ^ prefix) >> (shift + (pass == 1 ? 11 : 10))) == 0) atomicAdd(&hist[(key >> shift) & mask], 1);
+        });
         zeros = __reduce_add_sync(0xFFFFFFFFu, zeros);
-        if (zeros && (tid & 31) == 0) atomicAdd(&hist[0x80000000u >> 21], zeros);
+        if (zeros && lane == 0) atomicAdd(&hist[0x80000000u >> 21], zeros);
         __syncthreads();
         // Bins from the highest down, two a thread.
         const int d = 2047 - 2 * tid, upper = hist[d], lower = hist[d - 1];
@@ -127,33 +135,41 @@ static __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictPara
         prefix = s_prefix;
         want = s_want;
     }
-    const int run = run_length(len), t0 = min(tid * run, len), t1 = min(t0 + run, len);
-    int above = 0, equal = 0;
-    for (int t = t0; t < t1; ++t) {
-        const uint32_t key = order_key(w[t]);
-        const bool fixed = t < lo || t >= hi;
-        above += fixed || (!none && key > prefix);
-        equal += !fixed && !none && key == prefix;
-    }
-    int total;
-    const int equal_before = cta_scan(equal, sums, &total);
-    const int take = max(0, min(equal, want - equal_before));
-    int at = cta_scan(above + take, sums, &total), left = take;
-    for (int t = t0; t < t1; ++t) {
-        const float x = w[t];
+    // What a token is: kept for its place or its key, or equal to the cut-off.
+    auto kind = [&](int t, float x, bool& above, bool& equal) {
         const uint32_t key = order_key(x);
-        const bool fixed = t < lo || t >= hi;
-        bool in = fixed || (!none && key > prefix);
-        if (!in && !none && key == prefix && left > 0) {
-            in = true;
-            --left;
-        }
+        const bool in = t < len, fixed = in && (t < lo || t >= hi);
+        above = fixed || (in && !none && key > prefix);
+        equal = in && !fixed && !none && key == prefix;
+    };
+    int above = 0, equal = 0;  // of the warp's run
+    for_tokens([&](int t, float x) {
+        bool a, e;
+        kind(t, x, a, e);
+        above += __popc(__ballot_sync(0xFFFFFFFFu, a));
+        equal += __popc(__ballot_sync(0xFFFFFFFFu, e));
+    });
+    int total;
+    int left = want - cta_scan(lane == 0 ? equal : 0, sums, &total);  // equal ones that the run may keep
+    left = __shfl_sync(0xFFFFFFFFu, left, 0);
+    const int take = max(0, min(equal, left));
+    int at = cta_scan(lane == 0 ? above + take : 0, sums, &total);
+    at = __shfl_sync(0xFFFFFFFFu, at, 0);
+    const uint32_t below = (1u << lane) - 1;
+    for_tokens([&](int t, float x) {
+        bool a, e;
+        kind(t, x, a, e);
+        const uint32_t equals = __ballot_sync(0xFFFFFFFFu, e);
+        const bool in = a || (e && __popc(equals & below) < left);
+        const uint32_t ins = __ballot_sync(0xFFFFFFFFu, in);
         if (in) {
-            kept[at] = t;
-            ow[at] = x;
-            ++at;
+            const int place = at + __popc(ins & below);
+            kept[place] = t;
+            ow[place] = x;
         }
-    }
+        at += __popc(ins);
+        left -= __popc(equals);
+    });
 }
 
 // Largest |code| of four, as fp16 (exact; a NaN code stays one).
