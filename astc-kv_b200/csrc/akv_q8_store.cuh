@@ -91,7 +91,7 @@ struct Piece {
 // coding them. Rows that a growing block holds already are read, coded again
 // and written in place.
 template <int FMT, typename T, int PP>
-__global__ void __launch_bounds__(256) store_kernel(StoreParams p) {
+__global__ void __launch_bounds__(256, PP == 2 ? (sizeof(T) == 2 ? 6 : 4) : 1) store_kernel(StoreParams p) {
     __shared__ uint32_t red[8];
     const CacheDev& c = p.c;
     const int h = blockIdx.y, b = blockIdx.z >> 1, side = blockIdx.z & 1;
