@@ -346,10 +346,11 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     // A step kernel of one CTA leaves nothing to combine.
     const bool combine = plan.chunk ? plan.nsplits > 1 : !plan.cluster && plan.share_ctas > 1;
     const int64_t rows = combine ? static_cast<int64_t>(p.c.B) * p.c.H * p.R : 0;
-    // Tokens per CTA of the weights part: some 1000 CTAs where there are tokens
-    // enough, since each first works out the rows' log-sum-exps.
+    // Tokens per CTA of the weights part: one wave of CTAs where there are
+    // tokens enough, since each first works out the rows' log-sum-exps (B2,
+    // 131071 tokens: 126 us the whole call, with four times the CTAs 133).
     int wtokens = kCombineThreads;
-    while (wtokens < 2048 && static_cast<int64_t>(p.c.B) * p.c.H * p.c.T / wtokens > 8 * sm_count()) wtokens *= 2;
+    while (wtokens < 8192 && static_cast<int64_t>(p.c.B) * p.c.H * p.c.T / wtokens > 4 * sm_count()) wtokens *= 2;
     const int wblocks = plan.keep_scores ? (p.c.T + wtokens - 1) / wtokens : 0;
     // Partials of a row: of all rows alike, or as the shares fall.
     const int64_t pieces = plan.chunk ? plan.nsplits : plan.share_ctas / (static_cast<int64_t>(p.c.B) * p.c.H) + 1;
