@@ -410,7 +410,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         const bool in = my_row < rows;
         const int r = r0 + my_row;
         const int64_t part = unit + my_row + (SHARED && tile ? p.R : 0);
-        const bool none = blind || (!started && !isnan(l));
+        if (!alive) l = CUDART_NAN_F;  // gave up: the rows become NaN
+        const bool none = alive && (blind || (!started && !isnan(l)));
         const float inv = none ? 0.f : 1.f / l;
         const int64_t row = in ? out_row(p, b, h, r) : 0;
 #pragma unroll 1
@@ -418,7 +419,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             uint32_t o[16];
             tmem_ld16(o, o_at + 16 * g);
             tmem_wait_ld(o);
-            if (!in || 16 * g >= c.D || !alive) {
+            if (!in || 16 * g >= c.D) {
             } else if (p.nsplits > 1) {
                 uint4* to = reinterpret_cast<uint4*>(p.part_o + part * c.D + 16 * g);
 #pragma unroll
@@ -442,7 +443,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             __syncwarp();
         }
         if (in) {
-            if (!alive) l = CUDART_NAN_F;
             if (p.nsplits > 1) {
                 p.part_ml[part] = make_float2(none ? -CUDART_INF_F : isnan(l) ? l : base, l);
             } else {
