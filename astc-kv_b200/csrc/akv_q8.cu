@@ -93,7 +93,7 @@ int sm_count() {
 struct AttnPlan {
     int rows;         // per kv head
     bool chunk;       // the tcgen05 kernel, else the step kernel
-    bool cluster;     // the step kernel's clusters
+    int cluster;      // CTAs of the step kernel's clusters, 0 without
     int nt;           // groups of eight rows per CTA
     int split, nsplits;          // chunk kernel
     int share_ctas, share_min;   // step kernel
@@ -107,10 +107,11 @@ struct AttnPlan {
 // 80 us against 51; 32 rows, B8 x 8192 90 against 92).
 constexpr int kChunkMinRows = 33;
 
-// Tokens up to which a cluster of eight CTAs for each kv head (which all have
-// to fit the GPU at once) beats even shares of all CTAs and a second launch
-// (B1 x 4096, 32/8 heads: 16.0 us against 18.8).
-constexpr int kClusterTokens = 4096;
+// Tokens for each CTA of a cluster up to which a cluster for each kv head of
+// each sequence beats even shares of all CTAs and a second launch (32/8 heads:
+// B1 x 4096 in clusters of eight 16.0 us against 18.8; B64 x 300, a CTA each,
+// 22 against 30, the same ragged to 500 tokens 19 against 27).
+constexpr int kClusterTokens = 512;
 
 // Rows whose scores are stored for the token weights rather than computed
 // again: storing costs 8 bytes per row and token, a second pass over K
@@ -172,7 +173,10 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
         a.share_ctas = static_cast<int>(ctas > 0 ? ctas : 1);
         a.nsplits = 0;
         parts = 2 * static_cast<size_t>(a.share_ctas) * group;
-        a.cluster = a.split == 0 && a.rows <= 8 && bh * kStepCluster <= slots && c.max_tokens <= kClusterTokens;
+        // The largest cluster with which all units fit the GPU at once.
+        int size = kStepCluster;
+        while (size > 1 && bh * size > slots) size /= 2;
+        a.cluster = a.split == 0 && a.rows <= 8 && c.max_tokens <= kClusterTokens * size ? size : 0;
     }
     const auto up = [](size_t x) { return (x + 15) / 16 * 16; };
     a.part_ml = 0;
@@ -333,7 +337,7 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     p.q = d->q_dev; p.qB = d->q_stride[0]; p.qT = d->q_stride[1]; p.qH = d->q_stride[2];
     p.lens = d->seq_lens_dev; p.q_lens = d->q_lens_dev;
     p.split = plan.split; p.nsplits = plan.nsplits;
-    p.share_ctas = plan.chunk ? 0 : plan.cluster ? -1 : plan.share_ctas; p.share_min = plan.share_min; p.row_group = 8 * plan.nt;
+    p.share_ctas = plan.chunk ? 0 : plan.cluster ? -plan.cluster : plan.share_ctas; p.share_min = plan.share_min; p.row_group = 8 * plan.nt;
     p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
     p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     p.scores = plan.keep_scores ? reinterpret_cast<float*>(ws + plan.scores) : nullptr;

@@ -24,7 +24,7 @@ struct AttnParams {
     // Partials: of the chunk kernel [B][H][nsplits][R] rows, of the step
     // kernel two pieces for each CTA, row_group rows each (see Parts).
     int split, nsplits;         // tokens per split
-    int share_ctas;             // CTAs of the step kernel, 0 for the chunk kernel, -1 for the step kernel's clusters
+    int share_ctas;             // CTAs of the step kernel, 0 for the chunk kernel, minus the size of its clusters
     int share_min;              // chunks that a share has at least
     int row_group;
     float* part_o;              // ... [D], weighted by 2^-base

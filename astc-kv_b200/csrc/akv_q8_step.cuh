@@ -74,8 +74,8 @@ __device__ __forceinline__ float4 load_remote4(const void* p, int rank) {
 // P is the second part, so that one product does both. The power that the
 // products draw slows the clock: B32, 32768 tokens int8, run for seconds at the
 // 1000 W power cap, 402 us against 410 (349 against 345 in short runs).
-// CLUSTER: eight CTAs divide one unit and add up its pieces through distributed
-// shared memory; for little work, where the scan of the lengths and a second
+// CLUSTER: up to eight CTAs divide one unit and add up its pieces through
+// distributed shared memory; for little work, where the scan of the lengths and a second
 // launch would cost more than an even division saves (B1, 384 tokens, 9/3
 // heads: 8.2 us against 12.3; B8, 1024 tokens, 32/8 heads: 15.7 against 24.8).
 // DP: head_dim rounded up to 64, 128 or 256; NT: groups of 8 rows; PLO: P in
@@ -100,10 +100,10 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     const int groups = (p.R + ROWS - 1) / ROWS, units = c.H * groups;  // of a sequence
     int64_t at = 0, stop = 1;  // the next chunk of this CTA's share, its end
     int b, unit_of_b, chunk;
-    const int rank = CLUSTER ? blockIdx.x % kStepCluster : 0;
+    const int ranks = CLUSTER ? -p.share_ctas : 1, rank = CLUSTER ? blockIdx.x % ranks : 0;
     if constexpr (CLUSTER) {
-        b = blockIdx.x / kStepCluster / units;
-        unit_of_b = blockIdx.x / kStepCluster % units;
+        b = blockIdx.x / ranks / units;
+        unit_of_b = blockIdx.x / ranks % units;
         chunk = 0;
     } else {
         // Sequences without tokens or queries are nobody's share.
@@ -132,8 +132,8 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     const int n_chunks = share_chunks(p, b);
     int n_mine;
     if constexpr (CLUSTER) {
-        chunk = rank * n_chunks / kStepCluster;
-        n_mine = (rank + 1) * n_chunks / kStepCluster - chunk;
+        chunk = rank * n_chunks / ranks;
+        n_mine = (rank + 1) * n_chunks / ranks - chunk;
         at = stop;
     } else {
         n_mine = static_cast<int>(min(static_cast<int64_t>(n_chunks - chunk), stop - at));
@@ -511,13 +511,13 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     if constexpr (CLUSTER) {
         __syncthreads();
         cluster_sync();
-        // Row r is finished by CTA r % 8, its pieces in the order of the CTAs.
-        for (int r = rank; r < rows; r += kStepCluster) {
+        // Row r is finished by CTA r % ranks, its pieces in the order of the CTAs.
+        for (int r = rank; r < rows; r += ranks) {
             float top = -CUDART_INF_F, sum = 0.f;
             float2 v[kStepCluster];
 #pragma unroll
             for (int k = 0; k < kStepCluster; ++k) {
-                v[k] = load_remote2(&piece[r], k);
+                v[k] = k < ranks ? load_remote2(&piece[r], k) : make_float2(-CUDART_INF_F, 0.f);
                 top = fmaxf(top, v[k].x);
             }
 #pragma unroll

@@ -12,10 +12,10 @@ int launch_step(const AttnParams& p, cudaStream_t s) {
         if (p.share_ctas < 0) {
             cudaLaunchAttribute attr;
             attr.id = cudaLaunchAttributeClusterDimension;
-            attr.val.clusterDim.x = kStepCluster;
+            attr.val.clusterDim.x = static_cast<unsigned>(-p.share_ctas);
             attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
             cudaLaunchConfig_t cfg = {};
-            cfg.gridDim = dim3(static_cast<unsigned>(p.c.B * p.c.H * kStepCluster));
+            cfg.gridDim = dim3(static_cast<unsigned>(p.c.B) * p.c.H * static_cast<unsigned>(-p.share_ctas));
             cfg.blockDim = dim3(kStepThreads);
             cfg.stream = s;
             cfg.attrs = &attr;

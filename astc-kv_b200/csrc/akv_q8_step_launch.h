@@ -6,7 +6,7 @@
 namespace akv {
 namespace q8 {
 
-constexpr int kStepCluster = 8;   // CTAs of a cluster
+constexpr int kStepCluster = 8;   // CTAs of a cluster at most
 constexpr int kStepWarps = 4;     // warps of a CTA, a tile of 16 tokens each
 
 inline int launched() { return cudaPeekAtLastError() == cudaSuccess ? AKV_OK : (cudaGetLastError(), AKV_ERR_CUDA); }
