@@ -310,8 +310,18 @@ __device__ __forceinline__ Parts find_parts(const AttnParams& p, int b, int h, i
     return {i1 - i0 + 1, i0 == i1, rest + (s.start(i0) == at ? 0 : p.row_group), rest, step};
 }
 
-// Base-2 log-sum-exp of a row over its partials, by one warp; all lanes get it.
-__device__ __forceinline__ float combined_lse(const AttnParams& p, const Parts& parts) {
+// A row's sum of 2^score over its partials, sum * 2^top. The two stay apart
+// where outputs are divided by it: as one number, top + log2 sum, a score of
+// 1000 leaves 14 bits for the sum.
+struct RowSum {
+    float top, sum;  // -inf, 0: nothing seen; a NaN is in `sum`
+    __device__ __forceinline__ bool none() const { return top == -CUDART_INF_F && !isnan(sum); }
+    __device__ __forceinline__ float inverse() const { return none() ? 0.f : 1.f / sum; }
+    __device__ __forceinline__ float lse() const { return isnan(sum) ? sum : none() ? top : top + log2f(sum); }
+};
+
+// By one warp; all lanes get it.
+__device__ __forceinline__ RowSum combined_sum(const AttnParams& p, const Parts& parts) {
     const int lane = threadIdx.x & 31;
     float m = -CUDART_INF_F, l = 0.f;
     for (int s = lane; s < parts.n; s += 32) {
@@ -325,7 +335,7 @@ __device__ __forceinline__ float combined_lse(const AttnParams& p, const Parts& 
     for (int o = 16; o; o >>= 1) all = fmaxf(all, __shfl_xor_sync(0xFFFFFFFFu, all, o));
     l = m == -CUDART_INF_F && !isnan(l) ? 0.f : l * exp2f(m - all);
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, o);
-    return isnan(l) ? l : all == -CUDART_INF_F ? all : all + log2f(l);
+    return {all, l};
 }
 
 // Eight query rows as fragments of the second operand of S^T = K Q^T, in fp16
@@ -371,8 +381,9 @@ __device__ __forceinline__ void pack_rows(const AttnParams& p, int b, int h, int
 }
 
 // A row by one warp.
-__device__ __forceinline__ void combine_row(const AttnParams& p, const Parts& parts, float all, int64_t row) {
+__device__ __forceinline__ void combine_row(const AttnParams& p, const Parts& parts, const RowSum& all, int64_t row) {
     const int lanes = p.c.D / 4;
+    const float inv = all.inverse();
     for (int x = threadIdx.x & 31; x < lanes; x += 32) {
         float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int s0 = 0; s0 < parts.n; s0 += 4) {
@@ -388,19 +399,19 @@ __device__ __forceinline__ void combine_row(const AttnParams& p, const Parts& pa
             }
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float w = f[k] == -CUDART_INF_F ? 0.f : exp2f(f[k] - all);
+                const float w = f[k] == -CUDART_INF_F ? 0.f : exp2f(f[k] - all.top);
                 a.x = fmaf(v[k].x, w, a.x);
                 a.y = fmaf(v[k].y, w, a.y);
                 a.z = fmaf(v[k].z, w, a.z);
                 a.w = fmaf(v[k].w, w, a.w);
             }
         }
-        store4(p.out, p.out_dtype, row * p.c.D + 4 * x, a);
+        store4(p.out, p.out_dtype, row * p.c.D + 4 * x, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
     }
 }
 
 // The first blocks: `rows` rows of the output, each its partials weighted
-// by 2^(m - lse). Groups of D / 4 threads take every so many-th partial, four
+// by 2^(m - top), over the row's sum. Groups of D / 4 threads take every so many-th partial, four
 // loads in flight each (the kernel is bound by load latency: with one thread
 // per dimension 128 partials of 128 rows took 36 us); their sums are
 // added in a fixed order. Where partials are few a warp does a row (by_warp).
@@ -420,11 +431,12 @@ static __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnPar
         const int r = i % p.R, bh = i / p.R, h = bh % p.c.H, b = bh / p.c.H, D = p.c.D;
         const Parts parts = find_parts(p, b, h, r);  // every warp for itself
         if (parts.done) return;
-        const float all = combined_lse(p, parts);
+        const RowSum all = combined_sum(p, parts);
         const int64_t row = out_row(p, b, h, r);
         if (by_warp ? (tid & 31) == 0 : tid == 0) {
-            if (p.lse) p.lse[row] = all;
-            if (p.lse_out) p.lse_out[row] = all * 0.69314718055994531f;
+            const float lse = all.lse();
+            if (p.lse) p.lse[row] = lse;
+            if (p.lse_out) p.lse_out[row] = lse * 0.69314718055994531f;
         }
         if (by_warp) {
             combine_row(p, parts, all, row);
@@ -437,7 +449,7 @@ static __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnPar
             __syncthreads();
             if (s0 + tid < parts.n) {
                 const float m = p.part_ml[parts.row(s0 + tid)].x;
-                w[tid] = m == -CUDART_INF_F ? 0.f : exp2f(m - all);
+                w[tid] = m == -CUDART_INF_F ? 0.f : exp2f(m - all.top);
             }
             __syncthreads();
             const int n = min(kCombineThreads, parts.n - s0);
@@ -467,7 +479,8 @@ static __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnPar
             const float4 v = part[k * lanes + x];
             a.x += v.x; a.y += v.y; a.z += v.z; a.w += v.w;
         }
-        store4(p.out, p.out_dtype, row * D + 4 * x, a);
+        const float inv = all.inverse();
+        store4(p.out, p.out_dtype, row * D + 4 * x, make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv));
         return;
     }
     if (packs > 0) {
@@ -481,7 +494,7 @@ static __global__ void __launch_bounds__(kCombineThreads) combine_kernel(AttnPar
     const int h = bh % p.c.H;
     for (int r = tid >> 5; r < p.R; r += kCombineThreads / 32) {
         const Parts parts = find_parts(p, b, h, r);
-        const float v = parts.done ? p.lse[out_row(p, b, h, r)] : combined_lse(p, parts);
+        const float v = parts.done ? p.lse[out_row(p, b, h, r)] : combined_sum(p, parts).lse();
         if ((tid & 31) == 0) {
             lse[r] = v;
             ends[r] = seen_by(p, r / p.G, len, qlen);

@@ -1,0 +1,51 @@
+"""Attention of many rows (query tokens x heads of a kv head) over the 8-bit
+cache: the forms with 16-bit queries and outputs, whose kernel takes 33 rows
+and more, in one tile of rows, in two that share them, and with wide heads.
+Plain implementations and bounds are those of test_gpu_q8.py."""
+import math
+
+import pytest
+import torch
+
+from test_gpu_q8 import MOST, make
+
+pytestmark = pytest.mark.gpu
+
+# head_dim, query heads per kv head, query tokens: rows shared by two tiles, tiles of their own, several of them, wide heads.
+SHAPES = [(64, 1, 40), (128, 4, 32), (128, 2, 100), (64, 3, 90), (128, 4, 150), (256, 1, 40), (240, 2, 90)]
+
+
+def one_hot(fmt, D, G, n, T, size, sign, at, seed):
+    """A cache and queries whose scores are `size` times numbers of order one, the one of token `at` far above the
+    others. Returns also the score of `at` (scale 1)."""
+    cache, k, v = make(1, 2, T, D, fmt=fmt, block=32, seed=seed)
+    c = torch.zeros(k.shape, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    low, high = (-96, 97) if sign > 0 else (64, 121)
+    c[..., 0] = torch.randint(low // 8, high // 8, k.shape[:3], generator=g, device="cuda").float() * 8
+    c[:, :, at, 0] = 120 if sign > 0 else 16
+    cache.k.copy_(c.to(cache.k.dtype))  # multiples of 8: e4m3 holds them too
+    cache.k_scales.fill_(1 / 128)
+    q = torch.zeros(1, n, 2 * G, D, device="cuda")
+    q[..., 0] = sign * size
+    return cache, v, q, sign * size * float(c[0, 0, at, 0]) / 128
+
+
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 14, 2.0 ** 17])
+@pytest.mark.parametrize("D,G,n,T,od", [(D, G, n, n + 333, torch.bfloat16) for D, G, n in SHAPES] + [
+    (64, 3, 1, 9000, torch.float32), (128, 4, 1, 5000, torch.float32), (128, 8, 1, 700, torch.float32),
+    (128, 4, 5, 3000, torch.float32), (256, 2, 1, 6000, torch.float32), (128, 4, 20, 2000, torch.float32)])
+def test_large_scores_in_pieces(cuda, D, G, n, T, od, size):
+    """Rows whose tokens several CTAs divide: the pieces are divided by their sum, not by the log-sum-exp, whose last
+    bit is worth 2^-24 of the scores. One token has all the weight; an output is its V row, off by the rounding of the
+    weight (to fp16 with 16-bit outputs) and of the output."""
+    from astc_kv_cuda import Q8Attention
+    for at in (3, T - n):
+        cache, v, q, score = one_hot("int8", D, G, n, T, size, 1, at, seed=n)
+        lens = torch.full((1,), T, dtype=torch.int32, device="cuda")
+        call = Q8Attention(q.bfloat16(), cache, lens, scale=1.0, out_dtype=od, lse=True)
+        out = call.run().double().view(1, n, 2, G, D)
+        want = v[:, :, at].view(1, 1, 2, 1, D).expand_as(out)
+        off = 2.0 ** -18 + (2.0 ** -10 + 2.0 ** -8 if od == torch.bfloat16 else 0.0)
+        assert ((out - want).abs() <= off * want.abs()).all()
+        assert ((call.lse.double() - score).abs() <= 2.0 ** -20 * abs(score) + 2.0 ** -18).all()
