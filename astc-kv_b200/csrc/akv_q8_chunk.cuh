@@ -311,21 +311,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                 if (!alive) break;
                 fence_after();
             }
-            if (__any_sync(0xFFFFFFFFu, t0 + kChunkHalf > bound)) {
-                // What a row does not see becomes a score that no factor
-                // brings back.
-#pragma unroll 1
-                for (int g = 0; g < 4; ++g) {
-                    uint32_t s[16];
-                    tmem_ld16(s, s_at + 16 * g);
-                    tmem_wait_ld(s);
-#pragma unroll
-                    for (int k = 0; k < 16; ++k)
-                        if (t0 + 16 * g + k >= bound) s[k] = __float_as_uint(-3e38f);
-                    tmem_st16(s_at + 16 * g, s);
-                }
-                tmem_wait_st();
-            }
             if (__any_sync(0xFFFFFFFFu, !started)) {
                 // The largest t of the row's tokens.
                 float m = -CUDART_INF_F;
@@ -337,7 +322,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                     tmem_wait_ld(s);
 #pragma unroll
                     for (int k = 0; k < 16; ++k)
-                        if (t0 + 16 * g + k < bound) m = fmaxf(m, fmaf(__uint_as_float(s[k]), fmaxf(factor * mt.x, 1e-30f), mt.y));
+                        if (t0 + 16 * g + k < bound) m = fmaxf(m, fmaf(__uint_as_float(s[k]), factor * mt.x, mt.y));
                 }
                 if (!started && m != -CUDART_INF_F) {
                     base = m - 6.f;
@@ -346,8 +331,29 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                 __syncwarp();
             }
             uint32_t pk[32];
-            float add;
-            while (true) {
+            float add, shift = 0.f;
+            bool placed = false;  // S holds t, less `shift`, of this half
+            for (int tries = 0;; ++tries) {
+                // Where a row does not see every token, or has a base without
+                // the bits to bring an exact score within 15 of it, S becomes t
+                // itself: -inf for what is not seen, and scores that are
+                // rounded first, to the base's own multiples, so that one raise
+                // is enough to bring them below 15. (`tries` is a limit all the same.)
+                if (!placed && __any_sync(0xFFFFFFFFu, t0 + kChunkHalf > bound || fabsf(base) >= 1048576.f)) {
+#pragma unroll 1
+                    for (int g = 0; g < 4; ++g) {
+                        uint32_t s[16];
+                        tmem_ld16(s, s_at + 16 * g);
+                        const float4 mt = meta[g];
+                        tmem_wait_ld(s);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            s[k] = __float_as_uint(t0 + 16 * g + k < bound ? fmaf(__uint_as_float(s[k]), factor * mt.x, mt.y) - base : -CUDART_INF_F);
+                        tmem_st16(s_at + 16 * g, s);
+                    }
+                    tmem_wait_st();
+                    placed = true;
+                }
                 float m = -CUDART_INF_F;
                 add = 0.f;
                 uint32_t s[2][16];
@@ -358,8 +364,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                     tmem_wait_ld(x);
                     if (g < 3) tmem_ld16(s[(g + 1) & 1], s_at + 16 * (g + 1));
                     const float4 mt = meta[g];
-                    // A NaN scale has to stay one.
-                    const float f0 = factor * mt.x, f = f0 < 1e-30f ? 1e-30f : f0, off = mt.y - base;
+                    const float f = placed ? 1.f : factor * mt.x, off = placed ? -shift : mt.y - base;
                     const uint64_t f2 = pair_of(f, f), off2 = pair_of(off, off);
                     uint64_t sum = 0;
 #pragma unroll
@@ -374,12 +379,14 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
                     const float2 both = halves(sum);
                     add = fmaf(both.x + both.y, mt.z, add);
                 }
-                if (!__any_sync(0xFFFFFFFFu, m > 15.f)) break;
+                if (!__any_sync(0xFFFFFFFFu, m > 15.f) || tries == 8) break;
                 // Some row's p leaves fp16: raise its base, scale its sums, again.
                 const float up = m > 15.f ? m - 6.f : 0.f;
-                const float alpha = exp2_fast(-up);
-                base += up;
+                const float to = base + up, alpha = exp2_fast(base - to);
+                shift += to - base;
+                base = to;
                 l *= alpha;
+                if (!placed) shift = 0.f;
                 if (i > 0) {
                     // The last P V of the tile may still be running.
                     alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.pv_done[tile], (i - 1) & 1, &sm.abort));

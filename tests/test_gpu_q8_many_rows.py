@@ -49,3 +49,22 @@ def test_large_scores_in_pieces(cuda, D, G, n, T, od, size):
         off = 2.0 ** -18 + (2.0 ** -10 + 2.0 ** -8 if od == torch.bfloat16 else 0.0)
         assert ((out - want).abs() <= off * want.abs()).all()
         assert ((call.lse.double() - score).abs() <= 2.0 ** -20 * abs(score) + 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 22, 2.0 ** 27, 2.0 ** 29, 2.0 ** 33, 2.0 ** 70, 2.0 ** 120])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("D,G,n", SHAPES)
+def test_scores_of_any_magnitude(cuda, D, G, n, fmt, sign, size):
+    """The softmax weight of one token is 1 (up to rounding it to fp16), whatever the size of the scores; tokens that
+    are not seen do not count, even where every score is far below 0."""
+    from astc_kv_cuda import Q8Attention
+    T = n + 333
+    for at in (3, T - n):
+        cache, v, q, score = one_hot(fmt, D, G, n, T, size, sign, at, seed=n)
+        lens = torch.full((1,), T, dtype=torch.int32, device="cuda")
+        call = Q8Attention(q.bfloat16(), cache, lens, scale=1.0, out_dtype=torch.bfloat16, lse=True)
+        out = call.run().double().view(1, n, 2, G, D)
+        want = v[:, :, at].view(1, 1, 2, 1, D).expand_as(out)
+        assert ((out - want).abs() <= (2.0 ** -10 + 2.0 ** -8 + 2.0 ** -18) * want.abs()).all()
+        assert ((call.lse.double() - score).abs() <= 2.0 ** -20 * abs(score) + 2.0 ** -18).all()
