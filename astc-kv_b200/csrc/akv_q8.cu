@@ -155,6 +155,8 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
     }
     size_t parts;  // rows of partials
     if (a.chunk) {
+        // Whole steps: a step's tokens past the split's end would count as seen.
+        a.split = static_cast<int>((static_cast<int64_t>(a.split < c.max_tokens ? a.split : c.max_tokens) + kChunkTokens - 1) / kChunkTokens * kChunkTokens);
         a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);
         const int64_t limit = 0x7FFFFFFF / ((a.rows + group - 1) / group + 1);
         while (a.nsplits > limit) {  // the grid holds splits x row groups

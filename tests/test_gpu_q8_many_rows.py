@@ -2,12 +2,11 @@
 cache: the forms with 16-bit queries and outputs, whose kernel takes 33 rows
 and more, in one tile of rows, in two that share them, and with wide heads.
 Plain implementations and bounds are those of test_gpu_q8.py."""
-import math
 
 import pytest
 import torch
 
-from test_gpu_q8 import MOST, make
+from test_gpu_q8 import check_attention, make
 
 pytestmark = pytest.mark.gpu
 
@@ -68,3 +67,12 @@ def test_scores_of_any_magnitude(cuda, D, G, n, fmt, sign, size):
         want = v[:, :, at].view(1, 1, 2, 1, D).expand_as(out)
         assert ((out - want).abs() <= (2.0 ** -10 + 2.0 ** -8 + 2.0 ** -18) * want.abs()).all()
         assert ((call.lse.double() - score).abs() <= 2.0 ** -20 * abs(score) + 2.0 ** -18).all()
+
+
+@pytest.mark.parametrize("split", [16, 48, 64, 192, 512])
+@pytest.mark.parametrize("D,G,n", SHAPES)
+def test_splits_of_any_length(cuda, D, G, n, split):
+    """split_tokens may be any multiple of 16; what lies between a split's end and the next step's is not a token."""
+    cache, k, v = make(2, 2, n + 800, D, page=128 if D == 128 else 0, block=32, seed=D + n)
+    q = torch.randn(2, n, 2 * G, D, device="cuda").bfloat16()
+    check_attention(cache, k, v, q, [n + 800, n + 77], out_dtype=torch.bfloat16, split=split)
