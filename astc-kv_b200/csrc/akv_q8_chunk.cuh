@@ -521,8 +521,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             // The phase before a stage's first use counts as over.
             if (!bar_wait(&sm.k_empty[st], (j / STAGES & 1) ^ 1, &sm.abort)) break;
             if (tid < 8) {
-                const float lv = log2_fast(vs < 8.0779357e-28f ? 8.0779357e-28f : vs);  // a NaN stays one
-                sm.meta[j % kMetaSlots][tid] = make_float4(ks, lv, exp2_fast(-lv), 0.f);
+                // A NaN scale stays one in lv, for rows that see it, and not in
+                // the reciprocal, which all rows' sums take.
+                const float lv = log2_fast(vs < 8.0779357e-28f ? 8.0779357e-28f : vs);
+                sm.meta[j % kMetaSlots][tid] = make_float4(ks, lv, isnan(lv) ? 0.f : exp2_fast(-lv), 0.f);
             }
 #pragma unroll
             for (int i = 0; i < KP; ++i) {

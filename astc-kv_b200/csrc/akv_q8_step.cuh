@@ -331,9 +331,10 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
             }
         }
         const float ks = kscale;
-        // A NaN scale has to stay one.
+        // A NaN scale has to stay one: in lv, which makes the scores of what is
+        // seen NaN; in iv it would reach the sums of rows that do not see it.
         const float vs = vscale < 8.0779357e-28f ? 8.0779357e-28f : vscale;
-        const float lv = log2_fast(vs), iv = exp2_fast(-lv);
+        const float lv = log2_fast(vs), iv = isnan(lv) ? 0.f : exp2_fast(-lv);
         next_tile();
         load_k();
         load_v(v_next, vscale_next);

@@ -6,7 +6,7 @@ Plain implementations and bounds are those of test_gpu_q8.py."""
 import pytest
 import torch
 
-from test_gpu_q8 import check_attention, make
+from test_gpu_q8 import check_attention, make, plain_attention
 
 pytestmark = pytest.mark.gpu
 
@@ -76,3 +76,36 @@ def test_splits_of_any_length(cuda, D, G, n, split):
     cache, k, v = make(2, 2, n + 800, D, page=128 if D == 128 else 0, block=32, seed=D + n)
     q = torch.randn(2, n, 2 * G, D, device="cuda").bfloat16()
     check_attention(cache, k, v, q, [n + 800, n + 77], out_dtype=torch.bfloat16, split=split)
+
+
+@pytest.mark.parametrize("what", ["k_scales", "v_scales"])
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("D,G,n,od", [(D, G, n, torch.bfloat16) for D, G, n in SHAPES] + [
+    (64, 2, 4, torch.float32), (128, 4, 20, torch.float32), (128, 4, 4, torch.bfloat16), (256, 2, 50, torch.float32)])
+def test_nan_scale_shows_where_it_is_seen(cuda, D, G, n, od, fmt, what):
+    """A block with a NaN scale among the queries' own tokens: queries that see a token of it are NaN, queries that
+    end before it, queries past q_lens and queries that see nothing are as without it."""
+    from astc_kv_cuda import Q8Attention
+    T, block = n + 256, 16
+    cache, k, v = make(3, 2, T, D, fmt=fmt, block=block, seed=n + D)
+    lens, q_lens = [T, T - 5, n // 2], [n, n - 3, n]
+    q = torch.randn(3, n, 2 * G, D, device="cuda").bfloat16()
+    ref, lse, _, A, vmax = plain_attention(q, k, v, lens, q_lens)
+    first = []  # of the block's tokens
+    for b in range(3):
+        at = (lens[b] - 2) // block
+        getattr(cache, what)[b, :, at] = float("nan")
+        first.append(at * block)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    call = Q8Attention(q, cache, torch.tensor(lens, **i32), q_lens=torch.tensor(q_lens, **i32), out_dtype=od, lse=True)
+    out = call.run().double()
+    f = 2.0 ** -19 * A + 2.0 ** -18
+    tol = vmax * (f + (0.0 if od == torch.float32 else 2.0 ** -10)) + (0.0 if od == torch.float32 else 2.0 ** -8) * ref.abs() + 1e-30
+    for b in range(3):
+        for i in range(n):
+            end = lens[b] - q_lens[b] + i + 1 if i < q_lens[b] else 0  # tokens that the query sees
+            if end > first[b]:
+                assert out[b, i].isnan().all() and call.lse[b, i].isnan().all(), (b, i)
+            else:
+                assert ((out[b, i] - ref[b, i]).abs() <= tol[b, i]).all(), (b, i)
+                assert torch.equal(call.lse[b, i].isinf(), lse[b, i].isinf()) and not call.lse[b, i].isnan().any(), (b, i)
