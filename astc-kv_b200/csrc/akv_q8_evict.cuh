@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(256, PP == 2 ? 6 : 2) pack_kernel(EvictParams 
 #pragma unroll
         for (int k = 1; k < 8; ++k) top = max(top, red[side][k]);
         const float scale = block_scale<FMT>(top), inv = block_inverse(scale);
+        const bool numbers = !isnan(scale);  // see store_kernel
         uint8_t* codes = to.codes + code_offset(to, b, h, phys, in_page);
 #pragma unroll
         for (int k = 0; k < PP; ++k) {
@@ -255,7 +256,7 @@ __global__ void __launch_bounds__(256, PP == 2 ? 6 : 2) pack_kernel(EvictParams 
                 from_codes4<FMT>(u[j], f);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(__fmul_rn(f[e], sc[side][k]), inv);
-                u[j] = to_codes4<FMT>(f);
+                u[j] = numbers ? to_codes4<FMT>(f) : 0u;
             }
             reinterpret_cast<uint4*>(codes + r * to.sT)[i - r * per_row] = make_uint4(u[0], u[1], u[2], u[3]);
         }

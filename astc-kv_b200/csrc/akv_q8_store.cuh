@@ -151,6 +151,9 @@ __global__ void __launch_bounds__(256, PP == 2 ? (sizeof(T) == 2 ? 6 : 4) : 1) s
         }
     }
     const float inv = block_inverse(scale);
+    // A block with a NaN scale holds zeros: a NaN code would meet the softmax
+    // weight 0 of rows that do not see it, in the attention's products.
+    const bool numbers = !isnan(scale);
 #pragma unroll
     for (int k = 0; k < PP; ++k) {
         const int i = threadIdx.x + k * blockDim.x;
@@ -162,7 +165,7 @@ __global__ void __launch_bounds__(256, PP == 2 ? (sizeof(T) == 2 ? 6 : 4) : 1) s
             float f[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(v[k].get(4 * j + e), inv);
-            u[j] = to_codes4<FMT>(f);
+            u[j] = numbers ? to_codes4<FMT>(f) : 0u;
         }
         *reinterpret_cast<uint4*>(codes + r * s.sT + d) = make_uint4(u[0], u[1], u[2], u[3]);
     }

@@ -32,7 +32,9 @@ extern "C" {
  * Code strides are bytes and multiples of 16, codes 16-byte aligned; scale
  * strides are elements. All page_tokens rows of a page are the cache's own
  * memory (an eviction writes whole blocks). Scales are >= 0; a scale below 2^-90 counts as 2^-90
- * where V's softmax weights are formed. A NaN scale makes what reads it NaN.
+ * where V's softmax weights are formed. A NaN scale makes NaN of what sees a
+ * token of its block. Codes are numbers: an e4m3 NaN code, which no call here
+ * writes, may also show in queries that end before its token.
  */
 typedef struct AkvQ8Side {
     void* codes;
@@ -66,8 +68,8 @@ typedef struct AkvQ8Cache {
  * start[b] keeps its scale unless the new rows need a larger one, and then
  * its rows are rounded again under that one. Tokens are stored in order: what
  * a block holds from start[b] on is not kept. A block that is given an
- * infinity or a NaN gets a NaN scale; one whose scale would be subnormal is
- * stored as zeros.
+ * infinity or a NaN gets a NaN scale and codes of 0; one whose scale would be
+ * subnormal is stored as zeros.
  */
 typedef struct AkvQ8StoreDesc {
     AkvQ8Cache cache;

@@ -109,3 +109,33 @@ def test_nan_scale_shows_where_it_is_seen(cuda, D, G, n, od, fmt, what):
             else:
                 assert ((out[b, i] - ref[b, i]).abs() <= tol[b, i]).all(), (b, i)
                 assert torch.equal(call.lse[b, i].isinf(), lse[b, i].isinf()) and not call.lse[b, i].isnan().any(), (b, i)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("D,G,n,od", [(128, 4, 40, torch.bfloat16), (256, 1, 40, torch.bfloat16), (128, 4, 6, torch.float32),
+                                      (64, 1, 20, torch.float32)])
+def test_stored_nan_stays_with_its_block(cuda, D, G, n, od, fmt, bad):
+    """Queries that end before the block of a row that is not finite are as without it, after a store and after an eviction."""
+    from astc_kv_cuda import Q8Attention, Q8Cache, Q8Evict, q8_store
+    T, block = 192, 16
+    at = T - 3
+    x = [torch.randn(1, T, 2, D, device="cuda") for _ in range(2)]
+    caches = []
+    for value in (0.0, bad):
+        for y in x:
+            y[0, at, :, 5] = value
+        c = Q8Cache.zeros(1, 2, T, D, fmt=fmt, block_tokens=block)
+        caches.append(q8_store(c, *x, torch.zeros(1, dtype=torch.int32, device="cuda")))
+    w = torch.zeros(1, 2, T, device="cuda")
+    small = []
+    for c in caches:
+        small.append(Q8Cache.zeros(1, 2, T - block, D, fmt=fmt, block_tokens=block))
+        Q8Evict(c, small[-1], w, keep=T - block, recent=2 * block).run()
+    q = torch.randn(1, n, 2 * G, D, device="cuda").bfloat16()
+    for (good, poor), length in ((caches, T), (small, T - block)):
+        codes = [t.view(torch.uint8) for t in (poor.k, poor.v)]
+        assert fmt == "int8" or not any(((t & 127) == 127).any() for t in codes)
+        clean, out = (Q8Attention(q, c, out_dtype=od).run() for c in (good, poor))
+        sees = length - n + torch.arange(n, device="cuda") + 1 > length - block
+        assert out[0, sees].isnan().all() and torch.equal(out[0, ~sees], clean[0, ~sees])
