@@ -97,7 +97,7 @@ class AkvQ8EvictDesc(ct.Structure):
     _fields_ = [
         ("src", AkvQ8Cache), ("dst", AkvQ8Cache), ("weights_dev", ct.c_void_p), ("weights_stride", ct.c_int64),
         ("seq_lens_dev", ct.c_void_p), ("keep", ct.c_int32), ("sinks", ct.c_int32), ("recent", ct.c_int32),
-        ("reserved0", ct.c_int32), ("kept_dev", ct.c_void_p), ("out_lens_dev", ct.c_void_p), ("out_weights_dev", ct.c_void_p),
+        ("out_weights_tokens", ct.c_int32), ("kept_dev", ct.c_void_p), ("out_lens_dev", ct.c_void_p), ("out_weights_dev", ct.c_void_p),
         ("out_weights_stride", ct.c_int64),
     ]
 

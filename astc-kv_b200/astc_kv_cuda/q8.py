@@ -327,10 +327,11 @@ class Q8Attention(_Call):
 class Q8Evict(_Call):
     """Keep min(len, keep) tokens per sequence and kv head: the first `sinks`,
     the last `recent`, and those with the largest `weights` [B, H, T], packed
-    in their order into `dst`, a cache in other memory that holds whole blocks. run() returns (kept
-    token indices [B, H, keep] with -1 after the last, lengths [B], the kept
-    tokens' weights [B, H, dst.max_tokens], 0 after the last): what the next
-    steps go on with."""
+    in their order into `dst`, a cache in other memory that holds whole blocks.
+    run() returns (kept token indices [B, H, keep] with -1 after the last,
+    lengths [B], the kept tokens' weights [B, H, dst.max_tokens], 0 after the
+    last): what the next steps go on with, in this object's own tensors, which
+    its next run() writes anew."""
 
     _fn = "evict"
 
@@ -359,9 +360,10 @@ class Q8Evict(_Call):
         i32 = dict(dtype=torch.int32, device=src.device)
         self.kept = torch.empty(B, H, keep, **i32)
         self.lens = torch.empty(B, **i32)
-        self.weights = torch.zeros(B, H, dst.max_tokens, dtype=torch.float32, device=src.device)
+        self.weights = torch.empty(B, H, dst.max_tokens, dtype=torch.float32, device=src.device)
         d.kept_dev, d.out_lens_dev = self.kept.data_ptr(), self.lens.data_ptr()
         d.out_weights_dev, d.out_weights_stride = self.weights.data_ptr(), dst.max_tokens
+        d.out_weights_tokens = dst.max_tokens
         self.cache = dst
         self._prepare(d, src.device, weights, lens, self.kept, self.lens, self.weights, *_cache_tensors(src), *_cache_tensors(dst))
 

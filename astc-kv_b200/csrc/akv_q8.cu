@@ -394,11 +394,13 @@ int akv_q8_evict(const AkvQ8EvictDesc* d, void* stream) {
     if (!d->weights_dev || !d->kept_dev || !d->out_lens_dev || !d->out_weights_dev || d->weights_stride < a.max_tokens ||
         d->out_weights_stride < d->keep)
         return AKV_ERR_INVALID_ARGUMENT;
+    if (d->out_weights_tokens && (d->out_weights_tokens < d->keep || d->out_weights_tokens > d->out_weights_stride)) return AKV_ERR_INVALID_ARGUMENT;
     if (a.batch == 0) return AKV_OK;
     EvictParams p;
     p.src = to_dev(a); p.dst = to_dev(c);
     p.weights = d->weights_dev; p.wstride = d->weights_stride; p.lens = d->seq_lens_dev;
     p.keep = d->keep; p.sinks = d->sinks; p.recent = d->recent;
+    p.columns = d->out_weights_tokens ? d->out_weights_tokens : d->keep;
     p.kept = d->kept_dev; p.out_lens = d->out_lens_dev; p.out_weights = d->out_weights_dev; p.ostride = d->out_weights_stride;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (a.max_tokens <= 8 * kSelectThreads) select_kernel<8><<<dim3(a.kv_heads, a.batch), kSelectThreads, 0, s>>>(p);

@@ -14,6 +14,7 @@ struct EvictParams {
     int64_t wstride;
     const int32_t* lens;
     int keep, sinks, recent;
+    int columns;                // weights per row to be written, at least keep
     int32_t* kept;
     int32_t* out_lens;
     float* out_weights;
@@ -79,10 +80,8 @@ __global__ void __launch_bounds__(kSelectThreads) select_kernel(EvictParams p) {
     const int n = min(len, p.keep);
     allow_next_kernel();
     if (h == 0 && tid == 0) p.out_lens[b] = n;
-    for (int i = n + tid; i < p.keep; i += kSelectThreads) {
-        kept[i] = -1;
-        ow[i] = 0.f;
-    }
+    for (int i = n + tid; i < p.keep; i += kSelectThreads) kept[i] = -1;
+    for (int i = n + tid; i < p.columns; i += kSelectThreads) ow[i] = 0.f;
     if (len <= p.keep) {
         for (int i = tid; i < n; i += kSelectThreads) {
             kept[i] = i;

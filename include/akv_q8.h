@@ -149,7 +149,9 @@ int akv_q8_attention(const AkvQ8AttnDesc* desc, void* stream);
  * their block become zeros.
  *     kept[b][h][i]        token that row i was, -1 from min(len, keep) on
  *     out_lens[b]          min(len, keep)
- *     out_weights[b][h][i] its weight, 0 from min(len, keep) on
+ *     out_weights[b][h][i] its weight, 0 from min(len, keep) up to
+ *                          out_weights_tokens: dst.max_tokens there leaves no
+ *                          earlier tokens' weights where later ones will be
  */
 typedef struct AkvQ8EvictDesc {
     AkvQ8Cache src, dst;
@@ -157,7 +159,7 @@ typedef struct AkvQ8EvictDesc {
     int64_t weights_stride;
     const int32_t* seq_lens_dev;    /* [batch] or NULL (= src.max_tokens) */
     int32_t keep, sinks, recent;    /* sinks + recent <= keep <= dst.max_tokens */
-    int32_t reserved0;
+    int32_t out_weights_tokens;     /* weights written per row, keep to out_weights_stride; 0 = keep */
     int32_t* kept_dev;              /* [batch][kv_heads][keep] */
     int32_t* out_lens_dev;          /* [batch] */
     float* out_weights_dev;         /* [batch][kv_heads], rows out_weights_stride apart (>= keep) */

@@ -159,3 +159,11 @@ def test_python_refuses_cpu_tensors_and_other_dtypes():
         Q8Cache(codes.float(), codes.float(), scales, scales)
     with pytest.raises(ValueError):
         Q8Cache.zeros(1, 1, 64, 64, fmt="int4", device="cpu")
+
+
+def test_evict_refuses_counts_of_weights_that_do_not_fit():
+    lib = L.lib()
+    for tokens in (-1, 63, 97):
+        d = _evict()
+        d.out_weights_stride, d.out_weights_tokens = 96, tokens
+        assert lib.akv_q8_evict(ct.byref(d), None) == 1, tokens
