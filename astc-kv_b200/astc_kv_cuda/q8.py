@@ -180,7 +180,13 @@ class Q8Cache:
 
 
 class _Call:
-    """A prepared call: a C descriptor, the tensors it points to, and `_issue`."""
+    """A prepared call: a C descriptor, the tensors it points to, and `_issue`.
+
+    Outputs and workspace are the object's own, so its runs follow one another
+    on one stream, or on streams that the caller orders. The first run on
+    another stream than the one the object was built on waits for what that
+    one had been given by then: earlier work on the memory that it took.
+    """
 
     _fn = ""
 
@@ -190,21 +196,32 @@ class _Call:
         self._index = device.index if device.index is not None else 0
         self._tensors = [t for t in tensors if t is not None]
         self._issue_c = getattr(L.lib(), "akv_q8_" + self._fn)
+        home = torch.cuda.current_stream(device)
+        self._home, self._met = home.cuda_stream, set()
+        # What a capture records cannot be waited for outside of it.
+        self._built = None if torch.cuda.is_current_stream_capturing() else home.record_event()
 
     def _issue(self, stream: torch.cuda.Stream | None) -> None:
         if torch.cuda.current_device() != self._index:
             raise ValueError(f"the tensors are on {self.device}, which is not the current device")
-        if stream is None:
-            handle = _current_stream(self._index)
-        else:
-            handle = stream.cuda_stream
-            # The caller may drop this object while the stream still works on
-            # its memory.
-            for t in self._tensors:
-                t.record_stream(stream)
+        handle = _current_stream(self._index) if stream is None else stream.cuda_stream
+        if handle != self._home:
+            self._elsewhere(handle, torch.cuda.current_stream(self._index) if stream is None else stream)
         code = self._issue_c(self._dref, handle or None)
         if code:
             raise L.AkvError(code, "q8_" + self._fn)
+
+    def _elsewhere(self, handle: int, stream: torch.cuda.Stream) -> None:
+        """Before a run on another stream than the one the object was built on."""
+        if self._built is not None and handle not in self._met:
+            with torch.cuda.stream(stream):
+                capturing = torch.cuda.is_current_stream_capturing()
+            if not capturing:  # a capture waits for all streams before it begins
+                stream.wait_event(self._built)
+                self._met.add(handle)
+        # The caller may drop this object while the stream still works on its memory.
+        for t in self._tensors:
+            t.record_stream(stream)
 
 
 class Q8Store(_Call):

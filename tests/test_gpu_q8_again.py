@@ -58,3 +58,85 @@ def test_evict_writes_the_weights_it_is_told_to(cuda):
         torch.cuda.synchronize()
         assert (out[0, :, :40] < 1).all() and not out[0, :, 40:end].any() and not out[1, :, 20:end].any()
         assert (out[:, :, end:] == 7).all()
+
+
+def small_calls():
+    """By name, what builds a call on a small cache, with an input that only the call holds: each call that owns memory."""
+    from astc_kv_cuda import Q8Attention, Q8Cache, Q8Evict, Q8Restore
+    cache, _, _ = make(2, 2, 4096, 64, seed=3)
+    q0 = torch.randn(2, 8, 64, device="cuda").bfloat16()
+    w0 = torch.rand(2, 2, 4096, device="cuda")
+
+    def attention():
+        q = q0.clone()
+        return Q8Attention(q, cache)
+
+    def restore():
+        start = torch.full((2,), 7, dtype=torch.int32, device="cuda")
+        return Q8Restore(cache, start, 64)
+
+    def evict():
+        w = w0.clone()
+        return Q8Evict(cache, Q8Cache.zeros(2, 2, 1024, 64, block_tokens=32), w, keep=1024)
+    return {"attention": attention, "restore": restore, "evict": evict}
+
+
+def results(out):
+    return list(out) if isinstance(out, tuple) else [out]
+
+
+@pytest.mark.parametrize("op", ["attention", "restore", "evict"])
+def test_other_stream_waits_for_the_memory(cuda, op):
+    """Work that was given to the building stream before still writes to memory that the call got from its allocator."""
+    build = small_calls()[op]
+    want = [t.clone() for t in results(build().run())]
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        torch.cuda.synchronize()
+        torch.cuda._sleep(100_000_000)
+        junk = [torch.full_like(t, 77) for t in want for _ in range(3)]
+        del junk
+        got = results(build().run(side))
+        side.synchronize()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("explicit", [False, True])
+@pytest.mark.parametrize("op", ["attention", "restore", "evict"])
+def test_memory_stays_until_the_other_stream_is_done(cuda, op, explicit):
+    """The call and what it reads are dropped while the stream that it was given has not begun with it."""
+    build = small_calls()[op]
+    want = [t.clone() for t in results(build().run())]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        call = build()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)
+            if not explicit:
+                got = results(call.run())
+        if explicit:
+            got = results(call.run(side))
+        sizes = [t.numel() * t.element_size() for t in call._tensors]
+        del call
+        junk = [torch.full((n,), 77, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(2)]
+        torch.cuda.synchronize()
+        del junk
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_first_run_inside_a_graph(cuda):
+    """A call built outside runs for the first time while a graph is captured."""
+    for op, build in small_calls().items():
+        want = [t.clone() for t in results(build().run())]
+        call = build()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = results(call.run())
+        for t in got:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), op
