@@ -344,7 +344,8 @@ class Q8Attention(_Call):
 class Q8Evict(_Call):
     """Keep min(len, keep) tokens per sequence and kv head: the first `sinks`,
     the last `recent`, and those with the largest `weights` [B, H, T], packed
-    in their order into `dst`, a cache in other memory that holds whole blocks.
+    in their order into `dst`, a cache in other memory (or in pages of the same
+    pool that `src` has not got) that holds whole blocks.
     run() returns (kept token indices [B, H, keep] with -1 after the last,
     lengths [B], the kept tokens' weights [B, H, dst.max_tokens], 0 after the
     last): what the next steps go on with, in this object's own tensors, which
@@ -365,10 +366,10 @@ class Q8Evict(_Call):
         if weights.dtype != torch.float32 or weights.dim() != 3 or tuple(weights.shape[:2]) != (B, H) or \
                 weights.shape[2] < src.max_tokens or not weights.is_contiguous():
             raise ValueError("weights must be contiguous fp32 [B, H, >= max_tokens]")
-        for a in (src.k, src.v, src.k_scales, src.v_scales):
-            for b in (dst.k, dst.v, dst.k_scales, dst.v_scales):
-                if a.untyped_storage().data_ptr() == b.untyped_storage().data_ptr():
-                    raise ValueError("dst must not share memory with src")
+        # Two block tables may share a pool: which pages they give out is on the device.
+        one_pool = src.block_table is not None and dst.block_table is not None and src.block_table.data_ptr() != dst.block_table.data_ptr()
+        if not one_pool and any(_may_overlap(a, b) for a in _planes(src) for b in _planes(dst)):
+            raise ValueError("dst must not share memory with src")
         d = L.AkvQ8EvictDesc()
         d.src, d.dst = src._c, dst._c
         d.weights_dev, d.weights_stride = weights.data_ptr(), weights.shape[2]
@@ -389,8 +390,39 @@ class Q8Evict(_Call):
         return self.kept, self.lens, self.weights
 
 
+def _planes(c: Q8Cache) -> tuple:
+    return c.k, c.v, c.k_scales, c.v_scales
+
+
 def _cache_tensors(c: Q8Cache) -> tuple:
-    return c.k, c.v, c.k_scales, c.v_scales, c.block_table, c.status
+    return *_planes(c), c.block_table, c.status
+
+
+def _may_overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors may have bytes in common. Views of different strides count as
+    overlapping when the ranges do that they span; of equal strides, when an element of both
+    can be at one place."""
+    def span(t):
+        return (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    apart = b.data_ptr() - a.data_ptr()
+    if apart >= span(a) or -apart >= span(b):
+        return False
+    size = a.element_size()
+    if a.stride() != b.stride() or size != b.element_size() or apart % size:
+        return True
+    dims = sorted(((s, n, m) for s, n, m in zip(a.stride(), a.shape, b.shape) if s and n * m > 1), reverse=True)
+
+    def meet(left: int, dims: list) -> bool:
+        # Is left = sum of s * (i - j) with 0 <= i < n, 0 <= j < m?
+        if not dims:
+            return left == 0
+        s, n, m = dims[0]
+        up, down = sum(r * (x - 1) for r, x, _ in dims[1:]), sum(r * (y - 1) for r, _, y in dims[1:])
+        first, last = max(-(-(left - up) // s), 1 - m), min((left + down) // s, n - 1)
+        return any(meet(left - s * k, dims[1:]) for k in range(first, last + 1))
+    return meet(apart // size, dims)
 
 
 def q8_store(cache: Q8Cache, k: torch.Tensor, v: torch.Tensor, start: torch.Tensor, counts: torch.Tensor | None = None,

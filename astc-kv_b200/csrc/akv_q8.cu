@@ -389,7 +389,9 @@ int akv_q8_evict(const AkvQ8EvictDesc* d, void* stream) {
     if (d->keep <= 0 || d->keep > c.max_tokens || d->sinks < 0 || d->recent < 0 ||
         static_cast<int64_t>(d->sinks) + d->recent > d->keep)
         return AKV_ERR_INVALID_ARGUMENT;
-    if (a.k.codes == c.k.codes || a.v.codes == c.v.codes || a.k.scales == c.k.scales || a.v.scales == c.v.scales)
+    // Two tables may give out pages of one pool.
+    if (!(a.block_table_dev && c.block_table_dev && a.block_table_dev != c.block_table_dev) &&
+        (a.k.codes == c.k.codes || a.v.codes == c.v.codes || a.k.scales == c.k.scales || a.v.scales == c.v.scales))
         return AKV_ERR_INVALID_ARGUMENT;
     if (!d->weights_dev || !d->kept_dev || !d->out_lens_dev || !d->out_weights_dev || d->weights_stride < a.max_tokens ||
         d->out_weights_stride < d->keep)

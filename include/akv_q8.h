@@ -146,7 +146,8 @@ int akv_q8_attention(const AkvQ8AttnDesc* desc, void* stream);
  * order into `dst`, a cache in other memory with the same format, batch,
  * kv_heads and head_dim, whose blocks get scales of their own (as a store
  * of the restored rows would); its rows from min(len, keep) to the end of
- * their block become zeros.
+ * their block become zeros. Other memory are also other pages of the same
+ * pool: no page of dst's table may be in src's, which the call cannot see.
  *     kept[b][h][i]        token that row i was, -1 from min(len, keep) on
  *     out_lens[b]          min(len, keep)
  *     out_weights[b][h][i] its weight, 0 from min(len, keep) up to

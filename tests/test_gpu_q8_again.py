@@ -5,7 +5,7 @@ import ctypes as ct
 import pytest
 import torch
 
-from test_gpu_q8 import make, plain_choice
+from test_gpu_q8 import half_step, make, plain_choice, values_of, MOST
 
 pytestmark = pytest.mark.gpu
 
@@ -140,3 +140,55 @@ def test_first_run_inside_a_graph(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), op
+
+
+def check_packed(src_values, dst, kept, lens):
+    """`dst` holds the kept rows, each block under a scale of its own."""
+    for b, n in enumerate(lens):
+        for h in range(dst.kv_heads):
+            at = kept[b, h, :n].long()
+            for got, values in zip(values_of(dst), src_values):
+                rows = values[b, h, at]
+                pad = torch.zeros(-(-n // dst.block_tokens) * dst.block_tokens, dst.head_dim, dtype=torch.float64, device="cuda")
+                pad[:n] = rows
+                sc = (pad.view(-1, dst.block_tokens, dst.head_dim).abs().amax((1, 2)) / MOST[dst.fmt]).repeat_interleave(dst.block_tokens)[:n, None]
+                assert ((got[b, h, :n] - rows).abs() <= half_step(rows, sc, dst.fmt) * (1 + 2.0 ** -10)).all()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+def test_evict_into_other_pages_of_the_pool(cuda, fmt):
+    """A paged server has one pool: what a sequence keeps goes to pages that nobody has."""
+    from astc_kv_cuda import Q8Cache, Q8Evict
+    page, block, keep = 64, 32, 150
+    src, k, v = make(3, 2, 512, 64, fmt=fmt, block=block, page=page, spare=12, seed=4)
+    used = set(src.block_table.flatten().tolist())
+    free = torch.tensor([i for i in range(src.k.shape[0]) if i not in used][:9], dtype=torch.int32, device="cuda").view(3, 3)
+    dst = Q8Cache(src.k, src.v, src.k_scales, src.v_scales, block_tokens=block, block_table=free)
+    before = [t.clone() for t in (src.k.view(torch.int8), src.k_scales)]
+    w = torch.rand(3, 2, 512, device="cuda")
+    kept, lens, _ = Q8Evict(src, dst, w, torch.tensor([512, 100, 317], dtype=torch.int32, device="cuda"), keep=keep, sinks=3, recent=9).run()
+    assert lens.tolist() == [keep, 100, keep]
+    check_packed((k, v), dst, kept, lens.tolist())
+    others = sorted(set(range(src.k.shape[0])) - set(free.flatten().tolist()))
+    assert torch.equal(src.k.view(torch.int8)[others], before[0][others]) and torch.equal(src.k_scales[others], before[1][others])
+    with pytest.raises(ValueError):
+        Q8Evict(src, src, w, keep=keep)
+
+
+def test_evict_between_slices_of_one_tensor(cuda):
+    """The caches of two layers, K and V side by side, in one allocation; and slices that do overlap."""
+    from astc_kv_cuda import Q8Cache, Q8Evict
+    codes = torch.randint(-127, 128, (2, 2, 2, 3, 96, 64), device="cuda", dtype=torch.int8)  # batch, layer, K and V, ...
+    scales = torch.rand(2, 2, 2, 3, 3, device="cuda")
+
+    def cache(layer, t0, t1):
+        c, s = codes[:, layer, :, :, t0:t1], scales[:, layer, :, :, t0 // 32:t1 // 32]
+        return Q8Cache(c[:, 0], c[:, 1], s[:, 0], s[:, 1], block_tokens=32)
+    w = torch.rand(2, 3, 96, device="cuda")
+    for src, dst in ((cache(0, 0, 96), cache(1, 0, 96)), (cache(1, 0, 64), cache(1, 64, 96))):
+        values = values_of(src)
+        kept, lens, _ = Q8Evict(src, dst, w, keep=20).run()
+        check_packed(values, dst, kept, lens.tolist())
+    for src, dst in ((cache(0, 0, 96), cache(0, 64, 96)), (cache(1, 32, 96), cache(1, 0, 64))):
+        with pytest.raises(ValueError):
+            Q8Evict(src, dst, w, keep=20)

@@ -167,3 +167,18 @@ def test_evict_refuses_counts_of_weights_that_do_not_fit():
         d = _evict()
         d.out_weights_stride, d.out_weights_tokens = 96, tokens
         assert lib.akv_q8_evict(ct.byref(d), None) == 1, tokens
+
+
+def test_evict_within_a_pool_needs_two_tables():
+    lib = L.lib()
+    d = _evict()
+    for side in ("k", "v"):
+        getattr(d.dst, side).codes = getattr(d.src, side).codes
+        getattr(d.dst, side).scales = getattr(d.src, side).scales
+    for c in (d.src, d.dst):
+        c.block_table_dev, c.pages_per_seq, c.num_pages, c.batch = 4096, 1, 8, 0  # a batch of none: nothing is launched
+    assert lib.akv_q8_evict(ct.byref(d), None) == 1
+    d.dst.block_table_dev = 8192
+    assert lib.akv_q8_evict(ct.byref(d), None) == 0
+    d.dst.block_table_dev, d.dst.max_tokens = None, 128
+    assert lib.akv_q8_evict(ct.byref(d), None) == 1
