@@ -22,15 +22,16 @@ constexpr int kMaxGridYZ = 65535;
 
 bool valid_dtype(int t) { return t >= AKV_Q_F32 && t <= AKV_Q_F16; }
 
-bool valid_side(const AkvQ8Side& s) {
-    return s.codes && s.scales && reinterpret_cast<uintptr_t>(s.codes) % 16 == 0 && reinterpret_cast<uintptr_t>(s.scales) % 4 == 0 &&
+// A cache for no sequences needs no memory.
+bool valid_side(const AkvQ8Side& s, int batch) {
+    return (batch == 0 || (s.codes && s.scales)) && reinterpret_cast<uintptr_t>(s.codes) % 16 == 0 && reinterpret_cast<uintptr_t>(s.scales) % 4 == 0 &&
            s.stride_batch % 16 == 0 && s.stride_head % 16 == 0 && s.stride_page % 16 == 0 && s.stride_token % 16 == 0;
 }
 
 int check_cache(const AkvQ8Cache& c) {
     if (c.format != AKV_Q8_INT8 && c.format != AKV_Q8_E4M3) return AKV_ERR_INVALID_ARGUMENT;
     if (c.batch < 0 || c.kv_heads <= 0 || c.head_dim <= 0 || c.max_tokens <= 0 || c.page_tokens <= 0) return AKV_ERR_INVALID_ARGUMENT;
-    if (!valid_side(c.k) || !valid_side(c.v)) return AKV_ERR_INVALID_ARGUMENT;
+    if (!valid_side(c.k, c.batch) || !valid_side(c.v, c.batch)) return AKV_ERR_INVALID_ARGUMENT;
     if (c.block_tokens <= 0 || c.page_tokens % c.block_tokens) return AKV_ERR_INVALID_ARGUMENT;
     if (c.block_table_dev &&
         (c.pages_per_seq <= 0 || c.num_pages <= 0 || static_cast<int64_t>(c.pages_per_seq) * c.page_tokens < c.max_tokens))
@@ -389,15 +390,15 @@ int akv_q8_evict(const AkvQ8EvictDesc* d, void* stream) {
     if (d->keep <= 0 || d->keep > c.max_tokens || d->sinks < 0 || d->recent < 0 ||
         static_cast<int64_t>(d->sinks) + d->recent > d->keep)
         return AKV_ERR_INVALID_ARGUMENT;
-    // Two tables may give out pages of one pool.
-    if (!(a.block_table_dev && c.block_table_dev && a.block_table_dev != c.block_table_dev) &&
-        (a.k.codes == c.k.codes || a.v.codes == c.v.codes || a.k.scales == c.k.scales || a.v.scales == c.v.scales))
-        return AKV_ERR_INVALID_ARGUMENT;
-    if (!d->weights_dev || !d->kept_dev || !d->out_lens_dev || !d->out_weights_dev || d->weights_stride < a.max_tokens ||
-        d->out_weights_stride < d->keep)
-        return AKV_ERR_INVALID_ARGUMENT;
     if (d->out_weights_tokens && (d->out_weights_tokens < d->keep || d->out_weights_tokens > d->out_weights_stride)) return AKV_ERR_INVALID_ARGUMENT;
+    if (d->weights_stride < a.max_tokens || d->out_weights_stride < d->keep) return AKV_ERR_INVALID_ARGUMENT;
+    // Two tables may give out pages of one pool.
+    const auto same = [](const void* x, const void* y) { return x && x == y; };
+    if (!(a.block_table_dev && c.block_table_dev && a.block_table_dev != c.block_table_dev) &&
+        (same(a.k.codes, c.k.codes) || same(a.v.codes, c.v.codes) || same(a.k.scales, c.k.scales) || same(a.v.scales, c.v.scales)))
+        return AKV_ERR_INVALID_ARGUMENT;
     if (a.batch == 0) return AKV_OK;
+    if (!d->weights_dev || !d->kept_dev || !d->out_lens_dev || !d->out_weights_dev) return AKV_ERR_INVALID_ARGUMENT;
     EvictParams p;
     p.src = to_dev(a); p.dst = to_dev(c);
     p.weights = d->weights_dev; p.wstride = d->weights_stride; p.lens = d->seq_lens_dev;

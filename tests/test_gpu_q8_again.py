@@ -192,3 +192,22 @@ def test_evict_between_slices_of_one_tensor(cuda):
     for src, dst in ((cache(0, 0, 96), cache(0, 64, 96)), (cache(1, 32, 96), cache(1, 0, 64))):
         with pytest.raises(ValueError):
             Q8Evict(src, dst, w, keep=20)
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_no_sequences(cuda, paged):
+    """A batch of none: empty results, no error."""
+    from astc_kv_cuda import Q8Attention, Q8Cache, q8_evict, q8_restore, q8_store
+    i32 = dict(dtype=torch.int32, device="cuda")
+
+    def cache():
+        paging = dict(block_table=torch.empty(0, 2, **i32), page_tokens=64, num_pages=4) if paged else {}
+        return Q8Cache.zeros(0, 2, 128, 64, **paging)
+    src, dst, none = cache(), cache(), torch.empty(0, **i32)
+    x = torch.randn(0, 3, 2, 64, device="cuda")
+    q8_store(src, x, x, none)
+    assert q8_restore(src, none, 5)[0].shape == (0, 5, 2, 64)
+    w = torch.empty(0, 2, 128, device="cuda")
+    assert Q8Attention(torch.randn(0, 7, 8, 64, device="cuda"), src, none, weights=w, lse=True).run().shape == (0, 7, 8, 64)
+    kept, lens, _ = q8_evict(src, dst, w, none, keep=10)
+    assert kept.shape == (0, 2, 10) and lens.shape == (0,)

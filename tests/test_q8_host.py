@@ -182,3 +182,19 @@ def test_evict_within_a_pool_needs_two_tables():
     assert lib.akv_q8_evict(ct.byref(d), None) == 0
     d.dst.block_table_dev, d.dst.max_tokens = None, 128
     assert lib.akv_q8_evict(ct.byref(d), None) == 1
+
+
+def test_a_batch_of_none_needs_no_memory():
+    """Empty tensors have no address; there is nothing to do, and that is not an error."""
+    lib = L.lib()
+    s, r, a, e = L.AkvQ8StoreDesc(), L.AkvQ8RestoreDesc(), _attention(), _evict()
+    s.cache, r.cache = _cache(), _cache()
+    s.tokens = r.tokens = 4
+    for c in (s.cache, r.cache, a.cache, e.src, e.dst):
+        c.batch = 0
+        for side in (c.k, c.v):
+            side.codes = side.scales = None
+    a.q_dev = a.out_dev = e.weights_dev = e.kept_dev = e.out_lens_dev = e.out_weights_dev = None
+    assert lib.akv_q8_attention_workspace(ct.byref(a)) >= 16
+    for fn, d in ((lib.akv_q8_attention, a), (lib.akv_q8_evict, e), (lib.akv_q8_store, s), (lib.akv_q8_restore, r)):
+        assert fn(ct.byref(d), None) == 0
