@@ -322,7 +322,15 @@ size_t akv_q8_attention_workspace(const AkvQ8AttnDesc* d) { return check_attenti
 
 int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     if (int st = check_attention(d)) return st;
-    if (d->cache.batch == 0 || d->q_tokens == 0) return AKV_OK;
+    if (d->cache.batch == 0) return AKV_OK;
+    if (d->q_tokens == 0) {
+        // A sum over no queries.
+        if (!d->weights_dev || d->accumulate) return AKV_OK;
+        const AkvQ8Cache& c = d->cache;
+        return cudaMemset2DAsync(d->weights_dev, d->weights_stride * sizeof(float), 0, c.max_tokens * sizeof(float),
+                                 static_cast<size_t>(c.batch) * c.kv_heads, static_cast<cudaStream_t>(stream)) == cudaSuccess
+                   ? AKV_OK : (cudaGetLastError(), AKV_ERR_CUDA);
+    }
     const uintptr_t elem = d->q_dtype == AKV_Q_F32 ? 4 : 2;
     if (!d->q_dev || !d->out_dev || reinterpret_cast<uintptr_t>(d->q_dev) % elem || reinterpret_cast<uintptr_t>(d->out_dev) % 16)
         return AKV_ERR_INVALID_ARGUMENT;

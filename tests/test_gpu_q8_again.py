@@ -211,3 +211,15 @@ def test_no_sequences(cuda, paged):
     assert Q8Attention(torch.randn(0, 7, 8, 64, device="cuda"), src, none, weights=w, lse=True).run().shape == (0, 7, 8, 64)
     kept, lens, _ = q8_evict(src, dst, w, none, keep=10)
     assert kept.shape == (0, 2, 10) and lens.shape == (0,)
+
+
+def test_no_queries(cuda):
+    """A sum over no queries is 0, and adding it changes nothing."""
+    from astc_kv_cuda import Q8Attention
+    cache, _, _ = make(2, 3, 100, 64, seed=2)
+    q = torch.randn(2, 0, 6, 64, device="cuda").bfloat16()
+    w = torch.rand(2, 3, cache.max_tokens + 7, device="cuda")
+    first = w.clone()
+    assert Q8Attention(q, cache, weights=w).run().shape == (2, 0, 6, 64) and torch.equal(w, first)
+    Q8Attention(q, cache, weights=w, accumulate=False).run()
+    assert not w[:, :, :cache.max_tokens].any() and torch.equal(w[:, :, cache.max_tokens:], first[:, :, cache.max_tokens:])
