@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(256, PP == 2 ? (sizeof(T) == 2 ? 6 : 4) : 1) s
     const CacheDev& c = p.c;
     const int h = blockIdx.y, b = blockIdx.z >> 1, side = blockIdx.z & 1;
     const int start = p.start[b], count = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
+    if (count == 0) return;  // wherever it starts
     if (start < 0 || static_cast<int64_t>(start) + count > c.T) {
         if (threadIdx.x == 0 && blockIdx.x == 0) report(c.status, AKV_ERR_INVALID_ARGUMENT);
         if (start < 0 || start >= c.T) return;

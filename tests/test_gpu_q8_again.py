@@ -223,3 +223,17 @@ def test_no_queries(cuda):
     assert Q8Attention(q, cache, weights=w).run().shape == (2, 0, 6, 64) and torch.equal(w, first)
     Q8Attention(q, cache, weights=w, accumulate=False).run()
     assert not w[:, :, :cache.max_tokens].any() and torch.equal(w[:, :, cache.max_tokens:], first[:, :, cache.max_tokens:])
+
+
+def test_store_of_no_rows_anywhere(cuda):
+    """A sequence that brings no rows stores nothing outside the cache, wherever its start is."""
+    from astc_kv_cuda import Q8Cache, q8_store
+    c = Q8Cache.zeros(4, 1, 64, 16, block_tokens=16)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cache = Q8Cache(c.k, c.v, c.k_scales, c.v_scales, block_tokens=16, status=status)
+    x = torch.ones(4, 8, 1, 16, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    q8_store(cache, x, x, torch.tensor([-5, 64, 1 << 30, 3], **i32), torch.tensor([0, 0, -2, 1], **i32))
+    assert int(status) == 0 and (cache.k[3, 0, 3] == 127).all() and not cache.k[:3].any()
+    q8_store(cache, x, x, torch.tensor([-5, 64, 1 << 30, 3], **i32), torch.tensor([0, 0, 1, 1], **i32))
+    assert int(status) == 1
