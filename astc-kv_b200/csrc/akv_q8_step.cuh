@@ -377,11 +377,13 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
                     x = fmaxf(x, __shfl_xor_sync(0xFFFFFFFFu, x, 16));
                     // The row's largest p is to be 2^8 again; rows below
                     // their limit stay as they are.
+                    // (Rounded so that with large scores, too, what is below
+                    // the limit is less than 16 above the base.)
                     const bool up = x > limit[nt][k];
-                    const float to = up ? x - 8.f : base[nt][k];
+                    const float to = up ? __fadd_ru(x, -8.f) : base[nt][k];
                     const float alpha = limit[nt][k] == -CUDART_INF_F ? 0.f : exp2_fast(base[nt][k] - to);
                     base[nt][k] = to;
-                    limit[nt][k] = up ? to + 15.5f : limit[nt][k];
+                    limit[nt][k] = up ? __fadd_rd(to, 15.5f) : limit[nt][k];
                     l[nt][k] *= alpha;
 #pragma unroll
                     for (int i = 0; i < KS; ++i) {

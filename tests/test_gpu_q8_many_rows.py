@@ -139,3 +139,28 @@ def test_stored_nan_stays_with_its_block(cuda, D, G, n, od, fmt, bad):
         clean, out = (Q8Attention(q, c, out_dtype=od).run() for c in (good, poor))
         sees = length - n + torch.arange(n, device="cuda") + 1 > length - block
         assert out[0, sees].isnan().all() and torch.equal(out[0, ~sees], clean[0, ~sees])
+
+
+@pytest.mark.parametrize("size", [2.0 ** 18, 2.0 ** 22, 2.0 ** 23, 2.0 ** 24, 2.0 ** 25, 2.0 ** 26, 2.0 ** 27])
+@pytest.mark.parametrize("n,od", [(1, torch.float32), (1, torch.bfloat16), (2, torch.float32), (40, torch.bfloat16)])
+def test_large_scores_that_rise(cuda, n, od, size):
+    """Scores near `size` that rise by some 5 to 12 natural units every 64 tokens, where fp32 has few bits or none for the
+    differences: an output stays among the values that it averages."""
+    from astc_kv_cuda import Q8Attention
+    T, D, G = 1024, 64, 8
+    cache, _, v = make(8, 1, T, D, block=32, seed=1, spread=0.0)
+    cache.k.zero_()
+    cache.k[..., 0] = 64
+    cache.k[..., 1] = (torch.arange(T, device="cuda") // 64).to(torch.int8)
+    cache.k_scales.fill_(1 / 64)
+    q = torch.zeros(8, n, G, D, device="cuda")
+    q[..., 0] = size
+    q[..., 1] = 64 * torch.linspace(5.0, 12.0, 64, device="cuda").view(8, 1, G)
+    lens = torch.full((8,), T, dtype=torch.int32, device="cuda")
+    # Splits of all tokens, so that one warp goes through the rise.
+    call = Q8Attention(q.bfloat16() if n == 40 else q, cache, lens, scale=1.0, out_dtype=od, lse=True, split_tokens=T)
+    out = call.run().double()
+    top = v.abs().amax()
+    assert (out.abs() <= top * (1 + 2.0 ** -7)).all()  # a NaN or an infinity is not
+    score = q[..., 0].double() + q[..., 1].double() / 64 * (T // 64 - 1)
+    assert ((call.lse.double() - score).abs() <= 2.0 ** -19 * score + 16).all()
