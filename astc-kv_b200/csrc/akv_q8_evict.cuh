@@ -195,11 +195,12 @@ __global__ void __launch_bounds__(256, PP == 2 ? 6 : 2) pack_kernel(EvictParams 
     const int row0 = blockIdx.x * c.blk, per_row = c.D / 16;
     const int len = p.lens ? min(max(p.lens[b], 0), a.T) : a.T;
     const int n = min(min(len, p.keep) - row0, c.blk);
-    if (n <= 0) return;
     int in_page;
-    const int phys = page_of(c, b, row0, in_page);
+    const int phys = n > 0 ? page_of(c, b, row0, in_page) : -1;
+    // For the kept tokens; and before any return, so that the kernel does not
+    // end before the selection (the next one waits for this one alone).
+    wait_for_previous_kernel();
     if (phys < 0) return;
-    wait_for_previous_kernel();  // for the kept tokens
     uint4 w[2][PP];
     float sc[2][PP];
 #pragma unroll

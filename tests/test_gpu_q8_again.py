@@ -237,3 +237,21 @@ def test_store_of_no_rows_anywhere(cuda):
     assert int(status) == 0 and (cache.k[3, 0, 3] == 127).all() and not cache.k[:3].any()
     q8_store(cache, x, x, torch.tensor([-5, 64, 1 << 30, 3], **i32), torch.tensor([0, 0, 1, 1], **i32))
     assert int(status) == 1
+
+
+def test_restore_where_an_eviction_of_empty_sequences_says(cuda):
+    """A restore reads the lengths that the eviction before it wrote, also when there was nothing to pack."""
+    from astc_kv_cuda import Q8Cache, Q8Evict, Q8Restore
+    cache, _, _ = make(64, 2, 4096, 32, seed=5)
+    dst = Q8Cache.zeros(64, 2, 64, 32, block_tokens=32)
+    w = torch.rand(64, 2, 4096, device="cuda")
+    lens = torch.zeros(64, dtype=torch.int32, device="cuda")
+    evict = Q8Evict(cache, dst, w, lens, keep=32)
+    restore = Q8Restore(dst, evict.lens, 1)
+    dst.k[:, :, 0], dst.k[:, :, 32] = 1, 2
+    dst.k_scales.fill_(1.0)
+    for _ in range(200):
+        evict.lens.fill_(32)
+        evict.run()
+        k, _ = restore.run()
+        assert (k == 1).all()
