@@ -70,7 +70,9 @@ class Q8Cache:
     views whose last dimension is contiguous and whose other strides are
     multiples of 16 bytes. `max_tokens` (default: all there is room for)
     bounds a sequence. `status`: optional int32 [1] that kernels write an
-    error code to (a bad table entry, a store past the end).
+    error code to (a bad table entry, a store past the end, a wait inside a
+    kernel that ran out); without it such rows are dropped or read as zeros
+    and nothing says so.
     """
     k: torch.Tensor
     v: torch.Tensor
@@ -141,7 +143,7 @@ class Q8Cache:
     @classmethod
     def zeros(cls, batch: int, kv_heads: int, max_tokens: int, head_dim: int, *, fmt: str = "int8", block_tokens: int = 64,
               page_tokens: int = 0, block_table: torch.Tensor | None = None, num_pages: int = 0,
-              device: torch.device | str = "cuda") -> "Q8Cache":
+              status: torch.Tensor | None = None, device: torch.device | str = "cuda") -> "Q8Cache":
         """An empty cache: in one piece, or `num_pages` pages of `page_tokens` for a block table."""
         if fmt not in _FORMATS:
             raise ValueError("fmt must be 'int8' or 'fp8'")
@@ -155,7 +157,8 @@ class Q8Cache:
             return torch.zeros(n, kv_heads, rows, head_dim, dtype=torch.int8, device=device).view(_FORMATS[fmt])
         def scales():
             return torch.zeros(n, kv_heads, -(-rows // block_tokens), dtype=torch.float32, device=device)
-        return cls(codes(), codes(), scales(), scales(), block_tokens=block_tokens, block_table=block_table, max_tokens=max_tokens)
+        return cls(codes(), codes(), scales(), scales(), block_tokens=block_tokens, block_table=block_table, max_tokens=max_tokens,
+                   status=status)
 
     @property
     def device(self) -> torch.device:

@@ -255,3 +255,18 @@ def test_restore_where_an_eviction_of_empty_sequences_says(cuda):
         evict.run()
         k, _ = restore.run()
         assert (k == 1).all()
+
+
+@pytest.mark.parametrize("paged", [False, True])
+def test_empty_cache_with_a_status(cuda, paged):
+    from astc_kv_cuda import Q8Cache, q8_store
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    paging = dict(block_table=torch.tensor([[0, 1]], dtype=torch.int32, device="cuda"), page_tokens=32, num_pages=1) if paged else {}
+    cache = Q8Cache.zeros(1, 1, 64, 32, block_tokens=32, status=status, **paging)
+    x = torch.ones(1, 8, 1, 32, device="cuda")
+    q8_store(cache, x, x, torch.full((1,), 4, dtype=torch.int32, device="cuda"))
+    assert int(status) == 0
+    q8_store(cache, x, x, torch.full((1,), 32 if paged else 60, dtype=torch.int32, device="cuda"))
+    assert int(status) == (5 if paged else 1)
+    with pytest.raises(ValueError):
+        Q8Cache.zeros(1, 1, 64, 32, status=status.long())
