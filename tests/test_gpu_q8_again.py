@@ -270,3 +270,86 @@ def test_empty_cache_with_a_status(cuda, paged):
     assert int(status) == (5 if paged else 1)
     with pytest.raises(ValueError):
         Q8Cache.zeros(1, 1, 64, 32, status=status.long())
+
+
+def attention_off(cache, b, k, v, length, n, od):
+    """Attention of random queries of every sequence over its whole cache, of which `b`'s last `length` tokens are k, v
+    [H, length, D] and the rest is zeros: checks its outputs and weights."""
+    from astc_kv_cuda import Q8Attention
+    H, D, T, G = cache.kv_heads, cache.head_dim, cache.max_tokens, 4
+    q = torch.randn(cache.batch, n, H * G, D, device="cuda").bfloat16()
+    w = torch.zeros(cache.batch, H, T, device="cuda")
+    out = Q8Attention(q, cache, out_dtype=od, weights=w).run()[b].double()
+    qq = q[b].double().view(n, H, G, D).permute(1, 2, 0, 3)
+    s = torch.einsum("hgnd,htd->hgnt", qq, k) * D ** -0.5
+    A = float(torch.einsum("hgnd,htd->hgnt", qq.abs(), k.abs()).max()) * D ** -0.5
+    hidden = torch.arange(length, device="cuda") > torch.arange(length - n, length, device="cuda").view(n, 1)
+    e = s.masked_fill(hidden, float("-inf")).exp()
+    p = e / (e.sum(-1, keepdim=True) + (T - length))  # every other token has score 0 and value 0
+    ref = torch.einsum("hgnt,htd->nhgd", p, v).reshape(n, H * G, D)
+    f, vmax = 2.0 ** -19 * A + 2.0 ** -18, float(v.abs().max())
+    half = od != torch.float32
+    assert ((out - ref).abs() <= vmax * (f + (2.0 ** -10 if half else 0.0)) + (2.0 ** -8 if half else 0.0) * ref.abs()).all()
+    got = w[b, :, T - length:].double()
+    assert ((got - p.sum((1, 2))).abs() <= p.sum((1, 2)) * f + 2.0 ** -22 * got + 1e-30).all()
+
+
+def test_offsets_past_32_bits_of_one_piece(cuda):
+    """The last sequence of more than 2^32 bytes of codes: store, restore, both attention kernels with weights, eviction."""
+    from astc_kv_cuda import Q8Cache, q8_evict, q8_restore, q8_store
+    B, H, T, D, n = 34, 8, 131072, 128, 300
+    assert B * H * T * D > 1 << 32
+    cache = Q8Cache.zeros(B, H, T, D, block_tokens=128)
+    x, y = torch.randn(2, B, n, H, D, device="cuda").bfloat16()
+    q8_store(cache, x, y, torch.full((B,), T - n, dtype=torch.int32, device="cuda"))
+    back = q8_restore(cache, torch.full((B,), T - n, dtype=torch.int32, device="cuda"), n)
+    for got, rows in zip(back, (x, y)):
+        assert ((got - rows.float()).abs() <= rows.float().abs().amax((1, 2, 3), keepdim=True) / 127 * 0.51).all()
+    k, v = (t[-1].double().transpose(0, 1) for t in back)
+    attention_off(cache, B - 1, k, v, n, 4, torch.float32)
+    attention_off(cache, B - 1, k, v, n, 16, torch.bfloat16)
+    w = torch.zeros(B, H, T, device="cuda")
+    w[-1, :, -n:] = torch.rand(H, n, device="cuda") + 1
+    dst = Q8Cache.zeros(B, H, 128, D, block_tokens=128)
+    kept, _, _ = q8_evict(cache, dst, w, keep=128)
+    assert (kept[-1] >= T - n).all()
+    for h in range(H):
+        at = kept[-1, h].long() - (T - n)
+        for got, rows in zip(values_of(dst), (k, v)):
+            assert ((got[-1, h] - rows[h, at]).abs() <= rows[h, at].abs().max() / 127 * 0.51).all()
+
+
+def test_offsets_past_32_bits_of_pages(cuda):
+    """The last pages of a pool of more than 2^32 bytes: every call, and an eviction into other such pages."""
+    from astc_kv_cuda import Q8Cache, q8_evict, q8_restore, q8_store
+    pages, H, P, D, block, n = 17408, 8, 256, 128, 64, 1000
+    assert pages * H * P * D > 1 << 32
+    table = torch.tensor([[pages - 1, pages - 5, pages - 2, 3]], dtype=torch.int32, device="cuda")
+    cache = Q8Cache.zeros(1, H, 4 * P, D, fmt="fp8", block_tokens=block, page_tokens=P, block_table=table, num_pages=pages)
+    x, y = torch.randn(2, 1, n, H, D, device="cuda").bfloat16()
+    q8_store(cache, x, y, torch.full((1,), 4 * P - n, dtype=torch.int32, device="cuda"))
+    back = q8_restore(cache, torch.full((1,), 4 * P - n, dtype=torch.int32, device="cuda"), n)
+    for got, rows in zip(back, (x, y)):
+        assert ((got - rows.float()).abs() <= rows.float().abs() / 16 * 1.01 + rows.abs().max().float() / 448 * 2.0 ** -10).all()
+    k, v = (t[0].double().transpose(0, 1) for t in back)
+    attention_off(cache, 0, k, v, n, 4, torch.float32)
+    attention_off(cache, 0, k, v, n, 200, torch.bfloat16)
+    to = torch.tensor([[pages - 3, pages - 4]], dtype=torch.int32, device="cuda")
+    dst = Q8Cache(cache.k, cache.v, cache.k_scales, cache.v_scales, block_tokens=block, block_table=to)
+    w = torch.rand(1, H, 4 * P, device="cuda")
+    w[:, :, :4 * P - n] = -1
+    kept, lens, _ = q8_evict(cache, dst, w, keep=500)
+    full = [torch.zeros(1, H, 4 * P, D, dtype=torch.float64, device="cuda") for _ in range(2)]
+    for f, t in zip(full, (k, v)):
+        f[0, :, 4 * P - n:] = t
+    used = own_pages(dst)
+    check_packed(full, used, kept, lens.tolist())
+
+
+def own_pages(dst):
+    """`dst`'s pages in a pool of their own, so that only they are looked at."""
+    from astc_kv_cuda import Q8Cache
+    at = dst.block_table.flatten().long()
+    table = torch.arange(at.numel(), dtype=torch.int32, device="cuda").view(dst.block_table.shape)
+    pool = [t.view(torch.int8)[at].view(t.dtype) for t in (dst.k, dst.v)] + [t[at] for t in (dst.k_scales, dst.v_scales)]
+    return Q8Cache(*pool, block_tokens=dst.block_tokens, block_table=table)

@@ -164,3 +164,70 @@ def test_large_scores_that_rise(cuda, n, od, size):
     assert (out.abs() <= top * (1 + 2.0 ** -7)).all()  # a NaN or an infinity is not
     score = q[..., 0].double() + q[..., 1].double() / 64 * (T // 64 - 1)
     assert ((call.lse.double() - score).abs() <= 2.0 ** -19 * score + 16).all()
+
+
+@pytest.mark.parametrize("D,G,n", SHAPES)
+def test_bad_table_entries_read_as_zeros(cuda, D, G, n):
+    from astc_kv_cuda import Q8Cache
+    made, k, v = make(2, 2, 512, D, page=128, block=32, seed=10)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    cache = Q8Cache(made.k, made.v, made.k_scales, made.v_scales, block_tokens=32, block_table=made.block_table, status=status)
+    cache.block_table[0, 1], cache.block_table[1, 2] = 99999, -1
+    for x in (k, v):
+        x[0, :, 128:256] = 0
+        x[1, :, 256:384] = 0
+    q = torch.randn(2, n, 2 * G, D, device="cuda").bfloat16()
+    check_attention(cache, k, v, q, [512, 300], out_dtype=torch.bfloat16)
+    assert int(status) == 5
+
+
+@pytest.mark.parametrize("D,G,n", SHAPES)
+def test_runs_repeat_bit_for_bit(cuda, D, G, n):
+    """Outputs, log-sum-exps and token weights, which other kernels compute from them."""
+    from astc_kv_cuda import Q8Attention
+    cache, _, _ = make(3, 2, 3000, D, page=256, block=64, seed=12)
+    q = torch.randn(3, n, 2 * G, D, device="cuda").half()
+    lens = torch.tensor([3000, 1234, 177], dtype=torch.int32, device="cuda")
+    w = torch.zeros(3, 2, cache.max_tokens, device="cuda")
+    call = Q8Attention(q, cache, lens, weights=w, accumulate=False, out_dtype=torch.float16, lse=True)
+    a = call.run().clone(), call.lse.clone(), w.clone()
+    for _ in range(5):
+        call.run()
+        assert torch.equal(call.out, a[0]) and torch.equal(call.lse, a[1]) and torch.equal(w, a[2])
+
+
+@pytest.mark.parametrize("D,G,n", SHAPES)
+def test_in_a_graph(cuda, D, G, n):
+    """Store, attention with weights and eviction in one graph, which follows the lengths."""
+    from astc_kv_cuda import Q8Attention, Q8Cache, Q8Evict, Q8Store
+    i32 = dict(dtype=torch.int32, device="cuda")
+    T, keep = 1024, 96
+    lens, start = torch.zeros(2, **i32), torch.zeros(2, **i32)
+    cache, dst = Q8Cache.zeros(2, 2, T, D), Q8Cache.zeros(2, 2, 128, D)
+    x, y = (torch.zeros(2, n, 2, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    q = torch.zeros(2, n, 2 * G, D, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(2, 2, T, device="cuda")
+    calls = [Q8Store(cache, x, y, start), Q8Attention(q, cache, lens, out_dtype=torch.bfloat16, weights=w),
+             Q8Evict(cache, dst, w, lens, keep=keep, recent=8)]
+
+    def run():
+        return [t.clone() for c in calls for t in (lambda r: r if isinstance(r, tuple) else (r,))(c.run()) if torch.is_tensor(t)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    fresh = [t.clone() for t in (cache.k, cache.v, cache.k_scales, cache.v_scales, w)]
+    results = []
+    for replay in (True, False):
+        for t, f in zip((cache.k, cache.v, cache.k_scales, cache.v_scales, w), fresh):
+            t.copy_(f)
+        g = torch.Generator(device="cuda").manual_seed(3)
+        for at in (0, n, 2 * n):
+            start.copy_(torch.tensor([at, at // 2], **i32))
+            lens.copy_(start + n)
+            for t in (x, y, q):
+                t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+            if replay:
+                graph.replay()
+                results.append([t.clone() for t in got])
+            else:
+                assert all(torch.equal(a, b) for a, b in zip(results.pop(0), run()))
