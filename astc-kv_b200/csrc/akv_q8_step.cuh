@@ -27,6 +27,11 @@
 // raises it so that the largest P' is 2^8 again. A vote finds such scores;
 // after the first tiles they are rare.
 //
+// The tensor cores truncate as they add, which makes a long sum smaller than it
+// is. With fp32 outputs O is added, rounded to nearest, to a sum that waits in
+// shared memory, every 32 products (30010 tokens by one CTA, D 256: 1.6e-5 off
+// without that, of it 1.3e-5 too small, now 9e-7).
+//
 // The work, 64-token chunks of every (sequence, kv head, group of rows), is
 // divided evenly over the CTAs of one wave, whatever the lengths: a CTA's
 // share may start and end inside a unit, whose pieces the combine kernel adds
@@ -92,11 +97,13 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     __shared__ uint2 qs[KS][NT][QLO ? 2 : 1][32];
 
     __shared__ ShareScratch scratch;
+    __shared__ float carry[PLO ? 2 * NT : 1][kStepThreads];
 
     const CacheDev& c = p.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
     static_assert(!TWIN || (PLO && NT == 1), "twin rows carry P's second part");
     constexpr bool SECOND = PLO && !TWIN;  // P's second part in products of its own
+    constexpr int FOLD = SECOND ? 1024 : 2048;  // tokens after which O goes to its sum in shared memory (fp32 outputs)
     const int groups = (p.R + ROWS - 1) / ROWS, units = c.H * groups;  // of a sequence
     int64_t at = 0, stop = 1;  // the next chunk of this CTA's share, its end
     int b, unit_of_b, chunk;
@@ -304,7 +311,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
 #pragma unroll
         for (int i = 0; i < KS; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) { base[nt][k] = 0.f; limit[nt][k] = -CUDART_INF_F; l[nt][k] = 0.f; }
+        for (int k = 0; k < 2; ++k) { base[nt][k] = 0.f; limit[nt][k] = -CUDART_INF_F; l[nt][k] = 0.f; if (PLO) carry[2 * nt + k][threadIdx.x] = 1.f; }
     }
 
     auto tile = [&](int t0, const uint32_t (&vr)[4][VW], float vscale, uint32_t (&v_next)[4][VW], float& vscale_next) {
@@ -385,6 +392,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
                     base[nt][k] = to;
                     limit[nt][k] = up ? __fadd_rd(to, 15.5f) : limit[nt][k];
                     l[nt][k] *= alpha;
+                    if (PLO) carry[2 * nt + k][threadIdx.x] *= alpha;
 #pragma unroll
                     for (int i = 0; i < KS; ++i) {
                         o[i][nt][k] *= alpha;
@@ -427,12 +435,44 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
                 }
         }
     };
+    // O's sum, brought to the present base by `carry`: the lane's own part of
+    // the room that `red` takes at the end.
+    float4* const sums = reinterpret_cast<float4*>(&red[warp][0][0]) + lane;
     for (int t0 = t_begin + 16 * warp; t0 < t_end; t0 += 32 * kStepWarps) {
         tile(t0, va, vscale_a, vb, vscale_b);
         if (t0 + 16 * kStepWarps < t_end) tile(t0 + 16 * kStepWarps, vb, vscale_b, va, vscale_a);
+        if (PLO && t0 % FOLD >= FOLD - 32 * kStepWarps) {
+            const bool first = t0 - t_begin < FOLD;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const float f0 = carry[2 * nt][threadIdx.x], f1 = carry[2 * nt + 1][threadIdx.x];
+                carry[2 * nt][threadIdx.x] = carry[2 * nt + 1][threadIdx.x] = 1.f;
+#pragma unroll
+                for (int i = 0; i < KS; ++i) {
+                    float(&x)[4] = o[i][nt];
+                    float4 v = first ? make_float4(0.f, 0.f, 0.f, 0.f) : sums[(i * NT + nt) * 32];
+                    v = make_float4(fmaf(v.x, f0, x[0]), fmaf(v.y, f1, x[1]), fmaf(v.z, f0, x[2]), fmaf(v.w, f1, x[3]));
+                    sums[(i * NT + nt) * 32] = v;
+                    x[0] = x[1] = x[2] = x[3] = 0.f;
+                }
+            }
+        }
     }
 
     allow_next_kernel();
+    const int begun = t_begin + 16 * warp;
+    if (PLO && begun + (FOLD - 1 - begun % FOLD) / (32 * kStepWarps) * (32 * kStepWarps) < t_end) {  // there is a sum
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const float f0 = carry[2 * nt][threadIdx.x], f1 = carry[2 * nt + 1][threadIdx.x];
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                const float4 v = sums[(i * NT + nt) * 32];
+                float(&x)[4] = o[i][nt];
+                x[0] = fmaf(v.x, f0, x[0]); x[1] = fmaf(v.y, f1, x[1]); x[2] = fmaf(v.z, f0, x[2]); x[3] = fmaf(v.w, f1, x[3]);
+            }
+        }
+    }
     // Join the warps in their order: (m, l) first, then O under the common maximum.
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)

@@ -231,3 +231,21 @@ def test_in_a_graph(cuda, D, G, n):
                 results.append([t.clone() for t in got])
             else:
                 assert all(torch.equal(a, b) for a, b in zip(results.pop(0), run()))
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("D,G,n,T", [(64, 3, 1, 65536), (128, 4, 1, 65536), (128, 8, 1, 30010), (128, 4, 4, 40000), (256, 2, 1, 65536),
+                                     (256, 8, 3, 30010), (64, 9, 1, 1025), (64, 1, 1, 4099)])
+def test_long_sums_do_not_shrink(cuda, D, G, n, T, fmt):
+    """Outputs are means of equal values, summed by one warp group over all tokens: what is lost is what the sums lose. 32
+    sums that truncate at 2^-23, on the average at half of what they come to, make 2^-19; the parts of the softmax
+    weights (2^-22), the exponentials (2^-22) and the sums to nearest the rest of 2^-18."""
+    from astc_kv_cuda import Q8Attention
+    cache, _, _ = make(2, 1, T, D, fmt=fmt, block=32, seed=T)
+    cache.v.copy_(torch.full(cache.v.shape, 104.0, device="cuda").to(cache.v.dtype))
+    cache.v_scales.fill_(1 / 96)
+    q = torch.randn(2, n, G, D, device="cuda").bfloat16()
+    lens = torch.tensor([T, T - 777], dtype=torch.int32, device="cuda")
+    out = Q8Attention(q, cache, lens, scale=0.3 * D ** -0.5, split_tokens=(T + 15) // 16 * 16).run().double()
+    value = float(torch.tensor(1 / 96)) * 104
+    assert ((out - value).abs() <= 2.0 ** -18 * value).all()
