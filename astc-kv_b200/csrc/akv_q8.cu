@@ -108,6 +108,14 @@ struct AttnPlan {
 // 80 us against 51; 32 rows, B8 x 8192 90 against 92).
 constexpr int kChunkMinRows = 33;
 
+// Tokens that a tile of the tcgen05 kernel adds up at most where outputs are
+// fp16. The tensor cores truncate as they add: a sum over n tokens comes out
+// 6e-9 n too small (measured: 3e-5 at 8192, 8e-4 at 131072 tokens), which fp16
+// outputs, 2.4e-4 off by their rounding on the average, would show. A second
+// partial costs about 2.5 of this split's 128 steps. (bf16 outputs are eight
+// times coarser.)
+constexpr int64_t kChunkHalfTokens = 16384;
+
 // Tokens for each CTA of a cluster up to which a cluster for each kv head of
 // each sequence beats even shares of all CTAs and a second launch (32/8 heads:
 // B1 x 4096 in clusters of eight 16.0 us against 18.8; B64 x 300, a CTA each,
@@ -152,6 +160,10 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
         for (int64_t n = 2; n <= most && n <= steps; ++n)
             if (cost(n) <= limit) best = n;
         if (cost(1) <= least) best = best > 1 && limit > least ? best : 1;
+        if (d->out_dtype == AKV_Q_F16) {
+            const int64_t longest = kChunkHalfTokens / kChunkTokens * (shared ? 2 : 1), n = (steps + longest - 1) / longest;
+            best = best > n ? best : n;
+        }
         a.split = static_cast<int>((steps + best - 1) / best * kChunkTokens);
     }
     size_t parts;  // rows of partials

@@ -249,3 +249,22 @@ def test_long_sums_do_not_shrink(cuda, D, G, n, T, fmt):
     out = Q8Attention(q, cache, lens, scale=0.3 * D ** -0.5, split_tokens=(T + 15) // 16 * 16).run().double()
     value = float(torch.tensor(1 / 96)) * 104
     assert ((out - value).abs() <= 2.0 ** -18 * value).all()
+
+
+@pytest.mark.parametrize("n,H", [(16, 4), (100, 2)])
+def test_long_sums_of_fp16_outputs(cuda, n, H):
+    """Row tiles for 148 SMs, so that nothing but length asks for splits. Outputs are 64 known values, each rounded to
+    fp16, 2^-11 at most and at random: their mean is off by 2^-14.8, one standard deviation. Sums that lose 2^-27.3 of
+    themselves with every token, over 16384 of them, lose 2^-13.3."""
+    from astc_kv_cuda import Q8Attention, Q8Cache
+    B, G, T, D = 37, 4, 131072, 64
+    cache = Q8Cache.zeros(B, H, T, D, block_tokens=128)
+    cache.k.random_(-100, 101)
+    cache.v.copy_(torch.arange(64, 128, device="cuda").to(torch.int8).expand(cache.v.shape))
+    cache.k_scales.fill_(1 / 100)
+    cache.v_scales.fill_(1 / 96)
+    q = torch.randn(B, n, H * G, D, device="cuda").half()
+    out = Q8Attention(q, cache, out_dtype=torch.float16).run().double()
+    value = float(torch.tensor(1 / 96)) * torch.arange(64, 128, device="cuda").double()
+    off = (out / value - 1).mean(-1)
+    assert (off.abs() <= 2.0 ** -12).all()
