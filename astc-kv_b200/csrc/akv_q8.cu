@@ -144,8 +144,12 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
         // partial written and read; the number of splits, up to eight or one
         // wave, is that of the least cost over the waves. Where lengths may be
         // ragged more splits are taken for up to 15 %: short sequences then
-        // leave SMs to long ones (4 sequences of 559 to 8190 tokens, 9/3
-        // heads, 509 query tokens and their weights: 118 against 148 us).
+        // leave SMs to long ones. 4 x 128 query tokens, 32/8 heads, D 128, up
+        // to 8192 tokens, four splits against two: 241 to 8192 tokens 67 us
+        // against 100, all 8192 119 against 103; 4 x 509, 9/3 heads, D 64: 58
+        // against 89, and 100 against 90. Not where units fill the SMs, which
+        // then even the lengths out by themselves: 4 x 512 query tokens, four
+        // splits against one, ragged 234 against 159, equal 425 against 313.
         const int64_t units = bh * ((a.rows + group - 1) / group), sms = sm_count();
         const int64_t steps = (static_cast<int64_t>(c.max_tokens) + kChunkTokens - 1) / kChunkTokens;
         const int64_t most = units > 0 && sms / units > 8 ? sms / units : 8;
@@ -156,7 +160,7 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
         double least = cost(1);
         for (int64_t n = 2; n <= most && n <= steps; ++n) least = cost(n) < least ? cost(n) : least;
         int64_t best = 1;
-        const double limit = d->seq_lens_dev && c.batch > 1 ? 1.15 * least : least;
+        const double limit = d->seq_lens_dev && c.batch > 1 && units < sms ? 1.15 * least : least;
         for (int64_t n = 2; n <= most && n <= steps; ++n)
             if (cost(n) <= limit) best = n;
         if (cost(1) <= least) best = best > 1 && limit > least ? best : 1;

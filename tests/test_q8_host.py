@@ -198,3 +198,15 @@ def test_a_batch_of_none_needs_no_memory():
     assert lib.akv_q8_attention_workspace(ct.byref(a)) >= 16
     for fn, d in ((lib.akv_q8_attention, a), (lib.akv_q8_evict, e), (lib.akv_q8_store, s), (lib.akv_q8_restore, r)):
         assert fn(ct.byref(d), None) == 0
+
+
+@pytest.mark.parametrize("q_tokens,more", [(128, True), (512, False)])
+def test_ragged_lengths_ask_for_more_splits_of_few_rows_only(q_tokens, more):
+    """Partials take workspace. With rows for every SM, lengths do not change the splits."""
+    lib = L.lib()
+    d = _attention()
+    d.cache.batch, d.cache.kv_heads, d.cache.head_dim, d.cache.max_tokens, d.cache.page_tokens = 4, 8, 128, 8192, 8192
+    d.q_heads, d.q_tokens, d.out_dtype = 32, q_tokens, L.AKV_Q_BF16
+    without = lib.akv_q8_attention_workspace(ct.byref(d))
+    d.seq_lens_dev = 4096
+    assert (lib.akv_q8_attention_workspace(ct.byref(d)) > without) == more
