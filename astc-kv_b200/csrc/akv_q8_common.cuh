@@ -48,8 +48,8 @@ inline CacheDev to_dev(const AkvQ8Cache& c) {
 // Ordering with the kernel before or after on the stream when both are
 // launched as programmatic dependents (no effect otherwise): the next one may
 // be brought onto the SMs, and wait until everything before has finished. A
-// kernel waits in every CTA, whatever it does, since its end is all that the
-// next one's wait sees.
+// kernel waits in one CTA at least, whatever it has to do, since its end is
+// all that the next one's wait sees.
 __device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

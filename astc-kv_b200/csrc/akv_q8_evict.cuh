@@ -197,9 +197,10 @@ __global__ void __launch_bounds__(256, PP == 2 ? 6 : 2) pack_kernel(EvictParams 
     const int n = min(min(len, p.keep) - row0, c.blk);
     int in_page;
     const int phys = n > 0 ? page_of(c, b, row0, in_page) : -1;
-    // For the kept tokens; and before any return, so that the kernel does not
-    // end before the selection (the next one waits for this one alone).
-    wait_for_previous_kernel();
+    // For the kept tokens; and in a CTA of each row at least, so that the
+    // kernel does not end before the selection (the next one waits for this
+    // one alone).
+    if (phys >= 0 || blockIdx.x == 0) wait_for_previous_kernel();
     if (phys < 0) return;
     uint4 w[2][PP];
     float sc[2][PP];
@@ -243,7 +244,13 @@ __global__ void __launch_bounds__(256, PP == 2 ? 6 : 2) pack_kernel(EvictParams 
 #pragma unroll
         for (int k = 1; k < 8; ++k) top = max(top, red[side][k]);
         const float scale = block_scale<FMT>(top), inv = block_inverse(scale);
-        const bool numbers = !isnan(scale);  // see store_kernel
+        if (isnan(scale)) {  // see store_kernel
+#pragma unroll
+            for (int k = 0; k < PP; ++k) {
+                w[side][k] = make_uint4(0, 0, 0, 0);
+                sc[side][k] = 0.f;
+            }
+        }
         uint8_t* codes = to.codes + code_offset(to, b, h, phys, in_page);
 #pragma unroll
         for (int k = 0; k < PP; ++k) {
@@ -256,7 +263,7 @@ __global__ void __launch_bounds__(256, PP == 2 ? 6 : 2) pack_kernel(EvictParams 
                 from_codes4<FMT>(u[j], f);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(__fmul_rn(f[e], sc[side][k]), inv);
-                u[j] = numbers ? to_codes4<FMT>(f) : 0u;
+                u[j] = to_codes4<FMT>(f);
             }
             reinterpret_cast<uint4*>(codes + r * to.sT)[i - r * per_row] = make_uint4(u[0], u[1], u[2], u[3]);
         }

@@ -96,9 +96,9 @@ __global__ void __launch_bounds__(256, PP == 2 ? (sizeof(T) == 2 ? 6 : 4) : 1) s
     const CacheDev& c = p.c;
     const int h = blockIdx.y, b = blockIdx.z >> 1, side = blockIdx.z & 1;
     const int start = p.start[b], count = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
-    if (count == 0) return;  // wherever it starts
     if (start < 0 || static_cast<int64_t>(start) + count > c.T) {
-        if (threadIdx.x == 0 && blockIdx.x == 0) report(c.status, AKV_ERR_INVALID_ARGUMENT);
+        // (No rows are nowhere outside. Asked here, so that both loads are in flight at a time.)
+        if (count > 0 && threadIdx.x == 0 && blockIdx.x == 0) report(c.status, AKV_ERR_INVALID_ARGUMENT);
         if (start < 0 || start >= c.T) return;
     }
     const int end = start + min(count, c.T - start), shift = 31 - __clz(c.blk);
@@ -154,7 +154,12 @@ __global__ void __launch_bounds__(256, PP == 2 ? (sizeof(T) == 2 ? 6 : 4) : 1) s
     const float inv = block_inverse(scale);
     // A block with a NaN scale holds zeros: a NaN code would meet the softmax
     // weight 0 of rows that do not see it, in the attention's products.
-    const bool numbers = !isnan(scale);
+    if (isnan(scale)) {
+#pragma unroll
+        for (int k = 0; k < PP; ++k)
+#pragma unroll
+            for (int j = 0; j < static_cast<int>(sizeof(T)); ++j) v[k].w[j] = make_uint4(0, 0, 0, 0);
+    }
 #pragma unroll
     for (int k = 0; k < PP; ++k) {
         const int i = threadIdx.x + k * blockDim.x;
@@ -166,7 +171,7 @@ __global__ void __launch_bounds__(256, PP == 2 ? (sizeof(T) == 2 ? 6 : 4) : 1) s
             float f[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) f[e] = __fmul_rn(v[k].get(4 * j + e), inv);
-            u[j] = numbers ? to_codes4<FMT>(f) : 0u;
+            u[j] = to_codes4<FMT>(f);
         }
         *reinterpret_cast<uint4*>(codes + r * s.sT + d) = make_uint4(u[0], u[1], u[2], u[3]);
     }

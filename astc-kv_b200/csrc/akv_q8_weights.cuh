@@ -47,8 +47,8 @@ __global__ void __launch_bounds__(kWeightThreads) weights_kernel(AttnParams p) {
     const int first = blockIdx.x * kWeightTile;
     float* at = p.weights + static_cast<int64_t>(bh) * p.wstride;
     if (first >= len) {
-        // Also here, so that the kernel does not end before the one before it.
-        wait_for_previous_kernel();
+        // So that the kernel does not end before the one before it.
+        if (blockIdx.x == 0) wait_for_previous_kernel();
         if (!p.accumulate && threadIdx.x < kWeightTile && first + threadIdx.x < c.T) at[first + threadIdx.x] = 0.f;
         return;
     }
