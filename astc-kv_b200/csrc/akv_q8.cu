@@ -224,7 +224,7 @@ int launch_chunk(const AttnParams& p, cudaStream_t s) {
     const int parts = SHARED ? p.nsplits / 2 : p.nsplits;
     constexpr int rows = 128 * kChunkTiles<DP>;
     const dim3 grid(parts * ((p.R + rows - 1) / rows), p.c.H, p.c.B);
-    kern<<<grid, kChunkThreads, bytes, s>>>(p);
+    kern<<<grid, kChunkThreads<DP>, bytes, s>>>(p);
     return launched();
 }
 

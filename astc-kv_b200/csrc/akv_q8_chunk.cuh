@@ -54,7 +54,10 @@ template <int DP>
 constexpr int kChunkTiles = DP <= 128 ? 2 : 1;
 constexpr int kChunkTokens = 128;  // per step
 constexpr int kChunkHalf = 64;     // P goes to the tensor cores in two parts
-constexpr int kChunkThreads = 32 * 20;  // five warpgroups; warps 17-19 only give their registers away
+// Five warpgroups, whose last three warps only give their registers away; with
+// one tile four, of 128 registers a thread.
+template <int DP>
+constexpr int kChunkThreads = 32 * (kChunkTiles<DP> == 2 ? 20 : 16);
 constexpr int kMetaSlots = 4;      // K may be written three steps ahead of a softmax
 
 template <int DP>
@@ -177,7 +180,7 @@ __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (
 // SHARED: 128 rows or fewer a kv head; both tiles take the same rows and every
 // other step, as two splits.
 template <int FMT, int DP, bool SHARED>
-__global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
+__global__ void __launch_bounds__(kChunkThreads<DP>, 1) chunk_kernel(AttnParams p) {
     using Smem = ChunkSmem<DP>;
     constexpr int TILES = kChunkTiles<DP>, STAGES = TILES, ROWS = 128 * TILES;
     static_assert(!SHARED || TILES == 2, "two tiles to share rows");
@@ -185,7 +188,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     // The swizzle counts from 1024-byte boundaries.
     Smem& sm = *reinterpret_cast<Smem*>(smem_raw + (-smem_addr(smem_raw) & 1023));
     const CacheDev& c = p.c;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // With one tile there is no second group of softmax warps.
+    constexpr int THREADS = kChunkThreads<DP>, MISSING = TILES == 2 ? 0 : 4;
+    const int hw_warp = threadIdx.x >> 5, warp = hw_warp < 4 ? hw_warp : hw_warp + MISSING, lane = threadIdx.x & 31;
     const int tiles = (p.R + ROWS - 1) / ROWS;
     // Later rows see more tokens: they go first.
     const int parts = SHARED ? p.nsplits / 2 : p.nsplits;  // CTAs along the tokens
@@ -198,7 +203,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     const int steps = t_end > t_begin ? (t_end - t_begin + kChunkTokens - 1) / kChunkTokens : 0;
     if (steps == 0) {
         // Nothing to see for any row.
-        for (int i = threadIdx.x; i < rows; i += kChunkThreads) {
+        for (int i = threadIdx.x; i < rows; i += THREADS) {
             if (p.nsplits > 1) {
                 p.part_ml[unit + i] = make_float2(-CUDART_INF_F, 0.f);
                 if (SHARED) p.part_ml[unit + p.R + i] = make_float2(-CUDART_INF_F, 0.f);
@@ -209,7 +214,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
             if (p.lse_out) p.lse_out[row] = -CUDART_INF_F;
         }
         if (p.nsplits == 1)
-            for (int i = threadIdx.x; i < rows * c.D; i += kChunkThreads)
+            for (int i = threadIdx.x; i < rows * c.D; i += THREADS)
                 store_elem(p.out, p.out_dtype, out_row(p, b, h, r0 + i / c.D) * c.D + i % c.D, 0.f);
         return;
     }
@@ -287,13 +292,11 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
 
     // Steps of a tile: all, or every other one.
     const bool two = TILES == 2 && (SHARED || rows > 128);  // else the second tile rests
-    // Registers go to where they are needed: 2 x 136 + 2 x 80 + 48 = 5 x 96,
-    // with one tile 136 + 24 + 2 x 136 + 48.
-    if (TILES == 1 && warp >= 4 && warp < 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 24;");
-    } else if (warp < 8) {
+    // Registers go to where they are needed: 2 x 136 + 2 x 80 + 48 = 5 x 96
+    // (with one tile all have what they need).
+    if (warp < 8) {
         // ------------------------------------------------------------ softmax
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+        if (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         const int tile = warp >> 2;
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes
         const uint32_t s_tile = tmem + tile * 128 + lanes, o_at = tmem + 256 + tile * 128 + lanes;
@@ -461,11 +464,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     } else if (warp < 12) {
         // ---------------------------------------------------------- K to fp16
         if (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        else asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         // Four lanes a row of a 64-column tile, 32 rows at a time: the stores
         // of eight lanes (two rows, every other chunk) fall into different
         // banks.
-        const int tid = threadIdx.x - 256;
+        const int tid = threadIdx.x - 32 * (8 - MISSING);
         constexpr int KP = DP / 16;  // 16-byte pieces per lane and step
         const int k_row = tid >> 2, k_piece = tid & 3;
         int k_col[DP / 64];
@@ -546,7 +548,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
     } else if (warp < 16) {
         // ---------------------------------------------------------- V to fp16
         if (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-        else asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
         // Eight lanes take the 64 tokens of a tile row, eight tokens each.
         const int w = warp & 3;
         constexpr int VW = DP / 32;  // words of a token per lane
@@ -600,7 +601,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1) chunk_kernel(AttnParams p) {
         }
     } else {
         // --------------------------------------------------------- the products
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
         if (warp == 16) {
             // The whole warp goes through the loop, so that addresses stay in
             // uniform registers; one lane issues.
