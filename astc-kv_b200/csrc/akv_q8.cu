@@ -103,10 +103,14 @@ struct AttnPlan {
 };
 
 // Rows from which the tcgen05 kernel, whose CTA does 128 or 256 rows for the
-// price of one, is ahead of the step kernel, which does 16 (32/8 heads, D 128,
-// int8: 36 rows, B8 x 8192 tokens 78 us against 153; 32 rows, B1 x 32768 tokens
-// 80 us against 51; 32 rows, B8 x 8192 90 against 92).
-constexpr int kChunkMinRows = 33;
+// price of one, is ahead of the step kernel, which does 16 at a time (8 above
+// head_dim 128). Measured, 8 kv heads, step kernel against tcgen05, B8 x 8192
+// tokens: D 128 int8 20 rows 78 us against 81, 32 rows 81 against 82, 36 rows
+// 153 against 83; D 64 32 rows 50 against 59; D 256 int8 16 rows 106 against
+// 119, 20 rows 143 against 120, e4m3 101 against 114 and 134 against 115.
+// (B1 x 32768, D 128, 32 rows 47 against 43; B8 x 700, D 64, 20 rows 20
+// against 17: short of 33 rows neither is far ahead up to D 128.)
+int chunk_min_rows(int head_dim) { return head_dim <= 128 ? 33 : 17; }
 
 // Tokens that a tile of the tcgen05 kernel adds up at most where outputs are
 // fp16. The tensor cores truncate as they add: a sum over n tokens comes out
@@ -133,7 +137,7 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
     const int64_t bh = static_cast<int64_t>(c.batch) * c.kv_heads;
     a.rows = d->q_tokens * (d->q_heads / c.kv_heads);
     a.nt = c.head_dim <= 128 && a.rows > 8 ? 2 : 1;
-    a.chunk = a.rows >= kChunkMinRows && d->q_dtype != AKV_Q_F32 && d->out_dtype != AKV_Q_F32;
+    a.chunk = a.rows >= chunk_min_rows(c.head_dim) && d->q_dtype != AKV_Q_F32 && d->out_dtype != AKV_Q_F32;
     a.keep_scores = !a.chunk && d->weights_dev && a.rows <= 8 * a.nt && a.rows <= kScoreRows;
     a.split = d->split_tokens;
     const bool shared = a.chunk && a.rows <= 128 && c.head_dim <= 128;  // its two tiles share the rows and take every other step

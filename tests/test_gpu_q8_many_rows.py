@@ -268,3 +268,12 @@ def test_long_sums_of_fp16_outputs(cuda, n, H):
     value = float(torch.tensor(1 / 96)) * torch.arange(64, 128, device="cuda").double()
     off = (out / value - 1).mean(-1)
     assert (off.abs() <= 2.0 ** -12).all()
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("D", [144, 208, 256])
+@pytest.mark.parametrize("n", [8, 9, 16, 17, 24, 32])
+def test_wide_heads_of_few_rows(cuda, D, n, fmt):
+    cache, k, v = make(2, 2, 500, D, fmt=fmt, block=32, seed=n)
+    q = torch.randn(2, n, 2, D, device="cuda").half()
+    check_attention(cache, k, v, q, [500, 130], [n, n // 2], out_dtype=torch.float16)

@@ -210,3 +210,16 @@ def test_ragged_lengths_ask_for_more_splits_of_few_rows_only(q_tokens, more):
     without = lib.akv_q8_attention_workspace(ct.byref(d))
     d.seq_lens_dev = 4096
     assert (lib.akv_q8_attention_workspace(ct.byref(d)) > without) == more
+
+
+@pytest.mark.parametrize("head_dim,rows", [(64, 33), (128, 33), (144, 17), (256, 17)])
+def test_rows_from_which_the_kernel_for_many_rows_is_taken(head_dim, rows):
+    """It shows in the workspace: one step of that kernel has no partials, or two a row where two tiles share the rows."""
+    lib = L.lib()
+    for n in (rows - 1, rows):
+        d = _attention()
+        d.cache.batch, d.cache.kv_heads, d.cache.head_dim, d.cache.max_tokens = 1, 1, head_dim, 128
+        d.q_heads, d.q_tokens, d.out_dtype = 1, n, L.AKV_Q_BF16
+        parts = 2 * n if head_dim <= 128 else 0
+        want = (parts * 8 + 15) // 16 * 16 + parts * head_dim * 4 + 16
+        assert (lib.akv_q8_attention_workspace(ct.byref(d)) == want) == (n == rows)
