@@ -126,10 +126,14 @@ constexpr int64_t kChunkHalfTokens = 16384;
 // 22 against 30, the same ragged to 500 tokens 19 against 27).
 constexpr int kClusterTokens = 512;
 
-// Rows whose scores are stored for the token weights rather than computed
-// again: storing costs 8 bytes per row and token, a second pass over K
-// head_dim bytes per token.
-constexpr int kScoreRows = 16;
+// Scores are stored for the token weights, rather than computed again, where one
+// CTA of the step kernel has all rows. Storing costs 8 bytes per row
+// and token, a second pass over K head_dim bytes per token and the products;
+// stored against computed, B8 x 8192 tokens, 8 kv heads, int8: D 64 1 row 28 us
+// against 59, 16 rows 52 against 71; D 128 41 against 93 and 66 against 109;
+// D 256 8 rows 72 against 177. Stored scores take 4 bytes of workspace per row,
+// kv head and token of max_tokens.
+bool keeps_scores(const AttnPlan& a) { return !a.chunk && a.rows <= 8 * a.nt; }
 
 AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
     AttnPlan a = {};
@@ -138,7 +142,7 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
     a.rows = d->q_tokens * (d->q_heads / c.kv_heads);
     a.nt = c.head_dim <= 128 && a.rows > 8 ? 2 : 1;
     a.chunk = a.rows >= chunk_min_rows(c.head_dim) && d->q_dtype != AKV_Q_F32 && d->out_dtype != AKV_Q_F32;
-    a.keep_scores = !a.chunk && d->weights_dev && a.rows <= 8 * a.nt && a.rows <= kScoreRows;
+    a.keep_scores = d->weights_dev && keeps_scores(a);
     a.split = d->split_tokens;
     const bool shared = a.chunk && a.rows <= 128 && c.head_dim <= 128;  // its two tiles share the rows and take every other step
     const int group = a.chunk ? (c.head_dim <= 128 ? 256 : 128) : 8 * a.nt;  // rows of a CTA
