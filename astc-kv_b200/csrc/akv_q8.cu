@@ -4,6 +4,7 @@
 
 #include <atomic>
 #include <cmath>
+#include <initializer_list>
 
 #include "../../include/akv_q8.h"
 #include "akv_q8_attend.cuh"
@@ -22,6 +23,13 @@ constexpr int kMaxGridYZ = 65535;
 
 bool valid_dtype(int t) { return t >= AKV_Q_F32 && t <= AKV_Q_F16; }
 
+// Words that kernels read or write one at a time, or NULL.
+bool words(std::initializer_list<const void*> pointers) {
+    for (const void* p : pointers)
+        if (reinterpret_cast<uintptr_t>(p) % 4) return false;
+    return true;
+}
+
 // A cache for no sequences needs no memory.
 bool valid_side(const AkvQ8Side& s, int batch) {
     return (batch == 0 || (s.codes && s.scales)) && reinterpret_cast<uintptr_t>(s.codes) % 16 == 0 && reinterpret_cast<uintptr_t>(s.scales) % 4 == 0 &&
@@ -31,7 +39,7 @@ bool valid_side(const AkvQ8Side& s, int batch) {
 int check_cache(const AkvQ8Cache& c) {
     if (c.format != AKV_Q8_INT8 && c.format != AKV_Q8_E4M3) return AKV_ERR_INVALID_ARGUMENT;
     if (c.batch < 0 || c.kv_heads <= 0 || c.head_dim <= 0 || c.max_tokens <= 0 || c.page_tokens <= 0) return AKV_ERR_INVALID_ARGUMENT;
-    if (!valid_side(c.k, c.batch) || !valid_side(c.v, c.batch)) return AKV_ERR_INVALID_ARGUMENT;
+    if (!valid_side(c.k, c.batch) || !valid_side(c.v, c.batch) || !words({c.block_table_dev, c.status_dev})) return AKV_ERR_INVALID_ARGUMENT;
     if (c.block_tokens <= 0 || c.page_tokens % c.block_tokens) return AKV_ERR_INVALID_ARGUMENT;
     if (c.block_table_dev &&
         (c.pages_per_seq <= 0 || c.num_pages <= 0 || static_cast<int64_t>(c.pages_per_seq) * c.page_tokens < c.max_tokens))
@@ -74,6 +82,7 @@ int check_attention(const AkvQ8AttnDesc* d) {
         return AKV_ERR_INVALID_ARGUMENT;
     if (d->split_tokens < 0 || d->split_tokens % 16 || !(d->scale >= 0.f) || std::isinf(d->scale)) return AKV_ERR_INVALID_ARGUMENT;
     if (d->weights_dev && d->weights_stride < d->cache.max_tokens) return AKV_ERR_INVALID_ARGUMENT;
+    if (!words({d->seq_lens_dev, d->q_lens_dev, d->lse_dev, d->weights_dev})) return AKV_ERR_INVALID_ARGUMENT;
     const int64_t rows = static_cast<int64_t>(d->q_heads) * d->q_tokens;
     if (rows > 1 << 24 || rows * d->cache.batch > 1 << 30) return AKV_ERR_UNSUPPORTED;
     return AKV_OK;
@@ -284,7 +293,7 @@ int akv_q8_store(const AkvQ8StoreDesc* d, void* stream) {
     if (d->cache.batch == 0 || d->tokens == 0) return AKV_OK;
     const uintptr_t elem = d->dtype == AKV_Q_F32 ? 4 : 2;
     if (!d->k_dev || !d->v_dev || !d->start_dev || reinterpret_cast<uintptr_t>(d->k_dev) % elem ||
-        reinterpret_cast<uintptr_t>(d->v_dev) % elem)
+        reinterpret_cast<uintptr_t>(d->v_dev) % elem || !words({d->start_dev, d->counts_dev}))
         return AKV_ERR_INVALID_ARGUMENT;
     StoreParams p;
     p.c = to_dev(d->cache);
@@ -323,7 +332,7 @@ int akv_q8_restore(const AkvQ8RestoreDesc* d, void* stream) {
     if (int st = check_cache(d->cache)) return st;
     if (d->tokens < 0 || !valid_dtype(d->dtype)) return AKV_ERR_INVALID_ARGUMENT;
     if (d->cache.batch == 0 || d->tokens == 0) return AKV_OK;
-    if (!d->k_dev || !d->v_dev || reinterpret_cast<uintptr_t>(d->k_dev) % 16 || reinterpret_cast<uintptr_t>(d->v_dev) % 16)
+    if (!d->k_dev || !d->v_dev || reinterpret_cast<uintptr_t>(d->k_dev) % 16 || reinterpret_cast<uintptr_t>(d->v_dev) % 16 || !words({d->start_dev}))
         return AKV_ERR_INVALID_ARGUMENT;
     RestoreParams p;
     p.c = to_dev(d->cache);
@@ -430,7 +439,9 @@ int akv_q8_evict(const AkvQ8EvictDesc* d, void* stream) {
         (same(a.k.codes, c.k.codes) || same(a.v.codes, c.v.codes) || same(a.k.scales, c.k.scales) || same(a.v.scales, c.v.scales)))
         return AKV_ERR_INVALID_ARGUMENT;
     if (a.batch == 0) return AKV_OK;
-    if (!d->weights_dev || !d->kept_dev || !d->out_lens_dev || !d->out_weights_dev) return AKV_ERR_INVALID_ARGUMENT;
+    if (!d->weights_dev || !d->kept_dev || !d->out_lens_dev || !d->out_weights_dev ||
+        !words({d->weights_dev, d->kept_dev, d->out_lens_dev, d->out_weights_dev, d->seq_lens_dev}))
+        return AKV_ERR_INVALID_ARGUMENT;
     EvictParams p;
     p.src = to_dev(a); p.dst = to_dev(c);
     p.weights = d->weights_dev; p.wstride = d->weights_stride; p.lens = d->seq_lens_dev;

@@ -223,3 +223,39 @@ def test_rows_from_which_the_kernel_for_many_rows_is_taken(head_dim, rows):
         parts = 2 * n if head_dim <= 128 else 0
         want = (parts * 8 + 15) // 16 * 16 + parts * head_dim * 4 + 16
         assert (lib.akv_q8_attention_workspace(ct.byref(d)) == want) == (n == rows)
+
+
+def test_addresses_of_words_are_checked():
+    """int32 and fp32 arrays on odd addresses would fault on the GPU."""
+    lib = L.lib()
+
+    def store():
+        s = L.AkvQ8StoreDesc()
+        s.cache, s.tokens, s.dtype = _cache(), 4, L.AKV_Q_F16
+        s.k_dev = s.v_dev = s.start_dev = s.counts_dev = 4096
+        return s
+
+    def restore():
+        r = L.AkvQ8RestoreDesc()
+        r.cache, r.tokens = _cache(), 4
+        r.k_dev = r.v_dev = r.start_dev = 4096
+        return r
+
+    def attention():
+        d = _attention()
+        d.workspace_dev, d.workspace_bytes = 4096, 1 << 30
+        d.weights_stride = 128
+        return d
+    for make, fn, fields in ((store, lib.akv_q8_store, ("start_dev", "counts_dev")), (restore, lib.akv_q8_restore, ("start_dev",)),
+                             (attention, lib.akv_q8_attention, ("seq_lens_dev", "q_lens_dev", "lse_dev", "weights_dev")),
+                             (_evict, lib.akv_q8_evict, ("weights_dev", "kept_dev", "out_lens_dev", "out_weights_dev", "seq_lens_dev"))):
+        for field in fields:
+            d = make()
+            setattr(d, field, 4098)
+            assert fn(ct.byref(d), None) == 1, field
+        for field in ("block_table_dev", "status_dev"):
+            d = make()
+            c = d.src if hasattr(d, "src") else d.cache
+            c.pages_per_seq, c.num_pages = 1, 2
+            setattr(c, field, 4098)
+            assert fn(ct.byref(d), None) == 1, field
