@@ -14,7 +14,10 @@ re-issued with `run()`, and a function for a single call.
 * `Q8Restore` returns tokens as values.
 
 Lengths, positions and block tables are int32 CUDA tensors that are read when
-a call runs, so a program updates them in place between steps. Everything
+a call runs, so a program updates them in place between steps. A call's
+outputs and workspace are its own and written anew by every run: runs of one
+call follow one another, on one stream or on streams that the program orders.
+Everything
 below runs in libakv_cuda.so (C ABI: include/akv_q8.h, which has the formulas
 and the rules for empty rows, ties and values that are not finite).
 """
@@ -295,6 +298,12 @@ class Q8Attention(_Call):
     `self.lse` [B, n, Hq]. `weights` fp32 [B, H, >= max_tokens]: the softmax
     weight each token received, over the queries and the kv head's query
     heads, is added to it (`accumulate=False`: replaces it).
+
+    Splits and workspace go by the cache's max_tokens, not by the lengths; with
+    `weights` and up to 16 rows (queries x heads of a kv head; 8 above head_dim
+    128) the workspace holds 4 bytes per row, kv head and token of it. Where a
+    cache has much more room than tokens, a second Q8Cache over the same tensors
+    with a smaller `max_tokens` serves it faster.
     """
 
     _fn = "attention"

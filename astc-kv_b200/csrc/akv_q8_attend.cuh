@@ -110,8 +110,10 @@ __device__ __forceinline__ void load_q16(const AttnParams& p, int64_t at, float 
 }
 
 // The power of two that brings a query row's largest |x| to [2^14, 2^15), so
-// that fp16 holds the row: bf16 and fp16 rows exactly, down to 2^-38 of the
-// largest; fp32 rows in two parts. Rows of zeros, infinities or NaN stay.
+// that fp16 holds the row: bf16 elements exactly down to 2^-31 of the largest,
+// below that off by 2^-39 of it at most; fp16 elements exactly, but for the
+// last bit of subnormal ones in rows that reach 2^15; fp32 rows in two parts
+// (22 bits). Rows of zeros, infinities or NaN stay.
 __device__ __forceinline__ int row_exponent(float top) {
     const int e = static_cast<int>(__float_as_uint(top) >> 23) - 127;
     if (top == 0.f || e == 128) return 0;

@@ -22,22 +22,30 @@
 // Shared memory operands are K-major with the 128-byte swizzle: Q and K
 // [row][d], V transposed to [d][token] (eight tokens of a d are paired by byte
 // permutes in registers and stored as 16 bytes). Codes are exact in fp16, and
-// 16-bit query rows after a power of two.
+// 16-bit query rows after a power of two, as row_exponent says.
 //
 // Softmax: t = s * factor + log2 v - base per token block, p = 2^t, and the
 // row sum adds p / v (see the step kernel for V's scale in the exponent).
 // `base` follows the row maximum loosely: the first tokens set it so that
 // their largest p is 2^6, and only a t above 15 (p would leave fp16) moves it
-// and scales O, which after the first tokens hardly ever happens.
+// and scales O, which after the first tokens hardly ever happens. Where a row
+// does not see all of 64 tokens, and where scores are so large that fp32 has no
+// bits for differences to the base, S is rewritten as t first, -inf for what is
+// not seen.
 //
-// With head_dim above 128 a CTA has one tile of rows and one stage of K and V.
+// P is rounded to fp16 (2^-11 of itself at most), and O is added up by the
+// tensor cores, which truncate: 6e-9 of it per token of the split.
+//
+// With head_dim above 128 a CTA has one tile of rows, one stage of K and V, and
+// four warpgroups: K is warps 4-7, V 8-11, the issuing warp 12.
 //
 // Per step and tile the tensor cores need 1024 cycles (D = 128) and the
 // special-function units as many for the 128 x 128 exp2. Measured, 2048 query
 // tokens at the end of 32768, 32/8 heads, D 128: int8 1.17 ms = 917 TFLOP/s,
-// 55 % of the 1657 that a large library product reaches (e4m3 1.13 ms; 1.26 ms
-// int8 under the power cap); the tensor pipe is active 32 % of the time. What
-// bounds it is the latency of a tile's round (scores, softmax, P, values: some
+// 55 % of the 1657 that a large library product reaches (e4m3 1.12 ms; 1.25 ms
+// int8 under the power cap). In a capture of 1024 query tokens at the end of
+// 16384 the tensor pipe is active 39 % of the time; at D 256, 512 at the end of
+// 8192 (223 us, 597 TFLOP/s), 26 %. What bounds it is the latency of a tile's round (scores, softmax, P, values: some
 // 4500 cycles, two tiles in turn), not a unit's throughput. On the way: stalls
 // on the converters' loads 2.2 to 1.43 ms, uniform issue of the products and
 // separate K and V groups 1.31, S in one piece 1.17; four 16-column loads of S
@@ -80,8 +88,9 @@ __device__ __forceinline__ void bar_init(uint64_t* bar, int count) {
 __device__ __forceinline__ void bar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
-// Waits for the phase of `parity` to end, a bounded number of times; false
-// (and the CTA's abort flag) when it does not, or when another warp gave up.
+// Waits for the phase of `parity` to end, a bounded number of times (a try takes
+// about 1.5 us, all some 6 s); false (and the CTA's abort flag) when it does
+// not, or when another warp gave up.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, int parity, volatile int* abort) {
     for (int i = 0; i < 1 << 22; ++i) {
         uint32_t ok;

@@ -17,8 +17,8 @@
 //   and the output's d follow: fragment row g of tile i is byte 2i of lane
 //   group g's bytes, row g + 8 is byte 2i + 1.
 //
-// Codes are exact in fp16; a query row is exact in fp16 after a power of two
-// (fp32 queries in two parts); the block scale of K and the power go to the
+// Codes are exact in fp16; a 16-bit query row is after a power of two, as
+// row_exponent says (fp32 queries go in two parts); the block scale of K and the power go to the
 // fp32 score. V's block scale v is folded into the exponent: P' = 2^(s +
 // log2 v - m) and the row sum adds P' / v, so V needs no product. P' is
 // scaled to between 2^8 and 2^15.5 to use fp16's range; fp32 outputs carry it
@@ -36,12 +36,14 @@
 // divided evenly over the CTAs of one wave, whatever the lengths: a CTA's
 // share may start and end inside a unit, whose pieces the combine kernel adds
 // up. (Splits of one length left CTAs idle behind the longest sequence: five
-// drafted tokens over eight sequences of 205 to 8192 tokens 84 us, now 51.)
+// drafted tokens over eight sequences of 205 to 8192 tokens 84 us, with even
+// shares 72; what came after made it 51.)
 //
 // Measured (fp32 out, head_dim 128, 32/8 heads, B32, 32768 tokens: 2.15 GB):
-// int8 346 us = 6.21 TB/s, 97 % of a copy's 6.42 TB/s; e4m3 330 us; under the
-// power cap int8 398 us at 1.6 GHz. 392 warp instructions per 16 tokens, of
-// them 176 to turn codes into fp16; issue slots 54 % used, tensor pipe 16 %.
+// int8 355 us = 6.05 TB/s, 94 % of a copy's 6.42 TB/s; e4m3 336 us; under the
+// power cap int8 401 us at 1.6 GHz. 402 warp instructions per 16 tokens, of
+// them 176 to turn codes into fp16; issue slots 54 % used, tensor pipe 16 % (B8).
+// (Without the sum in shared memory 348, 331 and 396 us.)
 // What carried it there from 587 us: pointers that advance instead of index
 // arithmetic (587 to 398), query fragments in shared memory rather than
 // registers (398 to 385), V loaded a tile ahead (385 to 365), even shares.

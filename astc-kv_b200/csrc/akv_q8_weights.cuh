@@ -10,6 +10,11 @@
 // asynchronous copies one stage ahead. A token's two sums are added in a fixed
 // order, so the result does not depend on timing.
 //
+// A score is one chain of products here and two in the step kernel, so it may
+// differ in its last bits from the one that went into the log-sum-exp; measured
+// against 64 bits, weights of 40 to 1200 rows are 1e-7 to 6e-7 off, those of
+// plain fp32 1e-7 to 9e-7.
+//
 // Half the products of the attention itself and one exp2 a score, of which an
 // SM does 16 a cycle: 90 us for 3 x 452 query tokens against 18578, 16/16
 // heads, D 64, where it takes 274 us.

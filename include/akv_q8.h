@@ -69,7 +69,8 @@ typedef struct AkvQ8Cache {
  * its rows are rounded again under that one. Tokens are stored in order: what
  * a block holds from start[b] on is not kept. A block that is given an
  * infinity or a NaN gets a NaN scale and codes of 0; one whose scale would be
- * subnormal is stored as zeros.
+ * subnormal is stored as zeros. Rows past max_tokens are dropped, with a start
+ * outside [0, max_tokens) all rows of the sequence (see status_dev).
  */
 typedef struct AkvQ8StoreDesc {
     AkvQ8Cache cache;
@@ -111,9 +112,21 @@ int akv_q8_restore(const AkvQ8RestoreDesc* desc, void* stream);
  *                           softmax weight of t   (accumulate 1: +=, 0: =)
  * A query that sees nothing, and one past q_lens[b], gives zeros and
  * lse = -inf. With accumulate 0 the weights of tokens past seq_lens[b] become
- * 0, with 1 they stay. Scores, softmax and sums are fp32; with a 16-bit
- * output the softmax weights are rounded to fp16 before they meet V, with an
- * fp32 output they are carried in two fp16 parts.
+ * 0, with 1 they stay.
+ *
+ * Scores, softmax and sums are fp32. A score is a sum in the tensor cores,
+ * which truncate, of exact products (of 22 bits with fp32 queries): off by at
+ * most 2^-20 of the sum of |scale q K|. With an fp32 output the softmax weights
+ * meet V in two fp16 parts (22 bits) and long sums are rounded to nearest
+ * every 32 products; with a 16-bit output the weights are rounded to fp16,
+ * and from 33 rows (queries x heads of a kv head; 17 above head_dim 128)
+ * the values' sum comes out 6e-9 of itself per token of a split too small.
+ *
+ * Lengths are read by the kernels, so what the host decides, the splits of many
+ * rows and the size of the workspace, goes by max_tokens: a cache with much
+ * more room than tokens is served best through one with a smaller max_tokens
+ * over the same memory. Workspace: partials, and with weights of up to 16 rows
+ * (8 above head_dim 128) 4 bytes per row, kv head and token of max_tokens.
  */
 typedef struct AkvQ8AttnDesc {
     AkvQ8Cache cache;
