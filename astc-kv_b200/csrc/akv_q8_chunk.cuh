@@ -254,7 +254,10 @@ __global__ void __launch_bounds__(kChunkThreads<DP>, 1) chunk_kernel(AttnParams 
     bool blind = true;
     if (warp < 4 * TILES) {
         const int tile = warp >> 2, r = threadIdx.x & 127, at_row = SHARED ? r : threadIdx.x, row = r0 + at_row;
-        const bool in = at_row < rows;
+        // A row without tokens goes along unmasked, as zeros, and is dropped at
+        // the end.
+        const int seen = at_row < rows ? seen_by(p, row / p.G, len, qlen) : 0;
+        const bool in = seen > 0;
         const int64_t at = in ? q_row(p, b, h, row) : 0;
         uint32_t top = 0;
         if (in) {
@@ -288,9 +291,7 @@ __global__ void __launch_bounds__(kChunkThreads<DP>, 1) chunk_kernel(AttnParams 
             }
         }
         factor = p.c2 * power_of_two(-e);
-        // A row without tokens goes along unmasked and is dropped at the end.
-        const int seen = in ? seen_by(p, row / p.G, len, qlen) : 0;
-        blind = seen == 0;
+        blind = !in;
         bound = blind ? INT_MAX : seen;
         fence_async();
     }

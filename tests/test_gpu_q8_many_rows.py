@@ -277,3 +277,25 @@ def test_wide_heads_of_few_rows(cuda, D, n, fmt):
     cache, k, v = make(2, 2, 500, D, fmt=fmt, block=32, seed=n)
     q = torch.randn(2, n, 2, D, device="cuda").half()
     check_attention(cache, k, v, q, [500, 130], [n, n // 2], out_dtype=torch.float16)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), 3e38])
+@pytest.mark.parametrize("D,G,n,od", [(D, G, n, torch.bfloat16) for D, G, n in SHAPES] + [
+    (64, 2, 4, torch.float32), (128, 4, 20, torch.float32), (128, 4, 4, torch.bfloat16)])
+def test_queries_past_their_count_are_not_looked_at(cuda, D, G, n, od, value):
+    """What lies past q_lens (and in sequences without queries) reaches no output and no weight."""
+    from astc_kv_cuda import Q8Attention
+    cache, _, _ = make(3, 2, 300, D, block=32, seed=n)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    lens, q_lens = torch.tensor([300, 200, 250], **i32), torch.tensor([n - 1, n // 2, 0], **i32)
+    q = torch.randn(3, n, 2 * G, D, device="cuda").bfloat16()
+    results = []
+    for fill in (0.0, value):
+        for b, m in enumerate(q_lens.tolist()):
+            q[b, m:] = fill
+        w = torch.ones(3, 2, cache.max_tokens, device="cuda")
+        call = Q8Attention(q, cache, lens, q_lens=q_lens, out_dtype=od, lse=True, weights=w)
+        results.append((call.run(), call.lse, w))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    for b, m in enumerate(q_lens.tolist()):
+        assert not results[1][0][b, m:].any() and (results[1][1][b, m:] == float("-inf")).all()
