@@ -115,7 +115,7 @@ struct AttnPlan {
 // price of one, is ahead of the step kernel, which does 16 at a time (8 above
 // head_dim 128). Measured, 8 kv heads, step kernel against tcgen05, B8 x 8192
 // tokens: D 128 int8 20 rows 78 us against 81, 32 rows 81 against 82, 36 rows
-// 153 against 83; D 64 32 rows 50 against 59; D 256 int8 16 rows 106 against
+// 109 against 82; D 64 32 rows 50 against 59, 36 rows 67 against 60; D 256 int8 16 rows 106 against
 // 119, 20 rows 143 against 120, e4m3 101 against 114 and 134 against 115.
 // (B1 x 32768, D 128, 32 rows 47 against 43; B8 x 700, D 64, 20 rows 20
 // against 17: short of 33 rows neither is far ahead up to D 128.)
