@@ -191,7 +191,7 @@ class _Call:
     Outputs and workspace are the object's own, so its runs follow one another
     on one stream, or on streams that the caller orders. The first run on
     another stream than the one the object was built on waits for what that
-    one had been given by then: earlier work on the memory that it took.
+    one has been given so far: earlier work on the memory that the object took.
     """
 
     _fn = ""
@@ -202,10 +202,7 @@ class _Call:
         self._index = device.index if device.index is not None else 0
         self._tensors = [t for t in tensors if t is not None]
         self._issue_c = getattr(L.lib(), "akv_q8_" + self._fn)
-        home = torch.cuda.current_stream(device)
-        self._home, self._met = home.cuda_stream, set()
-        # What a capture records cannot be waited for outside of it.
-        self._built = None if torch.cuda.is_current_stream_capturing() else home.record_event()
+        self._home, self._met = _current_stream(self._index), set()
 
     def _issue(self, stream: torch.cuda.Stream | None) -> None:
         if torch.cuda.current_device() != self._index:
@@ -219,11 +216,11 @@ class _Call:
 
     def _elsewhere(self, handle: int, stream: torch.cuda.Stream) -> None:
         """Before a run on another stream than the one the object was built on."""
-        if self._built is not None and handle not in self._met:
-            with torch.cuda.stream(stream):
-                capturing = torch.cuda.is_current_stream_capturing()
-            if not capturing:  # a capture waits for all streams before it begins
-                stream.wait_event(self._built)
+        # (A capture waits for all streams before it begins.)
+        if handle not in self._met:
+            home = torch.cuda.ExternalStream(self._home, self.device) if self._home else torch.cuda.default_stream(self.device)
+            if not _capturing(stream) and not _capturing(home):
+                stream.wait_stream(home)
                 self._met.add(handle)
         # The caller may drop this object while the stream still works on its memory.
         for t in self._tensors:
@@ -400,6 +397,11 @@ class Q8Evict(_Call):
     def run(self, stream: torch.cuda.Stream | None = None) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         self._issue(stream)
         return self.kept, self.lens, self.weights
+
+
+def _capturing(stream: torch.cuda.Stream) -> bool:
+    with torch.cuda.stream(stream):
+        return torch.cuda.is_current_stream_capturing()
 
 
 def _planes(c: Q8Cache) -> tuple:

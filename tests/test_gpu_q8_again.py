@@ -353,3 +353,21 @@ def own_pages(dst):
     table = torch.arange(at.numel(), dtype=torch.int32, device="cuda").view(dst.block_table.shape)
     pool = [t.view(torch.int8)[at].view(t.dtype) for t in (dst.k, dst.v)] + [t[at] for t in (dst.k_scales, dst.v_scales)]
     return Q8Cache(*pool, block_tokens=dst.block_tokens, block_table=table)
+
+
+@pytest.mark.parametrize("op", ["attention", "restore", "evict"])
+def test_built_on_a_stream_of_its_own(cuda, op):
+    """A call built on a side stream and run on the default one waits for the side stream's work on its memory."""
+    build = small_calls()[op]
+    want = [t.clone() for t in results(build().run())]
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(100_000_000)
+            junk = [torch.full_like(t, 77) for t in want for _ in range(3)]
+            del junk
+            call = build()
+        got = results(call.run())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
