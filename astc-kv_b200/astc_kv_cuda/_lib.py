@@ -1,4 +1,4 @@
-"""ctypes binding of libakv_cuda.so (the C ABI in include/akv_cuda.h and include/akv_q8.h).
+"""ctypes binding of libakv_cuda.so (the C ABI in include/akv_cuda.h, akv_q8.h, akv_rotary.h and akv_q4.h).
 
 The library is the product path: nothing here falls back to CPU code. If the
 shared object is missing or fails to load, `lib()` raises.
@@ -102,7 +102,67 @@ class AkvQ8EvictDesc(ct.Structure):
     ]
 
 
-# Every symbol include/akv_cuda.h, include/akv_host.h and include/akv_q8.h declare.
+AKV_ROTARY_MAX_AXES, AKV_Q4_GROUP, AKV_Q4_TOKENS = 8, 32, 16
+
+
+class AkvRotary(ct.Structure):
+    _fields_ = [
+        ("table_dev", ct.c_void_p), ("positions", ct.c_int32), ("rotary_dim", ct.c_int32), ("axes", ct.c_int32),
+        ("interleaved", ct.c_int32), ("axis", ct.c_uint8 * 128),
+    ]
+
+
+class AkvRotateDesc(ct.Structure):
+    _fields_ = [
+        ("rotary", AkvRotary), ("batch", ct.c_int32), ("tokens", ct.c_int32), ("heads", ct.c_int32), ("head_dim", ct.c_int32),
+        ("dtype", ct.c_int32), ("inverse", ct.c_int32), ("x_dev", ct.c_void_p), ("out_dev", ct.c_void_p), ("x_stride", ct.c_int64 * 3),
+        ("out_stride", ct.c_int64 * 3), ("positions_dev", ct.c_void_p), ("status_dev", ct.c_void_p),
+    ]
+
+
+class AkvQ4Side(ct.Structure):
+    _fields_ = [
+        ("codes", ct.c_void_p), ("scales", ct.c_void_p),
+        ("stride_batch", ct.c_int64), ("stride_head", ct.c_int64), ("stride_page", ct.c_int64), ("stride_token", ct.c_int64),
+        ("scale_stride_batch", ct.c_int64), ("scale_stride_head", ct.c_int64), ("scale_stride_page", ct.c_int64),
+        ("scale_stride_group", ct.c_int64),
+    ]
+
+
+class AkvQ4Cache(ct.Structure):
+    _fields_ = [
+        ("batch", ct.c_int32), ("kv_heads", ct.c_int32), ("head_dim", ct.c_int32), ("max_tokens", ct.c_int32), ("page_tokens", ct.c_int32),
+        ("pages_per_seq", ct.c_int32), ("num_pages", ct.c_int32), ("reserved0", ct.c_int32),
+        ("block_table_dev", ct.c_void_p), ("k", AkvQ4Side), ("v", AkvQ4Side), ("status_dev", ct.c_void_p),
+    ]
+
+
+class AkvQ4AppendDesc(ct.Structure):
+    _fields_ = [
+        ("cache", AkvQ4Cache), ("rotary", AkvRotary), ("tokens", ct.c_int32), ("dtype", ct.c_int32), ("q_heads", ct.c_int32),
+        ("reserved0", ct.c_int32), ("k_dev", ct.c_void_p), ("v_dev", ct.c_void_p), ("q_dev", ct.c_void_p), ("q_out_dev", ct.c_void_p),
+        ("k_stride", ct.c_int64 * 3), ("v_stride", ct.c_int64 * 3), ("q_stride", ct.c_int64 * 3), ("start_dev", ct.c_void_p),
+        ("counts_dev", ct.c_void_p), ("positions_dev", ct.c_void_p),
+    ]
+
+
+class AkvQ4RestoreDesc(ct.Structure):
+    _fields_ = [
+        ("cache", AkvQ4Cache), ("tokens", ct.c_int32), ("dtype", ct.c_int32), ("start_dev", ct.c_void_p),
+        ("k_dev", ct.c_void_p), ("v_dev", ct.c_void_p),
+    ]
+
+
+class AkvQ4AttnDesc(ct.Structure):
+    _fields_ = [
+        ("cache", AkvQ4Cache), ("q_heads", ct.c_int32), ("q_tokens", ct.c_int32), ("q_dtype", ct.c_int32), ("out_dtype", ct.c_int32),
+        ("causal", ct.c_int32), ("split_tokens", ct.c_int32), ("scale", ct.c_float), ("reserved0", ct.c_int32),
+        ("q_dev", ct.c_void_p), ("q_stride", ct.c_int64 * 3), ("seq_lens_dev", ct.c_void_p), ("q_lens_dev", ct.c_void_p),
+        ("out_dev", ct.c_void_p), ("lse_dev", ct.c_void_p), ("workspace_dev", ct.c_void_p), ("workspace_bytes", ct.c_size_t),
+    ]
+
+
+# Every symbol that include/akv_cuda.h, akv_host.h, akv_q8.h, akv_rotary.h and akv_q4.h declare.
 EXPORTS = (
     "akv_cuda_error", "akv_cuda_abi_version", "akv_cuda_init", "akv_cuda_decode_blocks", "akv_cuda_decode_image",
     "akv_cuda_attention_workspace", "akv_cuda_attention_plan", "akv_cuda_attention_tail_workspace",
@@ -111,6 +171,8 @@ EXPORTS = (
     "akv_cuda_decode_attention_noalloc", "akv_cuda_restore_plane", "akv_cuda_struct_size",
     "akv_cuda_host_tables", "akv_host_encode", "akv_host_random_blocks",
     "akv_q8_store", "akv_q8_restore", "akv_q8_attention_workspace", "akv_q8_attention", "akv_q8_evict", "akv_q8_struct_size",
+    "akv_rotate", "akv_rotary_struct_size",
+    "akv_q4_append", "akv_q4_restore", "akv_q4_attention_workspace", "akv_q4_attention", "akv_q4_struct_size",
 )
 
 _lib = None
@@ -161,14 +223,17 @@ def lib() -> ct.CDLL:
         l.akv_cuda_host_tables.restype = sz
         l.akv_host_encode.argtypes = [vp, ct.c_uint, ct.c_uint, ct.c_int, ct.c_int, ct.c_int, vp, sz, ct.c_int]
         l.akv_host_random_blocks.argtypes = [i64, ct.c_int, ct.c_uint64, vp, ct.c_int]
-        for name, desc in (("store", AkvQ8StoreDesc), ("restore", AkvQ8RestoreDesc), ("attention", AkvQ8AttnDesc),
-                           ("evict", AkvQ8EvictDesc)):
-            f = getattr(l, "akv_q8_" + name)
+        for name, desc in (("q8_store", AkvQ8StoreDesc), ("q8_restore", AkvQ8RestoreDesc), ("q8_attention", AkvQ8AttnDesc),
+                           ("q8_evict", AkvQ8EvictDesc), ("rotate", AkvRotateDesc), ("q4_append", AkvQ4AppendDesc),
+                           ("q4_restore", AkvQ4RestoreDesc), ("q4_attention", AkvQ4AttnDesc)):
+            f = getattr(l, "akv_" + name)
             f.argtypes, f.restype = [ct.POINTER(desc), vp], ct.c_int
         l.akv_q8_attention_workspace.argtypes = [ct.POINTER(AkvQ8AttnDesc)]
         l.akv_q8_attention_workspace.restype = sz
-        l.akv_q8_struct_size.argtypes = [ct.c_int]
-        l.akv_q8_struct_size.restype = sz
+        l.akv_q4_attention_workspace.argtypes = [ct.POINTER(AkvQ4AttnDesc)]
+        l.akv_q4_attention_workspace.restype = sz
+        for f in (l.akv_q8_struct_size, l.akv_rotary_struct_size, l.akv_q4_struct_size):
+            f.argtypes, f.restype = [ct.c_int], sz
         for name in EXPORTS:
             f = getattr(l, name)
             if f.restype is ct.c_int or name in ("akv_cuda_init", "akv_cuda_decode_blocks", "akv_cuda_decode_image",
@@ -177,8 +242,11 @@ def lib() -> ct.CDLL:
                                                   "akv_host_encode", "akv_host_random_blocks"):
                 f.restype = ct.c_int
         if l.akv_cuda_struct_size(0) != ct.sizeof(AkvPlane) or l.akv_cuda_struct_size(1) != ct.sizeof(AkvAttnDesc) or any(
-                l.akv_q8_struct_size(i) != ct.sizeof(s) for i, s in enumerate(
-                    (AkvQ8Cache, AkvQ8StoreDesc, AkvQ8RestoreDesc, AkvQ8AttnDesc, AkvQ8EvictDesc))):
+                size(i) != ct.sizeof(s) for size, structs in (
+                    (l.akv_q8_struct_size, (AkvQ8Cache, AkvQ8StoreDesc, AkvQ8RestoreDesc, AkvQ8AttnDesc, AkvQ8EvictDesc)),
+                    (l.akv_rotary_struct_size, (AkvRotary, AkvRotateDesc)),
+                    (l.akv_q4_struct_size, (AkvQ4Cache, AkvQ4AppendDesc, AkvQ4RestoreDesc, AkvQ4AttnDesc)))
+                for i, s in enumerate(structs)):
             raise RuntimeError("libakv_cuda.so struct layout does not match this binding")
         _lib = l
     return _lib

@@ -186,7 +186,7 @@ class Q8Cache:
 
 
 class _Call:
-    """A prepared call: a C descriptor, the tensors it points to, and `_issue`.
+    """A prepared call (of the 8-bit cache, the 4-bit cache or the rotation): a C descriptor, the tensors it points to, and `_issue`.
 
     Outputs and workspace are the object's own, so its runs follow one another
     on one stream, or on streams that the caller orders. The first run on
@@ -194,14 +194,14 @@ class _Call:
     one has been given so far: earlier work on the memory that the object took.
     """
 
-    _fn = ""
+    _family, _fn = "q8_", ""
 
     def _prepare(self, desc, device: torch.device, *tensors) -> None:
         self.desc, self.device = desc, device
         self._dref = ct.byref(desc)
         self._index = device.index if device.index is not None else 0
         self._tensors = [t for t in tensors if t is not None]
-        self._issue_c = getattr(L.lib(), "akv_q8_" + self._fn)
+        self._issue_c = getattr(L.lib(), "akv_" + self._family + self._fn)
         self._home, self._met = _current_stream(self._index), set()
 
     def _issue(self, stream: torch.cuda.Stream | None) -> None:
@@ -212,7 +212,7 @@ class _Call:
             self._elsewhere(handle, torch.cuda.current_stream(self._index) if stream is None else stream)
         code = self._issue_c(self._dref, handle or None)
         if code:
-            raise L.AkvError(code, "q8_" + self._fn)
+            raise L.AkvError(code, self._family + self._fn)
 
     def _elsewhere(self, handle: int, stream: torch.cuda.Stream) -> None:
         """Before a run on another stream than the one the object was built on."""

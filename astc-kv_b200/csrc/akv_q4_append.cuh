@@ -1,0 +1,276 @@
+// Append and restore of the 4-bit KV cache.
+//
+// A lane holds eight consecutive channels of a token's head: 16 bytes of 16-bit
+// rows in, one word of codes out, and four lanes share a scale. The other half of its
+// rotated pairs is loaded a second time by this lane, which finds it in L1
+// (rows meet no barrier and no shared memory). A lane keeps its token's cosines and
+// sines for all heads that it goes through.
+#pragma once
+#include "akv_q4_common.cuh"
+#include "akv_rotary.cuh"
+
+namespace akv {
+namespace q4 {
+
+struct AppendParams {
+    CacheDev c;
+    RotaryDev r;
+    const void* x[3];             // K, V, Q rows
+    int64_t xB[3], xT[3], xH[3];  // elements
+    void* q_out;
+    const int32_t* start;
+    const int32_t* counts;
+    const int32_t* places;
+    int n, Hq;
+    int kv_splits, q_splits;      // CTAs that share a token's kv heads, query heads
+};
+
+constexpr int kAppendThreads = 256;
+
+// How K and Q are rotated.
+enum { kStay, kHalves, kInterleaved };
+
+// A lane's eight channels of a row and, of halves, the other ones of their
+// pairs. VEC: rows start on 16-byte boundaries and no piece is rotated in part;
+// without it elements are loaded one by one.
+template <typename T, bool VEC, int TURN>
+struct Lane {
+    Chunk<T, 8> own, other;
+
+    __device__ __forceinline__ void load(const T* row, const RotaryDev& r, int d) {
+        if (VEC) own.load(row + d);
+        else own.load_each(row + d);
+        if (TURN != kHalves || d >= r.R) return;
+        const int half = r.R / 2;
+        if constexpr (VEC) {
+            other.load(row + (d < half ? d + half : d - half));
+        } else {
+            T e[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) e[k] = row[d + k < half ? d + k + half : d + k < r.R ? d + k - half : d + k];
+            other.pack(e);
+        }
+    }
+    // `c`, `s`: of this lane's channels (of halves), or pairs (interleaved); the first channel of a pair of
+    // halves has its sine negated already.
+    __device__ __forceinline__ void get(const RotaryDev& r, int d, const float (&c)[8], const float (&s)[8], float (&x)[8]) const {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = own.get(k);
+        if constexpr (TURN != kStay) {
+            if (d >= r.R) return;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if (!VEC && d + k >= r.R) break;
+                if (TURN == kHalves) {
+                    x[k] = turned(x[k], other.get(k), c[k], s[k]);
+                } else if (k % 2 == 0) {
+                    const float a = x[k], z = x[k + 1];
+                    x[k] = turned(a, z, c[k / 2], -s[k / 2]);
+                    x[k + 1] = turned(z, a, c[k / 2], s[k / 2]);
+                }
+            }
+        }
+    }
+};
+
+// Cosines and sines as Lane::get takes them.
+template <bool VEC, int TURN>
+__device__ __forceinline__ void lane_turns(const RotaryDev& r, const int32_t* places, int64_t stride, int place, int d, float (&c)[8], float (&s)[8]) {
+    if (TURN == kStay || d >= r.R) return;
+    const int half = r.R / 2;
+    if constexpr (TURN == kInterleaved) {
+        if constexpr (VEC) {
+            float cc[4], ss[4];
+            load_turns<4>(r, places, stride, place, d / 2, cc, ss);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { c[k] = cc[k]; s[k] = ss[k]; }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float cc[1] = {0.f}, ss[1] = {0.f};
+                if (d + 2 * k < r.R) load_turns<1>(r, places, stride, place, d / 2 + k, cc, ss);
+                c[k] = cc[0];
+                s[k] = ss[0];
+            }
+        }
+    } else if constexpr (VEC) {
+        load_turns<8>(r, places, stride, place, d < half ? d : d - half, c, s);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s[k] = d < half ? -s[k] : s[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            float cc[1] = {0.f}, ss[1] = {0.f};
+            if (d + k < r.R) load_turns<1>(r, places, stride, place, d + k < half ? d + k : d + k - half, cc, ss);
+            c[k] = cc[0];
+            s[k] = d + k < half ? -ss[0] : ss[0];
+        }
+    }
+}
+
+// Scale of a group with the largest |x| `top` (a number).
+__device__ __forceinline__ __half group_scale(float top) { return __float2half_rn(fminf(__fdiv_rn(top, 6.f), kMostScale)); }
+
+__device__ __forceinline__ uint32_t group_codes(const float (&x)[8], float scale) {
+    const float inverse = scale > 0.f ? __frcp_rn(scale) : 0.f;
+    float y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) y[k] = scale > 0.f ? quotient(x[k], scale, inverse) : 0.f;
+    return to_codes(y);
+}
+
+// grid.x: tokens of all sequences, so many rows of D / 8 lanes a CTA; grid.y:
+// parts of the kv heads, then parts of the query heads.
+template <typename T, bool VEC, int TURN>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendParams p) {
+    const CacheDev& c = p.c;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lanes = c.D / 8, rows = 32 / lanes;  // of a warp
+    const int row_of_warp = lane / lanes, l = lane - row_of_warp * lanes, d = 8 * l;
+    const int64_t token = (static_cast<int64_t>(blockIdx.x) * (kAppendThreads / 32) + warp) * rows + row_of_warp, tokens = static_cast<int64_t>(c.B) * p.n;
+    const bool there = row_of_warp < rows && token < tokens;
+    const int b = there ? static_cast<int>(token / p.n) : 0, i = there ? static_cast<int>(token - static_cast<int64_t>(b) * p.n) : 0;
+    const int start = p.start[b], count = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
+    const bool counted = there && i < count;
+    float cs[8], sn[8];
+    if (TURN != kStay && counted && d < p.r.R) {
+        // A start outside the cache may be none of the table either.
+        const int place = static_cast<int>(min(static_cast<int64_t>(start) + i, static_cast<int64_t>(INT_MAX)));
+        const int32_t* places = p.places ? p.places + token : nullptr;
+        if (places_in(p.r, places, tokens, place)) {
+            lane_turns<VEC, TURN>(p.r, places, tokens, place, d, cs, sn);
+        } else {
+            if (l == 0) q8::report(c.status, AKV_ERR_INVALID_ARGUMENT);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) cs[k] = sn[k] = CUDART_NAN_F;
+        }
+    }
+    if (static_cast<int>(blockIdx.y) >= p.kv_splits) {
+        // Queries. (No lane waits for another here.)
+        if (!there) return;
+        const T* x = static_cast<const T*>(p.x[2]) + b * p.xB[2] + i * p.xT[2];
+        T* out = static_cast<T*>(p.q_out) + token * p.Hq * c.D + d;
+        for (int h0 = blockIdx.y - p.kv_splits; h0 < p.Hq; h0 += 2 * p.q_splits) {
+            Lane<T, VEC, TURN> v[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                if (counted && h0 + j * p.q_splits < p.Hq) v[j].load(x + (h0 + j * p.q_splits) * p.xH[2], p.r, d);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int h = h0 + j * p.q_splits;
+                if (h >= p.Hq) break;
+                float y[8];
+                if (counted) {
+                    v[j].get(p.r, d, cs, sn, y);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) y[k] = 0.f;
+                }
+                Chunk<T, 8> o;
+                o.set(y);
+                o.store(out + static_cast<int64_t>(h) * c.D);
+            }
+        }
+        return;
+    }
+    if (there && i == 0 && l == 0 && blockIdx.y == 0 && count > 0 && (start < 0 || static_cast<int64_t>(start) + count > c.T))
+        q8::report(c.status, AKV_ERR_INVALID_ARGUMENT);
+    const bool kept = counted && start >= 0 && start < c.T && i < c.T - start;
+    int row = 0;
+    const int phys = kept ? page_of(c, b, start + i, row) : -1;
+    if (!__any_sync(0xFFFFFFFFu, phys >= 0)) return;
+    const bool store = phys >= 0;
+    const uint32_t row_mask = (lanes == 32 ? 0xFFFFFFFFu : (1u << lanes) - 1) << (row_of_warp * lanes & 31);
+    const T* xk = static_cast<const T*>(p.x[0]) + b * p.xB[0] + i * p.xT[0];
+    const T* xv = static_cast<const T*>(p.x[1]) + b * p.xB[1] + i * p.xT[1];
+    for (int h0 = blockIdx.y; h0 < c.H; h0 += 2 * p.kv_splits) {
+        Lane<T, VEC, TURN> k2[2];
+        Lane<T, VEC, kStay> v2[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int h = h0 + j * p.kv_splits;
+            if (!store || h >= c.H) continue;
+            k2[j].load(xk + h * p.xH[0], p.r, d);
+            v2[j].load(xv + h * p.xH[1], p.r, d);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int h = h0 + j * p.kv_splits;
+            if (h >= c.H) break;
+            float x[2][8];
+            uint32_t top[2] = {0, 0};
+            if (store) {
+                k2[j].get(p.r, d, cs, sn, x[0]);
+                v2[j].get(p.r, d, cs, sn, x[1]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    top[0] = max(top[0], q8::abs_bits(x[0][e]));
+                    top[1] = max(top[1], q8::abs_bits(x[1][e]));
+                }
+            }
+#pragma unroll
+            for (int o = 1; o <= 2; o <<= 1) {
+                top[0] = max(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], o));
+                top[1] = max(top[1], __shfl_xor_sync(0xFFFFFFFFu, top[1], o));
+            }
+            const uint32_t inf = 0x7F800000u;
+            const bool bad = __ballot_sync(0xFFFFFFFFu, top[0] >= inf || top[1] >= inf) & row_mask;
+            if (!store) continue;
+#pragma unroll
+            for (int side = 0; side < 2; ++side) {
+                const SideDev& s = side ? c.v : c.k;
+                const bool none = side ? top[1] >= inf : bad;
+                const __half scale = none ? __ushort_as_half(side ? 0 : 0x7FFF) : group_scale(__uint_as_float(top[side]));
+                const uint32_t w = none ? 0u : group_codes(x[side], __half2float(scale));
+                *reinterpret_cast<uint32_t*>(s.codes + code_offset(s, b, h, phys, row) + 4 * l) = w;
+                if ((l & 3) == 0) s.scales[scale_offset(s, b, h, phys, row) + (l >> 2) * s.cG] = scale;
+            }
+        }
+    }
+}
+
+struct RestoreParams {
+    CacheDev c;
+    void* out[2];
+    const int32_t* start;
+    int n;
+};
+
+// One thread per eight channels, in the order of the output; grid.y: sequence x side.
+template <typename T>
+__global__ void __launch_bounds__(256) restore_kernel(RestoreParams p) {
+    const CacheDev& c = p.c;
+    const int b = blockIdx.y >> 1, side = blockIdx.y & 1;
+    const SideDev& s = side ? c.v : c.k;
+    const unsigned per_row = c.D / 8, per_token = per_row * c.H;
+    const unsigned i = blockIdx.x * 256u + threadIdx.x;
+    if (i >= per_token * p.n) return;
+    const unsigned ti = i / per_token, rest = i - ti * per_token;
+    const int h = rest / per_row, l = rest - h * per_row;
+    q8::wait_for_previous_kernel();
+    const int64_t t = static_cast<int64_t>(ti) + (p.start ? p.start[b] : 0);
+    int row = 0;
+    const int phys = t >= 0 && t < c.T ? page_of(c, b, static_cast<int>(t), row) : -1;
+    uint32_t w = 0;
+    __half scale = __float2half_rn(0.f);
+    if (phys >= 0) {
+        w = *reinterpret_cast<const uint32_t*>(s.codes + code_offset(s, b, h, phys, row) + 4 * l);
+        scale = s.scales[scale_offset(s, b, h, phys, row) + (l >> 2) * s.cG];
+    }
+    uint32_t v[4];
+    codes_to_half(w, v);
+    const __half2 both = __half2half2(scale);
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        v[k] = mul2(v[k], *reinterpret_cast<const uint32_t*>(&both));
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
+        x[2 * k] = f.x;
+        x[2 * k + 1] = f.y;
+    }
+    Chunk<T, 8> o;
+    o.set(x);
+    o.store(static_cast<T*>(p.out[side]) + (static_cast<int64_t>(b) * p.n * per_token + i) * 8);
+}
+
+}  // namespace q4
+}  // namespace akv
