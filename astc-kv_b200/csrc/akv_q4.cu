@@ -8,6 +8,7 @@
 
 #include "akv_q4_append.cuh"
 #include "akv_q4_attend.cuh"
+#include "akv_q4_chunk.cuh"
 
 namespace akv {
 namespace q4 {
@@ -97,11 +98,22 @@ int sm_count() {
 
 struct AttnPlan {
     int rows;         // per kv head
+    bool chunk;       // the tcgen05 kernel, else the step kernel
     int cluster;      // CTAs of the step kernel's clusters, 0 without
     int nt;           // groups of eight rows per CTA
-    int share_ctas, share_min;
+    int split, nsplits;          // chunk kernel
+    int share_ctas, share_min;   // step kernel
     size_t part_ml, part_o, bytes;  // offsets into the workspace, and its size
 };
+
+// Rows from which the tcgen05 kernel is taken, whose CTA does 128 or 256 rows
+// for the price of one, rather than the step kernel, which does 16 at a time
+// (8 above head_dim 128).
+int chunk_min_rows(int head_dim) { return head_dim <= 128 ? 33 : 17; }
+
+// Tokens that a tile of the tcgen05 kernel adds up at most where outputs are
+// fp16: as in the 8-bit cache, the truncated sum would show in fp16's rounding.
+constexpr int64_t kChunkHalfTokens = 16384;
 
 // Tokens for each CTA of a cluster up to which a cluster for each kv head of
 // each sequence is taken, rather than even shares of all CTAs and a second launch.
@@ -113,24 +125,85 @@ AttnPlan plan_attention(const AkvQ4AttnDesc* d) {
     const int64_t bh = static_cast<int64_t>(c.batch) * c.kv_heads;
     a.rows = d->q_tokens * (d->q_heads / c.kv_heads);
     a.nt = c.head_dim <= 128 && a.rows > 8 ? 2 : 1;
-    const int group = 8 * a.nt;
-    // One wave of CTAs (see the step kernel), two pieces each; no more CTAs
-    // than there can be chunks.
-    const int64_t chunks = bh * ((a.rows + group - 1) / group) * ((c.max_tokens + q8::kShareTokens - 1) / q8::kShareTokens);
-    const int64_t slots = static_cast<int64_t>(sm_count()) * (c.head_dim > 128 || a.nt == 2 ? 2 : 4);
-    a.share_min = d->split_tokens > q8::kShareTokens ? d->split_tokens / q8::kShareTokens : 1;
-    const int64_t ctas = chunks / a.share_min < slots ? chunks / a.share_min : slots;
-    a.share_ctas = static_cast<int>(ctas > 0 ? ctas : 1);
-    const size_t parts = 2 * static_cast<size_t>(a.share_ctas) * group;
-    // The largest cluster with which all units fit the GPU at once.
-    int size = q8::kStepCluster;
-    while (size > 1 && bh * size > slots) size /= 2;
-    a.cluster = d->split_tokens == 0 && a.rows <= 8 && c.max_tokens <= kClusterTokens * size ? size : 0;
+    a.chunk = a.rows >= chunk_min_rows(c.head_dim) && d->q_dtype != AKV_Q_F32 && d->out_dtype != AKV_Q_F32;
+    a.split = d->split_tokens;
+    const bool shared = a.chunk && a.rows <= 128 && c.head_dim <= 128;  // its two tiles share the rows and take every other step
+    const int group = a.chunk ? (c.head_dim <= 128 ? 256 : 128) : 8 * a.nt;  // rows of a CTA
+    const int64_t units = bh * ((a.rows + group - 1) / group), sms = sm_count();
+    size_t parts;  // rows of partials
+    if (a.chunk) {
+        const int64_t steps = (static_cast<int64_t>(c.max_tokens) + kChunkTokens - 1) / kChunkTokens;
+        if (a.split == 0) {
+            // One CTA per SM; the number of splits, up to eight or one wave, is
+            // that of the least cost over the waves, as in the 8-bit cache.
+            const int64_t most = units > 0 && sms / units > 8 ? sms / units : 8;
+            const auto cost = [&](int64_t n) {
+                const double each = static_cast<double>((steps + n - 1) / n) + 3.0 + (n > 1 ? 2.5 * c.head_dim / 128 : 0.0);
+                return static_cast<double>((units * n + sms - 1) / sms) * each;
+            };
+            double least = cost(1);
+            for (int64_t n = 2; n <= most && n <= steps; ++n) least = cost(n) < least ? cost(n) : least;
+            int64_t best = 1;
+            const double limit = d->seq_lens_dev && c.batch > 1 && units < sms ? 1.15 * least : least;
+            for (int64_t n = 2; n <= most && n <= steps; ++n)
+                if (cost(n) <= limit) best = n;
+            if (cost(1) <= least) best = best > 1 && limit > least ? best : 1;
+            if (d->out_dtype == AKV_Q_F16) {
+                const int64_t longest = kChunkHalfTokens / kChunkTokens * (shared ? 2 : 1), n = (steps + longest - 1) / longest;
+                best = best > n ? best : n;
+            }
+            a.split = static_cast<int>((steps + best - 1) / best * kChunkTokens);
+        }
+        // Whole steps: a step's tokens past the split's end would count as seen.
+        a.split = static_cast<int>((static_cast<int64_t>(a.split < c.max_tokens ? a.split : c.max_tokens) + kChunkTokens - 1) / kChunkTokens * kChunkTokens);
+        a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);
+        const int64_t limit = 0x7FFFFFFF / ((a.rows + group - 1) / group + 1);
+        while (a.nsplits > limit) {  // the grid holds splits x row groups
+            a.split *= 2;
+            a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);
+        }
+        if (shared) a.nsplits *= 2;
+        parts = a.nsplits > 1 ? static_cast<size_t>(bh) * a.nsplits * a.rows : 0;
+    } else {
+        // One wave of CTAs (see the step kernel), two pieces each; no more
+        // CTAs than there can be chunks.
+        const int64_t chunks = units * ((c.max_tokens + q8::kShareTokens - 1) / q8::kShareTokens);
+        const int64_t slots = sms * (c.head_dim > 128 || a.nt == 2 ? 2 : 4);
+        a.share_min = a.split > q8::kShareTokens ? a.split / q8::kShareTokens : 1;
+        const int64_t ctas = chunks / a.share_min < slots ? chunks / a.share_min : slots;
+        a.share_ctas = static_cast<int>(ctas > 0 ? ctas : 1);
+        parts = 2 * static_cast<size_t>(a.share_ctas) * group;
+        // The largest cluster with which all units fit the GPU at once.
+        int size = q8::kStepCluster;
+        while (size > 1 && bh * size > slots) size /= 2;
+        a.cluster = a.split == 0 && a.rows <= 8 && c.max_tokens <= kClusterTokens * size ? size : 0;
+    }
     const auto up = [](size_t x) { return (x + 15) / 16 * 16; };
     a.part_ml = 0;
     a.part_o = up(parts * sizeof(float2));
     a.bytes = a.part_o + up(parts * c.head_dim * sizeof(float)) + 16;
     return a;
+}
+
+template <int DP, bool SHARED>
+int launch_chunk(const Q4Params& p, cudaStream_t s) {
+    const auto kern = chunk_kernel<DP, SHARED>;
+    constexpr int bytes = sizeof(ChunkSmem<DP>) + 1024;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+        cudaGetLastError();
+        return AKV_ERR_CUDA;
+    }
+    const int parts = SHARED ? p.a.nsplits / 2 : p.a.nsplits;
+    constexpr int rows = 128 * kChunkTiles<DP>;
+    const dim3 grid(parts * ((p.a.R + rows - 1) / rows), p.c.H, p.c.B);
+    kern<<<grid, kChunkThreads<DP>, bytes, s>>>(p);
+    return q8::launched();
+}
+
+int launch_chunk(const Q4Params& p, cudaStream_t s) {
+    if (p.c.D > 128) return launch_chunk<256, false>(p, s);
+    if (p.a.R <= 128) return p.c.D > 64 ? launch_chunk<128, true>(p, s) : launch_chunk<64, true>(p, s);
+    return p.c.D > 64 ? launch_chunk<128, false>(p, s) : launch_chunk<64, false>(p, s);
 }
 
 template <typename T, bool VEC>
@@ -254,16 +327,17 @@ int akv_q4_attention(const AkvQ4AttnDesc* d, void* stream) {
     p.c2 = (d->scale > 0.f ? d->scale : 1.0f / std::sqrt(static_cast<float>(p.c.D))) * 1.4426950408889634f;
     p.q = d->q_dev; p.qB = d->q_stride[0]; p.qT = d->q_stride[1]; p.qH = d->q_stride[2];
     p.lens = d->seq_lens_dev; p.q_lens = d->q_lens_dev;
-    p.share_ctas = plan.cluster ? -plan.cluster : plan.share_ctas; p.share_min = plan.share_min; p.row_group = 8 * plan.nt;
+    p.split = plan.split; p.nsplits = plan.nsplits;
+    p.share_ctas = plan.chunk ? 0 : plan.cluster ? -plan.cluster : plan.share_ctas; p.share_min = plan.share_min; p.row_group = 8 * plan.nt;
     p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
     p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     p.out = d->out_dev; p.lse_out = d->lse_dev;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (int st = launch_step(pp, plan.nt, s)) return st;
+    if (int st = plan.chunk ? launch_chunk(pp, s) : launch_step(pp, plan.nt, s)) return st;
     // A step kernel of one CTA leaves nothing to combine.
-    if (plan.cluster || plan.share_ctas <= 1) return AKV_OK;
+    if (plan.chunk ? plan.nsplits <= 1 : plan.cluster || plan.share_ctas <= 1) return AKV_OK;
     const int64_t rows = static_cast<int64_t>(p.c.B) * p.c.H * p.R;
-    const int64_t pieces = plan.share_ctas / (static_cast<int64_t>(p.c.B) * p.c.H) + 1;
+    const int64_t pieces = plan.chunk ? plan.nsplits : plan.share_ctas / (static_cast<int64_t>(p.c.B) * p.c.H) + 1;
     const bool by_warp = pieces <= 16 && rows >= 1024;  // partials of a row: few, a warp's work
     constexpr int per = q8::kCombineThreads / 32;
     const int64_t blocks = by_warp ? (rows + per - 1) / per : rows;

@@ -109,7 +109,7 @@ __device__ __forceinline__ void lane_turns(const RotaryDev& r, const int32_t* pl
 }
 
 // Scale of a group with the largest |x| `top` (a number).
-__device__ __forceinline__ __half group_scale(float top) { return __float2half_rn(fminf(__fdiv_rn(top, 6.f), kMostScale)); }
+__device__ __forceinline__ __half group_scale(float top) { return __float2half_rn(fminf(__fmul_rn(top, 1.f / 6.f), kMostScale)); }
 
 __device__ __forceinline__ uint32_t group_codes(const float (&x)[8], float scale) {
     const float inverse = scale > 0.f ? __frcp_rn(scale) : 0.f;

@@ -1,0 +1,600 @@
+// Attention of many rows (query tokens x heads of a kv head) over the 4-bit
+// cache with 16-bit outputs: prompt chunks, on the fifth-generation tensor
+// cores.
+//
+// A CTA takes 256 rows of one kv head as two tiles of 128 and goes through a
+// split of the tokens 128 at a time. Its warps have roles, as in the 8-bit
+// cache's chunk kernel:
+//
+//   warps 0-3, 4-7  softmax of tile 0 and 1, one thread per row
+//   warps 8-11      K, warps 12-15 V: codes from global memory to values in
+//                   shared memory (the conversion is shared by all 256 rows)
+//   warp 16         one thread issues tcgen05.mma
+//
+// S = Q K^T (M 128 rows, N 128 tokens) and O += P V (N head_dim) accumulate in
+// tensor memory: two S tiles and two O tiles fill its 512 columns. P is
+// written as fp16 over its own S, 64 tokens at a time, and is the A operand of
+// the second product. While one tile's softmax runs, the other tile's products
+// do. The order of the issues is the order of execution, so an S that is there
+// tells that the P V before it is done.
+//
+// Shared memory operands are K-major with the 128-byte swizzle: Q and K
+// [row][d], V transposed to [d][token]. K and V are code * scale, the fp16
+// numbers that the format defines: scores and the values' sum need no scale,
+// and the softmax no more than one multiplication and addition a score.
+//
+// Softmax: t = s * factor - base, p = 2^t. `base` follows the row maximum
+// loosely: the first tokens set it so that their largest p is 2^6, and only a
+// row whose p of 64 tokens add up to more than 2^15 (no p leaves fp16 before)
+// moves it and scales O, which after the first tokens hardly ever happens.
+// So no maximum is taken. Where a row does not see all of 64 tokens, and where scores
+// are so large that fp32 has no bits for differences to the base, S is
+// rewritten as t first, -inf for what is not seen.
+//
+// P is rounded to fp16 (2^-11 of itself at most), and O is added up by the
+// tensor cores, which truncate: 6e-9 of it per token of the split.
+//
+// With head_dim above 128 a CTA has one tile of rows, one stage of K and V, and
+// four warpgroups: K is warps 4-7, V 8-11, the issuing warp 12.
+#pragma once
+#include "akv_q4_attend.cuh"
+#include "akv_q8_chunk.cuh"
+
+namespace akv {
+namespace q4 {
+
+using q8::kChunkHalf;
+using q8::kChunkThreads;
+using q8::kChunkTiles;
+using q8::kChunkTokens;
+using q8::add2;
+using q8::bar_arrive;
+using q8::bar_init;
+using q8::bar_wait;
+using q8::elect_lane;
+using q8::exp2_fast;
+using q8::fence_after;
+using q8::fence_async;
+using q8::fence_before;
+using q8::fma2;
+using q8::halves;
+using q8::mma_commit;
+using q8::mma_desc;
+using q8::mma_ss;
+using q8::mma_ts;
+using q8::operand_desc;
+using q8::pack_half2;
+using q8::pair_of;
+using q8::smem_addr;
+using q8::swizzled;
+using q8::tmem_ld16;
+using q8::tmem_st16;
+using q8::tmem_wait_ld;
+using q8::tmem_wait_st;
+
+template <int DP>
+struct ChunkSmem {
+    // Operand tiles of 64 x 16-bit columns, 128 bytes a row, swizzled.
+    uint8_t q[kChunkTiles<DP>][DP / 64][128 * 128];
+    uint8_t k[kChunkTiles<DP>][DP / 64][128 * 128];
+    uint8_t v[kChunkTiles<DP>][2][DP * 128];
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], pv_done[2], done;
+    uint32_t tmem;
+    int abort;
+};
+
+// The same as the streaming loads, or zeros without a load; nothing waits for what is loaded.
+template <int NWORDS>
+__device__ __forceinline__ void load_words_if(uint32_t (&w)[NWORDS], const uint8_t* p, bool in) {
+    if constexpr (NWORDS == 4) {
+        const uint4 v = q8::load_stream_if(p, in);
+        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+    } else if constexpr (NWORDS == 2) {
+        const uint2 v = q8::load_stream8_if(p, in);
+        w[0] = v.x; w[1] = v.y;
+    } else {
+        asm volatile(
+            "{\n.reg .pred p;\nsetp.ne.u32 p, %2, 0;\nmov.b32 %0, 0;\n@p ld.global.nc.L1::no_allocate.u32 %0, [%1];\n}\n"
+            : "=&r"(w[0]) : "l"(p), "r"(static_cast<uint32_t>(in)));
+    }
+}
+__device__ __forceinline__ uint32_t load_scale_if(const __half* p, bool in) {
+    uint16_t v;
+    asm volatile("{\n.reg .pred p;\nsetp.ne.u32 p, %2, 0;\nmov.b16 %0, 0;\n@p ld.global.nc.L1::no_allocate.u16 %0, [%1];\n}\n"
+                 : "=&h"(v) : "l"(p), "r"(static_cast<uint32_t>(in)));
+    return v;
+}
+
+
+// SHARED: 128 rows or fewer a kv head; both tiles take the same rows and every
+// other step, as two splits.
+template <int DP, bool SHARED>
+__global__ void __launch_bounds__(kChunkThreads<DP>, 1) chunk_kernel(Q4Params pp) {
+    using Smem = ChunkSmem<DP>;
+    const q8::AttnParams& p = pp.a;
+    constexpr int TILES = kChunkTiles<DP>, STAGES = TILES, ROWS = 128 * TILES;
+    static_assert(!SHARED || TILES == 2, "two tiles to share rows");
+    extern __shared__ uint8_t smem_raw[];
+    // The swizzle counts from 1024-byte boundaries.
+    Smem& sm = *reinterpret_cast<Smem*>(smem_raw + (-smem_addr(smem_raw) & 1023));
+    const CacheDev& c = pp.c;
+    // With one tile there is no second group of softmax warps.
+    constexpr int THREADS = kChunkThreads<DP>, MISSING = TILES == 2 ? 0 : 4;
+    const int hw_warp = threadIdx.x >> 5, warp = hw_warp < 4 ? hw_warp : hw_warp + MISSING, lane = threadIdx.x & 31;
+    const int tiles = (p.R + ROWS - 1) / ROWS;
+    // Later rows see more tokens: they go first.
+    const int parts = SHARED ? p.nsplits / 2 : p.nsplits;  // CTAs along the tokens
+    const int split = blockIdx.x % parts, r0 = (tiles - 1 - blockIdx.x / parts) * ROWS, h = blockIdx.y, b = blockIdx.z;
+    const int len = q8::len_of(p, b), qlen = q8::q_len_of(p, b), rows = min(ROWS, p.R - r0);
+    const int bh = b * c.H + h;
+    const int64_t unit = (static_cast<int64_t>(bh) * p.nsplits + (SHARED ? 2 * split : split)) * p.R + r0;
+    const int end = r0 / p.G < qlen ? q8::seen_by(p, min((r0 + rows - 1) / p.G, qlen - 1), len, qlen) : 0;
+    const int t_begin = split * p.split, t_end = min(t_begin + p.split, end);
+    const int steps = t_end > t_begin ? (t_end - t_begin + kChunkTokens - 1) / kChunkTokens : 0;
+    if (steps == 0) {
+        // Nothing to see for any row.
+        for (int i = threadIdx.x; i < rows; i += THREADS) {
+            if (p.nsplits > 1) {
+                p.part_ml[unit + i] = make_float2(-CUDART_INF_F, 0.f);
+                if (SHARED) p.part_ml[unit + p.R + i] = make_float2(-CUDART_INF_F, 0.f);
+                continue;
+            }
+            const int64_t row = q8::out_row(p, b, h, r0 + i);
+            if (p.lse_out) p.lse_out[row] = -CUDART_INF_F;
+        }
+        if (p.nsplits == 1)
+            for (int i = threadIdx.x; i < rows * c.D; i += THREADS)
+                q8::store_elem(p.out, p.out_dtype, q8::out_row(p, b, h, r0 + i / c.D) * c.D + i % c.D, 0.f);
+        return;
+    }
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            bar_init(&sm.k_full[i], 128);
+            bar_init(&sm.v_full[i], 128);
+            bar_init(&sm.k_empty[i], 1);
+            bar_init(&sm.v_empty[i], 1);
+            bar_init(&sm.pv_done[i], 1);
+            bar_init(&sm.s_full[i], 1);
+            bar_init(&sm.p_full[i][0], 128);
+            bar_init(&sm.p_full[i][1], 128);
+        }
+        bar_init(&sm.done, 1);
+        sm.abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 16) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sm.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+
+    // Query rows: thread = row, to fp16 after a power of two.
+    float factor = 0.f;
+    int bound = 0;
+    bool blind = true;
+    if (warp < 4 * TILES) {
+        const int tile = warp >> 2, r = threadIdx.x & 127, at_row = SHARED ? r : threadIdx.x, row = r0 + at_row;
+        // A row without tokens goes along unmasked, as zeros, and is dropped at
+        // the end.
+        const int seen = at_row < rows ? q8::seen_by(p, row / p.G, len, qlen) : 0;
+        const bool in = seen > 0;
+        const int64_t at = in ? q8::q_row(p, b, h, row) : 0;
+        uint32_t top = 0;
+        if (in) {
+#pragma unroll 4
+            for (int d = 0; d < c.D; d += 16) {
+                float x[16];
+                q8::load_q16(p, at + d, x);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) top = max(top, q8::abs_bits(x[k]));
+            }
+        }
+        const int e = q8::row_exponent(__uint_as_float(top));
+        const float up = q8::power_of_two(e);
+#pragma unroll 4
+        for (int d = 0; d < DP; d += 16) {
+            float x[16];
+            if (in && d < c.D) {
+                q8::load_q16(p, at + d, x);  // from L1
+            } else {
+#pragma unroll
+                for (int k = 0; k < 16; ++k) x[k] = 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                uint4 w;
+                w.x = pack_half2(x[8 * k] * up, x[8 * k + 1] * up);
+                w.y = pack_half2(x[8 * k + 2] * up, x[8 * k + 3] * up);
+                w.z = pack_half2(x[8 * k + 4] * up, x[8 * k + 5] * up);
+                w.w = pack_half2(x[8 * k + 6] * up, x[8 * k + 7] * up);
+                *reinterpret_cast<uint4*>(sm.q[tile][d / 64] + swizzled(r, d / 8 % 8 + k)) = w;
+            }
+        }
+        factor = p.c2 * q8::power_of_two(-e);
+        blind = !in;
+        bound = blind ? INT_MAX : seen;
+        fence_async();
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sm.tmem;
+
+    // Steps of a tile: all, or every other one.
+    const bool two = TILES == 2 && (SHARED || rows > 128);  // else the second tile rests
+    // Registers go to where they are needed: 2 x 136 + 2 x 80 + 48 = 5 x 96
+    // (with one tile all have what they need).
+    if (warp < 8) {
+        // ------------------------------------------------------------ softmax
+        if (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+        const int tile = warp >> 2;
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // this warp's 32 lanes
+        const uint32_t s_tile = tmem + tile * 128 + lanes, o_at = tmem + 256 + tile * 128 + lanes;
+        float base = 0.f, l = 0.f;
+        bool started = false;
+        bool alive = true;
+        const int my_steps = SHARED ? (steps + 1 - tile) / 2 : tile == 0 || two ? steps : 0;
+        for (int i = 0; i < 2 * my_steps && alive; ++i) {
+            const int turn = i >> 1, half = i & 1, j = SHARED ? 2 * turn + tile : turn;
+            const int t0 = t_begin + j * kChunkTokens + half * kChunkHalf;
+            const uint32_t s_at = s_tile + kChunkHalf * half;
+            if (half == 0) {
+                alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.s_full[tile], turn & 1, &sm.abort));
+                if (!alive) break;
+                fence_after();
+            }
+            // The largest s * factor - sub of the row's tokens; by the whole warp.
+            auto largest = [&](float sub, float f) {
+                float m = -CUDART_INF_F;
+#pragma unroll 1
+                for (int g = 0; g < 4; ++g) {
+                    uint32_t s[16];
+                    tmem_ld16(s, s_at + 16 * g);
+                    tmem_wait_ld(s);
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (t0 + 16 * g + k < bound) m = fmaxf(m, fmaf(__uint_as_float(s[k]), f, -sub));
+                }
+                return m;
+            };
+            if (__any_sync(0xFFFFFFFFu, !started)) {
+                const float m = largest(0.f, factor);
+                if (!started && m != -CUDART_INF_F) {
+                    base = m - 6.f;
+                    started = true;
+                }
+                __syncwarp();
+            }
+            uint32_t pk[32];
+            float add, shift = 0.f;
+            bool placed = false;  // S holds t, less `shift`, of this half
+            for (int tries = 0;; ++tries) {
+                // Where a row does not see every token, or has a base without
+                // the bits to bring an exact score near it, S becomes t
+                // itself: -inf for what is not seen, and scores that are
+                // rounded first, to the base's own multiples, so that one raise
+                // is enough. (`tries` is a limit all the same.)
+                if (!placed && __any_sync(0xFFFFFFFFu, t0 + kChunkHalf > bound || fabsf(base) >= 1048576.f)) {
+#pragma unroll 1
+                    for (int g = 0; g < 4; ++g) {
+                        uint32_t s[16];
+                        tmem_ld16(s, s_at + 16 * g);
+                        tmem_wait_ld(s);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            s[k] = __float_as_uint(t0 + 16 * g + k < bound ? __fmul_rn(__uint_as_float(s[k]), factor) - base : -CUDART_INF_F);
+                        tmem_st16(s_at + 16 * g, s);
+                    }
+                    tmem_wait_st();
+                    placed = true;
+                }
+                const float f = placed ? 1.f : factor, off = placed ? -shift : -base;
+                const uint64_t f2 = pair_of(f, f), off2 = pair_of(off, off);
+                uint64_t sums[2] = {0, 0};
+                uint32_t s[2][16];
+                tmem_ld16(s[0], s_at);
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    uint32_t(&x)[16] = s[g & 1];
+                    tmem_wait_ld(x);
+                    if (g < 3) tmem_ld16(s[(g + 1) & 1], s_at + 16 * (g + 1));
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2) {
+                        float2 t = halves(fma2(pair_of(x[k], x[k + 1]), f2, off2));
+                        t.x = exp2_fast(t.x);
+                        t.y = exp2_fast(t.y);
+                        sums[k / 2 & 1] = add2(sums[k / 2 & 1], pair_of(t.x, t.y));
+                        pk[8 * g + k / 2] = pack_half2(t.x, t.y);
+                    }
+                }
+                const float2 both = halves(add2(sums[0], sums[1]));
+                add = both.x + both.y;
+                const bool over = add > 32768.f;
+                if (!__any_sync(0xFFFFFFFFu, over) || tries == 8) break;
+                // Some row's p may leave fp16: raise its base, scale its sums, again.
+                const float m = largest(placed ? shift : base, f);
+                const float up = over ? m - 6.f : 0.f;
+                const float to = base + up, alpha = exp2_fast(base - to);
+                shift += to - base;
+                base = to;
+                l *= alpha;
+                if (!placed) shift = 0.f;
+                if (i > 0) {
+                    // The last P V of the tile may still be running.
+                    alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.pv_done[tile], (i - 1) & 1, &sm.abort));
+                    if (!alive) break;
+                    fence_after();
+#pragma unroll 1
+                    for (int g = 0; g < DP / 16; ++g) {
+                        uint32_t o[16];
+                        tmem_ld16(o, o_at + 16 * g);
+                        tmem_wait_ld(o);
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+                        tmem_st16(o_at + 16 * g, o);
+                    }
+                }
+            }
+            l += add;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) tmem_st16(s_at + 16 * g, pk + 16 * g);
+            tmem_wait_st();
+            fence_before();
+            bar_arrive(&sm.p_full[tile][half]);
+        }
+        // ---------------------------------------------------------- write rows
+        alive = __all_sync(0xFFFFFFFFu, alive && bar_wait(&sm.done, 0, &sm.abort));
+        fence_after();
+        const int my_row = SHARED ? threadIdx.x & 127 : threadIdx.x;
+        const bool in = my_row < rows;
+        const int r = r0 + my_row;
+        const int64_t part = unit + my_row + (SHARED && tile ? p.R : 0);
+        if (!alive) l = CUDART_NAN_F;  // gave up: the rows become NaN
+        const bool none = alive && (blind || (!started && !isnan(l)));
+        const float inv = none ? 0.f : 1.f / l;
+        const int64_t row = in ? q8::out_row(p, b, h, r) : 0;
+#pragma unroll 1
+        for (int g = 0; g < DP / 16; ++g) {
+            uint32_t o[16];
+            tmem_ld16(o, o_at + 16 * g);
+            tmem_wait_ld(o);
+            if (!in || 16 * g >= c.D) {
+            } else if (p.nsplits > 1) {
+                uint4* to = reinterpret_cast<uint4*>(p.part_o + part * c.D + 16 * g);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) to[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+            } else {
+                uint32_t w[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    const float x = none ? 0.f : __uint_as_float(o[2 * k]) * inv, y = none ? 0.f : __uint_as_float(o[2 * k + 1]) * inv;
+                    if (p.out_dtype == AKV_Q_BF16) {
+                        const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+                        w[k] = *reinterpret_cast<const uint32_t*>(&v);
+                    } else {
+                        w[k] = pack_half2(x, y);
+                    }
+                }
+                uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.out) + row * c.D + 16 * g);
+                to[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                to[1] = make_uint4(w[4], w[5], w[6], w[7]);
+            }
+            __syncwarp();
+        }
+        if (in) {
+            if (p.nsplits > 1) {
+                p.part_ml[part] = make_float2(none ? -CUDART_INF_F : isnan(l) ? l : base, l);
+            } else {
+                const float lse = none ? -CUDART_INF_F : isnan(l) ? l : base + log2f(l);
+                if (p.lse_out) p.lse_out[row] = lse * 0.69314718055994531f;
+            }
+        }
+    } else if (warp < 12) {
+        // -------------------------------------------------------- K's values
+        if (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        // A lane takes pieces of 32 channels, a scale each; two or four lanes
+        // a row. Eight lanes store 16 bytes each into different banks: pieces
+        // of the second 64-column tile go in another order, two words ahead.
+        const int tid = threadIdx.x - 32 * (8 - MISSING);
+        constexpr int LANES = DP / 32 < 4 ? DP / 32 : 4, PIECES = DP / 32 / LANES, ROWS_K = 128 / LANES;  // rows at a time, LANES times
+        const int k_row = tid / LANES, k_piece = tid % LANES, turn_k = k_piece & 2;
+        int k_at[PIECES];  // bytes of the row
+        int64_t s_off[PIECES];
+#pragma unroll
+        for (int k = 0; k < PIECES; ++k) {
+            const int piece = k_piece + 4 * k < c.D / 32 ? k_piece + 4 * k : 0;
+            k_at[k] = 16 * piece;
+            s_off[k] = piece * c.k.cG;
+        }
+        const uint8_t* head = c.k.codes + b * c.k.sB + h * c.k.sH;
+        const __half* scales = c.k.scales + b * c.k.cB + h * c.k.cH;
+        // Every step within one page: one look at the table for all its rows.
+        const bool one_page = c.page_shift == 31 || (c.P % kChunkTokens == 0 && t_begin % kChunkTokens == 0);
+        uint32_t kr[LANES][PIECES][4], ks[LANES][PIECES];
+        auto load_k = [&](int t0) {
+            int row = 0, phys = -1;
+            if (one_page && t0 < t_end) phys = page_of(c, b, t0, row);
+#pragma unroll
+            for (int i = 0; i < LANES; ++i) {
+                const int t = t0 + ROWS_K * i + k_row;
+                if (!one_page) phys = t < t_end ? page_of(c, b, t, row) : -1;
+                const bool in = phys >= 0 && t < t_end;
+                const int at = one_page ? row + ROWS_K * i + k_row : row;
+#pragma unroll
+                for (int k = 0; k < PIECES; ++k) {
+                    load_words_if(kr[i][k], head + phys * c.k.sP + at * c.k.sT + k_at[k], in);
+                    ks[i][k] = load_scale_if(scales + phys * c.k.cP + at + s_off[k], in);
+                }
+            }
+        };
+        load_k(t_begin);
+        for (int j = 0; j < steps; ++j) {
+            const int st = j % STAGES;
+            // The phase before a stage's first use counts as over.
+            if (!bar_wait(&sm.k_empty[st], (j / STAGES & 1) ^ 1, &sm.abort)) break;
+#pragma unroll
+            for (int i = 0; i < LANES; ++i)
+#pragma unroll
+                for (int k = 0; k < PIECES; ++k) {
+                    uint8_t* tile = sm.k[st][(k_piece >> 1) + 2 * k];
+                    const int r = ROWS_K * i + k_row;
+                    const uint32_t sc = __byte_perm(ks[i][k], 0, 0x1010);
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        uint32_t x[4];
+                        codes_to_half(turn_k ? kr[i][k][w ^ 2] : kr[i][k][w], x);
+                        *reinterpret_cast<uint4*>(tile + swizzled(r, 4 * (k_piece & 1) + (w ^ turn_k))) =
+                            make_uint4(mul2(x[0], sc), mul2(x[1], sc), mul2(x[2], sc), mul2(x[3], sc));
+                    }
+                }
+            fence_async();
+            bar_arrive(&sm.k_full[st]);
+            load_k(t_begin + (j + 1) * kChunkTokens);
+        }
+    } else if (warp < 16) {
+        // -------------------------------------------------------- V's values
+        if (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+        // Eight lanes take the 64 tokens of a tile row, eight tokens each, of
+        // channels that share a scale.
+        const int w = warp & 3;
+        constexpr int VW = DP / 64;  // words of a token per lane
+        const int v_tok = 64 * (w & 1) + 8 * (lane & 7), v_d = (w >> 1) * (DP / 2) + (lane >> 3) * (DP / 8);
+        const int v_from = v_d < c.D ? v_d : 0;
+        const uint8_t* head = c.v.codes + b * c.v.sB + h * c.v.sH + v_from / 2;
+        const __half* scales = c.v.scales + b * c.v.cB + h * c.v.cH + v_from / AKV_Q4_GROUP * c.v.cG;
+        uint32_t vr[8][VW];
+        uint32_t vs[4];  // scales of pairs of tokens
+        auto load_v = [&](int t0) {
+            const int t = t0 + v_tok;
+            int row = 0;
+            const int phys = t < t_end ? page_of(c, b, t, row) : -1;
+            const uint8_t* at = head + phys * c.v.sP + row * c.v.sT;
+            const int left = phys >= 0 ? t_end - t : 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                load_words_if(vr[i], at, i < left);
+                at += c.v.sT;
+            }
+            // (A page holds all of the eight tokens' scales.)
+            const __half* s_at = scales + phys * c.v.cP + row;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint2 s = q8::load_stream8_if(s_at + 4 * i, 4 * i < left);
+                vs[2 * i] = s.x;
+                vs[2 * i + 1] = s.y;
+            }
+            if (left < 8) {  // what lies past the end may hold anything
+#pragma unroll
+                for (int i = 0; i < 4; ++i) vs[i] = 2 * i + 1 < left ? vs[i] : 2 * i < left ? vs[i] & 0xFFFFu : 0u;
+            }
+        };
+        load_v(t_begin);
+        for (int j = 0; j < steps; ++j) {
+            const int st = j % STAGES;
+            if (!bar_wait(&sm.v_empty[st], (j / STAGES & 1) ^ 1, &sm.abort)) break;
+            uint8_t* tile = sm.v[st][w & 1];
+#pragma unroll
+            for (int x = 0; x < VW; ++x)
+#pragma unroll
+                for (int o = 0; o < 2; ++o) {  // even channels of the word, then odd ones
+                    uint32_t y[4][4];  // [pair of tokens][channel]
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const uint32_t u = vr[2 * q][x], z = vr[2 * q + 1][x];
+                        codes_to_half(o ? ((u >> 4) & 0x0F0F0F0Fu) | (z & 0xF0F0F0F0u) : (u & 0x0F0F0F0Fu) | ((z << 4) & 0xF0F0F0F0u), y[q]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        *reinterpret_cast<uint4*>(tile + swizzled(v_d + 8 * x + 2 * k + o, lane & 7)) =
+                            make_uint4(mul2(y[0][k], vs[0]), mul2(y[1][k], vs[1]), mul2(y[2][k], vs[2]), mul2(y[3][k], vs[3]));
+                }
+            fence_async();
+            bar_arrive(&sm.v_full[st]);
+            load_v(t_begin + (j + 1) * kChunkTokens);
+        }
+    } else {
+        // --------------------------------------------------------- the products
+        if (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+        if (warp == 16) {
+            // The whole warp goes through the loop, so that addresses stay in
+            // uniform registers; one lane issues.
+            constexpr uint32_t qk = mma_desc(128, kChunkTokens), pv = mma_desc(128, DP);
+            constexpr uint32_t kTile = 128 * 128 / 16, kStage = DP / 64 * kTile;
+            constexpr uint32_t vHalf = DP * 128 / 16, vStage = 2 * vHalf;
+            const uint32_t q0 = operand_desc(sm.q), k0 = operand_desc(sm.k), v0 = operand_desc(sm.v);
+            const bool lead = elect_lane();
+            auto scores = [&](int tile, int st) {
+                const uint32_t d = tmem + tile * 128, a = q0 + tile * kStage, x = k0 + st * kStage;
+                if (lead) {
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        const uint32_t off = k / 4 * kTile + k % 4 * 2;
+                        mma_ss(d, a + off, x + off, qk, k > 0);
+                    }
+                    mma_commit(&sm.s_full[tile]);
+                }
+            };
+            auto values = [&](int tile, int half, int st, bool add) {
+                const uint32_t d = tmem + 256 + tile * 128, a = tmem + tile * 128 + half * kChunkHalf, x = v0 + st * vStage + half * vHalf;
+                if (lead) {
+#pragma unroll
+                    for (int k = 0; k < kChunkHalf / 16; ++k) mma_ts(d, a + 8 * k, x + 2 * k, pv, add || k > 0);
+                    mma_commit(&sm.pv_done[tile]);
+                }
+            };
+            const int tiles_here = two ? 2 : 1;
+            bool alive = true;
+            // A tile's first scores; with both tiles on the same rows, the
+            // second tile's are those of step 1.
+            for (int tile = 0; tile < tiles_here && alive; ++tile) {
+                const int st = SHARED ? tile : 0;
+                if (SHARED && tile >= steps) break;
+                alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.k_full[st], 0, &sm.abort));
+                if (!alive) break;
+                fence_after();
+                scores(tile, st);
+                if (lead && (SHARED || tile == tiles_here - 1)) mma_commit(&sm.k_empty[st]);
+            }
+            for (int j = 0; j < steps && alive; ++j) {
+                // The step after this one of the same tiles.
+                const int st = j % STAGES, next = SHARED ? j + 2 : j + 1, nx = next % STAGES, turn = SHARED ? j >> 1 : j;
+                const bool more = next < steps;
+                alive = bar_wait(&sm.v_full[st], j / STAGES & 1, &sm.abort);
+                if (more && !SHARED) alive = bar_wait(&sm.k_full[nx], next / STAGES & 1, &sm.abort) && alive;
+                const int i_end = SHARED ? 2 * st + 2 : 2 * tiles_here;
+                for (int i = SHARED ? 2 * st : 0; i < i_end; ++i) {
+                    const int tile = i >> 1, half = i & 1;
+                    alive = __all_sync(0xFFFFFFFFu, alive && bar_wait(&sm.p_full[tile][half], turn & 1, &sm.abort));
+                    if (!alive) break;
+                    fence_after();
+                    values(tile, half, st, turn > 0 || half > 0);
+                    if (lead && i == i_end - 1) mma_commit(&sm.v_empty[st]);
+                    if (!more || half == 0) continue;
+                    if (SHARED) {
+                        alive = __all_sync(0xFFFFFFFFu, bar_wait(&sm.k_full[nx], next / STAGES & 1, &sm.abort));
+                        if (!alive) break;
+                        fence_after();
+                    }
+                    scores(tile, nx);
+                    if (lead && i == i_end - 1) mma_commit(&sm.k_empty[nx]);
+                }
+            }
+            // Also after giving up: nothing may be in flight when the tensor
+            // memory is given back.
+            if (lead) mma_commit(&sm.done);
+            int none = 0;
+            bar_wait(&sm.done, 0, &none);
+        }
+        __syncwarp();
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 16) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        if (lane == 0 && sm.abort) q8::report(c.status, AKV_ERR_TIMEOUT);
+    }
+}
+
+}  // namespace q4
+}  // namespace akv

@@ -68,9 +68,9 @@ typedef struct AkvQ4Cache {
  * first, as akv_rotate does but without rounding to `dtype`, at
  * positions[axis][b][i], or start[b] + i on every axis without positions.
  * Then, for each 32 channels of a token,
- *     scale = min(fp16(amax / 6), 10912), code = e2m1(x / scale),
- * the quotients rounded to fp32, fp16 and e2m1 to the nearest (ties to even),
- * codes beyond 6 to 6; with a scale of 0 the codes are 0. (Values beyond 65472
+ *     scale = min(fp16(amax * (1/6)), 10912), code = e2m1(x / scale),
+ * product and quotient (and 1/6) rounded to fp32, then to fp16 and e2m1, to the
+ * nearest (ties to even), codes beyond 6 to 6; with a scale of 0 the codes are 0. (Values beyond 65472
  * become 65472.) A token whose K or V row holds an infinity or a NaN gets NaN
  * as K's scales and 0 as K's codes; V's groups that hold one become 0. The
  * same where a position is outside the table. Rows past max_tokens are

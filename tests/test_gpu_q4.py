@@ -1,6 +1,6 @@
 """The 4-bit KV cache on the GPU against plain implementations in 64 bits.
 
-What is stored. The definition rounds amax / 6 to fp32 and fp16, x / scale to
+What is stored. The definition rounds amax * (1/6) to fp32 and fp16, x / scale to
 fp32 and e2m1, a rotated key's products and sums to fp32: the plain
 implementation does each of these operations in 64 bits and rounds it, and codes
 and scales have to be the same bits. A value is code * scale rounded to fp16,
@@ -404,7 +404,7 @@ def test_scores_of_any_magnitude(cuda, D, G, n, T, od, sign, size):
 def quantised(x):
     """x [..., D], fp32 numbers in 64 bits -> codes [..., D / 2], scales [..., D / 32]; not for infinities and NaN."""
     x = x.unflatten(-1, (-1, GROUP))
-    s = (x.abs().amax(-1) / 6).float().half().double().clamp(max=10912)
+    s = (x.abs().amax(-1) * float(np.float32(1) / np.float32(6))).float().half().double().clamp(max=10912)
     y = torch.where(s[..., None] > 0, x / s.clamp(min=2.0 ** -24)[..., None], 0).float().double()
     levels = torch.tensor(LEVELS, dtype=torch.float64, device=x.device)
     middles = (levels[1:] + levels[:-1]) / 2
