@@ -206,6 +206,9 @@ int launch_chunk(const Q4Params& p, cudaStream_t s) {
     return p.c.D > 64 ? launch_chunk<128, false>(p, s) : launch_chunk<64, false>(p, s);
 }
 
+// Tokens from which an append's queries get a launch of their own.
+constexpr int64_t kQueriesApart = 512;
+
 template <typename T, bool VEC>
 void launch_append(const AppendParams& p, int turn, dim3 grid, cudaStream_t s) {
     if (turn == kHalves) append_kernel<T, VEC, kHalves><<<grid, kAppendThreads, 0, s>>>(p);
@@ -264,27 +267,46 @@ int akv_q4_append(const AkvQ4AppendDesc* d, void* stream) {
     p.q_out = d->q_out_dev;
     p.start = d->start_dev; p.counts = d->counts_dev; p.places = d->positions_dev;
     p.n = d->tokens; p.Hq = queries ? d->q_heads : 0;
-    const int rows = 32 / (p.c.D / 8) * (kAppendThreads / 32);  // tokens of a CTA
+    // Two chunks of eight channels a lane, where both halves of the rotated and of the other channels hold whole groups.
+    const bool pairs = vec && (!turn || !d->rotary.interleaved) && p.r.R % 64 == 0 && (p.c.D - p.r.R) % 64 == 0;
+    const int rows = 32 / (p.c.D / (pairs ? 16 : 8)) * (kAppendThreads / 32);  // tokens of a CTA
     const int64_t blocks = (static_cast<int64_t>(p.c.B) * p.n + rows - 1) / rows;
     if (blocks > 0x7FFFFFFF) return AKV_ERR_UNSUPPORTED;
-    // As many heads a CTA as leave some waves of CTAs.
-    const int64_t want = (8 * static_cast<int64_t>(sm_count()) + blocks - 1) / blocks;
-    const auto split = [&](int heads) {
-        const int64_t least = (heads + 7) / 8, n = want > least ? want : least;
-        return static_cast<int>(n < heads ? n : heads);
+    // As many heads a CTA as leave a wave of CTAs, in whole rounds of a lane's loads.
+    const int64_t wave = 2 * static_cast<int64_t>(sm_count()), want = wave > blocks ? wave / blocks : 1;
+    const auto split = [&](int heads, int round) {
+        int rounds = 8 / round;
+        while (rounds > 1 && (heads + rounds * round - 1) / (rounds * round) < want) --rounds;
+        const int n = (heads + rounds * round - 1) / (rounds * round);
+        return n < want ? static_cast<int>(want < heads ? want : heads) : n;
     };
-    p.kv_splits = split(p.c.H);
-    p.q_splits = queries ? split(p.Hq) : 0;
+    p.kv_splits = split(p.c.H, kAppendHeads);
+    // Queries go along in this launch where they are few, or else in a launch of their own, whose kernel needs fewer registers.
+    const bool apart = queries && static_cast<int64_t>(p.c.B) * p.n >= kQueriesApart;
+    p.q_splits = queries && !apart ? split(p.Hq, pairs ? kRotateHeads : 2) : 0;
     if (p.kv_splits + p.q_splits > kMaxGridYZ) return AKV_ERR_UNSUPPORTED;
     const dim3 grid(static_cast<unsigned>(blocks), p.kv_splits + p.q_splits);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int how = !turn ? kStay : d->rotary.interleaved ? kInterleaved : kHalves;
     with_type(d->dtype, [&](auto t) {
         using T = decltype(t);
-        if (vec) launch_append<T, true>(p, how, grid, s);
+        if (pairs) {
+            if (p.q_splits) append_pairs_kernel<T, true, true><<<grid, kAppendThreads, 0, s>>>(p);
+            else if (turn) append_pairs_kernel<T, true, false><<<grid, kAppendThreads, 0, s>>>(p);
+            else append_pairs_kernel<T, false, false><<<grid, kAppendThreads, 0, s>>>(p);
+        } else if (vec) launch_append<T, true>(p, how, grid, s);
         else launch_append<T, false>(p, how, grid, s);
     });
-    return q8::launched();
+    if (const int st = q8::launched()) return st;
+    if (!apart) return AKV_OK;
+    RotateParams r = {};
+    r.r = p.r;
+    r.B = p.c.B; r.n = p.n; r.H = p.Hq; r.D = p.c.D;
+    r.x = d->q_dev; r.out = d->q_out_dev;
+    r.xB = p.xB[2]; r.xT = p.xT[2]; r.xH = p.xH[2];
+    r.oH = p.c.D; r.oT = r.oH * r.H; r.oB = r.oT * r.n;
+    r.places = p.places; r.start = p.start; r.counts = p.counts; r.status = p.c.status;
+    return launch_rotate(r, d->dtype, d->rotary.interleaved != 0, s);
 }
 
 int akv_q4_restore(const AkvQ4RestoreDesc* d, void* stream) {
@@ -297,7 +319,7 @@ int akv_q4_restore(const AkvQ4RestoreDesc* d, void* stream) {
     p.c = to_dev(d->cache);
     p.out[0] = d->k_dev; p.out[1] = d->v_dev;
     p.start = d->start_dev; p.n = d->tokens;
-    const int64_t pieces = static_cast<int64_t>(p.n) * p.c.H * (p.c.D / 8);  // of a sequence's side
+    const int64_t pieces = static_cast<int64_t>(p.n) * p.c.H * (p.c.D / 16);  // of a sequence's side
     if (pieces > 0x7FFFFF00) return AKV_ERR_UNSUPPORTED;
     const dim3 grid(static_cast<unsigned>((pieces + 255) / 256), 2 * p.c.B);
     int st = AKV_OK;

@@ -26,6 +26,7 @@ struct AppendParams {
 };
 
 constexpr int kAppendThreads = 256;
+constexpr int kAppendHeads = 2;  // of K and V, loads of so many in flight
 
 // How K and Q are rotated.
 enum { kStay, kHalves, kInterleaved };
@@ -112,10 +113,10 @@ __device__ __forceinline__ void lane_turns(const RotaryDev& r, const int32_t* pl
 __device__ __forceinline__ __half group_scale(float top) { return __float2half_rn(fminf(__fmul_rn(top, 1.f / 6.f), kMostScale)); }
 
 __device__ __forceinline__ uint32_t group_codes(const float (&x)[8], float scale) {
-    const float inverse = scale > 0.f ? __frcp_rn(scale) : 0.f;
+    const float inverse = inverse_of(scale);
     float y[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] = scale > 0.f ? quotient(x[k], scale, inverse) : 0.f;
+    for (int k = 0; k < 8; ++k) y[k] = quotient(x[k], scale, inverse);
     return to_codes(y);
 }
 
@@ -133,8 +134,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendParams p) 
     const bool counted = there && i < count;
     float cs[8], sn[8];
     if (TURN != kStay && counted && d < p.r.R) {
-        // A start outside the cache may be none of the table either.
-        const int place = static_cast<int>(min(static_cast<int64_t>(start) + i, static_cast<int64_t>(INT_MAX)));
+        const int place = place_of(start, i);
         const int32_t* places = p.places ? p.places + token : nullptr;
         if (places_in(p.r, places, tokens, place)) {
             lane_turns<VEC, TURN>(p.r, places, tokens, place, d, cs, sn);
@@ -228,6 +228,234 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(AppendParams p) 
     }
 }
 
+// ------------------------------------------------- pairs of chunks a lane
+//
+// The form that a model's prompts and steps take: 16-byte rows, pairs of
+// halves (or none), and halves that hold whole groups. A lane has two chunks of eight
+// channels, of rotated ones the two halves of eight pairs, so that nothing is
+// loaded twice, and two fp32 operations go in one instruction.
+
+__device__ __forceinline__ uint64_t pack2f(float a, float b) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ float2 unpack2f(uint64_t v) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+}
+__device__ __forceinline__ uint64_t fma2f(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2f(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// The sums of products have to be rounded by themselves. As pairs the compiler
+// makes a multiplication and an addition one operation (also where they are
+// written as two), so additions are done one by one.
+__device__ __forceinline__ uint64_t sum2f(uint64_t a, uint64_t b, float sign) {
+    const float2 x = unpack2f(a), y = unpack2f(b);
+    return sign < 0.f ? pack2f(__fsub_rn(x.x, y.x), __fsub_rn(x.y, y.y)) : pack2f(__fadd_rn(x.x, y.x), __fadd_rn(x.y, y.y));
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+}
+// The largest |x|, a NaN if one is.
+__device__ __forceinline__ float largest_of(const uint64_t (&x)[4]) {
+    float top[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 f = unpack2f(x[k]);
+        top[0] = max_nan(top[0], fabsf(f.x));
+        top[1] = max_nan(top[1], fabsf(f.y));
+    }
+    return max_nan(top[0], top[1]);
+}
+
+// Eight channels as four pairs of neighbours.
+template <typename T>
+__device__ __forceinline__ void chunk_values(const Chunk<T, 8>& v, uint64_t (&x)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = pack2f(v.get(2 * k), v.get(2 * k + 1));
+}
+
+// Codes of a chunk, given its group's scale.
+__device__ __forceinline__ uint32_t chunk_codes(const uint64_t (&x)[4], float scale) {
+    const float inverse = inverse_of(scale);
+    const uint64_t inv = pack2f(inverse, inverse), neg = pack2f(-scale, -scale);
+    float y[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint64_t q = mul2f(x[k], inv);  // see quotient()
+        const float2 f = unpack2f(fma2f(fma2f(q, neg, x[k]), inv, q));
+        y[2 * k] = f.x;
+        y[2 * k + 1] = f.y;
+    }
+    return to_codes(y);
+}
+
+// Grid as of append_kernel, with rows of D / 16 lanes. QUERIES: with parts for
+// the query heads.
+template <typename T, bool TURN, bool QUERIES>
+__global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 4 ? 1 : QUERIES ? 2 : 3) append_pairs_kernel(AppendParams p) {
+    const CacheDev& c = p.c;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lanes = c.D / 16, rows = 32 / lanes;  // of a warp
+    const int row_of_warp = lane / lanes, u = lane - row_of_warp * lanes;
+    const int64_t token = (static_cast<int64_t>(blockIdx.x) * (kAppendThreads / 32) + warp) * rows + row_of_warp, tokens = static_cast<int64_t>(c.B) * p.n;
+    const bool there = row_of_warp < rows && token < tokens;
+    const int b = there ? static_cast<int>(token / p.n) : 0, i = there ? static_cast<int>(token - static_cast<int64_t>(b) * p.n) : 0;
+    const int start = p.start[b], count = p.counts ? min(max(p.counts[b], 0), p.n) : p.n;
+    const bool counted = there && i < count;
+    // The lane's chunks: of the rotated channels, then of the others, half of them apart.
+    const int R = TURN ? p.r.R : 0;
+    const bool turn = TURN && 16 * u < R;
+    const int d0 = turn ? 8 * u : R + 8 * (u - R / 16), d1 = d0 + (turn ? R / 2 : (c.D - R) / 2);
+    uint64_t cs[4], sn[4];
+    if (turn && counted) {
+        const int place = place_of(start, i);
+        const int32_t* places = p.places ? p.places + token : nullptr;
+        float cc[8], ss[8];
+        if (places_in(p.r, places, tokens, place)) {
+            load_turns<8>(p.r, places, tokens, place, d0, cc, ss);
+        } else {
+            if (u == 0) q8::report(c.status, AKV_ERR_INVALID_ARGUMENT);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) cc[k] = ss[k] = CUDART_NAN_F;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            cs[k] = pack2f(cc[2 * k], cc[2 * k + 1]);
+            sn[k] = pack2f(ss[2 * k], ss[2 * k + 1]);
+        }
+    }
+    auto rotate = [&](uint64_t (&x)[4], uint64_t (&z)[4]) {
+        if constexpr (TURN) {
+            if (!turn) return;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint64_t e = sum2f(mul2f(x[k], cs[k]), mul2f(z[k], sn[k]), -1.f), f = sum2f(mul2f(z[k], cs[k]), mul2f(x[k], sn[k]), 1.f);
+                x[k] = e;
+                z[k] = f;
+            }
+        }
+    };
+    if (QUERIES && static_cast<int>(blockIdx.y) >= p.kv_splits) {
+        // Queries. (No lane waits for another here.)
+        if (!there) return;
+        const T* x = static_cast<const T*>(p.x[2]) + b * p.xB[2] + i * p.xT[2];
+        T* out = static_cast<T*>(p.q_out) + token * p.Hq * c.D;
+        for (int h0 = blockIdx.y - p.kv_splits; h0 < p.Hq; h0 += kRotateHeads * p.q_splits) {
+            Chunk<T, 8> v[kRotateHeads][2];
+#pragma unroll
+            for (int j = 0; j < kRotateHeads; ++j) {
+                const int h = h0 + j * p.q_splits;
+                if (!counted || h >= p.Hq) break;
+                v[j][0].load(x + h * p.xH[2] + d0);
+                v[j][1].load(x + h * p.xH[2] + d1);
+            }
+#pragma unroll
+            for (int j = 0; j < kRotateHeads; ++j) {
+                const int h = h0 + j * p.q_splits;
+                if (h >= p.Hq) break;
+                Chunk<T, 8> o[2];
+                if (counted) {
+                    uint64_t y[2][4];
+                    chunk_values(v[j][0], y[0]);
+                    chunk_values(v[j][1], y[1]);
+                    rotate(y[0], y[1]);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float f[8];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const float2 g = unpack2f(y[e][k]);
+                            f[2 * k] = g.x;
+                            f[2 * k + 1] = g.y;
+                        }
+                        o[e].set(f);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int k = 0; k < Chunk<T, 8>::kWords; ++k) o[e].w[k] = 0;
+                }
+                o[0].store(out + static_cast<int64_t>(h) * c.D + d0);
+                o[1].store(out + static_cast<int64_t>(h) * c.D + d1);
+            }
+        }
+        return;
+    }
+    if (there && i == 0 && u == 0 && blockIdx.y == 0 && count > 0 && (start < 0 || static_cast<int64_t>(start) + count > c.T))
+        q8::report(c.status, AKV_ERR_INVALID_ARGUMENT);
+    const bool kept = counted && start >= 0 && start < c.T && i < c.T - start;
+    int row = 0;
+    const int phys = kept ? page_of(c, b, start + i, row) : -1;
+    if (!__any_sync(0xFFFFFFFFu, phys >= 0)) return;
+    const bool store = phys >= 0;
+    const uint32_t row_mask = (lanes == 32 ? 0xFFFFFFFFu : (1u << lanes) - 1) << (row_of_warp * lanes & 31);
+    const T* in[2] = {static_cast<const T*>(p.x[0]) + b * p.xB[0] + i * p.xT[0], static_cast<const T*>(p.x[1]) + b * p.xB[1] + i * p.xT[1]};
+    uint8_t* codes[2] = {c.k.codes + code_offset(c.k, b, 0, phys, row), c.v.codes + code_offset(c.v, b, 0, phys, row)};
+    __half* scales[2] = {c.k.scales + scale_offset(c.k, b, 0, phys, row), c.v.scales + scale_offset(c.v, b, 0, phys, row)};
+    for (int h0 = blockIdx.y; h0 < c.H; h0 += kAppendHeads * p.kv_splits) {
+        Chunk<T, 8> v[kAppendHeads][2][2];  // [head][side][chunk]
+#pragma unroll
+        for (int j = 0; j < kAppendHeads; ++j) {
+            const int h = h0 + j * p.kv_splits;
+#pragma unroll
+            for (int side = 0; side < 2; ++side)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    v[j][side][e].clear();  // a lane that stores nothing goes along with zeros
+                    if (store && h < c.H) v[j][side][e].load(in[side] + h * p.xH[side] + (e ? d1 : d0));
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < kAppendHeads; ++j) {
+            const int h = h0 + j * p.kv_splits;
+            if (h >= c.H) break;
+            bool mine = true;  // of this lane's groups, whether all are numbers
+            // V, then K, which has to know of V.
+#pragma unroll
+            for (int side = 1; side >= 0; --side) {
+                const SideDev& s = side ? c.v : c.k;
+                uint64_t x[2][4];
+                float top[2];
+                chunk_values(v[j][side][0], x[0]);
+                chunk_values(v[j][side][1], x[1]);
+                if (side == 0) rotate(x[0], x[1]);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) top[e] = side == 0 || sizeof(T) == 4 ? largest_of(x[e]) : v[j][side][e].largest();
+#pragma unroll
+                for (int o = 1; o <= 2; o <<= 1) {
+                    top[0] = max_nan(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], o));
+                    top[1] = max_nan(top[1], __shfl_xor_sync(0xFFFFFFFFu, top[1], o));
+                }
+                const bool fine[2] = {top[0] < CUDART_INF_F, top[1] < CUDART_INF_F};
+                mine = mine && fine[0] && fine[1];
+                bool bad = false;
+                if (side == 0) bad = __ballot_sync(0xFFFFFFFFu, !mine) & row_mask;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const bool none = side ? !fine[e] : bad;
+                    const __half scale = none ? __ushort_as_half(side ? 0 : 0x7FFF) : group_scale(top[e]);
+                    const uint32_t w = none ? 0u : chunk_codes(x[e], __half2float(scale));
+                    const int d = e ? d1 : d0;
+                    if (store) *reinterpret_cast<uint32_t*>(codes[side] + h * s.sH + d / 2) = w;
+                    if (store && (u & 3) == 0) scales[side][h * s.cH + (d / AKV_Q4_GROUP) * s.cG] = scale;
+                }
+            }
+        }
+    }
+}
+
 struct RestoreParams {
     CacheDev c;
     void* out[2];
@@ -235,13 +463,13 @@ struct RestoreParams {
     int n;
 };
 
-// One thread per eight channels, in the order of the output; grid.y: sequence x side.
+// One thread per sixteen channels, in the order of the output; grid.y: sequence x side.
 template <typename T>
 __global__ void __launch_bounds__(256) restore_kernel(RestoreParams p) {
     const CacheDev& c = p.c;
     const int b = blockIdx.y >> 1, side = blockIdx.y & 1;
     const SideDev& s = side ? c.v : c.k;
-    const unsigned per_row = c.D / 8, per_token = per_row * c.H;
+    const unsigned per_row = c.D / 16, per_token = per_row * c.H;
     const unsigned i = blockIdx.x * 256u + threadIdx.x;
     if (i >= per_token * p.n) return;
     const unsigned ti = i / per_token, rest = i - ti * per_token;
@@ -250,26 +478,36 @@ __global__ void __launch_bounds__(256) restore_kernel(RestoreParams p) {
     const int64_t t = static_cast<int64_t>(ti) + (p.start ? p.start[b] : 0);
     int row = 0;
     const int phys = t >= 0 && t < c.T ? page_of(c, b, static_cast<int>(t), row) : -1;
-    uint32_t w = 0;
+    uint2 w = make_uint2(0, 0);
     __half scale = __float2half_rn(0.f);
     if (phys >= 0) {
-        w = *reinterpret_cast<const uint32_t*>(s.codes + code_offset(s, b, h, phys, row) + 4 * l);
-        scale = s.scales[scale_offset(s, b, h, phys, row) + (l >> 2) * s.cG];
+        w = *reinterpret_cast<const uint2*>(s.codes + code_offset(s, b, h, phys, row) + 8 * l);
+        scale = s.scales[scale_offset(s, b, h, phys, row) + (l >> 1) * s.cG];
     }
-    uint32_t v[4];
-    codes_to_half(w, v);
     const __half2 both = __half2half2(scale);
-    float x[8];
+    T* out = static_cast<T*>(p.out[side]) + (static_cast<int64_t>(b) * p.n * per_token + i) * 16;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        v[k] = mul2(v[k], *reinterpret_cast<const uint32_t*>(&both));
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
-        x[2 * k] = f.x;
-        x[2 * k + 1] = f.y;
+    for (int e = 0; e < 2; ++e) {
+        uint32_t v[4];
+        codes_to_half(e ? w.y : w.x, v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = mul2(v[k], *reinterpret_cast<const uint32_t*>(&both));
+        Chunk<T, 8> o;
+        if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o.w[k] = v[k];
+        } else {
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[k]));
+                x[2 * k] = f.x;
+                x[2 * k + 1] = f.y;
+            }
+            o.set(x);
+        }
+        o.store(out + 8 * e);
     }
-    Chunk<T, 8> o;
-    o.set(x);
-    o.store(static_cast<T*>(p.out[side]) + (static_cast<int64_t>(b) * p.n * per_token + i) * 8);
 }
 
 }  // namespace q4

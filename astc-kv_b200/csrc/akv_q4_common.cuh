@@ -89,13 +89,21 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
 // that fp16 holds, 65472.
 constexpr float kMostScale = 10912.f;
 
-// x / scale rounded to nearest, given the rounded reciprocal of the scale: the
-// quotient's estimate and one correction by its exact remainder (Markstein's
-// theorem). Ties between two codes have to be seen as ties: a 16-bit x is
-// often a small multiple of the scale.
+// x / scale rounded to nearest, given the scale's approximate reciprocal (a
+// unit in the last place off at most): the estimate q of the quotient and one
+// correction by its remainder, which is exact (Markstein). q + remainder *
+// inverse is then off by 2^-45 of itself before its one rounding, and a
+// quotient of 24 bits by 11 is 2^-36 away at least from what would round
+// another way. Ties between two codes have to be seen as ties: a 16-bit x is
+// often a small multiple of the scale. 0 for a scale of 0.
 __device__ __forceinline__ float quotient(float x, float scale, float inverse) {
     const float q = __fmul_rn(x, inverse);
     return __fmaf_rn(__fmaf_rn(-q, scale, x), inverse, q);
+}
+__device__ __forceinline__ float inverse_of(float scale) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(scale));
+    return scale > 0.f ? y : 0.f;
 }
 
 }  // namespace q4

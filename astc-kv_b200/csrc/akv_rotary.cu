@@ -5,12 +5,11 @@
 #include "akv_q8_step_launch.h"
 #include "akv_rotary.cuh"
 
-using namespace akv;
-
+namespace akv {
 namespace {
 
 template <typename T, int N>
-void launch_rotate(const RotateParams& p, bool interleaved, unsigned blocks, cudaStream_t s) {
+void launch(const RotateParams& p, bool interleaved, unsigned blocks, cudaStream_t s) {
     if constexpr (N < 8) {  // interleaved, four pairs are 16 bytes
         if (interleaved) {
             rotate_kernel<T, N, true><<<blocks, kRotateThreads, 0, s>>>(p);
@@ -21,6 +20,31 @@ void launch_rotate(const RotateParams& p, bool interleaved, unsigned blocks, cud
 }
 
 }  // namespace
+
+int launch_rotate(RotateParams p, int dtype, bool interleaved, cudaStream_t s) {
+    const int N = rotate_width(p, interleaved, dtype == AKV_Q_F32 ? 4 : 2);
+    p.splits = rotate_splits(p, N);
+    if (p.splits == 0) return AKV_ERR_UNSUPPORTED;
+    const int64_t threads = static_cast<int64_t>(p.B) * p.n * p.splits * ((p.D + 2 * N - 1) / (2 * N));
+    const unsigned blocks = static_cast<unsigned>((threads + kRotateThreads - 1) / kRotateThreads);
+    if (dtype == AKV_Q_F32) {
+        if (N == 4) launch<float, 4>(p, interleaved, blocks, s);
+        else launch<float, 1>(p, interleaved, blocks, s);
+    } else if (dtype == AKV_Q_BF16) {
+        if (N == 8) launch<__nv_bfloat16, 8>(p, false, blocks, s);
+        else if (N == 4) launch<__nv_bfloat16, 4>(p, interleaved, blocks, s);
+        else launch<__nv_bfloat16, 1>(p, interleaved, blocks, s);
+    } else {
+        if (N == 8) launch<__half, 8>(p, false, blocks, s);
+        else if (N == 4) launch<__half, 4>(p, interleaved, blocks, s);
+        else launch<__half, 1>(p, interleaved, blocks, s);
+    }
+    return q8::launched();
+}
+
+}  // namespace akv
+
+using namespace akv;
 
 extern "C" {
 
@@ -52,41 +76,8 @@ int akv_rotate(const AkvRotateDesc* d, void* stream) {
     p.xB = d->x_stride[0]; p.xT = d->x_stride[1]; p.xH = d->x_stride[2];
     p.oB = d->out_stride[0]; p.oT = d->out_stride[1]; p.oH = d->out_stride[2];
     p.places = d->positions_dev; p.status = d->status_dev;
-    // The widest pieces that sizes and addresses allow: 8 pairs (16 bytes of
-    // either half), 4 pairs, else one.
-    const auto aligned = [&](int64_t bytes) {
-        bool a = reinterpret_cast<uintptr_t>(p.x) % bytes == 0 && reinterpret_cast<uintptr_t>(p.out) % bytes == 0;
-        for (const int64_t st : {p.xB, p.xT, p.xH, p.oB, p.oT, p.oH}) a = a && st * elem % bytes == 0;
-        return a;
-    };
-    int N = 1;
-    if (elem == 2 && !d->rotary.interleaved && p.r.R % 16 == 0 && p.D % 16 == 0 && aligned(16)) N = 8;
-    else if (p.r.R % 8 == 0 && p.D % 8 == 0 && aligned(4 * elem)) N = 4;
-    const int64_t tokens = static_cast<int64_t>(p.B) * p.n, units = (p.D + 2 * N - 1) / (2 * N);
-    // Eight heads a thread where that leaves some waves of threads, fewer else.
-    const int64_t few = static_cast<int64_t>(148) * 2048;
-    int64_t splits = (p.H + 7) / 8;
-    const int64_t want = (few + tokens * units - 1) / (tokens * units);
-    if (splits < want) splits = want < p.H ? want : p.H;
-    if (tokens * units * splits > 0x7FFFFF00) splits = 1;
-    if (tokens * units * splits > 0x7FFFFF00) return AKV_ERR_UNSUPPORTED;
-    p.splits = static_cast<int>(splits);
-    const unsigned blocks = static_cast<unsigned>((tokens * units * splits + kRotateThreads - 1) / kRotateThreads);
-    const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool inter = d->rotary.interleaved != 0;
-    if (d->dtype == AKV_Q_F32) {
-        if (N == 4) launch_rotate<float, 4>(p, inter, blocks, s);
-        else launch_rotate<float, 1>(p, inter, blocks, s);
-    } else if (d->dtype == AKV_Q_BF16) {
-        if (N == 8) launch_rotate<__nv_bfloat16, 8>(p, false, blocks, s);
-        else if (N == 4) launch_rotate<__nv_bfloat16, 4>(p, inter, blocks, s);
-        else launch_rotate<__nv_bfloat16, 1>(p, inter, blocks, s);
-    } else {
-        if (N == 8) launch_rotate<__half, 8>(p, false, blocks, s);
-        else if (N == 4) launch_rotate<__half, 4>(p, inter, blocks, s);
-        else launch_rotate<__half, 1>(p, inter, blocks, s);
-    }
-    return q8::launched();
+    p.start = p.counts = nullptr;
+    return launch_rotate(p, d->dtype, d->rotary.interleaved != 0, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

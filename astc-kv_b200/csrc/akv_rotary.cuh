@@ -8,7 +8,11 @@
 // are rounded one by one (no fused multiply-add), so that every call that
 // rotates a value gets the same bits.
 #pragma once
+#include <climits>
+
 #include <math_constants.h>
+
+#include <initializer_list>
 
 #include "../../include/akv_rotary.h"
 #include "akv_q8_common.cuh"
@@ -19,6 +23,7 @@ struct RotaryDev {
     const float* table;
     int positions, R, axes;
     uint32_t used;           // axes that a pair takes
+    uint32_t alike;          // bit i: pairs 4i to 4i + 3 take one axis
     bool whole_rows;         // rows of the table start on 16-byte boundaries
     uint8_t axis[128];
 };
@@ -28,10 +33,12 @@ inline RotaryDev to_dev(const AkvRotary& r) {
     d.table = r.table_dev;
     d.positions = r.positions; d.R = r.rotary_dim; d.axes = r.axes;
     d.used = 0;
+    d.alike = ~0u;
     d.whole_rows = r.rotary_dim % 4 == 0;
     for (int i = 0; i < r.rotary_dim / 2; ++i) {
         d.axis[i] = r.axis[i];
         d.used |= 1u << r.axis[i];
+        if (i % 4 && r.axis[i] != r.axis[i - 1]) d.alike &= ~(1u << i / 4);
     }
     return d;
 }
@@ -60,15 +67,19 @@ __device__ __forceinline__ bool places_in(const RotaryDev& r, const int32_t* pla
 template <int N>
 __device__ __forceinline__ void load_turns(const RotaryDev& r, const int32_t* places, int64_t stride, int place, int first, float (&c)[N], float (&s)[N]) {
     const int64_t row = r.R;  // floats
-    if (N >= 4 && r.whole_rows && (r.axes == 1 || !places)) {
-        const float4* at = reinterpret_cast<const float4*>(r.table + (places ? __ldg(places) : place) * row + 2 * first);
+    if constexpr (N >= 4) {
+        constexpr uint32_t all = (1u << N / 4) - 1;
+        const int axis = r.axis[first];
+        if (r.whole_rows && (!places || ((r.alike >> first / 4 & all) == all && axis == r.axis[first + N - 4]))) {
+            const float4* at = reinterpret_cast<const float4*>(r.table + (places ? __ldg(places + axis * stride) : place) * row + 2 * first);
 #pragma unroll
-        for (int k = 0; k < N / 2; ++k) {
-            const float4 v = __ldg(at + k);
-            c[2 * k] = v.x; s[2 * k] = v.y;
-            c[N > 1 ? 2 * k + 1 : 0] = v.z; s[N > 1 ? 2 * k + 1 : 0] = v.w;
+            for (int k = 0; k < N / 2; ++k) {
+                const float4 v = __ldg(at + k);
+                c[2 * k] = v.x; s[2 * k] = v.y;
+                c[2 * k + 1] = v.z; s[2 * k + 1] = v.w;
+            }
+            return;
         }
-        return;
     }
 #pragma unroll
     for (int k = 0; k < N; ++k) {
@@ -82,6 +93,11 @@ __device__ __forceinline__ void load_turns(const RotaryDev& r, const int32_t* pl
 // x cos + other sin: the first of a pair gives -sin.
 __device__ __forceinline__ float turned(float x, float other, float c, float s) { return __fadd_rn(__fmul_rn(x, c), __fmul_rn(other, s)); }
 
+__device__ __forceinline__ __half low_of(__half2 v) { return __low2half(v); }
+__device__ __forceinline__ __half high_of(__half2 v) { return __high2half(v); }
+__device__ __forceinline__ __nv_bfloat16 low_of(__nv_bfloat162 v) { return __low2bfloat16(v); }
+__device__ __forceinline__ __nv_bfloat16 high_of(__nv_bfloat162 v) { return __high2bfloat16(v); }
+
 // N consecutive elements as they are in memory.
 template <typename T, int N>
 struct Chunk {
@@ -93,7 +109,11 @@ struct Chunk {
         if constexpr (kBytes >= 16) {
 #pragma unroll
             for (int k = 0; k < kBytes / 16; ++k) {
-                const uint4 v = *(reinterpret_cast<const uint4*>(at) + k);
+                // (Volatile, so that all of a round's loads stay ahead of its arithmetic; not from the
+                // read-only path: out may be x.)
+                uint4 v;
+                asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(reinterpret_cast<const uint4*>(at) + k) : "memory");
                 w[4 * k] = v.x; w[4 * k + 1] = v.y; w[4 * k + 2] = v.z; w[4 * k + 3] = v.w;
             }
         } else if constexpr (kBytes == 8) {
@@ -115,6 +135,23 @@ struct Chunk {
             *reinterpret_cast<uint32_t*>(at) = w[0];
         } else {
             *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(w[0]);
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int k = 0; k < kWords; ++k) w[k] = 0;
+    }
+    // The largest |element| of 16-bit ones, a NaN if one is.
+    __device__ __forceinline__ float largest() const {
+        if constexpr (sizeof(T) == 2) {
+            using T2 = std::conditional_t<std::is_same<T, __nv_bfloat16>::value, __nv_bfloat162, __half2>;
+            T2 m = __habs2(*reinterpret_cast<const T2*>(&w[0]));
+#pragma unroll
+            for (int k = 1; k < kWords; ++k) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const T2*>(&w[k])));
+            const T top = __hmax_nan(low_of(m), high_of(m));
+            return static_cast<float>(top);
+        } else {
+            return 0.f;
         }
     }
     // Element by element, wherever it starts.
@@ -164,9 +201,14 @@ struct RotateParams {
     const void* x;
     void* out;
     int64_t xB, xT, xH, oB, oT, oH;  // elements
-    const int32_t* places;
+    const int32_t* places;     // or NULL: the tokens' places in a cache, start[b] + i
+    const int32_t* start;
+    const int32_t* counts;     // tokens of each sequence, zeros past them; or NULL
     int32_t* status;
 };
+
+// Token i of a sequence that begins at `start`. (A start outside a cache may be none of the table either.)
+__device__ __forceinline__ int place_of(int start, int i) { return static_cast<int>(min(static_cast<int64_t>(start) + i, static_cast<int64_t>(INT_MAX))); }
 
 constexpr int kRotateThreads = 256;
 constexpr int kRotateHeads = 4;  // loads of so many heads in flight
@@ -176,6 +218,7 @@ constexpr int kRotateHeads = 4;  // loads of so many heads in flight
 // what it writes and nothing else, out may be x.
 template <typename T, int N, bool INTER>
 __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(RotateParams p) {
+    constexpr bool ONE = INTER && sizeof(Chunk<T, 2 * N>) == 16;  // both pieces are 16 bytes in a row
     const unsigned units = (p.D + 2 * N - 1) / (2 * N);
     const unsigned i = blockIdx.x * static_cast<unsigned>(kRotateThreads) + threadIdx.x, rest = i / units, u = i - rest * units;
     const unsigned token = rest / p.splits, split = rest - token * p.splits;
@@ -187,11 +230,13 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(RotateParams p) 
     const T* x = static_cast<const T*>(p.x) + b * p.xB + t * p.xT;
     T* out = static_cast<T*>(p.out) + b * p.oB + t * p.oT;
     float c[N], s[N];
-    if (turn) {
-        const int32_t* places = p.places + token;
+    const bool counted = !p.counts || t < p.counts[b];
+    if (turn && counted) {
+        const int32_t* places = p.places ? p.places + token : nullptr;
         const int64_t stride = static_cast<int64_t>(p.B) * p.n;
-        if (places_in(p.r, places, stride, 0)) {
-            load_turns<N>(p.r, places, stride, 0, N * u, c, s);
+        const int place = p.start ? place_of(p.start[b], t) : 0;
+        if (places_in(p.r, places, stride, place)) {
+            load_turns<N>(p.r, places, stride, place, N * u, c, s);
             if (p.inverse) {
 #pragma unroll
                 for (int k = 0; k < N; ++k) s[k] = -s[k];
@@ -208,14 +253,27 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(RotateParams p) 
         for (int j = 0; j < kRotateHeads; ++j) {
             const int h = h0 + j * p.splits;
             if (h >= p.H) break;
-            v[j][0].load(x + h * p.xH + at0);
-            if (second) v[j][1].load(x + h * p.xH + at1);
+            v[j][0].clear();
+            v[j][1].clear();
+            if (!counted) continue;
+            if constexpr (ONE) {
+                Chunk<T, 2 * N> both;
+                both.load(x + h * p.xH + at0);
+#pragma unroll
+                for (int k = 0; k < Chunk<T, N>::kWords; ++k) {
+                    v[j][0].w[k] = both.w[k];
+                    v[j][1].w[k] = both.w[k + Chunk<T, N>::kWords];
+                }
+            } else {
+                v[j][0].load(x + h * p.xH + at0);
+                if (second) v[j][1].load(x + h * p.xH + at1);
+            }
         }
 #pragma unroll
         for (int j = 0; j < kRotateHeads; ++j) {
             const int h = h0 + j * p.splits;
             if (h >= p.H) break;
-            if (turn) {
+            if (turn && counted) {
                 float y1[N], y2[N];
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
@@ -236,10 +294,49 @@ __global__ void __launch_bounds__(kRotateThreads) rotate_kernel(RotateParams p) 
                 v[j][0].set(y1);
                 v[j][1].set(y2);
             }
-            v[j][0].store(out + h * p.oH + at0);
-            if (second) v[j][1].store(out + h * p.oH + at1);
+            if constexpr (ONE) {
+                Chunk<T, 2 * N> both;
+#pragma unroll
+                for (int k = 0; k < Chunk<T, N>::kWords; ++k) {
+                    both.w[k] = v[j][0].w[k];
+                    both.w[k + Chunk<T, N>::kWords] = v[j][1].w[k];
+                }
+                both.store(out + h * p.oH + at0);
+            } else {
+                v[j][0].store(out + h * p.oH + at0);
+                if (second) v[j][1].store(out + h * p.oH + at1);
+            }
         }
     }
 }
+
+// How wide rotate_kernel's pieces may be: 8 pairs (16 bytes of either half), 4
+// pairs, else one; for the addresses and strides (bytes) of its rows.
+inline int rotate_width(const RotateParams& p, bool interleaved, int64_t elem) {
+    const auto aligned = [&](int64_t bytes) {
+        bool a = reinterpret_cast<uintptr_t>(p.x) % bytes == 0 && reinterpret_cast<uintptr_t>(p.out) % bytes == 0;
+        for (const int64_t st : {p.xB, p.xT, p.xH, p.oB, p.oT, p.oH}) a = a && st * elem % bytes == 0;
+        return a;
+    };
+    if (elem == 2 && !interleaved && p.r.R % 16 == 0 && p.D % 16 == 0 && aligned(16)) return 8;
+    return p.r.R % 8 == 0 && p.D % 8 == 0 && aligned(interleaved ? 16 : 4 * elem) ? 4 : 1;
+}
+
+// Threads that share a token's heads. Eight heads a thread (4 x 8191 tokens, 40
+// heads, D 128, bf16: 109 us, with four 121, with twenty 111), twenty where
+// positions have several axes and a thread takes longer to begin (113 us against
+// 118), fewer where that leaves SMs with few threads (2 x 4097 tokens, 16 heads, D 72:
+// 10.3 us, with 2048 threads an SM asked for 12.4). 0 where the grid would be too large.
+inline int rotate_splits(const RotateParams& p, int N) {
+    const int64_t units = static_cast<int64_t>(p.B) * p.n * ((p.D + 2 * N - 1) / (2 * N)), few = 148 * 640;
+    const int64_t want = (few + units - 1) / units, heads = p.r.axes > 1 && p.places ? 20 : 8;
+    int64_t splits = (p.H + heads - 1) / heads;
+    if (splits < want) splits = want < p.H ? want : p.H;
+    if (units * splits > 0x7FFFFF00) splits = 1;
+    return units * splits > 0x7FFFFF00 ? 0 : static_cast<int>(splits);
+}
+
+// Launches rotate_kernel; dtype AKV_Q_*. Defined in akv_rotary.cu.
+int launch_rotate(RotateParams p, int dtype, bool interleaved, cudaStream_t s);
 
 }  // namespace akv
