@@ -20,13 +20,13 @@ INCLUDE = ROOT.parent / "include"
 LIB = PKG / "libakv_cuda.so"
 
 SOURCES = ["akv_cuda.cu", "akv_q8.cu", "akv_q8_step_int8.cu", "akv_q8_step_e4m3.cu", "akv_rotary.cu", "akv_q4.cu",
-           "akv_q4_step.cu", "akv_tables.cpp", "akv_encode.cpp"]
+           "akv_q4_step_dense.cu", "akv_q4_step_strided.cu", "akv_tables.cpp", "akv_encode.cpp"]
 HEADERS = ["akv_astc_device.cuh", "akv_common.cuh", "akv_decode_kernels.cuh", "akv_attention_kernels.cuh", "akv_tables.h",
            "akv_attn_fp16.cuh",
            "akv_attn_fast.cuh", "akv_decode_fast.cuh",
            "akv_q8_common.cuh", "akv_q8_store.cuh", "akv_q8_attend.cuh", "akv_q8_chunk.cuh", "akv_q8_step.cuh", "akv_q8_step_launch.cuh", "akv_q8_step_launch.h",
            "akv_q8_weights.cuh", "akv_q8_evict.cuh",
-           "akv_rotary.cuh", "akv_q4_common.cuh", "akv_q4_append.cuh", "akv_q4_attend.cuh", "akv_q4_step.cuh", "akv_q4_chunk.cuh"]
+           "akv_rotary.cuh", "akv_q4_common.cuh", "akv_q4_append.cuh", "akv_q4_attend.cuh", "akv_q4_step.cuh", "akv_q4_step_launch.cuh", "akv_q4_chunk.cuh"]
 
 
 def nvcc() -> str:

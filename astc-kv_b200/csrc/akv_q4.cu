@@ -355,7 +355,9 @@ int akv_q4_attention(const AkvQ4AttnDesc* d, void* stream) {
     p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     p.out = d->out_dev; p.lse_out = d->lse_dev;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (int st = plan.chunk ? launch_chunk(pp, s) : launch_step(pp, plan.nt, s)) return st;
+    const int row = pp.c.D / 2;
+    const bool dense = (pp.c.D == 64 || pp.c.D == 128 || pp.c.D == 256) && pp.c.k.sT == row && pp.c.v.sT == row;
+    if (int st = plan.chunk ? launch_chunk(pp, s) : dense ? launch_step_dense(pp, plan.nt, s) : launch_step_strided(pp, plan.nt, s)) return st;
     // A step kernel of one CTA leaves nothing to combine.
     if (plan.chunk ? plan.nsplits <= 1 : plan.cluster || plan.share_ctas <= 1) return AKV_OK;
     const int64_t rows = static_cast<int64_t>(p.c.B) * p.c.H * p.R;

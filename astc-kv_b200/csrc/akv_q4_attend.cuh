@@ -14,8 +14,10 @@ struct Q4Params {
     CacheDev c;
 };
 
-// nt: groups of eight rows per CTA, 1 or 2.
-int launch_step(const Q4Params& p, int nt, cudaStream_t s);
+// Host launchers of the step kernel, one translation unit each (the kernel has
+// many instances; they compile side by side). nt: groups of eight rows per CTA, 1 or 2.
+int launch_step_dense(const Q4Params& p, int nt, cudaStream_t s);    // see the kernel's DENSE
+int launch_step_strided(const Q4Params& p, int nt, cudaStream_t s);
 
 }  // namespace q4
 }  // namespace akv

@@ -50,6 +50,13 @@ __device__ __forceinline__ void load_words(uint32_t (&w)[NWORDS], const uint8_t*
     }
 }
 
+// Not volatile: only the numbers order products.
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b.x), "r"(b.y));
+}
+
 // A lane's part of a tile of 16 tokens, as loaded.
 template <int DP>
 struct Tile {
@@ -62,12 +69,14 @@ struct Tile {
 
 // DP: head_dim rounded up to 64, 128 or 256; NT: groups of 8 rows; PLO: P in
 // two parts; QLO: queries in two parts; TWIN, CLUSTER: see the 8-bit cache's step kernel.
-template <int DP, int NT, bool PLO, bool QLO, bool TWIN, bool CLUSTER>
+// DENSE: head_dim is DP and the rows of codes follow one another.
+template <int DP, int NT, bool PLO, bool QLO, bool TWIN, bool CLUSTER, bool DENSE>
 __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) step_kernel(Q4Params pp) {
     constexpr int KS = DP / 16;       // k-steps of S, d-tiles of O
     constexpr int ROWS = 8 * NT;
     constexpr int KP = Tile<DP>::KP, KW = Tile<DP>::KW, VW = Tile<DP>::VW;
     static_assert(!TWIN || (PLO && NT == 1), "twin rows carry P's second part");
+    constexpr int TURN = 16 * kStepWarps;       // tokens from a tile to the warp's next
     constexpr bool SECOND = PLO && !TWIN;       // P's second part in products of its own
     constexpr int FOLD = SECOND ? 1024 : 2048;  // tokens after which O goes to its sum in shared memory (fp32 outputs)
     __shared__ __align__(16) float red[kStepWarps][ROWS][DP];
@@ -139,54 +148,48 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     const int64_t part = (2 * static_cast<int64_t>(blockIdx.x) + (first ? 0 : 1)) * ROWS;  // where a piece of a unit goes
     const int t_begin = chunk * kShareTokens, t_end = min(t_begin + n_mine * kShareTokens, len);
 
-    // The tile to be loaded next: its first token, its place in its page, and
-    // pointers that move along with it and start anew in every page.
-    int t_load = t_begin + 16 * warp, page = t_load / c.P, row = t_load - page * c.P;
-    bool mapped = false;
+    // The tile to be loaded next: its first token and pointers that move along
+    // with it. Up to fast_end tiles are whole and in the same page; what comes
+    // there is looked up anew. (Votes where all lanes agree anyway: the
+    // compiler then keeps the warp together at no cost.)
+    int t_load = t_begin + 16 * warp, fast_end = 0, left = 0;  // left: tokens of the tile that there are, 0 where it is not mapped
+    bool fast = false;
     const uint8_t *k_at = nullptr, *v_at = nullptr;
     const __half *ks_at[KP], *vs_at = nullptr;
-    auto enter_page = [&]() {
-        mapped = false;
+    const int64_t k_row = DENSE ? DP / 2 : c.k.sT, v_row = DENSE ? DP / 2 : c.v.sT;
+    auto find_tile = [&]() {
+        left = 0;
+        fast_end = INT_MIN;
+        fast = false;
         if (t_load >= t_end) return;
-        int phys = page;
-        if (c.table) {
-            phys = __ldg(c.table + static_cast<int64_t>(b) * c.pps + page);
-            if (static_cast<unsigned>(phys) >= static_cast<unsigned>(c.num_pages)) {
-                q8::report(c.status, AKV_ERR_BAD_BLOCK_TABLE);
-                return;
-            }
-        }
-        mapped = true;
-        k_at = c.k.codes + code_offset(c.k, b, h, phys, row) + token_k * c.k.sT;
-        v_at = c.v.codes + code_offset(c.v, b, h, phys, row) + token_v * c.v.sT + v_col / 2;
+        int row;
+        const int phys = page_of(c, b, t_load, row);
+        if (phys < 0) return;
+        left = min(t_end - t_load, 16);
+        fast_end = min(t_end, t_load - row + c.P) - 15;
+        fast = t_load < fast_end;
+        k_at = c.k.codes + code_offset(c.k, b, h, phys, row) + token_k * k_row;
+        v_at = c.v.codes + code_offset(c.v, b, h, phys, row) + token_v * v_row + v_col / 2;
 #pragma unroll
         for (int j = 0; j < KP; ++j) ks_at[j] = c.k.scales + scale_offset(c.k, b, h, phys, row) + k_group[j] * c.k.cG + (token_k & ~3);
         vs_at = c.v.scales + scale_offset(c.v, b, h, phys, row) + v_col / AKV_Q4_GROUP * c.v.cG + token_v;
     };
-    const int64_t k_step = 16 * kStepWarps * c.k.sT, v_step = 16 * kStepWarps * c.v.sT;
     auto next_tile = [&]() {
-        t_load += 16 * kStepWarps;
-        row += 16 * kStepWarps;
-        if (row >= c.P) {
-            do {
-                row -= c.P;
-                ++page;
-            } while (row >= c.P);
-            enter_page();
-        } else {
-            k_at += k_step;
-            v_at += v_step;
+        t_load += TURN;
+        k_at += TURN * k_row;
+        v_at += TURN * v_row;
 #pragma unroll
-            for (int j = 0; j < KP; ++j) ks_at[j] += 16 * kStepWarps;
-            vs_at += 16 * kStepWarps;
-        }
+        for (int j = 0; j < KP; ++j) ks_at[j] += TURN;
+        vs_at += TURN;
+        fast = __all_sync(0xFFFFFFFFu, t_load < fast_end);
+        if (!fast) find_tile();
     };
     auto load_k = [&](Tile<DP>& t) {
-        if (mapped && t_load + 16 <= t_end) {
+        if (fast) {
 #pragma unroll
             for (int j = 0; j < KP; ++j) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) load_words(t.k[i][j], k_at + 2 * i * c.k.sT + k_col[j] / 2);
+                for (int i = 0; i < 2; ++i) load_words(t.k[i][j], k_at + 2 * i * k_row + k_col[j] / 2);
                 t.ks[j] = load_scales(ks_at[j]);
             }
             return;
@@ -194,39 +197,39 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
 #pragma unroll
         for (int j = 0; j < KP; ++j) {
             t.ks[j] = make_uint2(0, 0);
-            if (mapped && t_load < t_end) t.ks[j] = load_scales(ks_at[j]);  // a page's scales reach to the tile's end
+            if (left > 0) t.ks[j] = load_scales(ks_at[j]);  // a page's scales reach to the tile's end
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int w = 0; w < KW; ++w) t.k[i][j][w] = 0;
-                if (mapped && t_load + token_k + 2 * i < t_end) load_words(t.k[i][j], k_at + 2 * i * c.k.sT + k_col[j] / 2);
+                if (token_k + 2 * i < left) load_words(t.k[i][j], k_at + 2 * i * k_row + k_col[j] / 2);
             }
         }
     };
     auto load_v = [&](Tile<DP>& t) {
-        if (mapped && t_load + 16 <= t_end) {
+        if (fast) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_words(t.v[i], v_at + i * c.v.sT);
+            for (int i = 0; i < 4; ++i) load_words(t.v[i], v_at + i * v_row);
             t.vs = load_scales(vs_at);
             return;
         }
         t.vs = make_uint2(0, 0);
-        const int left = mapped ? t_end - t_load - token_v : 0;  // what lies past the end may hold anything: codes and scales are 0 there
-        if (left > 0) {
+        const int mine = left - token_v;  // what lies past the end may hold anything: codes and scales are 0 there
+        if (mine > 0) {
             t.vs = load_scales(vs_at);
-            if (left < 4) t.vs.y &= left == 3 ? 0xFFFFu : 0u;
-            if (left < 2) t.vs.x &= 0xFFFFu;
+            if (mine < 4) t.vs.y &= mine == 3 ? 0xFFFFu : 0u;
+            if (mine < 2) t.vs.x &= 0xFFFFu;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
 #pragma unroll
             for (int w = 0; w < VW; ++w) t.v[i][w] = 0;
-            if (i < left) load_words(t.v[i], v_at + i * c.v.sT);
+            if (i < mine) load_words(t.v[i], v_at + i * v_row);
         }
     };
 
     Tile<DP> ta, tb;
-    enter_page();
+    find_tile();
     load_k(ta);
     load_v(ta);
     next_tile();
@@ -326,10 +329,10 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
                     for (int nt = 0; nt < NT; ++nt) {
                         float(&acc)[4] = k & 1 ? s1[nt] : s[nt];
                         const uint2 q = qs[k][nt][0][lane];
-                        q8::mma16816(acc, a[2 * e], z[2 * e], a[2 * e + 1], z[2 * e + 1], q.x, q.y);
+                        mma(acc, a[2 * e], z[2 * e], a[2 * e + 1], z[2 * e + 1], q);
                         if (QLO) {
                             const uint2 ql = qs[k][nt][QLO ? 1 : 0][lane];
-                            q8::mma16816(acc, a[2 * e], z[2 * e], a[2 * e + 1], z[2 * e + 1], ql.x, ql.y);
+                            mma(acc, a[2 * e], z[2 * e], a[2 * e + 1], z[2 * e + 1], ql);
                         }
                     }
                 }
@@ -339,16 +342,22 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
         next_tile();
         load_k(t);
 
-        const bool all_seen = t0 + 16 <= bound_min;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[nt][k] = (s[nt][k] + s1[nt][k]) * factor[nt][k & 1];
+        if (__any_sync(0xFFFFFFFFu, t0 + 16 > bound_min)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (t0 + token_k + 2 * (k >> 1) >= bound[nt][k & 1]) s[nt][k] = -CUDART_INF_F;
+        }
         bool above = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                s[nt][k] = (s[nt][k] + s1[nt][k]) * factor[nt][k & 1];
-                if (!all_seen && t0 + token_k + 2 * (k >> 1) >= bound[nt][k & 1]) s[nt][k] = -CUDART_INF_F;
-                above |= s[nt][k] > limit[nt][k & 1];
-            }
+            for (int k = 0; k < 4; ++k) above |= s[nt][k] > limit[nt][k & 1];
         if (__any_sync(0xFFFFFFFFu, above)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -412,8 +421,8 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float(&acc)[4] = o[4 * w + e][nt];
-                    q8::mma16816(acc, even[0][e], odd[0][e], even[1][e], odd[1][e], ph[nt][0], ph[nt][1]);
-                    if (SECOND) q8::mma16816(acc, even[0][e], odd[0][e], even[1][e], odd[1][e], pl[SECOND ? nt : 0][0], pl[SECOND ? nt : 0][1]);
+                    mma(acc, even[0][e], odd[0][e], even[1][e], odd[1][e], make_uint2(ph[nt][0], ph[nt][1]));
+                    if (SECOND) mma(acc, even[0][e], odd[0][e], even[1][e], odd[1][e], make_uint2(pl[SECOND ? nt : 0][0], pl[SECOND ? nt : 0][1]));
                 }
         }
         load_v(t);
@@ -421,10 +430,10 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     // O's sum, brought to the present base by `carry`: the lane's own part of
     // the room that `red` takes at the end.
     float4* const sums = reinterpret_cast<float4*>(&red[warp][0][0]) + lane;
-    for (int t0 = t_begin + 16 * warp; t0 < t_end; t0 += 32 * kStepWarps) {
+    for (int t0 = t_begin + 16 * warp; __any_sync(0xFFFFFFFFu, t0 < t_end); t0 += 2 * TURN) {
         tile(t0, ta);
-        if (t0 + 16 * kStepWarps < t_end) tile(t0 + 16 * kStepWarps, tb);
-        if (PLO && t0 % FOLD >= FOLD - 32 * kStepWarps) {
+        if (__any_sync(0xFFFFFFFFu, t0 + TURN < t_end)) tile(t0 + TURN, tb);
+        if (PLO && __any_sync(0xFFFFFFFFu, t0 % FOLD >= FOLD - 2 * TURN)) {
             const bool begun = t0 - t_begin >= FOLD;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
