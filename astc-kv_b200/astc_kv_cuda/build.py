@@ -26,7 +26,7 @@ HEADERS = ["akv_astc_device.cuh", "akv_common.cuh", "akv_decode_kernels.cuh", "a
            "akv_attn_fast.cuh", "akv_decode_fast.cuh",
            "akv_q8_common.cuh", "akv_q8_store.cuh", "akv_q8_attend.cuh", "akv_q8_chunk.cuh", "akv_q8_step.cuh", "akv_q8_step_launch.cuh", "akv_q8_step_launch.h",
            "akv_q8_weights.cuh", "akv_q8_evict.cuh",
-           "akv_rotary.cuh", "akv_q4_common.cuh", "akv_q4_append.cuh", "akv_q4_attend.cuh", "akv_q4_step.cuh", "akv_q4_step_launch.cuh", "akv_q4_chunk.cuh"]
+           "akv_rotary.cuh", "akv_q4_common.cuh", "akv_q4_append.cuh", "akv_q4_attend.cuh", "akv_q4_loads.cuh", "akv_q4_step.cuh", "akv_q4_step_launch.cuh", "akv_q4_chunk.cuh"]
 
 
 def nvcc() -> str:

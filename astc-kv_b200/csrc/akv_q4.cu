@@ -196,7 +196,7 @@ int launch_chunk(const Q4Params& p, cudaStream_t s) {
     const int parts = SHARED ? p.a.nsplits / 2 : p.a.nsplits;
     constexpr int rows = 128 * kChunkTiles<DP>;
     const dim3 grid(parts * ((p.a.R + rows - 1) / rows), p.c.H, p.c.B);
-    kern<<<grid, kChunkThreads<DP>, bytes, s>>>(p);
+    kern<<<grid, kChunkThreads<DP, SHARED>, bytes, s>>>(p);
     return q8::launched();
 }
 

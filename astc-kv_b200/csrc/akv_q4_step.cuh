@@ -21,7 +21,7 @@
 //   channels, by a shift and a three-input operation each; the conversion then
 //   gives token pairs, and their scales multiply as a pair.
 #pragma once
-#include "akv_q4_attend.cuh"
+#include "akv_q4_loads.cuh"
 
 namespace akv {
 namespace q4 {
@@ -30,25 +30,6 @@ using q8::kShareTokens;
 using q8::kStepCluster;
 using q8::kStepThreads;
 using q8::kStepWarps;
-
-__device__ __forceinline__ uint2 load_scales(const __half* p) {
-    uint2 v;
-    asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-    return v;
-}
-// NWORDS words, 4 to 16 bytes.
-template <int NWORDS>
-__device__ __forceinline__ void load_words(uint32_t (&w)[NWORDS], const uint8_t* p) {
-    if constexpr (NWORDS == 4) {
-        const uint4 v = q8::load_stream(p);
-        w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-    } else if constexpr (NWORDS == 2) {
-        const uint2 v = q8::load_stream8(p);
-        w[0] = v.x; w[1] = v.y;
-    } else {
-        asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
-    }
-}
 
 // Not volatile: only the numbers order products.
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint2 b) {
