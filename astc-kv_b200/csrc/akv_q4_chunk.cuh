@@ -123,7 +123,7 @@ struct ChunkSmem {
     uint8_t k[kChunkTiles<DP>][DP / 64][128 * 128];
     uint8_t v[kChunkTiles<DP>][2][DP * 128];
     float factor[kChunkTiles<DP>][128];
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], pv_done[2], done;
+    uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2][2], pv_done[2], done;
     uint32_t tmem;
     int abort;
 };
@@ -210,6 +210,7 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
             bar_init(&sm.p_full[i][1], 128);
             bar_init(&sm.pv_done[i], 1);
         }
+        bar_init(&sm.q_full, 32 * SOFT);
         bar_init(&sm.done, 1);
         sm.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -218,6 +219,11 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&sm.tmem)) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = sm.tmem;
 
     const int tile = warp >> 2, tile_row = threadIdx.x & 127, my_row = SHARED ? tile_row : threadIdx.x;  // of a softmax thread
     int bound = 0;
@@ -231,7 +237,7 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
         // A warp's 32 query rows (16-bit here), to fp16 after a power of two.
         // DP / 8 lanes load a row, so that it is read in one piece.
         constexpr int LANES = DP / 8, AT_ONCE = 32 / LANES, ROUND = 8;
-        const uint32_t sees = __ballot_sync(0xFFFFFFFFu, !blind);
+        const int64_t own = blind ? 0 : q8::q_row(p, b, h, r0 + my_row);  // (a division: once a row)
         const bool bf16 = p.q_dtype == AKV_Q_BF16;
         const int mine = lane / LANES, d = lane % LANES * 8;
 #pragma unroll 1
@@ -241,8 +247,9 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
             for (int k = 0; k < ROUND; ++k) {
                 const int i = i0 + AT_ONCE * k + mine;  // of the warp's rows
                 raw[k] = make_uint4(0, 0, 0, 0);
-                if ((sees >> i & 1) && d < c.D) {
-                    const uint16_t* at = static_cast<const uint16_t*>(p.q) + q8::q_row(p, b, h, r0 + my_row - lane + i) + d;
+                const bool sees = !__shfl_sync(0xFFFFFFFFu, blind, i);
+                const uint16_t* at = static_cast<const uint16_t*>(p.q) + __shfl_sync(0xFFFFFFFFu, own, i) + d;
+                if (sees && d < c.D) {
                     if (p.q_vec) {
                         raw[k] = __ldg(reinterpret_cast<const uint4*>(at));
                     } else {
@@ -275,11 +282,9 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
             }
         }
         fence_async();
+        bar_arrive(&sm.q_full);
+        __syncwarp();
     }
-    fence_before();
-    __syncthreads();
-    fence_after();
-    const uint32_t tmem = sm.tmem;
 
     if (warp < SOFT) {
         // ------------------------------------------------------------ softmax
@@ -461,19 +466,23 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
         __syncwarp();
         const int first = my_row - lane, there = min(rows - first, 32);  // the warp's rows
         constexpr int AT_ONCE = PER < 32 ? 32 / PER : 1;
+        const int64_t own = my_row < rows ? q8::out_row(p, b, h, r0 + my_row) : 0;
 #pragma unroll 4
-        for (int r = lane / PER % AT_ONCE; r < there; r += AT_ONCE)
+        for (int i = 0; i < 32; i += AT_ONCE) {
+            const int r = i + lane / PER % AT_ONCE;
+            const int64_t to = p.nsplits > 1 ? part + first + r : __shfl_sync(0xFFFFFFFFu, own, r);
 #pragma unroll
             for (int k = lane % PER; k < PER; k += 32) {
-                if (4 * k >= c.D) continue;
+                if (r >= there || 4 * k >= c.D) continue;
                 const float4 v = room[r * PER + (k ^ (r & (PER - 1)))];
-                if (p.nsplits > 1) *reinterpret_cast<float4*>(p.part_o + (part + first + r) * c.D + 4 * k) = v;
-                else q8::store4(p.out, p.out_dtype, q8::out_row(p, b, h, r0 + first + r) * c.D + 4 * k, v);
+                if (p.nsplits > 1) *reinterpret_cast<float4*>(p.part_o + to * c.D + 4 * k) = v;
+                else q8::store4(p.out, p.out_dtype, to * c.D + 4 * k, v);
             }
+        }
         if (my_row < rows) {
             if (p.nsplits > 1) p.part_ml[part + my_row] = make_float2(none ? -CUDART_INF_F : isnan(l) ? l : base, l);
             else if (p.lse_out)
-                p.lse_out[q8::out_row(p, b, h, r0 + my_row)] = (none ? -CUDART_INF_F : isnan(l) ? l : base + log2f(l)) * 0.69314718055994531f;
+                p.lse_out[own] = (none ? -CUDART_INF_F : isnan(l) ? l : base + log2f(l)) * 0.69314718055994531f;
         }
     } else if (warp < MMA) {
         // --------------------------------------------------- K's and V's values
@@ -651,7 +660,7 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
             }
         };
         const int tiles_here = two ? 2 : 1;
-        bool alive = true;
+        bool alive = bar_wait(&sm.q_full, 0, &sm.abort);
         // A tile's first scores; with both tiles on the same rows, the
         // second tile's are those of step 1.
         for (int tile = 0; tile < tiles_here && alive; ++tile) {
