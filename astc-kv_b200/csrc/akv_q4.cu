@@ -108,7 +108,14 @@ struct AttnPlan {
 
 // Rows from which the tcgen05 kernel is taken, whose CTA does 128 or 256 rows
 // for the price of one, rather than the step kernel, which does 16 at a time
-// (8 above head_dim 128).
+// (8 above head_dim 128) and starts sooner. Measured, step and chunk kernel in us:
+//   head_dim 128, 8 heads, 32768 tokens      20 rows 37, 34   32 rows 38, 35   40 rows 47, 35
+//   head_dim 128, 8 x 8 heads, 8192 tokens   20 rows 57, 66   32 rows 60, 68   40 rows 81, 69
+//   head_dim 128, 2 x 8 heads, 512 tokens    20 rows 15, 17   32 rows 16, 18   40 rows 24, 20
+//   head_dim 64, 4 x 3 heads, 8192 tokens    20 rows 20, 19   32 rows 22, 20   40 rows 24, 20
+//   head_dim 256, 2 x 2 heads, 8192 tokens   16 rows 22, 24   20 rows 29, 25   32 rows 31, 25
+// (One sequence of two heads and 512 tokens would be better off with the step
+// kernel even at 128 rows, 14 against 18 us; lengths are not known here.)
 int chunk_min_rows(int head_dim) { return head_dim <= 128 ? 33 : 17; }
 
 // Tokens that a tile of the tcgen05 kernel adds up at most where outputs are
@@ -116,8 +123,12 @@ int chunk_min_rows(int head_dim) { return head_dim <= 128 ? 33 : 17; }
 constexpr int64_t kChunkHalfTokens = 16384;
 
 // Tokens for each CTA of a cluster up to which a cluster for each kv head of
-// each sequence is taken, rather than even shares of all CTAs and a second launch.
-constexpr int kClusterTokens = 512;
+// each sequence is taken, rather than even shares of all CTAs and a second
+// launch. Measured at head_dim 128, cluster and shares in us, 4096 / 8192 /
+// 16384 tokens: one sequence of 8 heads 10.8, 14.2 / 14.4, 16.1 / 21.8, 18.0;
+// eight of them 16.0, 24.1 / 23.9, 30.7 / 39.7, 43.6 (head_dim 64, 3 heads:
+// 8.5, 10.7 / 10.8, 12.1 / 15.6, 15.2).
+constexpr int kClusterTokens = 1024;
 
 AttnPlan plan_attention(const AkvQ4AttnDesc* d) {
     AttnPlan a = {};
@@ -135,7 +146,12 @@ AttnPlan plan_attention(const AkvQ4AttnDesc* d) {
         const int64_t steps = (static_cast<int64_t>(c.max_tokens) + kChunkTokens - 1) / kChunkTokens;
         if (a.split == 0) {
             // One CTA per SM; the number of splits, up to eight or one wave, is
-            // that of the least cost over the waves, as in the 8-bit cache.
+            // that of the least cost over the waves, as in the 8-bit cache. Where
+            // sequences have lengths of their own and do not fill the SMs, as many
+            // more as cost 15 % at most if all are full: short ones leave SMs free
+            // that the long ones' splits then use. Measured, with and without, in us:
+            // 32 + 8 heads, 4 x 128 of 8192 tokens, ragged 60, 85, all full 100, 86;
+            // 3 x 300 of 8192 93, 133 and 165, 135; 64 + 8 heads, 8 x 5 of 8192 40, 54 and 69, 56.
             const int64_t most = units > 0 && sms / units > 8 ? sms / units : 8;
             const auto cost = [&](int64_t n) {
                 const double each = static_cast<double>((steps + n - 1) / n) + 3.0 + (n > 1 ? 2.5 * c.head_dim / 128 : 0.0);
@@ -206,8 +222,22 @@ int launch_chunk(const Q4Params& p, cudaStream_t s) {
     return p.c.D > 64 ? launch_chunk<128, false>(p, s) : launch_chunk<64, false>(p, s);
 }
 
-// Tokens from which an append's queries get a launch of their own.
-constexpr int64_t kQueriesApart = 512;
+// Tokens from which an append's queries get a launch of their own, whose kernel
+// needs fewer registers, beside the kernel with two chunks a lane and beside the
+// general one. Measured with 32 + 2 x 8 heads, together and apart in us:
+//   tokens                 1024       2048       4096       8192      32768
+//   head_dim 128      7.2,  9.0  9.7, 11.7   20, 21     41, 38    152, 127
+//   head_dim  64      5.9,  7.2  7.4,  8.7   11, 12     21, 21     81,  72
+//   96, general       8.4,  8.6   13, 12     28, 20     55, 38    223, 136
+//   160, general       13,  11    27, 19     52, 35    108, 70    425, 247
+constexpr int64_t kQueriesApart = 8192, kQueriesApartGeneral = 2048;
+
+// Tokens from which an append takes the kernel with two chunks a lane, where it
+// can, which has longer to go before its first load. Measured likewise, the
+// general kernel and that one in us, at 1 / 64 / 128 / 1024 / 32768 tokens:
+// head_dim 128 2.8, 3.3 / 3.6, 3.7 / 4.4, 4.0 / 8.5, 7.2 / 154, 127; head_dim
+// 256 3.0, 3.5 / 4.2, 4.2 / 4.9, 4.2 / 14, 11 / 301, 242.
+constexpr int64_t kPairsTokens = 128;
 
 template <typename T, bool VEC>
 void launch_append(const AppendParams& p, int turn, dim3 grid, cudaStream_t s) {
@@ -268,9 +298,10 @@ int akv_q4_append(const AkvQ4AppendDesc* d, void* stream) {
     p.start = d->start_dev; p.counts = d->counts_dev; p.places = d->positions_dev;
     p.n = d->tokens; p.Hq = queries ? d->q_heads : 0;
     // Two chunks of eight channels a lane, where both halves of the rotated and of the other channels hold whole groups.
-    const bool pairs = vec && (!turn || !d->rotary.interleaved) && p.r.R % 64 == 0 && (p.c.D - p.r.R) % 64 == 0;
+    const int64_t tokens = static_cast<int64_t>(p.c.B) * p.n;
+    const bool pairs = vec && tokens >= kPairsTokens && (!turn || !d->rotary.interleaved) && p.r.R % 64 == 0 && (p.c.D - p.r.R) % 64 == 0;
     const int rows = 32 / (p.c.D / (pairs ? 16 : 8)) * (kAppendThreads / 32);  // tokens of a CTA
-    const int64_t blocks = (static_cast<int64_t>(p.c.B) * p.n + rows - 1) / rows;
+    const int64_t blocks = (tokens + rows - 1) / rows;
     if (blocks > 0x7FFFFFFF) return AKV_ERR_UNSUPPORTED;
     // As many heads a CTA as leave a wave of CTAs, in whole rounds of a lane's loads.
     const int64_t wave = 2 * static_cast<int64_t>(sm_count()), want = wave > blocks ? wave / blocks : 1;
@@ -281,8 +312,7 @@ int akv_q4_append(const AkvQ4AppendDesc* d, void* stream) {
         return n < want ? static_cast<int>(want < heads ? want : heads) : n;
     };
     p.kv_splits = split(p.c.H, kAppendHeads);
-    // Queries go along in this launch where they are few, or else in a launch of their own, whose kernel needs fewer registers.
-    const bool apart = queries && static_cast<int64_t>(p.c.B) * p.n >= kQueriesApart;
+    const bool apart = queries && tokens >= (pairs ? kQueriesApart : kQueriesApartGeneral);
     p.q_splits = queries && !apart ? split(p.Hq, pairs ? kRotateHeads : 2) : 0;
     if (p.kv_splits + p.q_splits > kMaxGridYZ) return AKV_ERR_UNSUPPORTED;
     const dim3 grid(static_cast<unsigned>(blocks), p.kv_splits + p.q_splits);

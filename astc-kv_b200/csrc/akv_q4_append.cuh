@@ -401,9 +401,25 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 4 ? 1 : QUERIES ?
     if (!__any_sync(0xFFFFFFFFu, phys >= 0)) return;
     const bool store = phys >= 0;
     const uint32_t row_mask = (lanes == 32 ? 0xFFFFFFFFu : (1u << lanes) - 1) << (row_of_warp * lanes & 31);
-    const T* in[2] = {static_cast<const T*>(p.x[0]) + b * p.xB[0] + i * p.xT[0], static_cast<const T*>(p.x[1]) + b * p.xB[1] + i * p.xT[1]};
-    uint8_t* codes[2] = {c.k.codes + code_offset(c.k, b, 0, phys, row), c.v.codes + code_offset(c.v, b, 0, phys, row)};
-    __half* scales[2] = {c.k.scales + scale_offset(c.k, b, 0, phys, row), c.v.scales + scale_offset(c.v, b, 0, phys, row)};
+    // Where the lane's first chunk of the next head is, stepped from head to
+    // head: multiplied out for each, offsets were a quarter of the instructions
+    // (51 against 43 us for 4 x 8192 tokens of 8 heads).
+    const int h_first = blockIdx.y;
+    const T* in[2];
+    uint8_t* codes[2];
+    __half* scales[2];
+    const int apart = d1 - d0;
+    int64_t in_step[2], code_step[2], scale_step[2];
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+        const SideDev& s = side ? c.v : c.k;
+        in_step[side] = p.kv_splits * p.xH[side];
+        code_step[side] = p.kv_splits * s.sH;
+        scale_step[side] = p.kv_splits * s.cH;
+        in[side] = static_cast<const T*>(p.x[side]) + b * p.xB[side] + i * p.xT[side] + h_first * p.xH[side] + d0;
+        codes[side] = s.codes + code_offset(s, b, h_first, phys, row) + d0 / 2;
+        scales[side] = s.scales + scale_offset(s, b, h_first, phys, row) + d0 / AKV_Q4_GROUP * s.cG;
+    }
     for (int h0 = blockIdx.y; h0 < c.H; h0 += kAppendHeads * p.kv_splits) {
         Chunk<T, 8> v[kAppendHeads][2][2];  // [head][side][chunk]
 #pragma unroll
@@ -414,8 +430,10 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 4 ? 1 : QUERIES ?
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     v[j][side][e].clear();  // a lane that stores nothing goes along with zeros
-                    if (store && h < c.H) v[j][side][e].load(in[side] + h * p.xH[side] + (e ? d1 : d0));
+                    if (store && h < c.H) v[j][side][e].load(in[side] + e * apart);
                 }
+            in[0] += in_step[0];
+            in[1] += in_step[1];
         }
 #pragma unroll
         for (int j = 0; j < kAppendHeads; ++j) {
@@ -447,10 +465,11 @@ __global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 4 ? 1 : QUERIES ?
                     const bool none = side ? !fine[e] : bad;
                     const __half scale = none ? __ushort_as_half(side ? 0 : 0x7FFF) : group_scale(top[e]);
                     const uint32_t w = none ? 0u : chunk_codes(x[e], __half2float(scale));
-                    const int d = e ? d1 : d0;
-                    if (store) *reinterpret_cast<uint32_t*>(codes[side] + h * s.sH + d / 2) = w;
-                    if (store && (u & 3) == 0) scales[side][h * s.cH + (d / AKV_Q4_GROUP) * s.cG] = scale;
+                    if (store) *reinterpret_cast<uint32_t*>(codes[side] + e * apart / 2) = w;
+                    if (store && (u & 3) == 0) scales[side][e * apart / AKV_Q4_GROUP * s.cG] = scale;
                 }
+                codes[side] += code_step[side];
+                scales[side] += scale_step[side];
             }
         }
     }

@@ -203,6 +203,24 @@ def test_one_token_of_few_heads(cuda, T, lens, G):
     check_attention(cache, k, v, q.half(), lens, out_dtype=torch.float16)
 
 
+@pytest.mark.parametrize("D,H,T,lens", [(64, 3, 8192, [8192, 4097]), (128, 1, 8177, [8177, 0]), (256, 1, 8000, [7999, 1]), (128, 2, 8208, [8208, 8193])])
+def test_one_token_of_long_sequences(cuda, D, H, T, lens):
+    cache, k, v = make(2, H, T, D, seed=T + D, page=48)
+    q = torch.randn(2, 4 * H, D, device="cuda")
+    check_attention(cache, k, v, q, lens)
+    check_attention(cache, k, v, q.bfloat16(), lens, out_dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("D,G,n,T", [(64, 3, 6, 16400), (128, 4, 5, 8190), (128, 1, 31, 8500), (96, 2, 16, 8200), (256, 2, 9, 6000)])
+@pytest.mark.parametrize("od", [torch.bfloat16, torch.float16])
+def test_few_tokens_of_large_caches(cuda, D, G, n, T, od):
+    """Seventeen to thirty-two rows (eighteen above head_dim 128) over long sequences."""
+    cache, k, v = make(2, 4, T, D, seed=D + n, page=80)
+    q = torch.randn(2, n, 4 * G, D, device="cuda").to(od)
+    check_attention(cache, k, v, q, [T, n + 3], [n, n - 2], out_dtype=od)
+    check_attention(cache, k, v, q, [T - 130, 1000], out_dtype=od, split=512)
+
+
 @pytest.mark.parametrize("n", [1, 4, 50])
 def test_not_causal_and_scale(cuda, n):
     cache, k, v = make(2, 1, 333, 64, seed=3)
@@ -480,6 +498,33 @@ def test_append_shapes(cuda, D, R, H, Hq, n, dt, interleaved):
     check_append(cache, k, v, [40, 60], rotary=rot, places=places_of(1, 2, n, 200)[0])
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("D,R,H,Hq,n", [(128, 128, 8, 32, 64), (64, 64, 3, 9, 71), (128, 64, 2, 16, 133), (256, 128, 1, 8, 66), (256, 256, 2, 2, 65)])
+def test_append_many_tokens(cuda, D, R, H, Hq, n, dt):
+    from astc_kv_cuda import Q4Cache, Rotary
+    rot = Rotary.make(R, 300, theta=1000.0)
+    cache = Q4Cache.zeros(2, H, 208, D)
+    qkv = torch.randn(2, n, Hq + 2 * H, D, device="cuda").to(dt)
+    q, k, v = qkv[:, :, :Hq], qkv[:, :, Hq:Hq + H], qkv[:, :, Hq + H:]
+    check_append(cache, k, v, [0, 55], rotary=rot, q=q)
+    check_append(cache, k, v, [3, 17], [n, n // 2], rotary=rot)
+    check_append(cache, k, v, [40, 1], [0, n])
+    check_append(cache, k, v, [40, 60], rotary=rot, places=places_of(1, 2, n, 300)[0], q=q)
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dt", TYPES)
+def test_append_queries_of_thousands_of_tokens(cuda, dt, interleaved):
+    from astc_kv_cuda import Q4Cache, Rotary
+    n = 4100
+    rot = Rotary.make(64, n + 60, sections=(8, 12, 12), interleaved=interleaved)
+    cache = Q4Cache.zeros(2, 1, n + 59, 64)
+    qkv = torch.randn(2, n, 5, 64, device="cuda").to(dt)
+    q, k, v = qkv[:, :, :3], qkv[:, :, 3:4], qkv[:, :, 4:]
+    check_append(cache, k, v, [0, 59], [n, n - 37], rotary=rot, q=q)
+    check_append(cache, k, v, [59, 1], rotary=rot, places=places_of(3, 2, n, n + 60), q=q)
+
+
 @pytest.mark.parametrize("sections", [(16, 16), (8, 12, 12)])
 @pytest.mark.parametrize("page", [16, 48, 256])
 def test_append_axes_into_pages(cuda, sections, page):
@@ -531,12 +576,12 @@ def test_append_sizes_from_the_smallest_to_the_largest(cuda):
 
 
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("D", [64, 96, 256])
-def test_append_of_values_that_are_not_finite(cuda, dt, D):
+@pytest.mark.parametrize("D,n", [(64, 40), (96, 40), (256, 40), (64, 70), (128, 64), (256, 64)])
+def test_append_of_values_that_are_not_finite(cuda, dt, D, n):
     """The token's K gets NaN scales and codes of 0, the groups of V that hold one become 0; other tokens and heads are as ever."""
     from astc_kv_cuda import Q4Cache, q4_append, q4_restore
-    cache, clean = Q4Cache.zeros(2, 3, 64, D), Q4Cache.zeros(2, 3, 64, D)
-    k, v = torch.randn(2, 2, 40, 3, D, device="cuda").to(dt)
+    cache, clean = Q4Cache.zeros(2, 3, 96, D), Q4Cache.zeros(2, 3, 96, D)
+    k, v = torch.randn(2, 2, n, 3, D, device="cuda").to(dt)
     start = torch.zeros(2, dtype=torch.int32, device="cuda")
     q4_append(clean, k, v, start)
     bad = [("k", 0, 7, 1, 5, math.nan), ("v", 0, 8, 2, D - 1, math.inf), ("k", 1, 0, 0, D // 2, -math.inf), ("v", 1, 39, 1, 0, -math.nan),
@@ -547,7 +592,7 @@ def test_append_of_values_that_are_not_finite(cuda, dt, D):
     tokens = {(b, h, t) for _, b, t, h, _, _ in bad}
     for b in range(2):
         for h in range(3):
-            for t in range(40):
+            for t in range(n):
                 if (b, h, t) not in tokens:
                     assert torch.equal(cache.k[b, h, t], clean.k[b, h, t]) and torch.equal(cache.k_scales[b, h, :, t], clean.k_scales[b, h, :, t])
                     assert torch.equal(cache.v[b, h, t], clean.v[b, h, t]) and torch.equal(cache.v_scales[b, h, :, t], clean.v_scales[b, h, :, t])
