@@ -312,7 +312,14 @@ int akv_q4_append(const AkvQ4AppendDesc* d, void* stream) {
         return n < want ? static_cast<int>(want < heads ? want : heads) : n;
     };
     p.kv_splits = split(p.c.H, kAppendHeads);
-    const bool apart = queries && tokens >= (pairs ? kQueriesApart : kQueriesApartGeneral);
+    RotateParams r = {};
+    r.r = p.r;
+    r.B = p.c.B; r.n = p.n; r.H = p.Hq; r.D = p.c.D;
+    r.x = d->q_dev; r.out = d->q_out_dev;
+    r.xB = p.xB[2]; r.xT = p.xT[2]; r.xH = p.xH[2];
+    r.oH = p.c.D; r.oT = r.oH * r.H; r.oB = r.oT * r.n;
+    r.places = p.places; r.start = p.start; r.counts = p.counts; r.status = p.c.status;
+    const bool apart = queries && tokens >= (pairs ? kQueriesApart : kQueriesApartGeneral) && rotate_fits(r, d->dtype, d->rotary.interleaved != 0);
     p.q_splits = queries && !apart ? split(p.Hq, pairs ? kRotateHeads : 2) : 0;
     if (p.kv_splits + p.q_splits > kMaxGridYZ) return AKV_ERR_UNSUPPORTED;
     const dim3 grid(static_cast<unsigned>(blocks), p.kv_splits + p.q_splits);
@@ -328,15 +335,7 @@ int akv_q4_append(const AkvQ4AppendDesc* d, void* stream) {
         else launch_append<T, false>(p, how, grid, s);
     });
     if (const int st = q8::launched()) return st;
-    if (!apart) return AKV_OK;
-    RotateParams r = {};
-    r.r = p.r;
-    r.B = p.c.B; r.n = p.n; r.H = p.Hq; r.D = p.c.D;
-    r.x = d->q_dev; r.out = d->q_out_dev;
-    r.xB = p.xB[2]; r.xT = p.xT[2]; r.xH = p.xH[2];
-    r.oH = p.c.D; r.oT = r.oH * r.H; r.oB = r.oT * r.n;
-    r.places = p.places; r.start = p.start; r.counts = p.counts; r.status = p.c.status;
-    return launch_rotate(r, d->dtype, d->rotary.interleaved != 0, s);
+    return apart ? launch_rotate(r, d->dtype, d->rotary.interleaved != 0, s) : AKV_OK;
 }
 
 int akv_q4_restore(const AkvQ4RestoreDesc* d, void* stream) {

@@ -1,10 +1,21 @@
 // Append and restore of the 4-bit KV cache.
 //
-// A lane holds eight consecutive channels of a token's head: 16 bytes of 16-bit
-// rows in, one word of codes out, and four lanes share a scale. The other half of its
-// rotated pairs is loaded a second time by this lane, which finds it in L1
-// (rows meet no barrier and no shared memory). A lane keeps its token's cosines and
-// sines for all heads that it goes through.
+// Both move each value once: 4 bytes of two 16-bit values in and 9 bits out, or the
+// other way, so memory bounds them where tokens are many, and the launch where
+// they are few.
+//
+// append_kernel: a lane holds eight consecutive channels of a token's head: 16
+// bytes of 16-bit rows in, one word of codes out, and four lanes share a scale. The
+// other half of its rotated pairs is loaded a second time by this lane, which
+// finds it in L1 (rows meet no barrier and no shared memory). A lane keeps its
+// token's cosines and sines for all heads that it goes through.
+// append_pairs_kernel: both halves of eight pairs a lane, see there.
+//
+// Measured with 8 heads of 128 channels, bf16, rotated, 4 x 8192 tokens (134 MB
+// in, 38 MB out): pairs 41 us, 4.2 TB/s, 64 % of a copy's rate (issue, 47 % of the
+// cycles, and the wait for two heads' loads; 36 us without rotation); the
+// general kernel 66 interleaved and 70 with 96 channels. With 32 query heads 128.
+// One token of 64 sequences 3.4 us. Restore of the 4 x 8192 tokens 35 us, 4.9 TB/s.
 #pragma once
 #include "akv_q4_common.cuh"
 #include "akv_rotary.cuh"
@@ -26,7 +37,9 @@ struct AppendParams {
 };
 
 constexpr int kAppendThreads = 256;
-constexpr int kAppendHeads = 2;  // of K and V, loads of so many in flight
+// Of K and V, loads of so many heads in flight: with one, two and four 4 x 8192
+// tokens of 16-bit rows take 44, 41 and 70 us (registers).
+constexpr int kAppendHeads = 2;
 
 // How K and Q are rotated.
 enum { kStay, kHalves, kInterleaved };
@@ -302,9 +315,10 @@ __device__ __forceinline__ uint32_t chunk_codes(const uint64_t (&x)[4], float sc
 }
 
 // Grid as of append_kernel, with rows of D / 16 lanes. QUERIES: with parts for
-// the query heads.
+// the query heads. Two CTAs an SM of fp32 rows (with the registers of one 75 us
+// for 4 x 8192 tokens, so 55).
 template <typename T, bool TURN, bool QUERIES>
-__global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 4 ? 1 : QUERIES ? 2 : 3) append_pairs_kernel(AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, sizeof(T) == 4 || QUERIES ? 2 : 3) append_pairs_kernel(AppendParams p) {
     const CacheDev& c = p.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lanes = c.D / 16, rows = 32 / lanes;  // of a warp
     const int row_of_warp = lane / lanes, u = lane - row_of_warp * lanes;
@@ -482,7 +496,8 @@ struct RestoreParams {
     int n;
 };
 
-// One thread per sixteen channels, in the order of the output; grid.y: sequence x side.
+// One thread per sixteen channels (eight bytes of codes, 32 or 64 of values), in
+// the order of the output, so that stores are whole lines; grid.y: sequence x side.
 template <typename T>
 __global__ void __launch_bounds__(256) restore_kernel(RestoreParams p) {
     const CacheDev& c = p.c;

@@ -7,9 +7,15 @@
 // cache's chunk kernel:
 //
 //   warps 0-3, 4-7  softmax of tile 0 and 1, one thread per row
-//   warps 8-11      K, warps 12-15 V: codes from global memory to values in
-//                   shared memory (the conversion is shared by all 256 rows)
-//   warp 16         one thread issues tcgen05.mma
+//   warps 8-11      K and V: codes from global memory to values in shared
+//                   memory (the conversion is shared by all 256 rows)
+//   warp 12         one thread issues tcgen05.mma
+//
+// Thirteen warps leave a thread 128 registers; with four code warps each for K
+// and V, and 96 registers, 2048 query tokens of 32768 take 971 us, so 957. Up to
+// 128 rows are one tile twice (SHARED), which take every other step: steps come
+// faster, and four code warps each for K and V are better, 41 against 45 us
+// (8 x 5 tokens, 64/8 heads, to 8192).
 //
 // S = Q K^T (M 128 rows, N 128 tokens) and O += P V (N head_dim) accumulate in
 // tensor memory: two S tiles and two O tiles fill its 512 columns. P is
@@ -35,7 +41,17 @@
 // tensor cores, which truncate: 6e-9 of it per token of the split.
 //
 // With head_dim above 128 a CTA has one tile of rows, one stage of K and V, and
-// four warpgroups: K is warps 4-7, V 8-11, the issuing warp 12.
+// K is warps 4-7, V 8-11, the issuing warp 12 (2 x 512 tokens of 8192, 8/1
+// heads, head_dim 256: 108 us; with four code warps for both 132).
+//
+// Measured, 2048 query tokens of 32768, 32/8 heads, head_dim 128, bf16: 948-957
+// us in short runs, 1120 TFLOP/s or 67 % of a library product's; 1130 us (942
+// TFLOP/s, 67 % of what such products sustain) at the power cap. Of a step of two tiles the
+// tensor cores work 60 % of the time, instructions issue in 43 % of the cycles;
+// what bounds it is the round S -> softmax -> P -> S of a tile, whose softmax is
+// bound by exp2 and the conversions to fp16 (a step's 32768 scores). Two softmax
+// warpgroups a tile, half of the columns each, took 1302 us, two issuing warps 1115
+// where one took 1010. Short cases are bound by the start: 1 x 512 tokens of 4096 59 us.
 #pragma once
 #include "akv_q4_loads.cuh"
 #include "akv_q8_chunk.cuh"

@@ -336,6 +336,11 @@ inline int rotate_splits(const RotateParams& p, int N) {
     return units * splits > 0x7FFFFF00 ? 0 : static_cast<int>(splits);
 }
 
+// Whether one launch holds them.
+inline bool rotate_fits(const RotateParams& p, int dtype, bool interleaved) {
+    return rotate_splits(p, rotate_width(p, interleaved, dtype == AKV_Q_F32 ? 4 : 2)) > 0;
+}
+
 // Launches rotate_kernel; dtype AKV_Q_*. Defined in akv_rotary.cu.
 int launch_rotate(RotateParams p, int dtype, bool interleaved, cudaStream_t s);
 
