@@ -28,7 +28,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib as L
-from .q8 import _DTYPES, _Call, _int32, _on, _rows
+from .q8 import _DTYPES, _Call, _int32, _may_overlap, _on, _rows
 from .rotary import Rotary
 
 _GROUP, _TOKENS = L.AKV_Q4_GROUP, L.AKV_Q4_TOKENS
@@ -44,8 +44,9 @@ class Q4Cache:
     `block_table` int32 [B, pages_per_seq]. The lower channel of a byte is in
     its lower half. Codes and scales may be views whose last dimension is
     contiguous and whose other strides are multiples of 16 bytes (codes) or 4
-    elements (scales). `max_tokens` (default: all there is room for) bounds a
-    sequence. `status`: optional int32 [1] that kernels write an error code to
+    elements (scales). Sequences may share pages that they only read; what two
+    appends write to one place is either one's. `max_tokens` (default: all there is
+    room for) bounds a sequence. `status`: optional int32 [1] that kernels write an error code to
     (a bad table entry, tokens past the end, a position outside the rotary
     table, a wait inside a kernel that ran out); without it such rows are
     dropped, NaN or read as zeros and nothing says so.
@@ -263,6 +264,8 @@ class Q4Attention(_Call):
             out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
         if out.shape != q.shape or out.dtype not in _DTYPES or not out.is_contiguous():
             raise ValueError("out must be contiguous fp32/bf16/fp16 with the shape of q")
+        if _may_overlap(q, out):
+            raise ValueError("out must not share memory with q")
         d.out_dtype, d.out_dev = _DTYPES[out.dtype], out.data_ptr()
         d.causal, d.split_tokens, d.scale = int(causal), split_tokens, scale
         d.seq_lens_dev = _int32("lens", lens, (B,))

@@ -155,7 +155,8 @@ class _Rotation(torch.autograd.Function):
 
 def rotate(x: torch.Tensor, rotary: Rotary, positions: torch.Tensor, *, inverse: bool = False, stream: torch.cuda.Stream | None = None,
            **kw) -> torch.Tensor:
-    """One `Rotate`; x may require a gradient (on the current stream, without out)."""
+    """One `Rotate`; x may require a gradient (on the current stream, without out). As with any operation of autograd, a
+    backward pass is captured into a CUDA graph only while no graph recorded outside the capture holds the same leaves."""
     if x.requires_grad and torch.is_grad_enabled():
         if stream is not None or kw:
             raise ValueError("a rotation that records a gradient runs on the current stream and takes no out or status")
