@@ -2,6 +2,10 @@
 finite next to others, pages that sequences share, calls at the same time on
 several streams, outputs on top of inputs, a rotation's backward pass in a CUDA
 graph."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -114,3 +118,10 @@ def test_backward_of_a_rotation_in_a_graph(cuda, interleaved):
         graph.replay()
         got = grad.clone()
         assert torch.equal(got, step())
+
+
+@pytest.mark.parametrize("args", [["--prompt", "1500", "--steps", "5"], ["--prompt", "70", "--steps", "40", "--page", "16"]])
+def test_the_example_runs(cuda, args):
+    done = subprocess.run([sys.executable, str(Path(__file__).resolve().parents[1] / "examples" / "q4_serving.py"), *args],
+                          capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stdout + done.stderr
