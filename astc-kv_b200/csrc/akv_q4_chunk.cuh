@@ -44,14 +44,15 @@
 // K is warps 4-7, V 8-11, the issuing warp 12 (2 x 512 tokens of 8192, 8/1
 // heads, head_dim 256: 108 us; with four code warps for both 132).
 //
-// Measured, 2048 query tokens of 32768, 32/8 heads, head_dim 128, bf16: 948-957
-// us in short runs, 1120 TFLOP/s or 67 % of a library product's; 1130 us (942
-// TFLOP/s, 67 % of what such products sustain) at the power cap. Of a step of two tiles the
+// Measured, 2048 query tokens of 32768, 32/8 heads, head_dim 128, bf16: 949 us
+// in short runs, 1122 TFLOP/s or 67 % of a library product's; 1116 us (954
+// TFLOP/s, 68 % of what such products sustain) at the power cap. Of a step of two tiles the
 // tensor cores work 60 % of the time, instructions issue in 43 % of the cycles;
 // what bounds it is the round S -> softmax -> P -> S of a tile, whose softmax is
 // bound by exp2 and the conversions to fp16 (a step's 32768 scores). Two softmax
 // warpgroups a tile, half of the columns each, took 1302 us, two issuing warps 1115
-// where one took 1010. Short cases are bound by the start: 1 x 512 tokens of 4096 59 us.
+// where one took 1010. Short cases are bound by the start: 1 x 512 tokens of 4096 58 us, 39 of
+// 75 15 us, of which queries into shared memory 4 and rows out 4.
 #pragma once
 #include "akv_q4_loads.cuh"
 #include "akv_q8_chunk.cuh"
@@ -171,7 +172,6 @@ __device__ __forceinline__ uint32_t load_scale_if(const __half* p, bool in) {
     return v;
 }
 
-
 // SHARED: 128 rows or fewer a kv head; both tiles take the same rows and every
 // other step, as two splits.
 template <int DP, bool SHARED>
@@ -279,11 +279,12 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
 #pragma unroll
             for (int k = 0; k < ROUND; ++k) {
                 const uint32_t v[4] = {raw[k].x, raw[k].y, raw[k].z, raw[k].w};
-                uint32_t top = 0, w[4];  // the order of the magnitudes is that of their bits
+                uint32_t w[4], both = 0;  // the order of the magnitudes is that of their bits
 #pragma unroll
-                for (int j = 0; j < 4; ++j) top = max(top, max(v[j] & 0x7FFFu, v[j] >> 16 & 0x7FFFu));
+                for (int j = 0; j < 4; ++j) both = __vmaxu2(both, v[j] & 0x7FFF7FFFu);
 #pragma unroll
-                for (int j = 1; j < LANES; j <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, j));
+                for (int j = 1; j < LANES; j <<= 1) both = __vmaxu2(both, __shfl_xor_sync(0xFFFFFFFFu, both, j));
+                const uint32_t top = max(both & 0xFFFFu, both >> 16);
                 const int e = q8::row_exponent(bf16 ? __uint_as_float(top << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(top))));
                 const float up = q8::power_of_two(e);
 #pragma unroll
@@ -463,37 +464,48 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
         const float inv = p.nsplits > 1 ? 1.f : none ? 0.f : 1.f / l;
         const int64_t part = unit + (SHARED && tile ? p.R : 0);
         // A warp's rows go through its own part of the operands' room, which
-        // nothing reads any more once all products are done, so that they are written in one piece each. Pieces of 16 bytes lie crosswise.
+        // nothing reads any more once all products are done, so that they are
+        // written in one piece each. Pieces of 16 bytes lie crosswise.
         constexpr int PER = DP / 4;  // pieces of a row
         float4* const room = reinterpret_cast<float4*>(&sm.q[0][0][0]) + static_cast<int64_t>(warp) * 32 * PER;
-#pragma unroll 1
-        for (int g = 0; g < DP / 16; ++g) {
-            uint32_t o[16];
-            tmem_ld16(o, o_at + 16 * g);
-            tmem_wait_ld(o);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const float4 v = none ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                      : make_float4(__uint_as_float(o[4 * k]) * inv, __uint_as_float(o[4 * k + 1]) * inv,
-                                                    __uint_as_float(o[4 * k + 2]) * inv, __uint_as_float(o[4 * k + 3]) * inv);
-                room[lane * PER + ((4 * g + k) ^ (lane & (PER - 1)))] = v;
-            }
-        }
-        __syncwarp();
-        const int first = my_row - lane, there = min(rows - first, 32);  // the warp's rows
-        constexpr int AT_ONCE = PER < 32 ? 32 / PER : 1;
+        const int there = min(rows - (my_row - lane), 32);  // the warp's rows
         const int64_t own = my_row < rows ? q8::out_row(p, b, h, r0 + my_row) : 0;
-#pragma unroll 4
-        for (int i = 0; i < 32; i += AT_ONCE) {
-            const int r = i + lane / PER % AT_ONCE;
-            const int64_t to = p.nsplits > 1 ? part + first + r : __shfl_sync(0xFFFFFFFFu, own, r);
+        if (there > 0) {
+#pragma unroll 1
+            for (int g = 0; g < DP / 16; ++g) {
+                uint32_t o[16];
+                tmem_ld16(o, o_at + 16 * g);
+                tmem_wait_ld(o);
 #pragma unroll
-            for (int k = lane % PER; k < PER; k += 32) {
-                if (r >= there || 4 * k >= c.D) continue;
-                const float4 v = room[r * PER + (k ^ (r & (PER - 1)))];
-                if (p.nsplits > 1) *reinterpret_cast<float4*>(p.part_o + to * c.D + 4 * k) = v;
-                else q8::store4(p.out, p.out_dtype, to * c.D + 4 * k, v);
+                for (int k = 0; k < 4; ++k) {
+                    const float4 v = none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                          : make_float4(__uint_as_float(o[4 * k]) * inv, __uint_as_float(o[4 * k + 1]) * inv,
+                                                        __uint_as_float(o[4 * k + 2]) * inv, __uint_as_float(o[4 * k + 3]) * inv);
+                    room[lane * PER + ((4 * g + k) ^ (lane & (PER - 1)))] = v;
+                }
             }
+            __syncwarp();
+            const int64_t mine = p.nsplits > 1 ? part + my_row : own;
+            // Four pieces a lane at once, so that none waits for the one before.
+            auto write = [&](auto store) {
+#pragma unroll 1
+                for (int m = 0; m < PER && m * 32 / PER < there; m += 4) {
+                    float4 v[4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int at = 32 * (m + u) + lane, r = at / PER, k = at % PER;
+                        v[u] = room[r * PER + (k ^ (r & (PER - 1)))];
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int at = 32 * (m + u) + lane, r = at / PER, k = at % PER;
+                        const int64_t to = __shfl_sync(0xFFFFFFFFu, mine, r);
+                        if (r < there && 4 * k < c.D) store(to * c.D + 4 * k, v[u]);
+                    }
+                }
+            };
+            if (p.nsplits > 1) write([&](int64_t at, float4 v) { *reinterpret_cast<float4*>(p.part_o + at) = v; });
+            else write([&](int64_t at, float4 v) { q8::store4(p.out, p.out_dtype, at, v); });
         }
         if (my_row < rows) {
             if (p.nsplits > 1) p.part_ml[part + my_row] = make_float2(none ? -CUDART_INF_F : isnan(l) ? l : base, l);
