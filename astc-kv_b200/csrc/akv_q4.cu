@@ -118,9 +118,11 @@ struct AttnPlan {
 // kernel even at 128 rows, 14 against 18 us; lengths are not known here.)
 int chunk_min_rows(int head_dim) { return head_dim <= 128 ? 33 : 17; }
 
-// Tokens that a tile of the tcgen05 kernel adds up at most where outputs are
-// fp16: as in the 8-bit cache, the truncated sum would show in fp16's rounding.
-constexpr int64_t kChunkHalfTokens = 16384;
+// Tokens that a tile of the tcgen05 kernel adds up at most, also where a caller
+// asks for longer splits: the tensor cores truncate as they add, and a sum over n tokens comes
+// out about 6e-9 n too small (measured, bf16 out, 6.5e-3 at a million tokens in one sum),
+// which has to stay below what the output's rounding takes, 2^-11 (fp16) and 2^-8 (bf16) at most.
+constexpr int64_t kChunkHalfTokens = 16384, kChunkBf16Tokens = 131072;
 
 // Tokens for each CTA of a cluster up to which a cluster for each kv head of
 // each sequence is taken, rather than even shares of all CTAs and a second
@@ -144,6 +146,8 @@ AttnPlan plan_attention(const AkvQ4AttnDesc* d) {
     size_t parts;  // rows of partials
     if (a.chunk) {
         const int64_t steps = (static_cast<int64_t>(c.max_tokens) + kChunkTokens - 1) / kChunkTokens;
+        // (Two tiles that take every other step share a split.)
+        const int64_t longest = (d->out_dtype == AKV_Q_F16 ? kChunkHalfTokens : kChunkBf16Tokens) * (shared ? 2 : 1);
         if (a.split == 0) {
             // One CTA per SM; the number of splits, up to eight or one wave, is
             // that of the least cost over the waves, as in the 8-bit cache. Where
@@ -164,12 +168,11 @@ AttnPlan plan_attention(const AkvQ4AttnDesc* d) {
             for (int64_t n = 2; n <= most && n <= steps; ++n)
                 if (cost(n) <= limit) best = n;
             if (cost(1) <= least) best = best > 1 && limit > least ? best : 1;
-            if (d->out_dtype == AKV_Q_F16) {
-                const int64_t longest = kChunkHalfTokens / kChunkTokens * (shared ? 2 : 1), n = (steps + longest - 1) / longest;
-                best = best > n ? best : n;
-            }
+            const int64_t n = (steps * kChunkTokens + longest - 1) / longest;
+            best = best > n ? best : n;
             a.split = static_cast<int>((steps + best - 1) / best * kChunkTokens);
         }
+        if (a.split > longest) a.split = static_cast<int>(longest);
         // Whole steps: a step's tokens past the split's end would count as seen.
         a.split = static_cast<int>((static_cast<int64_t>(a.split < c.max_tokens ? a.split : c.max_tokens) + kChunkTokens - 1) / kChunkTokens * kChunkTokens);
         a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);

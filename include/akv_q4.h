@@ -127,10 +127,11 @@ int akv_q4_restore(const AkvQ4RestoreDesc* desc, void* stream);
  * which truncate, of exact products (of 22 bits with fp32 queries): off by at
  * most 2^-20 of the sum of |scale q K|. With an fp32 output the softmax weights
  * meet V in two fp16 parts (22 bits) and long sums are rounded to nearest
- * every 32 products; with a 16-bit output the weights are rounded to fp16,
- * and where a call goes to the tcgen05 kernel (many rows, queries x heads of a
- * kv head) the values' sum comes out 6e-9 of itself per token of a split too
- * small.
+ * every 32 products; with a 16-bit output the weights are rounded to fp16, and
+ * where a call goes to the tcgen05 kernel (many rows, queries x heads of a
+ * kv head) the values' sum comes out about 6e-9 of itself per token of a split too
+ * small. Splits there are of 16384 tokens at most with an fp16 output and of
+ * 131072 with a bf16 one (of twice as many up to 128 rows and head_dim 128, as two sums).
  *
  * Lengths are read by the kernels, so what the host decides, the splits of many
  * rows and the size of the workspace, goes by max_tokens: a cache with much
@@ -142,7 +143,8 @@ typedef struct AkvQ4AttnDesc {
     int32_t q_heads, q_tokens;
     int32_t q_dtype, out_dtype;     /* AKV_Q_* */
     int32_t causal;
-    int32_t split_tokens;           /* tokens per split at least, a multiple of 16; 0 = library choice */
+    int32_t split_tokens;           /* tokens per split at least (many rows and a 16-bit output: up to what a sum may
+                                       hold, see above), a multiple of 16; 0 = library choice */
     float scale;                    /* 0 = head_dim^-0.5 */
     int32_t reserved0;
     const void* q_dev;              /* element strides batch / token / head */

@@ -1,0 +1,65 @@
+"""Long sums in the 4-bit cache's attention.
+
+Every token has the same score, so an output is the mean of V's values over all
+tokens, which 64 bits hold; V's values are positive and the means lie anywhere between two
+numbers of the output's type, so that what a sum loses shows in the mean of the
+relative errors. Tensor cores truncate as they add: about 2^-27.3 of a sum is lost with
+every token that they add up, here taken as 2^-27. The rounding of an output is off by 2^-11 (fp16),
+2^-8 (bf16) at most and at random, evenly spread in between: divided by
+the root of 3 one standard deviation, of the mean of 256 values a sixteenth of
+that; four of those are 2^-13.8 and 2^-10.8 times the root of 1/3, below 2^-13 and 2^-10 by far.
+All sequences read one page.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+P = 1024
+NOISE = {torch.float16: 4 * 2.0 ** -11 / 3 ** 0.5 / 16, torch.bfloat16: 4 * 2.0 ** -8 / 3 ** 0.5 / 16}
+
+
+def one_page(B, H, T, D):
+    """A cache of B sequences of T tokens that are all the same page, keys of 0, and V's mean [H, D]."""
+    from astc_kv_cuda import Q4Cache
+    from test_gpu_q4 import values
+    g = torch.Generator(device="cuda").manual_seed(T + D)
+    k = torch.zeros(1, H, P, D // 2, dtype=torch.uint8, device="cuda")
+    ks = torch.ones(1, H, D // 32, P, dtype=torch.float16, device="cuda")
+    c = torch.randint(1, 8, (2, 1, H, P, D // 2), generator=g, device="cuda", dtype=torch.uint8)
+    v = c[0] | c[1] << 4
+    vs = (1 + torch.rand(1, H, D // 32, P, generator=g, device="cuda")).half()
+    table = torch.zeros(B, T // P, dtype=torch.int32, device="cuda")
+    return Q4Cache(k, v, ks, vs, block_table=table), values(v, vs)[0].mean(1)
+
+
+def lost(B, H, T, D, n, od, split):
+    """The mean relative error of each row and of all of its values."""
+    from astc_kv_cuda import Q4Attention
+    assert H * D == 256
+    cache, mean = one_page(B, H, T, D)
+    q = torch.randn(B, n, H, D, device="cuda").half()
+    out = Q4Attention(q, cache, out_dtype=od, causal=False, split_tokens=split).run().double()
+    return (out / mean - 1).mean((-2, -1))
+
+
+@pytest.mark.parametrize("D,n,od,T,split", [
+    # Row tiles for every SM, so that nothing but length asks for splits; splits as long as the cache.
+    (64, 100, torch.float16, 1 << 17, 0), (64, 100, torch.float16, 1 << 17, 1 << 17), (128, 300, torch.float16, 1 << 17, 1 << 17),
+    (256, 100, torch.float16, 1 << 17, 1 << 17),
+    (64, 100, torch.bfloat16, 1 << 20, 0), (64, 300, torch.bfloat16, 1 << 20, 0), (128, 100, torch.bfloat16, 1 << 20, 1 << 20),
+    (256, 40, torch.bfloat16, 1 << 20, 0)])
+def test_many_rows_of_16_bits(cuda, D, n, od, T, split):
+    """Sums of 16384 tokens at most with fp16 outputs, of 131072 with bf16 ones."""
+    most = 16384 if od == torch.float16 else 131072
+    off = lost(148 if n <= 128 else 74, 256 // D, T, D, n, od, split)
+    assert (off.abs() <= most * 2.0 ** -27 + NOISE[od]).all(), float(off.abs().max())
+
+
+def test_splits_stay_what_was_asked_for_where_sums_are_short(cuda):
+    """The longest sum bounds splits from above alone: the workspace of shorter ones is that of a library's choice of them."""
+    from astc_kv_cuda import Q4Attention
+    cache, _ = one_page(1, 4, 1 << 18, 64)
+    q = torch.randn(1, 300, 4, 64, device="cuda").half()
+    size = {s: Q4Attention(q, cache, out_dtype=torch.bfloat16, split_tokens=s).workspace.numel() for s in (32768, 65536, 131072, 262144)}
+    assert size[32768] > size[65536] > size[131072] == size[262144]
