@@ -103,6 +103,7 @@ struct AttnPlan {
     int nt;           // groups of eight rows per CTA
     int split, nsplits;          // chunk kernel
     int share_ctas, share_min;   // step kernel
+    bool long_sums;              // see kStepLong
     size_t part_ml, part_o, bytes;  // offsets into the workspace, and its size
 };
 
@@ -191,6 +192,11 @@ AttnPlan plan_attention(const AkvQ4AttnDesc* d) {
         a.share_min = a.split > q8::kShareTokens ? a.split / q8::kShareTokens : 1;
         const int64_t ctas = chunks / a.share_min < slots ? chunks / a.share_min : slots;
         a.share_ctas = static_cast<int>(ctas > 0 ? ctas : 1);
+        // The chunks of a CTA at most: fewer CTAs share shorter lengths, of at least share_min chunks each.
+        int64_t share = (chunks + a.share_ctas - 1) / a.share_ctas;
+        if (a.share_min > 1 && share < 2 * static_cast<int64_t>(a.share_min)) share = 2 * static_cast<int64_t>(a.share_min);
+        const int64_t tokens = share * q8::kShareTokens;
+        a.long_sums = (tokens < c.max_tokens ? tokens : c.max_tokens) > (d->out_dtype == AKV_Q_F16 ? kStepLong : kStepLongBf16);
         parts = 2 * static_cast<size_t>(a.share_ctas) * group;
         // The largest cluster with which all units fit the GPU at once.
         int size = q8::kStepCluster;
@@ -372,6 +378,7 @@ int akv_q4_attention(const AkvQ4AttnDesc* d, void* stream) {
     char* ws = static_cast<char*>(d->workspace_dev);
     Q4Params pp = {};
     pp.c = to_dev(d->cache);
+    pp.long_sums = plan.long_sums;
     q8::AttnParams& p = pp.a;
     p.c.B = pp.c.B; p.c.H = pp.c.H; p.c.D = pp.c.D; p.c.T = pp.c.T; p.c.status = pp.c.status;
     p.Hq = d->q_heads; p.G = d->q_heads / d->cache.kv_heads; p.n = d->q_tokens; p.R = plan.rows;

@@ -61,23 +61,26 @@ struct Tile {
 
 // DP: head_dim rounded up to 64, 128 or 256; NT: groups of 8 rows; PLO: P in
 // two parts; QLO: queries in two parts; TWIN, CLUSTER: see the 8-bit cache's step kernel.
-// DENSE: head_dim is DP and the rows of codes follow one another.
-template <int DP, int NT, bool PLO, bool QLO, bool TWIN, bool CLUSTER, bool DENSE>
+// DENSE: head_dim is DP and the rows of codes follow one another. FOLDS: sums
+// are put by, as with P in two parts, or where a CTA may go through too many tokens.
+template <int DP, int NT, bool PLO, bool QLO, bool TWIN, bool CLUSTER, bool DENSE, bool FOLDS>
 __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) step_kernel(Q4Params pp) {
     constexpr int KS = DP / 16;       // k-steps of S, d-tiles of O
     constexpr int ROWS = 8 * NT;
     constexpr int KP = Tile<DP>::KP, KW = Tile<DP>::KW, VW = Tile<DP>::VW;
     static_assert(!TWIN || (PLO && NT == 1), "twin rows carry P's second part");
+    static_assert(FOLDS || !PLO, "short sums are part of P's second part");
     constexpr int TURN = 16 * kStepWarps;       // tokens from a tile to the warp's next
     constexpr bool SECOND = PLO && !TWIN;       // P's second part in products of its own
-    constexpr int FOLD = SECOND ? 1024 : 2048;  // tokens after which O goes to its sum in shared memory (fp32 outputs)
+    // Tokens after which O goes to its sum in shared memory (FOLDS), which is rounded to nearest.
+    constexpr int FOLD = !PLO ? kStepLong : SECOND ? 1024 : 2048;
     __shared__ __align__(16) float red[kStepWarps][ROWS][DP];
     __shared__ float2 ml[kStepWarps][ROWS];
     __shared__ float row_scale[ROWS];
     __shared__ float2 piece[CLUSTER ? ROWS : 1];
     __shared__ uint2 qs[KS][NT][QLO ? 2 : 1][32];
     __shared__ q8::ShareScratch scratch;
-    __shared__ float carry[PLO ? 2 * NT : 1][kStepThreads];
+    __shared__ float carry[FOLDS ? 2 * NT : 1][kStepThreads];
 
     const q8::AttnParams& p = pp.a;
     const CacheDev& c = pp.c;
@@ -291,7 +294,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
 #pragma unroll
         for (int i = 0; i < KS; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) { base[nt][k] = 0.f; limit[nt][k] = -CUDART_INF_F; l[nt][k] = 0.f; if (PLO) carry[2 * nt + k][threadIdx.x] = 1.f; }
+        for (int k = 0; k < 2; ++k) { base[nt][k] = 0.f; limit[nt][k] = -CUDART_INF_F; l[nt][k] = 0.f; if (FOLDS) carry[2 * nt + k][threadIdx.x] = 1.f; }
     }
 
     auto tile = [&](int t0, Tile<DP>& t) {
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
                     base[nt][k] = to;
                     limit[nt][k] = up ? __fadd_rd(to, 15.5f) : limit[nt][k];
                     l[nt][k] *= alpha;
-                    if (PLO) carry[2 * nt + k][threadIdx.x] *= alpha;
+                    if (FOLDS) carry[2 * nt + k][threadIdx.x] *= alpha;
 #pragma unroll
                     for (int i = 0; i < KS; ++i) {
                         o[i][nt][k] *= alpha;
@@ -425,7 +428,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     for (int t0 = t_begin + 16 * warp; __any_sync(0xFFFFFFFFu, t0 < t_end); t0 += 2 * TURN) {
         tile(t0, ta);
         if (__any_sync(0xFFFFFFFFu, t0 + TURN < t_end)) tile(t0 + TURN, tb);
-        if (PLO && __any_sync(0xFFFFFFFFu, t0 % FOLD >= FOLD - 2 * TURN)) {
+        if (FOLDS && __any_sync(0xFFFFFFFFu, t0 % FOLD >= FOLD - 2 * TURN)) {
             const bool begun = t0 - t_begin >= FOLD;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -445,7 +448,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
 
     q8::allow_next_kernel();
     const int begun = t_begin + 16 * warp;
-    if (PLO && begun + (FOLD - 1 - begun % FOLD) / (32 * kStepWarps) * (32 * kStepWarps) < t_end) {  // there is a sum
+    if (FOLDS && begun + (FOLD - 1 - begun % FOLD) / (32 * kStepWarps) * (32 * kStepWarps) < t_end) {  // there is a sum
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const float f0 = carry[2 * nt][threadIdx.x], f1 = carry[2 * nt + 1][threadIdx.x];

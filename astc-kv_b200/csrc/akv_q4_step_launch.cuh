@@ -20,11 +20,17 @@ int launch(const Q4Params& p, cudaStream_t s) {
             cfg.stream = s;
             cfg.attrs = &attr;
             cfg.numAttrs = 1;
-            return cudaLaunchKernelEx(&cfg, step_kernel<DP, 1, PLO, QLO, TWIN, true, DENSE>, p) == cudaSuccess
+            return cudaLaunchKernelEx(&cfg, step_kernel<DP, 1, PLO, QLO, TWIN, true, DENSE, PLO>, p) == cudaSuccess
                        ? AKV_OK : (cudaGetLastError(), AKV_ERR_CUDA);
         }
     }
-    step_kernel<DP, NT, PLO, QLO, TWIN, false, DENSE><<<p.a.share_ctas, kStepThreads, 0, s>>>(p);
+    if constexpr (!PLO) {
+        if (p.long_sums) {
+            step_kernel<DP, NT, PLO, QLO, TWIN, false, DENSE, true><<<p.a.share_ctas, kStepThreads, 0, s>>>(p);
+            return q8::launched();
+        }
+    }
+    step_kernel<DP, NT, PLO, QLO, TWIN, false, DENSE, PLO><<<p.a.share_ctas, kStepThreads, 0, s>>>(p);
     return q8::launched();
 }
 

@@ -56,6 +56,15 @@ def test_many_rows_of_16_bits(cuda, D, n, od, T, split):
     assert (off.abs() <= most * 2.0 ** -27 + NOISE[od]).all(), float(off.abs().max())
 
 
+@pytest.mark.parametrize("od", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,n", [(64, 1), (64, 16), (128, 1), (128, 9), (256, 1)])
+def test_few_rows_of_16_bits(cuda, D, n, od):
+    """As many sequences as there are CTAs, so that each goes through all tokens of one, four warps each."""
+    most = 16384 if od == torch.float16 else 131072
+    off = lost(148 * 4 * D // 256 if n == 1 and D < 256 else 296 * D // 256, 256 // D, (1 << 20 if od == torch.float16 else 1 << 21), D, n, od, 0)
+    assert (off.abs() <= most * 2.0 ** -27 + NOISE[od]).all(), float(off.abs().max())
+
+
 def test_splits_stay_what_was_asked_for_where_sums_are_short(cuda):
     """The longest sum bounds splits from above alone: the workspace of shorter ones is that of a library's choice of them."""
     from astc_kv_cuda import Q4Attention
