@@ -17,6 +17,7 @@ from collections.abc import Sequence
 from dataclasses import dataclass
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _lib as L
 from .q8 import _DTYPES, _Call, _int32, _may_overlap, _on, _rows
@@ -139,25 +140,45 @@ class Rotate(_Call):
 
 
 class _Rotation(torch.autograd.Function):
+    """A rotation is linear: both of its derivatives are rotations of the same positions, recorded where they are needed again."""
+
     @staticmethod
-    def forward(ctx, x, rotary, positions, inverse):
-        ctx.rotary, ctx.inverse = rotary, inverse
-        ctx.save_for_backward(positions)
+    def forward(x, rotary, positions, inverse):
         return Rotate(x, rotary, positions, inverse=inverse).run()
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    def setup_context(ctx, inputs, output):
+        _, ctx.rotary, positions, ctx.inverse = inputs
+        ctx.save_for_backward(positions)
+        ctx.save_for_forward(positions)
+
+    @staticmethod
     def backward(ctx, grad):
-        # (A broadcast gradient, of a sum for example, has no contiguous last dimension.)
-        grad = grad if grad.stride(-1) == 1 or grad.shape[-1] == 1 else grad.contiguous()
-        return Rotate(grad, ctx.rotary, ctx.saved_tensors[0], inverse=not ctx.inverse).run(), None, None, None
+        return rotate(_contiguous(grad), ctx.rotary, ctx.saved_tensors[0], inverse=not ctx.inverse), None, None, None
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        return rotate(_contiguous(tangent), ctx.rotary, ctx.saved_tensors[0], inverse=ctx.inverse)
+
+
+def _contiguous(x: torch.Tensor) -> torch.Tensor:
+    # (A broadcast gradient, of a sum for example, has no contiguous last dimension.)
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+_transforming = getattr(torch._C, "_are_functorch_transforms_active", lambda: False)
+
+
+def _derived(x: torch.Tensor) -> bool:
+    """Whether a derivative by x may be taken, backward, forward or by a transform of torch.func."""
+    return x.requires_grad and torch.is_grad_enabled() or unpack_dual(x).tangent is not None or _transforming()
 
 
 def rotate(x: torch.Tensor, rotary: Rotary, positions: torch.Tensor, *, inverse: bool = False, stream: torch.cuda.Stream | None = None,
            **kw) -> torch.Tensor:
-    """One `Rotate`; x may require a gradient (on the current stream, without out). As with any operation of autograd, a
-    backward pass is captured into a CUDA graph only while no graph recorded outside the capture holds the same leaves."""
-    if x.requires_grad and torch.is_grad_enabled():
+    """One `Rotate`; x may require a gradient or have a tangent (on the current stream, without out). As with any operation of
+    autograd, a backward pass is captured into a CUDA graph only while no graph recorded outside the capture holds the same leaves."""
+    if _derived(x):
         if stream is not None or kw:
             raise ValueError("a rotation that records a gradient runs on the current stream and takes no out or status")
         return _Rotation.apply(x, rotary, positions, inverse)

@@ -1,0 +1,53 @@
+"""More of the rotary positions on the GPU: derivatives of other kinds than the backward pass."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from test_gpu_rotary import TYPES, places_of, same, turned
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dt", TYPES)
+def test_tangents_are_rotated(cuda, dt, interleaved):
+    from astc_kv_cuda import Rotary, rotate
+    rot = Rotary.make(48, 30, sections=(8, 16), interleaved=interleaved)
+    axes = [0] * 8 + [1] * 16
+    at = places_of(2, 2, 5, 30, seed=3)
+    x, v = (torch.randn(2, 5, 3, 64, device="cuda").to(dt) for _ in range(2))
+    want = turned(v, rot.table, axes, at, interleaved)
+    with forward_ad.dual_level():
+        y = forward_ad.unpack_dual(rotate(forward_ad.make_dual(x, v), rot, at))
+        same(y.primal, turned(x, rot.table, axes, at, interleaved))
+        same(y.tangent, want)
+    y, t = torch.func.jvp(lambda z: rotate(z, rot, at), (x,), (v,))
+    same(t, want)
+    # Along with a gradient: of the tangent's sum by the tangent.
+    w = v.clone().requires_grad_()
+    with forward_ad.dual_level():
+        t = forward_ad.unpack_dual(rotate(forward_ad.make_dual(x, w), rot, at)).tangent
+        same(torch.autograd.grad(t.sum(), w)[0], turned(torch.ones_like(v), rot.table, axes, at, interleaved, True))
+
+
+def test_second_derivatives(cuda):
+    """f = sum(y^3) / 3 of y = R x: the Hessian times v is R^T (2 y u) with u = R v. With X = |x1| + |x2| of a pair and V likewise,
+    y is off by 2^-22 X, u by 2^-22 V, and eight more roundings make 2 y u off by 2 X V 2^-20; the last rotation adds up
+    two of those and its own 2^-22 (4 X V): 2^-17 X V covers them."""
+    from astc_kv_cuda import Rotary, rotate
+    rot = Rotary.make(64, 30)
+    at = places_of(1, 2, 5, 30)
+    x, v = (torch.randn(2, 5, 3, 64, device="cuda") for _ in range(2))
+    x.requires_grad_()
+    g, = torch.autograd.grad((rotate(x, rot, at) ** 3).sum() / 3, x, create_graph=True)
+    h, = torch.autograd.grad(g, x, v)
+
+    def turn(z, inverse=False):
+        return turned(z, rot.table, [0] * 32, at, False, inverse)
+    y, u = turn(x.detach()), turn(v)
+    want = turn((2 * y * u).float(), True)
+
+    def size(z):
+        z = z.detach().double().abs()
+        return (z[..., :32] + z[..., 32:]).repeat(1, 1, 1, 2)
+    assert ((h.double() - want).abs() <= 2.0 ** -17 * size(x) * size(v)).all()

@@ -1,0 +1,63 @@
+"""`rotate` and derivatives, without a GPU: a plain rotation stands in for the call, and the recording around it is checked."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from astc_kv_cuda import rotary
+
+
+class Plain:
+    """What Rotate does, in 64 bits and without a record."""
+
+    def __init__(self, x, table, positions, *, inverse=False, out=None):
+        x.data_ptr()  # as Rotate: memory, or an error
+        cs = table[positions.long()][:, :, None]
+        c, s = cs[..., 0], cs[..., 1] * (-1 if inverse else 1)
+        a, b = x.detach().chunk(2, -1)
+        self.out = torch.cat([a * c - b * s, b * c + a * s], -1)
+
+    def run(self, stream=None):
+        return self.out
+
+
+@pytest.fixture
+def given(monkeypatch):
+    monkeypatch.setattr(rotary, "Rotate", Plain)
+    g = torch.Generator().manual_seed(0)
+    angle = torch.randn(9, 3, dtype=torch.float64, generator=g)
+    table = torch.stack([angle.cos(), angle.sin()], -1) * 1.5
+    x, v = torch.randn(2, 2, 4, 2, 6, dtype=torch.float64, generator=g)
+    return x, v, table, torch.randint(0, 9, (2, 4), generator=g)
+
+
+def test_tangents_are_rotated(given):
+    x, v, table, at = given
+    want = Plain(v, table, at).run()
+    with forward_ad.dual_level():
+        y = rotary.rotate(forward_ad.make_dual(x, v), table, at)
+        assert torch.equal(forward_ad.unpack_dual(y).tangent, want)
+        y = rotary.rotate(forward_ad.make_dual(x, v[..., :1].expand_as(v)), table, at)  # broadcast
+        assert torch.equal(forward_ad.unpack_dual(y).tangent, Plain(v[..., :1].expand_as(v), table, at).run())
+    assert torch.equal(torch.func.jvp(lambda z: rotary.rotate(z, table, at), (x,), (v,))[1], want)
+
+
+@pytest.mark.parametrize("inverse", [False, True])
+def test_derivatives_of_any_order(given, inverse):
+    x, _, table, at = given
+    x = x.requires_grad_()
+    assert torch.autograd.gradcheck(lambda z: rotary.rotate(z, table, at, inverse=inverse), x, check_forward_ad=True)
+    assert torch.autograd.gradgradcheck(lambda z: rotary.rotate(z, table, at, inverse=inverse).sin(), x, check_fwd_over_rev=True)
+
+
+def test_transforms(given):
+    x, v, table, at = given
+
+    def f(z):
+        return rotary.rotate(z, table, at).sin().sum()
+    leaf = x.clone().requires_grad_()
+    g, = torch.autograd.grad(f(leaf), leaf, create_graph=True)
+    assert torch.equal(torch.func.grad(f)(x), g)
+    h, = torch.autograd.grad(g, leaf, v)
+    assert torch.allclose(torch.func.jvp(torch.func.grad(f), (x,), (v,))[1], h, rtol=1e-12)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(f)(x[None])
