@@ -18,6 +18,7 @@ from dataclasses import dataclass
 
 import torch
 from torch.autograd.forward_ad import unpack_dual
+from torch.autograd.graph import increment_version
 
 from . import _lib as L
 from .q8 import _DTYPES, _Call, _int32, _may_overlap, _on, _rows
@@ -98,7 +99,9 @@ class Rotate(_Call):
     a tensor that does not overlap it; its own contiguous one by default.
     `inverse`: turns back, which is the gradient. A token with a position
     outside the table becomes NaN in the rotated channels, and `status`
-    (optional int32 [1]) gets an error code."""
+    (optional int32 [1]) gets an error code. Records no gradient (see `rotate`):
+    an `out` that requires one is refused where gradients are recorded, and
+    autograd learns that a given `out` was written."""
 
     _family, _fn = "", "rotate"
 
@@ -114,6 +117,7 @@ class Rotate(_Call):
             raise ValueError("heads need as many channels as the pairs have, and at most 256")
         if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
             raise ValueError("status must be int32")
+        self._given = out is not None
         if out is None:
             out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         if out.dtype != x.dtype:
@@ -135,6 +139,10 @@ class Rotate(_Call):
         self._prepare(d, x.device, x, out, rotary.table, positions, status)
 
     def run(self, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
+        if self._given:
+            if self.out.requires_grad and torch.is_grad_enabled():
+                raise ValueError("a rotation into a given tensor records no gradient, which this one requires")
+            increment_version(self.out)
         self._issue(stream)
         return self.out
 

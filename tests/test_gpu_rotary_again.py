@@ -51,3 +51,34 @@ def test_second_derivatives(cuda):
         z = z.detach().double().abs()
         return (z[..., :32] + z[..., 32:]).repeat(1, 1, 1, 2)
     assert ((h.double() - want).abs() <= 2.0 ** -17 * size(x) * size(v)).all()
+
+
+def test_autograd_sees_what_is_written(cuda):
+    """A rotation in place of what a backward pass needs is an error there, and one that would need a record is refused."""
+    from astc_kv_cuda import Rotary, Rotate, rotate
+    rot = Rotary.make(64, 30)
+    at = places_of(1, 2, 5, 30)
+    x = torch.randn(2, 5, 3, 64, device="cuda")
+    w = torch.randn(64, device="cuda", requires_grad=True)
+    for write in (lambda: rotate(x, rot, at, out=x), Rotate(x, rot, at, out=x).run):
+        loss = (x * w).sum()  # keeps x
+        write()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    other, loss = x.clone(), (x * w).sum()
+    Rotate(x, rot, at, out=other).run()
+    loss.backward()
+    y = torch.randn(2, 5, 3, 64, device="cuda", requires_grad=True) * 2
+    before = y.detach().clone()
+    call = Rotate(y, rot, at, out=y)
+    for run in (call.run, lambda: rotate(x, rot, at, out=y)):
+        with pytest.raises(ValueError):
+            run()
+    assert torch.equal(y, before)
+    with torch.no_grad():
+        call.run()
+    same(y.detach(), turned(before, rot.table, [0] * 32, at, False))
+    with torch.inference_mode():
+        z = before.clone()
+        rotate(z, rot, at, out=z)
+    same(z, turned(before, rot.table, [0] * 32, at, False))
