@@ -174,19 +174,23 @@ def _contiguous(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
+# Whether a transform of torch.func is at work.
 _transforming = getattr(torch._C, "_are_functorch_transforms_active", lambda: False)
 
 
 def _derived(x: torch.Tensor) -> bool:
-    """Whether a derivative by x may be taken, backward, forward or by a transform of torch.func."""
-    return x.requires_grad and torch.is_grad_enabled() or unpack_dual(x).tangent is not None or _transforming()
+    """Whether a derivative by x is recorded, backward or forward."""
+    return x.requires_grad and torch.is_grad_enabled() or unpack_dual(x).tangent is not None
 
 
 def rotate(x: torch.Tensor, rotary: Rotary, positions: torch.Tensor, *, inverse: bool = False, stream: torch.cuda.Stream | None = None,
            **kw) -> torch.Tensor:
     """One `Rotate`; x may require a gradient or have a tangent (on the current stream, without out). As with any operation of
-    autograd, a backward pass is captured into a CUDA graph only while no graph recorded outside the capture holds the same leaves."""
-    if _derived(x):
+    autograd, a backward pass is captured into a CUDA graph only while no graph recorded outside the capture holds the same leaves.
+    The table gets no gradient: one that requires it is refused."""
+    if _derived(rotary.table):
+        raise ValueError("the rotary table takes no gradient")
+    if _derived(x) or _transforming():
         if stream is not None or kw:
             raise ValueError("a rotation that records a gradient runs on the current stream and takes no out or status")
         return _Rotation.apply(x, rotary, positions, inverse)

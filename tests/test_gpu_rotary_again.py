@@ -82,3 +82,16 @@ def test_autograd_sees_what_is_written(cuda):
         z = before.clone()
         rotate(z, rot, at, out=z)
     same(z, turned(before, rot.table, [0] * 32, at, False))
+
+
+def test_learned_frequencies_are_refused(cuda):
+    from astc_kv_cuda import Rotary, rotate
+    f = torch.rand(32, device="cuda", requires_grad=True)
+    at = places_of(1, 2, 5, 30)
+    x = torch.randn(2, 5, 3, 64, device="cuda")
+    for z in (x, x.clone().requires_grad_()):
+        with pytest.raises(ValueError):
+            rotate(z, Rotary.make(64, 30, frequencies=f), at)
+        with torch.no_grad():
+            rot = Rotary.make(64, 30, frequencies=f)
+        same(rotate(z, rot, at).detach(), turned(x if z is x else z.detach(), rot.table, [0] * 32, at, False))

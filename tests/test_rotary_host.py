@@ -1,4 +1,6 @@
 """`rotate` and derivatives, without a GPU: a plain rotation stands in for the call, and the recording around it is checked."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -11,7 +13,7 @@ class Plain:
 
     def __init__(self, x, table, positions, *, inverse=False, out=None):
         x.data_ptr()  # as Rotate: memory, or an error
-        cs = table[positions.long()][:, :, None]
+        cs = table.table[positions.long()][:, :, None]
         c, s = cs[..., 0], cs[..., 1] * (-1 if inverse else 1)
         a, b = x.detach().chunk(2, -1)
         self.out = torch.cat([a * c - b * s, b * c + a * s], -1)
@@ -27,7 +29,7 @@ def given(monkeypatch):
     angle = torch.randn(9, 3, dtype=torch.float64, generator=g)
     table = torch.stack([angle.cos(), angle.sin()], -1) * 1.5
     x, v = torch.randn(2, 2, 4, 2, 6, dtype=torch.float64, generator=g)
-    return x, v, table, torch.randint(0, 9, (2, 4), generator=g)
+    return x, v, SimpleNamespace(table=table), torch.randint(0, 9, (2, 4), generator=g)
 
 
 def test_tangents_are_rotated(given):
@@ -61,3 +63,14 @@ def test_transforms(given):
     assert torch.allclose(torch.func.jvp(torch.func.grad(f), (x,), (v,))[1], h, rtol=1e-12)
     with pytest.raises(RuntimeError):
         torch.func.vmap(f)(x[None])
+
+
+def test_a_table_that_requires_a_gradient(given):
+    x, v, rot, at = given
+    learned = SimpleNamespace(table=rot.table.clone().requires_grad_())
+    with pytest.raises(ValueError):
+        rotary.rotate(x, learned, at)
+    with torch.no_grad():
+        assert torch.equal(rotary.rotate(x, learned, at), rotary.rotate(x, rot, at))
+    with forward_ad.dual_level(), pytest.raises(ValueError):
+        rotary.rotate(x, SimpleNamespace(table=forward_ad.make_dual(rot.table, rot.table)), at)
