@@ -125,12 +125,13 @@ __device__ __forceinline__ void lane_turns(const RotaryDev& r, const int32_t* pl
 // Scale of a group with the largest |x| `top` (a number).
 __device__ __forceinline__ __half group_scale(float top) { return __float2half_rn(fminf(__fmul_rn(top, 1.f / 6.f), kMostScale)); }
 
+// (0 with a scale of 0: a quotient keeps the sign of what it is of.)
 __device__ __forceinline__ uint32_t group_codes(const float (&x)[8], float scale) {
     const float inverse = inverse_of(scale);
     float y[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) y[k] = quotient(x[k], scale, inverse);
-    return to_codes(y);
+    return scale > 0.f ? to_codes(y) : 0u;
 }
 
 // grid.x: tokens of all sequences, so many rows of D / 8 lanes a CTA; grid.y:
@@ -311,7 +312,7 @@ __device__ __forceinline__ uint32_t chunk_codes(const uint64_t (&x)[4], float sc
         y[2 * k] = f.x;
         y[2 * k + 1] = f.y;
     }
-    return to_codes(y);
+    return scale > 0.f ? to_codes(y) : 0u;
 }
 
 // Grid as of append_kernel, with rows of D / 16 lanes. QUERIES: with parts for
