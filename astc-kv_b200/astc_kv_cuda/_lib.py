@@ -156,7 +156,7 @@ class AkvQ4RestoreDesc(ct.Structure):
 class AkvQ4AttnDesc(ct.Structure):
     _fields_ = [
         ("cache", AkvQ4Cache), ("q_heads", ct.c_int32), ("q_tokens", ct.c_int32), ("q_dtype", ct.c_int32), ("out_dtype", ct.c_int32),
-        ("causal", ct.c_int32), ("split_tokens", ct.c_int32), ("scale", ct.c_float), ("reserved0", ct.c_int32),
+        ("causal", ct.c_int32), ("split_tokens", ct.c_int32), ("scale", ct.c_float), ("wait_tries", ct.c_int32),
         ("q_dev", ct.c_void_p), ("q_stride", ct.c_int64 * 3), ("seq_lens_dev", ct.c_void_p), ("q_lens_dev", ct.c_void_p),
         ("out_dev", ct.c_void_p), ("lse_dev", ct.c_void_p), ("workspace_dev", ct.c_void_p), ("workspace_bytes", ct.c_size_t),
     ]

@@ -77,7 +77,7 @@ int check_attention(const AkvQ4AttnDesc* d) {
     if (int st = check_cache(d->cache)) return st;
     if (d->q_heads <= 0 || d->q_heads % d->cache.kv_heads || d->q_tokens < 0 || !valid_dtype(d->q_dtype) || !valid_dtype(d->out_dtype))
         return AKV_ERR_INVALID_ARGUMENT;
-    if (d->split_tokens < 0 || d->split_tokens % 16 || !(d->scale >= 0.f) || std::isinf(d->scale)) return AKV_ERR_INVALID_ARGUMENT;
+    if (d->split_tokens < 0 || d->split_tokens % 16 || d->wait_tries < 0 || !(d->scale >= 0.f) || std::isinf(d->scale)) return AKV_ERR_INVALID_ARGUMENT;
     if (!words({d->seq_lens_dev, d->q_lens_dev, d->lse_dev})) return AKV_ERR_INVALID_ARGUMENT;
     const int64_t rows = static_cast<int64_t>(d->q_heads) * d->q_tokens;
     if (rows > 1 << 24 || rows * d->cache.batch > 1 << 30) return AKV_ERR_UNSUPPORTED;
@@ -379,6 +379,7 @@ int akv_q4_attention(const AkvQ4AttnDesc* d, void* stream) {
     Q4Params pp = {};
     pp.c = to_dev(d->cache);
     pp.long_sums = plan.long_sums;
+    pp.wait_tries = d->wait_tries ? d->wait_tries : kWaitTries;
     q8::AttnParams& p = pp.a;
     p.c.B = pp.c.B; p.c.H = pp.c.H; p.c.D = pp.c.D; p.c.T = pp.c.T; p.c.status = pp.c.status;
     p.Hq = d->q_heads; p.G = d->q_heads / d->cache.kv_heads; p.n = d->q_tokens; p.R = plan.rows;

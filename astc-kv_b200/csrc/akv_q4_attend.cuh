@@ -13,6 +13,7 @@ struct Q4Params {
     q8::AttnParams a;   // of a.c only B, H, D, T and status are set
     CacheDev c;
     bool long_sums;     // of a CTA of the step kernel, see kStepLong
+    int wait_tries;     // of a wait in the tcgen05 kernel
 };
 
 // Tokens that a CTA of the step kernel with a 16-bit output may go through in one sum, or

@@ -87,10 +87,12 @@ using q8::tmem_st16;
 using q8::tmem_wait_ld;
 using q8::tmem_wait_st;
 
-// Waits, as a warp, for the phase of `parity` to end, a bounded number of times (a
-// try takes about 1.5 us, all some 6 s); false (and the CTA's abort flag) when
-// it does not, or when another warp gave up. Decided by votes, so that the
-// compiler knows that the warp stays together.
+// Tries of a wait: one takes about 4.5 us, all some 19 s.
+constexpr int kWaitTries = 1 << 22;
+
+// Waits, as a warp, for the phase of `parity` to end, at most `tries` times; false
+// (and the CTA's abort flag) when it does not, or when another warp gave up.
+// Decided by votes, so that the compiler knows that the warp stays together.
 __device__ __forceinline__ bool bar_try(uint64_t* bar, int parity) {
     uint32_t ok;
     asm volatile(
@@ -98,10 +100,10 @@ __device__ __forceinline__ bool bar_try(uint64_t* bar, int parity) {
         : "=r"(ok) : "r"(smem_addr(bar)), "r"(parity) : "memory");
     return __all_sync(0xFFFFFFFFu, ok);
 }
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, int parity, volatile int* abort) {
+__device__ __forceinline__ bool bar_wait(uint64_t* bar, int parity, volatile int* abort, int tries) {
     if (bar_try(bar, parity)) return true;
 #pragma unroll 1
-    for (int i = 0; i < 1 << 22; ++i) {
+    for (int i = 0; i < tries; ++i) {
         if (bar_try(bar, parity)) return true;
         if (__any_sync(0xFFFFFFFFu, *abort)) return false;
     }
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
             bar_init(&sm.pv_done[i], 1);
         }
         bar_init(&sm.q_full, 32 * SOFT);
-        bar_init(&sm.done, 1);
+        bar_init(&sm.done, 2);
         sm.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -396,7 +398,7 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
                 if (!placed) shift = 0.f;
                 if (phase > 0) {
                     // The last P V of the tile may still be running.
-                    alive = bar_wait(&sm.pv_done[tile], (phase - 1) & 1, &sm.abort);
+                    alive = bar_wait(&sm.pv_done[tile], (phase - 1) & 1, &sm.abort, pp.wait_tries);
                     if (!alive) break;
                     fence_after();
 #pragma unroll 1
@@ -414,7 +416,7 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
         };
         for (int turn = 0; turn < my_steps && alive; ++turn) {
             const int t0 = t_begin + (SHARED ? 2 * turn + tile : turn) * kChunkTokens;
-            alive = bar_wait(&sm.s_full[tile], turn & 1, &sm.abort);
+            alive = bar_wait(&sm.s_full[tile], turn & 1, &sm.abort, pp.wait_tries);
             if (!alive) break;
             fence_after();
             uint32_t x[32], y[32];
@@ -457,22 +459,25 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
             }
         }
         // ---------------------------------------------------------- write rows
-        alive = alive && bar_wait(&sm.done, 0, &sm.abort);
+        alive = alive && bar_wait(&sm.done, 0, &sm.abort, pp.wait_tries);
         fence_after();
-        if (!alive) l = CUDART_NAN_F;  // gave up: the rows become NaN
+        // `done` ends as well where the issuing warp gave up, some products short.
+        alive = alive && !__any_sync(0xFFFFFFFFu, *static_cast<volatile int*>(&sm.abort));
+        if (!alive) l = CUDART_NAN_F;  // the rows become NaN
         const bool none = alive && (blind || (!started && !isnan(l)));
         const float inv = p.nsplits > 1 ? 1.f : none ? 0.f : 1.f / l;
         const int64_t part = unit + (SHARED && tile ? p.R : 0);
         // A warp's rows go through its own part of the operands' room, which
-        // nothing reads any more once all products are done, so that they are
-        // written in one piece each. Pieces of 16 bytes lie crosswise.
+        // nothing uses any more once all products are done, so that they are
+        // written in one piece each. Pieces of 16 bytes lie crosswise. (After giving
+        // up a code warp may still store there.)
         constexpr int PER = DP / 4;  // pieces of a row
         float4* const room = reinterpret_cast<float4*>(&sm.q[0][0][0]) + static_cast<int64_t>(warp) * 32 * PER;
         const int there = min(rows - (my_row - lane), 32);  // the warp's rows
         const int64_t own = my_row < rows ? q8::out_row(p, b, h, r0 + my_row) : 0;
         if (there > 0) {
 #pragma unroll 1
-            for (int g = 0; g < DP / 16; ++g) {
+            for (int g = 0; g < (alive ? DP / 16 : 0); ++g) {
                 uint32_t o[16];
                 tmem_ld16(o, o_at + 16 * g);
                 tmem_wait_ld(o);
@@ -494,7 +499,7 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
                         const int at = 32 * (m + u) + lane, r = at / PER, k = at % PER;
-                        v[u] = room[r * PER + (k ^ (r & (PER - 1)))];
+                        v[u] = alive ? room[r * PER + (k ^ (r & (PER - 1)))] : make_float4(CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F, CUDART_NAN_F);
                     }
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
@@ -616,7 +621,7 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
             const int st = j % STAGES;
             if (does_k) {
                 // The phase before a stage's first use counts as over.
-                if (!bar_wait(&sm.k_empty[st], (j / STAGES & 1) ^ 1, &sm.abort)) break;
+                if (!bar_wait(&sm.k_empty[st], (j / STAGES & 1) ^ 1, &sm.abort, pp.wait_tries)) break;
 #pragma unroll
                 for (int i = 0; i < LANES; ++i)
 #pragma unroll
@@ -637,7 +642,7 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
                 load_k(t_begin + (j + 1) * kChunkTokens);
             }
             if (does_v) {
-                if (!bar_wait(&sm.v_empty[st], (j / STAGES & 1) ^ 1, &sm.abort)) break;
+                if (!bar_wait(&sm.v_empty[st], (j / STAGES & 1) ^ 1, &sm.abort, pp.wait_tries)) break;
                 uint8_t* tile_v = sm.v[st][w & 1];
 #pragma unroll
                 for (int x = 0; x < VW; ++x)
@@ -688,13 +693,13 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
             }
         };
         const int tiles_here = two ? 2 : 1;
-        bool alive = bar_wait(&sm.q_full, 0, &sm.abort);
+        bool alive = bar_wait(&sm.q_full, 0, &sm.abort, pp.wait_tries);
         // A tile's first scores; with both tiles on the same rows, the
         // second tile's are those of step 1.
         for (int tile = 0; tile < tiles_here && alive; ++tile) {
             const int st = SHARED ? tile : 0;
             if (SHARED && tile >= steps) break;
-            alive = bar_wait(&sm.k_full[st], 0, &sm.abort);
+            alive = bar_wait(&sm.k_full[st], 0, &sm.abort, pp.wait_tries);
             if (!alive) break;
             fence_after();
             scores(tile, st);
@@ -704,19 +709,19 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
             // The step after this one of the same tiles.
             const int st = j % STAGES, next = SHARED ? j + 2 : j + 1, nx = next % STAGES, turn = SHARED ? j >> 1 : j;
             const bool more = next < steps;
-            alive = bar_wait(&sm.v_full[st], j / STAGES & 1, &sm.abort);
-            if (more && !SHARED) alive = bar_wait(&sm.k_full[nx], next / STAGES & 1, &sm.abort) && alive;
+            alive = bar_wait(&sm.v_full[st], j / STAGES & 1, &sm.abort, pp.wait_tries);
+            if (more && !SHARED) alive = bar_wait(&sm.k_full[nx], next / STAGES & 1, &sm.abort, pp.wait_tries) && alive;
             const int i_end = SHARED ? 2 * st + 2 : 2 * tiles_here;
             for (int i = SHARED ? 2 * st : 0; i < i_end; ++i) {
                 const int tile = i >> 1, half = i & 1;
-                alive = alive && bar_wait(&sm.p_full[i >> 1][i & 1], turn & 1, &sm.abort);
+                alive = alive && bar_wait(&sm.p_full[i >> 1][i & 1], turn & 1, &sm.abort, pp.wait_tries);
                 if (!alive) break;
                 fence_after();
                 values(tile, half, st, turn > 0 || half > 0);
                 if (lead && i == i_end - 1) mma_commit(&sm.v_empty[st]);
                 if (!more || half == 0) continue;
                 if (SHARED) {
-                    alive = bar_wait(&sm.k_full[nx], next / STAGES & 1, &sm.abort);
+                    alive = bar_wait(&sm.k_full[nx], next / STAGES & 1, &sm.abort, pp.wait_tries);
                     if (!alive) break;
                     fence_after();
                 }
@@ -726,9 +731,12 @@ __global__ void __launch_bounds__(kChunkThreads<DP, SHARED>, 1) chunk_kernel(Q4P
         }
         // Also after giving up: nothing may be in flight when the tensor
         // memory is given back.
-        if (lead) mma_commit(&sm.done);
+        if (lead) {
+            mma_commit(&sm.done);
+            bar_arrive(&sm.done);  // hands on whether the flag is set
+        }
         int none = 0;
-        bar_wait(&sm.done, 0, &none);
+        bar_wait(&sm.done, 0, &none, kWaitTries);
         __syncwarp();
     }
     fence_before();

@@ -145,7 +145,8 @@ typedef struct AkvQ4AttnDesc {
     int32_t split_tokens;           /* tokens per split at least (many rows and a 16-bit output: up to what a sum may
                                        hold, see above), a multiple of 16; 0 = library choice */
     float scale;                    /* 0 = head_dim^-0.5 */
-    int32_t reserved0;
+    int32_t wait_tries;             /* tries, of about 4.5 us, of a wait inside a kernel before it gives up (status_dev);
+                                       0 = library choice, some 19 s */
     const void* q_dev;              /* element strides batch / token / head */
     int64_t q_stride[3];
     const int32_t* seq_lens_dev;    /* [batch] or NULL (= max_tokens) */
