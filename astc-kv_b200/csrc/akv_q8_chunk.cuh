@@ -89,7 +89,7 @@ __device__ __forceinline__ void bar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_addr(bar)) : "memory");
 }
 // Waits for the phase of `parity` to end, a bounded number of times (a try takes
-// about 1.5 us, all some 6 s); false (and the CTA's abort flag) when it does
+// about 4.5 us, all some 19 s); false (and the CTA's abort flag) when it does
 // not, or when another warp gave up.
 __device__ __forceinline__ bool bar_wait(uint64_t* bar, int parity, volatile int* abort) {
     for (int i = 0; i < 1 << 22; ++i) {
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kChunkThreads<DP>, 1) chunk_kernel(AttnParams 
             bar_init(&sm.p_full[i][0], 128);
             bar_init(&sm.p_full[i][1], 128);
         }
-        bar_init(&sm.done, 1);
+        bar_init(&sm.done, 2);
         sm.abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -426,11 +426,13 @@ __global__ void __launch_bounds__(kChunkThreads<DP>, 1) chunk_kernel(AttnParams 
         // ---------------------------------------------------------- write rows
         alive = __all_sync(0xFFFFFFFFu, alive && bar_wait(&sm.done, 0, &sm.abort));
         fence_after();
+        // `done` ends as well where the issuing warp gave up, some products short.
+        alive = alive && !__any_sync(0xFFFFFFFFu, *static_cast<volatile int*>(&sm.abort));
         const int my_row = SHARED ? threadIdx.x & 127 : threadIdx.x;
         const bool in = my_row < rows;
         const int r = r0 + my_row;
         const int64_t part = unit + my_row + (SHARED && tile ? p.R : 0);
-        if (!alive) l = CUDART_NAN_F;  // gave up: the rows become NaN
+        if (!alive) l = CUDART_NAN_F;  // the rows become NaN
         const bool none = alive && (blind || (!started && !isnan(l)));
         const float inv = none ? 0.f : 1.f / l;
         const int64_t row = in ? out_row(p, b, h, r) : 0;
@@ -679,7 +681,10 @@ __global__ void __launch_bounds__(kChunkThreads<DP>, 1) chunk_kernel(AttnParams 
             }
             // Also after giving up: nothing may be in flight when the tensor
             // memory is given back.
-            if (lead) mma_commit(&sm.done);
+            if (lead) {
+                mma_commit(&sm.done);
+                bar_arrive(&sm.done);  // hands on whether the flag is set
+            }
             int none = 0;
             bar_wait(&sm.done, 0, &none);
         }
