@@ -121,13 +121,13 @@ struct AttnPlan {
 // against 17: short of 33 rows neither is far ahead up to D 128.)
 int chunk_min_rows(int head_dim) { return head_dim <= 128 ? 33 : 17; }
 
-// Tokens that a tile of the tcgen05 kernel adds up at most where outputs are
-// fp16. The tensor cores truncate as they add: a sum over n tokens comes out
-// 6e-9 n too small (measured: 3e-5 at 8192, 8e-4 at 131072 tokens), which fp16
-// outputs, 2.4e-4 off by their rounding on the average, would show. A second
-// partial costs about 2.5 of this split's 128 steps. (bf16 outputs are eight
-// times coarser.)
-constexpr int64_t kChunkHalfTokens = 16384;
+// Tokens that a tile of the tcgen05 kernel adds up at most, also where a caller
+// asks for longer splits. The tensor cores truncate as they add: a sum over n tokens comes out
+// 6e-9 n too small (measured: 3e-5 at 8192, 8e-4 at 131072, 6.7e-3 at a million tokens), which fp16
+// outputs, 2.4e-4 off by their rounding on the average, would show, and bf16
+// ones, which are eight times coarser, later. A second
+// partial costs about 2.5 of this split's 128 steps.
+constexpr int64_t kChunkHalfTokens = 16384, kChunkBf16Tokens = 131072;
 
 // Tokens for each CTA of a cluster up to which a cluster for each kv head of
 // each sequence beats even shares of all CTAs and a second launch (32/8 heads:
@@ -155,6 +155,8 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
     a.split = d->split_tokens;
     const bool shared = a.chunk && a.rows <= 128 && c.head_dim <= 128;  // its two tiles share the rows and take every other step
     const int group = a.chunk ? (c.head_dim <= 128 ? 256 : 128) : 8 * a.nt;  // rows of a CTA
+    // (Two tiles that take every other step share a split.)
+    const int64_t longest = (d->out_dtype == AKV_Q_F16 ? kChunkHalfTokens : kChunkBf16Tokens) * (shared ? 2 : 1);
     if (a.split == 0 && a.chunk) {
         // One CTA per SM. In steps of 128 tokens a CTA costs its share of the
         // tokens, about three to start and, when split, 2.5 (D 128) for a
@@ -181,14 +183,13 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
         for (int64_t n = 2; n <= most && n <= steps; ++n)
             if (cost(n) <= limit) best = n;
         if (cost(1) <= least) best = best > 1 && limit > least ? best : 1;
-        if (d->out_dtype == AKV_Q_F16) {
-            const int64_t longest = kChunkHalfTokens / kChunkTokens * (shared ? 2 : 1), n = (steps + longest - 1) / longest;
-            best = best > n ? best : n;
-        }
+        const int64_t n = (steps * kChunkTokens + longest - 1) / longest;
+        best = best > n ? best : n;
         a.split = static_cast<int>((steps + best - 1) / best * kChunkTokens);
     }
     size_t parts;  // rows of partials
     if (a.chunk) {
+        if (a.split > longest) a.split = static_cast<int>(longest);
         // Whole steps: a step's tokens past the split's end would count as seen.
         a.split = static_cast<int>((static_cast<int64_t>(a.split < c.max_tokens ? a.split : c.max_tokens) + kChunkTokens - 1) / kChunkTokens * kChunkTokens);
         a.nsplits = static_cast<int>((static_cast<int64_t>(c.max_tokens) + a.split - 1) / a.split);

@@ -121,6 +121,8 @@ int akv_q8_restore(const AkvQ8RestoreDesc* desc, void* stream);
  * every 32 products; with a 16-bit output the weights are rounded to fp16,
  * and from 33 rows (queries x heads of a kv head; 17 above head_dim 128)
  * the values' sum comes out 6e-9 of itself per token of a split too small.
+ * Splits there are of 16384 tokens at most with an fp16 output and of 131072
+ * with a bf16 one (of twice as many up to 128 rows and head_dim 128, as two sums).
  *
  * Lengths are read by the kernels, so what the host decides, the splits of many
  * rows and the size of the workspace, goes by max_tokens: a cache with much
@@ -133,7 +135,8 @@ typedef struct AkvQ8AttnDesc {
     int32_t q_heads, q_tokens;
     int32_t q_dtype, out_dtype;     /* AKV_Q_* */
     int32_t causal, accumulate;
-    int32_t split_tokens;           /* tokens per split at least, a multiple of 16; 0 = library choice */
+    int32_t split_tokens;           /* tokens per split at least (many rows and a 16-bit output: up to what a sum may
+                                       hold, see above), a multiple of 16; 0 = library choice */
     float scale;                    /* 0 = head_dim^-0.5 */
     const void* q_dev;              /* element strides batch / token / head */
     int64_t q_stride[3];
