@@ -103,7 +103,7 @@ struct AttnPlan {
     int nt;           // groups of eight rows per CTA
     int split, nsplits;          // chunk kernel
     int share_ctas, share_min;   // step kernel
-    bool long_sums;              // see kStepLong
+    bool long_sums;              // see q8::kStepLong
     size_t part_ml, part_o, bytes;  // offsets into the workspace, and its size
 };
 
@@ -192,11 +192,7 @@ AttnPlan plan_attention(const AkvQ4AttnDesc* d) {
         a.share_min = a.split > q8::kShareTokens ? a.split / q8::kShareTokens : 1;
         const int64_t ctas = chunks / a.share_min < slots ? chunks / a.share_min : slots;
         a.share_ctas = static_cast<int>(ctas > 0 ? ctas : 1);
-        // The chunks of a CTA at most: fewer CTAs share shorter lengths, of at least share_min chunks each.
-        int64_t share = (chunks + a.share_ctas - 1) / a.share_ctas;
-        if (a.share_min > 1 && share < 2 * static_cast<int64_t>(a.share_min)) share = 2 * static_cast<int64_t>(a.share_min);
-        const int64_t tokens = share * q8::kShareTokens;
-        a.long_sums = (tokens < c.max_tokens ? tokens : c.max_tokens) > (d->out_dtype == AKV_Q_F16 ? kStepLong : kStepLongBf16);
+        a.long_sums = q8::step_sums_long(chunks, a.share_ctas, a.share_min, c.max_tokens, d->out_dtype);
         parts = 2 * static_cast<size_t>(a.share_ctas) * group;
         // The largest cluster with which all units fit the GPU at once.
         int size = q8::kStepCluster;
@@ -378,7 +374,6 @@ int akv_q4_attention(const AkvQ4AttnDesc* d, void* stream) {
     char* ws = static_cast<char*>(d->workspace_dev);
     Q4Params pp = {};
     pp.c = to_dev(d->cache);
-    pp.long_sums = plan.long_sums;
     pp.wait_tries = d->wait_tries ? d->wait_tries : kWaitTries;
     q8::AttnParams& p = pp.a;
     p.c.B = pp.c.B; p.c.H = pp.c.H; p.c.D = pp.c.D; p.c.T = pp.c.T; p.c.status = pp.c.status;
@@ -391,6 +386,7 @@ int akv_q4_attention(const AkvQ4AttnDesc* d, void* stream) {
     p.lens = d->seq_lens_dev; p.q_lens = d->q_lens_dev;
     p.split = plan.split; p.nsplits = plan.nsplits;
     p.share_ctas = plan.chunk ? 0 : plan.cluster ? -plan.cluster : plan.share_ctas; p.share_min = plan.share_min; p.row_group = 8 * plan.nt;
+    p.long_sums = plan.long_sums;
     p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
     p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     p.out = d->out_dev; p.lse_out = d->lse_dev;

@@ -73,7 +73,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     constexpr int TURN = 16 * kStepWarps;       // tokens from a tile to the warp's next
     constexpr bool SECOND = PLO && !TWIN;       // P's second part in products of its own
     // Tokens after which O goes to its sum in shared memory (FOLDS), which is rounded to nearest.
-    constexpr int FOLD = !PLO ? kStepLong : SECOND ? 1024 : 2048;
+    constexpr int FOLD = !PLO ? q8::kStepLong : SECOND ? 1024 : 2048;
     __shared__ __align__(16) float red[kStepWarps][ROWS][DP];
     __shared__ float2 ml[kStepWarps][ROWS];
     __shared__ float row_scale[ROWS];

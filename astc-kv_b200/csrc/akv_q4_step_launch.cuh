@@ -25,7 +25,7 @@ int launch(const Q4Params& p, cudaStream_t s) {
         }
     }
     if constexpr (!PLO) {
-        if (p.long_sums) {
+        if (p.a.long_sums) {
             step_kernel<DP, NT, PLO, QLO, TWIN, false, DENSE, true><<<p.a.share_ctas, kStepThreads, 0, s>>>(p);
             return q8::launched();
         }

@@ -107,6 +107,7 @@ struct AttnPlan {
     int nt;           // groups of eight rows per CTA
     int split, nsplits;          // chunk kernel
     int share_ctas, share_min;   // step kernel
+    bool long_sums;              // see kStepLong
     bool keep_scores; // the step kernel stores its scores for the token weights
     size_t part_ml, part_o, scores, lse, q_rows, q_factors, bytes;  // offsets into the workspace, and its size
 };
@@ -209,6 +210,7 @@ AttnPlan plan_attention(const AkvQ8AttnDesc* d) {
         const int64_t ctas = chunks / a.share_min < slots ? chunks / a.share_min : slots;
         a.share_ctas = static_cast<int>(ctas > 0 ? ctas : 1);
         a.nsplits = 0;
+        a.long_sums = step_sums_long(chunks, a.share_ctas, a.share_min, c.max_tokens, d->out_dtype);
         parts = 2 * static_cast<size_t>(a.share_ctas) * group;
         // The largest cluster with which all units fit the GPU at once.
         int size = kStepCluster;
@@ -383,6 +385,7 @@ int akv_q8_attention(const AkvQ8AttnDesc* d, void* stream) {
     p.lens = d->seq_lens_dev; p.q_lens = d->q_lens_dev;
     p.split = plan.split; p.nsplits = plan.nsplits;
     p.share_ctas = plan.chunk ? 0 : plan.cluster ? -plan.cluster : plan.share_ctas; p.share_min = plan.share_min; p.row_group = 8 * plan.nt;
+    p.long_sums = plan.long_sums;
     p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
     p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     p.scores = plan.keep_scores ? reinterpret_cast<float*>(ws + plan.scores) : nullptr;

@@ -27,6 +27,7 @@ struct AttnParams {
     int share_ctas;             // CTAs of the step kernel, 0 for the chunk kernel, minus the size of its clusters
     int share_min;              // chunks that a share has at least
     int row_group;
+    bool long_sums;             // of a CTA of the step kernel with a 16-bit output, see kStepLong
     float* part_o;              // ... [D], weighted by 2^-base
     float2* part_ml;            // base (-inf: nothing seen), sum
     uint2* q_rows;              // query rows as fragments for the weights kernel, see pack_rows
@@ -217,6 +218,23 @@ struct Shares {
 __device__ __forceinline__ Shares make_shares(const AttnParams& p, int64_t chunks) {
     const int64_t most = p.share_min == 1 ? chunks : chunks / p.share_min;
     return {chunks, static_cast<int>(max(static_cast<int64_t>(1), min(most, static_cast<int64_t>(p.share_ctas))))};
+}
+
+// Tokens that a CTA of the step kernels with a 16-bit output may go through in one sum, or
+// puts its sum by after: the tensor cores truncate as they add, so a sum over n tokens
+// comes out about 6e-9 n too small, which an output's rounding (2^-11, fp16; 2^-8,
+// bf16) has to cover. Of these tokens a warp adds up a quarter. (With every sum put
+// by after 16384 tokens 32 sequences of 32768, 4-bit cache, 32/8 heads of 128 channels, bf16,
+// took 242 us where they take 232, although none of their sums is that long.)
+constexpr int kStepLong = 65536, kStepLongBf16 = 8 * kStepLong;
+
+// Whether a CTA may go through more, of `chunks` at most that `ctas` share.
+inline bool step_sums_long(int64_t chunks, int ctas, int share_min, int max_tokens, int out_dtype) {
+    // Fewer CTAs share shorter lengths, of at least share_min chunks each.
+    int64_t share = (chunks + ctas - 1) / ctas;
+    if (share_min > 1 && share < 2 * static_cast<int64_t>(share_min)) share = 2 * static_cast<int64_t>(share_min);
+    const int64_t tokens = share * kShareTokens;
+    return (tokens < max_tokens ? tokens : max_tokens) > (out_dtype == AKV_Q_F16 ? kStepLong : kStepLongBf16);
 }
 
 struct ShareScratch {

@@ -86,8 +86,9 @@ __device__ __forceinline__ float4 load_remote4(const void* p, int rank) {
 // launch would cost more than an even division saves (B1, 384 tokens, 9/3
 // heads: 8.2 us against 12.3; B8, 1024 tokens, 32/8 heads: 15.7 against 24.8).
 // DP: head_dim rounded up to 64, 128 or 256; NT: groups of 8 rows; PLO: P in
-// two parts; QLO: queries in two parts.
-template <int FMT, int DP, int NT, bool PLO, bool QLO, bool TWIN, bool CLUSTER>
+// two parts; QLO: queries in two parts. FOLDS: sums are put by, as with P in two
+// parts, or where a CTA may go through too many tokens.
+template <int FMT, int DP, int NT, bool PLO, bool QLO, bool TWIN, bool CLUSTER, bool FOLDS>
 __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) step_kernel(AttnParams p) {
     constexpr int KS = DP / 16;       // k-steps of S, d-tiles of O
     constexpr int VW = DP / 32;       // words of a V row per lane
@@ -99,13 +100,15 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     __shared__ uint2 qs[KS][NT][QLO ? 2 : 1][32];
 
     __shared__ ShareScratch scratch;
-    __shared__ float carry[PLO ? 2 * NT : 1][kStepThreads];
+    __shared__ float carry[FOLDS ? 2 * NT : 1][kStepThreads];
 
     const CacheDev& c = p.c;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, cc = lane & 3;
     static_assert(!TWIN || (PLO && NT == 1), "twin rows carry P's second part");
     constexpr bool SECOND = PLO && !TWIN;  // P's second part in products of its own
-    constexpr int FOLD = SECOND ? 1024 : 2048;  // tokens after which O goes to its sum in shared memory (fp32 outputs)
+    static_assert(FOLDS || !PLO, "short sums are part of P's second part");
+    // Tokens after which O goes to its sum in shared memory (FOLDS), which is rounded to nearest.
+    constexpr int FOLD = !PLO ? kStepLong : SECOND ? 1024 : 2048;
     const int groups = (p.R + ROWS - 1) / ROWS, units = c.H * groups;  // of a sequence
     int64_t at = 0, stop = 1;  // the next chunk of this CTA's share, its end
     int b, unit_of_b, chunk;
@@ -313,7 +316,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
 #pragma unroll
         for (int i = 0; i < KS; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) { base[nt][k] = 0.f; limit[nt][k] = -CUDART_INF_F; l[nt][k] = 0.f; if (PLO) carry[2 * nt + k][threadIdx.x] = 1.f; }
+        for (int k = 0; k < 2; ++k) { base[nt][k] = 0.f; limit[nt][k] = -CUDART_INF_F; l[nt][k] = 0.f; if (FOLDS) carry[2 * nt + k][threadIdx.x] = 1.f; }
     }
 
     auto tile = [&](int t0, const uint32_t (&vr)[4][VW], float vscale, uint32_t (&v_next)[4][VW], float& vscale_next) {
@@ -394,7 +397,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
                     base[nt][k] = to;
                     limit[nt][k] = up ? __fadd_rd(to, 15.5f) : limit[nt][k];
                     l[nt][k] *= alpha;
-                    if (PLO) carry[2 * nt + k][threadIdx.x] *= alpha;
+                    if (FOLDS) carry[2 * nt + k][threadIdx.x] *= alpha;
 #pragma unroll
                     for (int i = 0; i < KS; ++i) {
                         o[i][nt][k] *= alpha;
@@ -443,7 +446,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
     for (int t0 = t_begin + 16 * warp; t0 < t_end; t0 += 32 * kStepWarps) {
         tile(t0, va, vscale_a, vb, vscale_b);
         if (t0 + 16 * kStepWarps < t_end) tile(t0 + 16 * kStepWarps, vb, vscale_b, va, vscale_a);
-        if (PLO && t0 % FOLD >= FOLD - 32 * kStepWarps) {
+        if (FOLDS && t0 % FOLD >= FOLD - 32 * kStepWarps) {
             const bool first = t0 - t_begin < FOLD;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -463,7 +466,7 @@ __global__ void __launch_bounds__(kStepThreads, DP == 256 || NT == 2 ? 2 : 4) st
 
     allow_next_kernel();
     const int begun = t_begin + 16 * warp;
-    if (PLO && begun + (FOLD - 1 - begun % FOLD) / (32 * kStepWarps) * (32 * kStepWarps) < t_end) {  // there is a sum
+    if (FOLDS && begun + (FOLD - 1 - begun % FOLD) / (32 * kStepWarps) * (32 * kStepWarps) < t_end) {  // there is a sum
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const float f0 = carry[2 * nt][threadIdx.x], f1 = carry[2 * nt + 1][threadIdx.x];

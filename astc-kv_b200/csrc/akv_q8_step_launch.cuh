@@ -20,11 +20,17 @@ int launch_step(const AttnParams& p, cudaStream_t s) {
             cfg.stream = s;
             cfg.attrs = &attr;
             cfg.numAttrs = 1;
-            return cudaLaunchKernelEx(&cfg, step_kernel<FMT, DP, 1, PLO, QLO, TWIN, true>, p) == cudaSuccess
+            return cudaLaunchKernelEx(&cfg, step_kernel<FMT, DP, 1, PLO, QLO, TWIN, true, PLO>, p) == cudaSuccess
                        ? AKV_OK : (cudaGetLastError(), AKV_ERR_CUDA);
         }
     }
-    step_kernel<FMT, DP, NT, PLO, QLO, TWIN, false><<<p.share_ctas, kStepThreads, 0, s>>>(p);
+    if constexpr (!PLO) {
+        if (p.long_sums) {
+            step_kernel<FMT, DP, NT, PLO, QLO, TWIN, false, true><<<p.share_ctas, kStepThreads, 0, s>>>(p);
+            return launched();
+        }
+    }
+    step_kernel<FMT, DP, NT, PLO, QLO, TWIN, false, PLO><<<p.share_ctas, kStepThreads, 0, s>>>(p);
     return launched();
 }
 

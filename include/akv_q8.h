@@ -118,11 +118,10 @@ int akv_q8_restore(const AkvQ8RestoreDesc* desc, void* stream);
  * which truncate, of exact products (of 22 bits with fp32 queries): off by at
  * most 2^-20 of the sum of |scale q K|. With an fp32 output the softmax weights
  * meet V in two fp16 parts (22 bits) and long sums are rounded to nearest
- * every 32 products; with a 16-bit output the weights are rounded to fp16,
- * and from 33 rows (queries x heads of a kv head; 17 above head_dim 128)
- * the values' sum comes out 6e-9 of itself per token of a split too small.
- * Splits there are of 16384 tokens at most with an fp16 output and of 131072
- * with a bf16 one (of twice as many up to 128 rows and head_dim 128, as two sums).
+ * every 32 products; with a 16-bit output the weights are rounded to fp16, and
+ * the values' sum loses about 6e-9 of itself per token that the tensor cores
+ * add up, never more than 16384 tokens with an fp16 output and 131072 with a
+ * bf16 one; such sums are added in fp32.
  *
  * Lengths are read by the kernels, so what the host decides, the splits of many
  * rows and the size of the workspace, goes by max_tokens: a cache with much

@@ -41,3 +41,13 @@ def test_many_rows_of_16_bits(cuda, D, n, od, T, split, fmt):
     most = 16384 if od == torch.float16 else 131072
     off = lost(148 if n <= 128 else 74, 256 // D, T, D, n, od, split, fmt)
     assert (off.abs() <= most * 2.0 ** -27 + NOISE[od] + WEIGHTS).all(), float(off.abs().max())
+
+
+@pytest.mark.parametrize("fmt", ["int8", "fp8"])
+@pytest.mark.parametrize("od", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("D,n", [(64, 1), (64, 16), (128, 1), (128, 9), (256, 1)])
+def test_few_rows_of_16_bits(cuda, D, n, od, fmt):
+    """As many sequences as there are CTAs, so that each goes through all tokens of one, four warps each."""
+    most = 16384 if od == torch.float16 else 131072
+    off = lost(148 * 4 * D // 256 if n == 1 and D < 256 else 296 * D // 256, 256 // D, (1 << 20 if od == torch.float16 else 1 << 21), D, n, od, 0, fmt)
+    assert (off.abs() <= most * 2.0 ** -27 + NOISE[od] + WEIGHTS).all(), float(off.abs().max())
