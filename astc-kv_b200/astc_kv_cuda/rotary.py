@@ -92,6 +92,35 @@ class Rotary:
         return _int32("positions", positions, shape[1:] if positions.dim() == 2 and self.axis_count == 1 else shape)
 
 
+def _overlaps_itself(t: torch.Tensor) -> bool:
+    """Whether two elements of a tensor are at one place."""
+    if t.numel() == 0:
+        return False
+    dims = sorted([(s, n) for s, n in zip(t.stride(), t.shape) if n > 1], reverse=True)
+    extent = 1
+    for s, n in reversed(dims):  # nested, as most are?
+        if s < extent:
+            break
+        extent += s * (n - 1)
+    else:
+        return False
+
+    def meet(left: int, dims: list) -> bool:
+        # Is left = sum of s * i with -n < i < n?
+        if not dims:
+            return left == 0
+        (s, n), span = dims[0], sum(r * (m - 1) for r, m in dims[1:])
+        if abs(left) > span + s * (n - 1) or s == 0:
+            return left == 0
+        return any(meet(left - s * i, dims[1:]) for i in range(max(-(-(left - span) // s), 1 - n), min((left + span) // s, n - 1) + 1))
+
+    for k, (s, n) in enumerate(dims):
+        rest = dims[k + 1:]
+        if s == 0 or any(meet(s * i, rest) for i in range(1, min(n - 1, sum(r * (m - 1) for r, m in rest) // s) + 1)):
+            return True
+    return False
+
+
 class Rotate(_Call):
     """Rotate x [B, n, H, D] at `positions` int32 [B, n], or [axes, B, n] with
     several axes, read when the call runs. x may be a strided view, for example
@@ -131,8 +160,8 @@ class Rotate(_Call):
         same = d.x_dev == d.out_dev and all(a == b or s < 2 for a, b, s in zip(x.stride(), out.stride(), x.shape))
         if not same and _may_overlap(x, out):
             raise ValueError("out must be x or not overlap it")
-        if any(s == 0 and m > 1 for s, m in zip(out.stride(), out.shape)):
-            raise ValueError("out must not be a broadcast view")
+        if self._given and _overlaps_itself(out):
+            raise ValueError("out must not have two elements at one place")
         d.positions_dev = rotary._places(positions, B, n)
         d.status_dev = None if status is None else status.data_ptr()
         self.out = out

@@ -95,3 +95,16 @@ def test_learned_frequencies_are_refused(cuda):
         with torch.no_grad():
             rot = Rotary.make(64, 30, frequencies=f)
         same(rotate(z, rot, at).detach(), turned(x if z is x else z.detach(), rot.table, [0] * 32, at, False))
+
+
+def test_outputs_that_overlap_themselves_are_refused(cuda):
+    from astc_kv_cuda import Rotary, rotate
+    rot = Rotary.make(64, 30)
+    at = places_of(1, 2, 5, 30)
+    x = torch.randn(2, 5, 3, 64, device="cuda")
+    room = torch.zeros(4096, device="cuda")
+    for stride in ((960, 192, 32, 1), (960, 96, 64, 1), (64, 192, 64, 1), (0, 192, 64, 1)):
+        with pytest.raises(ValueError):
+            rotate(x, rot, at, out=room.as_strided(x.shape, stride))
+    for stride in ((960, 192, 64, 1), (192, 384, 64, 1), (64, 384, 128, 1)):
+        same(rotate(x, rot, at, out=room.as_strided(x.shape, stride)), turned(x, rot.table, [0] * 32, at, False))

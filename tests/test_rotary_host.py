@@ -74,3 +74,17 @@ def test_a_table_that_requires_a_gradient(given):
         assert torch.equal(rotary.rotate(x, learned, at), rotary.rotate(x, rot, at))
     with forward_ad.dual_level(), pytest.raises(ValueError):
         rotary.rotate(x, SimpleNamespace(table=forward_ad.make_dual(rot.table, rot.table)), at)
+
+
+@pytest.mark.parametrize("shape,stride,overlaps", [
+    ((2, 3, 4, 8), (96, 32, 8, 1), False), ((2, 3, 4, 8), (96, 32, 0, 1), True), ((2, 3, 1, 8), (96, 32, 0, 1), False), ((2, 3, 4, 8), (8, 16, 48, 1), False),
+    ((1, 3, 2, 32), (7, 64, 96, 1), False), ((1, 3, 2, 32), (7, 64, 80, 1), True), ((1, 9, 2, 32), (7, 16, 144, 1), True), ((2, 9, 2, 32), (1, 64, 1000, 2), False),
+    ((2, 9, 2, 32), (31, 64, 1000, 1), True), ((0, 3, 4, 8), (0, 0, 0, 1), False), ((2, 2, 2, 2), (4, 2, 3, 1), True), ((1, 1, 1, 1), (0, 0, 0, 0), False),
+    ((3, 100000, 64, 128), (819200000, 8192, 128, 1), False), ((3, 100000, 64, 128), (819199999, 8192, 128, 1), True),
+    ((3, 100000, 64, 128), (128, 24576, 384, 1), False)])
+def test_an_output_that_overlaps_itself(shape, stride, overlaps):
+    t = torch.empty(1, dtype=torch.bfloat16, device="meta").as_strided(shape, stride)
+    assert rotary._overlaps_itself(t) == overlaps
+    if t.numel() < 10000:
+        places = sum(torch.arange(n).mul(s).view([-1 if i == k else 1 for i in range(4)]) for k, (n, s) in enumerate(zip(shape, stride)))
+        assert (places.unique().numel() < t.numel()) == overlaps
