@@ -234,12 +234,16 @@ class Q4Attention(_Call):
     sequence out of n (the rest of the output is zero). `causal`: query i sees
     tokens up to its own; otherwise every query sees the whole sequence.
     `out_dtype` fp32 (default) or a 16-bit type, which also lets the softmax
-    weights meet V as fp16. `lse=True` keeps ln sum exp of the scores in
+    weights meet V as fp16. Prompts want a 16-bit one: many rows (queries x
+    heads of a kv head) of 16-bit queries and outputs go to another kernel, which
+    takes 0.95 ms for 2048 tokens of 32768 (32/8 heads of 128 channels) where fp32
+    outputs take 6.3. `lse=True` keeps ln sum exp of the scores in
     `self.lse` [B, n, Hq].
 
     Splits and workspace go by the cache's max_tokens, not by the lengths:
     where a cache has much more room than tokens, a second Q4Cache over the
-    same tensors with a smaller `max_tokens` serves it faster.
+    same tensors with a smaller `max_tokens` serves it faster (256 query tokens
+    of 4096, 32/8 heads: room for 4096 39 us, for 131072 80).
     """
 
     _family, _fn = "q4_", "attention"

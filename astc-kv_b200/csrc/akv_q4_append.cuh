@@ -6,16 +6,18 @@
 //
 // append_kernel: a lane holds eight consecutive channels of a token's head: 16
 // bytes of 16-bit rows in, one word of codes out, and four lanes share a scale. The
-// other half of its rotated pairs is loaded a second time by this lane, which
-// finds it in L1 (rows meet no barrier and no shared memory). A lane keeps its
+// other half of its rotated pairs is loaded a second time by this lane, with the
+// same loads, which ask L1 not to keep lines (rows meet no barrier and no shared memory). A lane keeps its
 // token's cosines and sines for all heads that it goes through.
 // append_pairs_kernel: both halves of eight pairs a lane, see there.
 //
 // Measured with 8 heads of 128 channels, bf16, rotated, 4 x 8192 tokens (134 MB
-// in, 38 MB out): pairs 41 us, 4.2 TB/s, 64 % of a copy's rate (issue, 47 % of the
-// cycles, and the wait for two heads' loads; 36 us without rotation); the
-// general kernel 66 interleaved and 70 with 96 channels. With 32 query heads 128.
-// One token of 64 sequences 3.4 us. Restore of the 4 x 8192 tokens 35 us, 4.9 TB/s.
+// in, 38 MB out): pairs 41 to 43 us, 4.2 TB/s, 64 % of a copy's rate, with no unit full
+// (issue 47 % of the cycles, DRAM 24 %, 20 % of the warps that an SM can hold; 36 us
+// without rotation); the general kernel 66 to 68 interleaved and 70 to 72 with 96 channels.
+// With 32 query heads 128 to 132.
+// One token of 64 sequences 3.4 us. Restore of the 4 x 8192 tokens 36 us, 4.8 TB/s (no unit
+// full: issue 64 %, DRAM 36 %).
 #pragma once
 #include "akv_q4_common.cuh"
 #include "akv_rotary.cuh"

@@ -24,10 +24,12 @@
 // Measured: 32 sequences of 32768 tokens, 32/8 heads, head_dim 128, 234 us in
 // short runs with bf16 out, 5.2 TB/s or 79 % of a copy's rate; 248 us with
 // fp32 out (sums rounded apart); 265 us at the power cap. One sequence of 384
-// tokens, 9/3 heads: 6 us on the device. What bounds the long ones is not memory
-// but the units that turn codes into operands: of 286 instructions a tile of 16
-// tokens 66 are conversions and 64 fp16 multiplications, both at half rate or
-// less (15 tiles of 2.3 KB a microsecond and SM). More loads in flight, Q kept in
+// tokens, 9/3 heads: 6 us on the device. In the long ones no unit is full: a tile of 16
+// tokens has 519 cycles of a quarter SM, in which 286 instructions issue
+// (56 %); 66 conversions at 3.6 cycles and 64 fp16 multiplications at 2.0 take 46 % and
+// 25 %, DRAM is busy 53 to 79 %. 16 ragged sequences of 283,000 tokens in all, in
+// pages of 256, fp32 out: 99 us; the same tokens in equal sequences of one piece 78
+// with fp16 out, of which ragged lengths add 12, pages 5 and fp32 sums 4 us. More loads in flight, Q kept in
 // registers, three or five CTAs an SM changed nothing; a place in the page found
 // by one comparison a tile, rows a known distance apart (DENSE) and masks only
 // at the ends took 260 us to 234.

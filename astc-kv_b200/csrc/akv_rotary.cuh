@@ -325,7 +325,7 @@ inline int rotate_width(const RotateParams& p, bool interleaved, int64_t elem) {
 // Threads that share a token's heads. Eight heads a thread (4 x 8191 tokens, 40
 // heads, D 128, bf16: 109 us, with four 121, with twenty 111), twenty where
 // positions have several axes and a thread takes longer to begin (113 us against
-// 118), fewer where that leaves SMs with few threads (2 x 4097 tokens, 16 heads, D 72:
+// 118; both with 40 heads, no other number was measured), fewer where that leaves SMs with few threads (2 x 4097 tokens, 16 heads, D 72:
 // 10.3 us, with 2048 threads an SM asked for 12.4). 0 where the grid would be too large.
 inline int rotate_splits(const RotateParams& p, int N) {
     const int64_t units = static_cast<int64_t>(p.B) * p.n * ((p.D + 2 * N - 1) / (2 * N)), few = 148 * 640;
