@@ -72,3 +72,44 @@ def test_splits_stay_what_was_asked_for_where_sums_are_short(cuda):
     q = torch.randn(1, 300, 4, 64, device="cuda").half()
     size = {s: Q4Attention(q, cache, out_dtype=torch.bfloat16, split_tokens=s).workspace.numel() for s in (32768, 65536, 131072, 262144)}
     assert size[32768] > size[65536] > size[131072] == size[262144]
+
+
+def two_pages(B, T, D, H, kinds, weight):
+    """Order of the pages [T / P], 0 and 1, and q [B, 1, H, D], alike in all channels: keys of the first page are 0, of the second 1 in
+    every channel, which then weighs exp(q D / sqrt(D)) times as much, 150 to 3000."""
+    n = T // P
+    order = torch.zeros(n, dtype=torch.long, device="cuda")
+    order[kinds[0] * n // 16:kinds[1] * n // 16] = 1
+    a = torch.arange(40, 40 + B * H, device="cuda").remainder(24).add(40).view(B, 1, H, 1) / 64 * weight
+    return order, a.expand(B, 1, H, D).half().contiguous()
+
+
+def weighted(order, log_weight, means):
+    """Softmax means [B, 1, H, D] of two pages' means [2, H, D]."""
+    n1 = int(order.sum())
+    w = torch.exp(log_weight)[..., None] * n1
+    return (means[0] * (len(order) - n1) + means[1] * w) / (len(order) - n1 + w)
+
+
+@pytest.mark.parametrize("od,T", [(torch.float16, 1 << 17), (torch.bfloat16, 1 << 20)])
+@pytest.mark.parametrize("kinds", [(15, 16), (9, 10), (0, 1), (3, 14)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_largest_scores_anywhere_in_long_sums(cuda, D, kinds, od, T):
+    """Sums are put by under one base and joined under another. A weight is one of two numbers, rounded to fp16 (2^-11); sums lose 2^-27 a
+    token, and an output is rounded."""
+    from astc_kv_cuda import Q4Attention, Q4Cache
+    from test_gpu_q4 import HALF_ULP, values
+    H = 256 // D
+    B = 148 * (4 if D < 256 else 2) // H
+    g = torch.Generator(device="cuda").manual_seed(D)
+    c = torch.randint(1, 8, (2, 2, H, P, D // 2), generator=g, device="cuda", dtype=torch.uint8)
+    v, vs = c[0] | c[1] << 4, (1 + torch.rand(2, H, D // 32, P, generator=g, device="cuda")).half()
+    k = torch.zeros(2, H, P, D // 2, dtype=torch.uint8, device="cuda")
+    k[1] = 0x22
+    order, q = two_pages(B, T, D, H, kinds, (64 / D) ** 0.5)
+    cache = Q4Cache(k, v, torch.ones_like(vs), vs, block_table=order.to(torch.int32).expand(B, -1).contiguous())
+    log_weight = q[..., 0].double() * D ** 0.5
+    out = Q4Attention(q, cache, out_dtype=od, causal=False).run().double()
+    want = weighted(order, log_weight, values(v, vs).mean(2))
+    most = 16384 if od == torch.float16 else 131072
+    assert ((out / want - 1).abs() <= 2.0 ** -11 + 2.0 ** -18 + most * 2.0 ** -27 + HALF_ULP[od]).all(), float((out / want - 1).abs().max())

@@ -51,3 +51,26 @@ def test_few_rows_of_16_bits(cuda, D, n, od, fmt):
     most = 16384 if od == torch.float16 else 131072
     off = lost(148 * 4 * D // 256 if n == 1 and D < 256 else 296 * D // 256, 256 // D, (1 << 20 if od == torch.float16 else 1 << 21), D, n, od, 0, fmt)
     assert (off.abs() <= most * 2.0 ** -27 + NOISE[od] + WEIGHTS).all(), float(off.abs().max())
+
+
+@pytest.mark.parametrize("od,T", [(torch.float16, 1 << 17), (torch.bfloat16, 1 << 20)])
+@pytest.mark.parametrize("kinds", [(15, 16), (9, 10), (0, 1), (3, 14)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_largest_scores_anywhere_in_long_sums(cuda, D, kinds, od, T):
+    """As with 4 bits; the power of two that a weight is rounded with holds V's scale, here one number."""
+    from astc_kv_cuda import Q8Attention, Q8Cache
+    from test_gpu_q4 import HALF_ULP
+    from test_gpu_q4_long import two_pages, weighted
+    H = 256 // D
+    B = 148 * (4 if D < 256 else 2) // H
+    g = torch.Generator(device="cuda").manual_seed(D)
+    v = torch.randint(32, 120, (2, H, P, D), generator=g, device="cuda").to(torch.int8)
+    k = torch.zeros_like(v)
+    k[1] = 64
+    scales = torch.full((2, H, P // 64), 1 / 64, device="cuda")
+    order, q = two_pages(B, T, D, H, kinds, (64 / D) ** 0.5)
+    cache = Q8Cache(k, v, scales, torch.ones_like(scales), block_table=order.to(torch.int32).expand(B, -1).contiguous())
+    out = Q8Attention(q, cache, out_dtype=od, causal=False).run().double()
+    want = weighted(order, q[..., 0].double() * D ** 0.5, v.double().mean(2))
+    most = 16384 if od == torch.float16 else 131072
+    assert ((out / want - 1).abs() <= 2.0 ** -11 + 2.0 ** -18 + most * 2.0 ** -27 + HALF_ULP[od]).all(), float((out / want - 1).abs().max())
