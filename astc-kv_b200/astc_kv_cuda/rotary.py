@@ -169,8 +169,8 @@ class Rotate(_Call):
 
     def run(self, stream: torch.cuda.Stream | None = None) -> torch.Tensor:
         if self._given:
-            if self.out.requires_grad and torch.is_grad_enabled():
-                raise ValueError("a rotation into a given tensor records no gradient, which this one requires")
+            if _derived(self.out):
+                raise ValueError("a rotation into a given tensor records no gradient or tangent, which this one has")
             increment_version(self.out)
         self._issue(stream)
         return self.out
@@ -219,7 +219,7 @@ def rotate(x: torch.Tensor, rotary: Rotary, positions: torch.Tensor, *, inverse:
     The table gets no gradient: one that requires it is refused."""
     if _derived(rotary.table):
         raise ValueError("the rotary table takes no gradient")
-    if _derived(x) or _transforming():
+    if _derived(x) or _transforming() and stream is None and not kw:
         if stream is not None or kw:
             raise ValueError("a rotation that records a gradient runs on the current stream and takes no out or status")
         return _Rotation.apply(x, rotary, positions, inverse)

@@ -75,6 +75,14 @@ def test_autograd_sees_what_is_written(cuda):
         with pytest.raises(ValueError):
             run()
     assert torch.equal(y, before)
+    with forward_ad.dual_level():
+        z = forward_ad.make_dual(x, x)
+        with pytest.raises(ValueError):
+            rotate(x.clone(), rot, at, out=z)
+    # (What a transform does not look at stays as it is outside.)
+    out = torch.empty_like(x)
+    torch.func.grad(lambda s: (rotate(x, rot, at, out=out) * s).sum())(torch.ones(1, device="cuda"))
+    same(out, turned(x, rot.table, [0] * 32, at, False))
     with torch.no_grad():
         call.run()
     same(y.detach(), turned(before, rot.table, [0] * 32, at, False))
